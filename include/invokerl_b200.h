@@ -262,6 +262,62 @@ IKRL_API int ikrl_logits_logprob_bwd(const void* logits, int64_t ld, const int64
                             const float* dlogp, int64_t N, int32_t V, void* dlogits,
                             int64_t ld_out, void* stream);
 
+/* ---- K4: losses over token distributions (no counterpart in the reference) ---------------------- */
+
+/* Distillation from a teacher's top log-probs and cross entropy, per row, with their gradients; on
+ * logits in memory here and through the LM head below.
+ *
+ * Rows have logits x [V], z = x / temperature, p = softmax(z).  Distillation: each row has K teacher
+ * entries (id, log-prob), q = exp(log-prob), in any order, K <= 256.  An entry counts when its id is
+ * >= 0 and its log-prob is above -inf, and a repeated id at its first place only; a row without
+ * entries has loss 0 and no gradient; an id >= V makes the row's loss and gradient NaN.  Outcomes
+ * are the entries' columns and, with `tail`, one more: any other column, of student mass p_t (the
+ * sum over those columns) and teacher mass q_t = 1 - sum q (0 when that is below 2^-20).
+ *   IKRL_DISTILL_FORWARD  KL(q | p); without `tail`, q is renormalised over the entries
+ *   IKRL_DISTILL_REVERSE  KL(p | q), the tail's log q_t taken from max(1 - sum q, 2^-20)
+ *   IKRL_DISTILL_JSD      beta KL(q | m) + (1 - beta) KL(p | m), m = beta q + (1 - beta) p
+ * The last two need `tail` (IKRL_ERR_UNSUPPORTED without).  Logits may be -inf (masked columns).
+ *
+ * Cross entropy: (lse - x_y) + label_smoothing * (x_y - mean_v x) + z_loss * lse^2 with
+ * lse = logsumexp(x); targets int64, -100 gives loss 0 and no gradient, others outside [0, V) NaN. */
+enum { IKRL_DISTILL_FORWARD = 0, IKRL_DISTILL_REVERSE = 1, IKRL_DISTILL_JSD = 2 };
+typedef struct {
+  int32_t kind;      /* IKRL_DISTILL_* */
+  int32_t tail;      /* 1: the other columns are one more outcome */
+  float beta;        /* IKRL_DISTILL_JSD: weight of the teacher, in (0, 1) */
+  float temperature; /* > 0; the teacher's log-probs are taken as given at this temperature */
+} ikrl_distill_params;
+
+/* A teacher's top log-probs: the K largest logits of each row (1 <= K <= 256, K <= V), largest first,
+ * of equal ones the lower column first, NaN before all: ids int64 [N][K] and logp fp32 [N][K] =
+ * log softmax(x / temperature) over the whole row.  logits as below. */
+IKRL_API int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V, int32_t K,
+                              float temperature, float* logp, int64_t* ids, void* stream);
+
+/* Bytes of the row state a forward writes and its backward reads (256-byte aligned, caller-owned):
+ * K entries a row, K = 1 for a cross entropy. */
+IKRL_API size_t ikrl_row_loss_state_bytes(int64_t N, int32_t K);
+
+/* logits [N, ld] of `dtype` (IKRL_DTYPE_BF16 or IKRL_DTYPE_F32; row stride ld >= V, any alignment of
+ * the rows), V <= 2^21.  loss [N] fp32.  The backward writes dlogits (the same dtype, row stride
+ * ld_out) = dloss[r] * d loss[r] / d logits[r]; rows with dloss == 0 are zeros and are not read.  It
+ * reads the logits again: they must be unchanged.  Both directions run inside a stream capture. */
+IKRL_API int ikrl_logits_distill_fwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V,
+                                     const int64_t* teacher_ids, const float* teacher_logp, int32_t K,
+                                     const ikrl_distill_params* params, float* loss, void* state,
+                                     size_t state_bytes, void* stream);
+IKRL_API int ikrl_logits_distill_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V,
+                                     int32_t K, const ikrl_distill_params* params, const void* state,
+                                     size_t state_bytes, const float* dloss, void* dlogits, int64_t ld_out,
+                                     void* stream);
+IKRL_API int ikrl_logits_cross_entropy_fwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V,
+                                           const int64_t* targets, float label_smoothing, float z_loss,
+                                           float* loss, void* state, size_t state_bytes, void* stream);
+IKRL_API int ikrl_logits_cross_entropy_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V,
+                                           float label_smoothing, float z_loss, const void* state,
+                                           size_t state_bytes, const float* dloss, void* dlogits,
+                                           int64_t ld_out, void* stream);
+
 /* ---- K1: fused LM-head log-prob (tcgen05 / TMEM / TMA) --------------------------------------- */
 
 /* Replaces the LM head + cross-entropy of invokerl/policy.py:124-191 (`_chunked_lm_head_ce`,
@@ -347,6 +403,34 @@ IKRL_API int ikrl_lmhead_logprob_fwd_noalloc(const void* hidden, const void* wei
  * kernel recorded when a bounded wait expired (its outputs are then NaN).  No counterpart in the
  * reference. */
 IKRL_API int ikrl_lmhead_noalloc_status(int32_t* status_out, void* stream);
+
+/* The K4 losses through the LM head: logits = hidden W^T of bf16 hidden [N, H] and weight [V, H], as
+ * ikrl_lmhead_logprob_fwd / _bwd and with their rules (H a multiple of 8, alignments, row skipping
+ * and the one host synchronisation of the backward outside a stream capture, chunk_rows,
+ * dweight_dtype and accumulation, ikrl_lmhead_status on the workspace).  The [N, V] logits are never
+ * in memory.  state: ikrl_row_loss_state_bytes(N, K), K = 1 for the cross entropy, as the forward
+ * left it; dloss[N] fp32 is the upstream gradient of the row losses. */
+IKRL_API size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int32_t K);
+IKRL_API size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
+                                                         int32_t dweight_dtype, int32_t accumulate_dweight);
+IKRL_API int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,
+                                     const float* teacher_logp, int64_t N, int32_t H, int32_t V, int32_t K,
+                                     const ikrl_distill_params* params, float* loss, void* state,
+                                     size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
+IKRL_API int ikrl_lmhead_distill_bwd(const void* hidden, const void* weight, int64_t N, int32_t H, int32_t V,
+                                     int32_t K, const ikrl_distill_params* params, const void* state,
+                                     size_t state_bytes, const float* dloss, int64_t chunk_rows, void* dhidden,
+                                     void* dweight, int32_t dweight_dtype, int32_t accumulate_dweight, void* ws,
+                                     size_t ws_bytes, void* stream);
+IKRL_API int ikrl_lmhead_cross_entropy_fwd(const void* hidden, const void* weight, const int64_t* targets,
+                                           int64_t N, int32_t H, int32_t V, float label_smoothing, float z_loss,
+                                           float* loss, void* state, size_t state_bytes, void* ws,
+                                           size_t ws_bytes, void* stream);
+IKRL_API int ikrl_lmhead_cross_entropy_bwd(const void* hidden, const void* weight, int64_t N, int32_t H,
+                                           int32_t V, float label_smoothing, float z_loss, const void* state,
+                                           size_t state_bytes, const float* dloss, int64_t chunk_rows,
+                                           void* dhidden, void* dweight, int32_t dweight_dtype,
+                                           int32_t accumulate_dweight, void* ws, size_t ws_bytes, void* stream);
 
 /* Selects the K1 GEMM kernel for later calls in this process: CTA pairs (tcgen05 cta_group::2,
  * clusters of two; the default) or single CTAs (enable = 0).  Returns the previous setting.  The

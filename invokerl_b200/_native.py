@@ -23,6 +23,10 @@ IKRL_DTYPE_BF16 = 1
 IKRL_KL_SCHULMAN = 0
 IKRL_KL_SIMPLE = 1
 IKRL_KL_NONE = 2
+IKRL_DISTILL_FORWARD = 0
+IKRL_DISTILL_REVERSE = 1
+IKRL_DISTILL_JSD = 2
+MAX_ENTRIES = 256  # teacher entries of a row, and the k of a top-k
 IKRL_LOSS_GRPO = 0
 IKRL_LOSS_PPO = 1
 # Launch knobs of ikrl_set_tuning (include/invokerl_b200.h, IKRL_TUNE_*).
@@ -77,6 +81,10 @@ class LossParams(ctypes.Structure):
         ("vf_coef", c_float),
         ("vf_clip_eps", c_float),
     ]
+
+
+class DistillParams(ctypes.Structure):
+    _fields_ = [("kind", c_int32), ("tail", c_int32), ("beta", c_float), ("temperature", c_float)]
 
 
 # name -> (restype, argtypes).  Pointers are passed as c_void_p (device addresses).
@@ -135,6 +143,51 @@ _SIGNATURES: dict[str, tuple] = {
     "ikrl_lmhead_logprob_bwd": (
         ctypes.c_int,
         [_P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int64, _P, _P, c_int32, c_int32, _P, c_size_t, _P],
+    ),
+    "ikrl_row_loss_state_bytes": (c_size_t, [c_int64, c_int32]),
+    "ikrl_logits_topk": (
+        ctypes.c_int,
+        [_P, c_int32, c_int64, c_int64, c_int32, c_int32, c_float, _P, _P, _P],
+    ),
+    "ikrl_logits_distill_fwd": (
+        ctypes.c_int,
+        [_P, c_int32, c_int64, c_int64, c_int32, _P, _P, c_int32, POINTER(DistillParams), _P, _P, c_size_t, _P],
+    ),
+    "ikrl_logits_distill_bwd": (
+        ctypes.c_int,
+        [_P, c_int32, c_int64, c_int64, c_int32, c_int32, POINTER(DistillParams), _P, c_size_t, _P, _P, c_int64, _P],
+    ),
+    "ikrl_logits_cross_entropy_fwd": (
+        ctypes.c_int,
+        [_P, c_int32, c_int64, c_int64, c_int32, _P, c_float, c_float, _P, _P, c_size_t, _P],
+    ),
+    "ikrl_logits_cross_entropy_bwd": (
+        ctypes.c_int,
+        [_P, c_int32, c_int64, c_int64, c_int32, c_float, c_float, _P, c_size_t, _P, _P, c_int64, _P],
+    ),
+    "ikrl_lmhead_row_loss_fwd_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32]),
+    "ikrl_lmhead_row_loss_bwd_workspace_bytes": (
+        c_size_t,
+        [c_int64, c_int32, c_int32, c_int64, c_int32, c_int32],
+    ),
+    "ikrl_lmhead_distill_fwd": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, POINTER(DistillParams), _P, _P, c_size_t, _P, c_size_t,
+         _P],
+    ),
+    "ikrl_lmhead_distill_bwd": (
+        ctypes.c_int,
+        [_P, _P, c_int64, c_int32, c_int32, c_int32, POINTER(DistillParams), _P, c_size_t, _P, c_int64, _P, _P,
+         c_int32, c_int32, _P, c_size_t, _P],
+    ),
+    "ikrl_lmhead_cross_entropy_fwd": (
+        ctypes.c_int,
+        [_P, _P, _P, c_int64, c_int32, c_int32, c_float, c_float, _P, _P, c_size_t, _P, c_size_t, _P],
+    ),
+    "ikrl_lmhead_cross_entropy_bwd": (
+        ctypes.c_int,
+        [_P, _P, c_int64, c_int32, c_int32, c_float, c_float, _P, c_size_t, _P, c_int64, _P, _P, c_int32, c_int32,
+         _P, c_size_t, _P],
     ),
     "ikrl_lmhead_status": (ctypes.c_int, [_P, POINTER(c_int32), _P]),
     "ikrl_lmhead_cache_row_elems": (ctypes.c_int, [c_int32, POINTER(c_int64), POINTER(c_int64)]),
@@ -337,6 +390,7 @@ def sz(x: int) -> c_size_t:
 
 __all__ = [
     "IkrlError",
+    "DistillParams",
     "LossParams",
     "lib",
     "call",

@@ -22,6 +22,7 @@
 // Every mbarrier wait is bounded (sm100::kWaitTimeoutNs); on expiry the CTA records an error,
 // drains its in-flight copies and MMAs, frees TMEM and exits.
 #include "common.cuh"
+#include "row_dist.cuh"
 #include "sm100.cuh"
 
 #include <atomic>
@@ -51,8 +52,24 @@ constexpr uint32_t kMnAtomBytes = 64 * BK * 2;  // one 64-wide MN slab of an MN-
 
 // EPI_LSE_CACHED: the forward's epilogue that also fills the logit cache (its own instantiation,
 // so the plain forward carries none of the cache's code).
-enum Epi : int { EPI_LSE = 0, EPI_DLOGITS = 1, EPI_STORE_BF16 = 2, EPI_F32 = 3, EPI_LSE_CACHED = 4 };
+// EPI_TAIL, EPI_DTAIL: forward and backward of the row losses (row_dist.cuh).  EPI_TAIL takes each
+// row's entry columns out of the accumulator, stores their logits and keeps the running sum of the
+// others; EPI_DTAIL forms the gradient of the others.
+enum Epi : int {
+  EPI_LSE = 0,
+  EPI_DLOGITS = 1,
+  EPI_STORE_BF16 = 2,
+  EPI_F32 = 3,
+  EPI_LSE_CACHED = 4,
+  EPI_TAIL = 5,
+  EPI_DTAIL = 6
+};
 constexpr bool is_lse(int epi) { return epi == EPI_LSE || epi == EPI_LSE_CACHED; }
+constexpr bool is_dlogits(int epi) { return epi == EPI_DLOGITS || epi == EPI_DTAIL; }
+// The epilogue whose launch rules (pacing, splits) an epilogue follows.
+constexpr int epi_kind(int epi) {
+  return (epi == EPI_LSE_CACHED || epi == EPI_TAIL) ? (int)EPI_LSE : (epi == EPI_DTAIL ? (int)EPI_DLOGITS : epi);
+}
 enum F32Mode : int { F32_STORE = 0, F32_ADD = 1, F32_ADD_TO_BF16 = 2 };
 
 struct GemmParams {
@@ -90,6 +107,13 @@ struct GemmParams {
   float* cache_m;         // [slots][n_mchunks] chunk maxima, log2 units
   int64_t ld_cache;
   int n_mchunks;
+  // Row losses (TAIL, DTAIL)
+  float c;                // log2(e) / temperature
+  const int* cols;        // [M][n_cols] entry columns ascending, kNoEntry behind the last (TAIL)
+  int n_cols;
+  float* xk;              // [M][n_cols] logits at the entries (TAIL)
+  float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
+  const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
 };
 
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err) {
@@ -153,6 +177,32 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
     if (row_ok && p.slot != nullptr) cslot = p.slot[grow];
     cslot0 = __shfl_sync(0xffffffffu, cslot, 0);
     cache_run = stage_smem != 0 && __all_sync(0xffffffffu, cslot >= 0 && cslot == cslot0 + lane);
+  }
+  // TAIL: the row's next entry column at or after the columns read so far
+  const int* next_col = nullptr;
+  int next = kNoEntry, at = 0;
+  float sum_x = 0.f;
+  auto advance = [&]() { next = ++at < p.n_cols ? next_col[at] : kNoEntry; };
+  if constexpr (EPI == EPI_TAIL) {
+    if (row_ok) {
+      next_col = p.cols + (int64_t)grow * p.n_cols;
+      int hi = p.n_cols;
+      const int from = t_begin * TILE_N;
+      while (at < hi) {
+        const int mid = (at + hi) >> 1;
+        if (next_col[mid] < from) at = mid + 1;
+        else hi = mid;
+      }
+      if (at < p.n_cols) next = next_col[at];
+    }
+  }
+  float level = 0.f;
+  if constexpr (EPI == EPI_DTAIL) {
+    if (row_ok) {
+      lse2 = p.lse[grow] * p.c;
+      gval = p.g[grow];
+      level = p.level[grow];
+    }
   }
   if constexpr (EPI == EPI_DLOGITS) {
     if (row_ok) {
@@ -229,10 +279,48 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       }
       if (cslot >= 0) p.cache_m[(int64_t)cslot * p.n_mchunks + (col0 >> 5)] = cm;
       }  // EPI_LSE_CACHED
-    } else if constexpr (EPI == EPI_DLOGITS) {
+    } else if constexpr (EPI == EPI_TAIL) {
+      if (p.part_x != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sum_x += i < nvalid ? v[i] : 0.f;
+      }
+      // Entries in this chunk leave it: their logits to xk, -inf in their place.
+      while (next < col0) advance();  // entries of other warps' columns
+      while (next < col0 + nvalid) {
+        const int rel = next - col0;
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i == rel) {
+            x = v[i];
+            v[i] = -INFINITY;
+          }
+        p.xk[(int64_t)grow * p.n_cols + at] = x;
+        advance();
+      }
+      float cm = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < nvalid) cm = fmaxf(cm, v[i]);
+      const float from = cm == -INFINITY ? 0.f : cm;  // a chunk of entries only sums to 0
+      float cs = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) cs += i < nvalid ? fast_exp2((v[i] - from) * p.c) : 0.f;
+      if (cm > run_m) {
+        run_s = fmaf(run_s, fast_exp2((run_m - cm) * p.c), cs);
+        run_m = cm;
+      } else {
+        run_s = fmaf(cs, cm == -INFINITY ? 1.f : fast_exp2((cm - run_m) * p.c), run_s);
+      }
+    } else if constexpr (is_dlogits(EPI)) {
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
+        if constexpr (EPI == EPI_DTAIL) {
+          w[i >> 1] = pack_bf16x2(fmaf(gval, fast_exp2(fmaf(v[i], p.c, -lse2)), level),
+                                  fmaf(gval, fast_exp2(fmaf(v[i + 1], p.c, -lse2)), level));
+          continue;
+        }
         const float p0 = fast_exp2(fmaf(v[i], kLog2e, -lse2));
         const float p1 = fast_exp2(fmaf(v[i + 1], kLog2e, -lse2));
         const float d0 = gval * (((int64_t)(col0 + i) == tgt ? 1.f : 0.f) - p0);
@@ -366,7 +454,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       }
     }
   }
-  if constexpr (EPI == EPI_DLOGITS || EPI == EPI_LSE_CACHED) {
+  if constexpr (is_dlogits(EPI) || EPI == EPI_LSE_CACHED) {
     // Every TMA store of this warp has completed before the CTA can exit.
     if (stage_smem != 0 && lane == 0) bulk_wait_all();
     __syncwarp();
@@ -377,6 +465,14 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       p.part_m[(int64_t)set * p.M + grow] = run_m;
       p.part_s[(int64_t)set * p.M + grow] = run_s;
       if (found) p.part_t[grow] = tval;
+    }
+  }
+  if constexpr (EPI == EPI_TAIL) {
+    if (row_ok && !*abort_v) {
+      const int64_t o = (int64_t)(split * GROUPS + group) * p.M + grow;
+      p.part_m[o] = run_m;
+      p.part_s[o] = run_s;
+      if (p.part_x != nullptr) p.part_x[o] = sum_x;
     }
   }
   return ok;
@@ -1024,7 +1120,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     // ---------------- epilogue (both CTAs, own 128 rows x 512 columns) ----------------
     const uint32_t af[2] = {smem_u32(&acc_full[0]), smem_u32(&acc_full[1])};
     const uint32_t ae[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
-    const uint32_t stage = ((EPI == EPI_DLOGITS || EPI == EPI_LSE_CACHED) && p.ds_tma)
+    const uint32_t stage = ((is_dlogits(EPI) || EPI == EPI_LSE_CACHED) && p.ds_tma)
                                ? smem_base + kWideStages * kWideStageBytes + (uint32_t)(warp - 2) * kDsStageBytes
                                : 0u;
     int jb = 0;
@@ -1223,7 +1319,7 @@ int pace_array(unsigned** out) {
 bool pacing_enabled(int epi, int K) {
   int64_t mask = tuning(IKRL_TUNE_PACE);
   if (mask < 0) mask = K >= 2048 ? 15 : 14;
-  return (mask >> (epi == EPI_LSE_CACHED ? EPI_LSE : epi)) & 1;
+  return (mask >> epi_kind(epi)) & 1;
 }
 bool persistent_pairs() { return tuning(IKRL_TUNE_PERSISTENT) != 0; }
 
@@ -1232,7 +1328,7 @@ int launch_gemm_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorM
                      int m_tiles, cudaStream_t s) {
   GemmParams p = p_in;
   auto kern = WIDE ? lmhead_gemm_wide_kernel<EPI, A_MN, B_MN> : lmhead_gemm_pair_kernel<EPI, A_MN, B_MN>;
-  p.ds_tma = (WIDE && c != nullptr && (EPI == EPI_DLOGITS || EPI == EPI_LSE_CACHED)) ? 1 : 0;
+  p.ds_tma = (WIDE && c != nullptr && (is_dlogits(EPI) || EPI == EPI_LSE_CACHED)) ? 1 : 0;
   const uint32_t smem_bytes = WIDE ? (p.ds_tma ? kWideDsSmemBytes : kWideSmemBytes) : kPairSmemBytes;
   IKRL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes));
   IKRL_REQUIRE(p.split_major == 1, IKRL_ERR_UNSUPPORTED, "pair kernel needs a split-major grid");
@@ -1375,7 +1471,7 @@ K1Plan plan_k1(int epi, int64_t m_tiles, int N, int K, int splits_hint, int nsm)
     pl.tiles_per_split = 1;
   } else {
     pl.tiles_per_split = (int)cdiv64(pl.n_tiles, splits_hint);
-    if (epi == EPI_DLOGITS && pl.kind != 0 && persistent && balance_splits_enabled())
+    if (is_dlogits(epi) && pl.kind != 0 && persistent && balance_splits_enabled())
       pl.tiles_per_split = balanced_tiles_per_split(m_tiles, pl.n_tiles, splits_hint, npairs);
   }
   pl.splits = (int)cdiv64(pl.n_tiles, pl.tiles_per_split);
@@ -1841,6 +1937,36 @@ __global__ void scatter_rows_kernel(const uint4* __restrict__ src, const int* __
   }
 }
 
+// Row losses, backward: what the dS epilogue multiplies and adds for compacted row k (row idx[k]; k
+// itself when idx is null), gs = g coef and level_out = g level; 0 for rows without a gradient.
+__global__ void row_scale_kernel(const float* __restrict__ dloss, const int64_t* __restrict__ row_ids,
+                                 const float* __restrict__ coef, const int* __restrict__ idx, int64_t n, float level,
+                                 float* __restrict__ gs, float* __restrict__ level_out) {
+  const int64_t k = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (k >= n) return;
+  const int64_t r = idx ? idx[k] : k;
+  const float g = dloss[r];
+  const bool on = g != 0.f && row_ids[r] != kRowNone;
+  gs[k] = on ? g * coef[r] : 0.f;
+  level_out[k] = on ? g * level : 0.f;
+}
+
+// Row losses, backward: the gradient at the entries of chunk rows [c0, c0 + rows) goes over what the
+// dS epilogue wrote there.  One block of threads per 256 entries.
+__global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __restrict__ cols,
+                                  const float* __restrict__ grad, int K, const int* __restrict__ idx, int64_t c0,
+                                  int64_t rows, uint16_t* __restrict__ ds, int64_t ld_ds) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= rows * K) return;
+  const int64_t k = i / K;
+  const int e = (int)(i - k * K);
+  const int64_t r = idx ? idx[c0 + k] : c0 + k;
+  const int col = cols[r * K + e];
+  if (col == kNoEntry) return;
+  const float g = dloss[r];
+  ds[k * ld_ds + col] = g != 0.f ? f32_to_bf16_rn(g * grad[r * K + e]) : (uint16_t)0;
+}
+
 // Row skipping is on unless IKRL_TUNE_SKIP_ZERO_ROWS = 0.
 bool skip_zero_rows_enabled() { return tuning(IKRL_TUNE_SKIP_ZERO_ROWS) != 0; }
 
@@ -1881,6 +2007,15 @@ struct CacheArgs {
 size_t cache_fwd_workspace_bytes(int64_t N, int H, int V) {
   const size_t base = fwd_layout(N, H, V).total;
   return base + ((((size_t)std::max<int64_t>(1, cdiv64(N, kCompactRows)) * 4) + 255) & ~size_t(255));
+}
+
+// Workspace of a row loss: its forward's partial sums of all logits and logits at the entries stand
+// behind the forward's own, its backward's levels behind the backward's own.
+static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+static size_t row_level_bytes(int64_t N) { return align256((size_t)N * 4); }
+static size_t row_loss_fwd_bytes(int64_t N, int H, int V, int K) {
+  const FwdLayout L = fwd_layout(N, H, V);
+  return L.total + align256((size_t)kWideGroups * L.splits * N * 4) + align256((size_t)N * K * 4);
 }
 
 static int lmhead_fwd_impl(const char* what, const void* hidden, const void* weight, const int64_t* ids, int64_t N, int32_t H,
@@ -1946,14 +2081,24 @@ static int lmhead_fwd_impl(const char* what, const void* hidden, const void* wei
 }
 
 
+// A row loss (row_dist.cuh) behind the LM head's backward: the state its forward left, and its level
+// (the constant part of the gradient).
+struct RowLossBwd {
+  RowState st;
+  int K;
+  float c, level;
+};
+
 // cache_slot / cache_q / cache_m: the logit cache a forward filled (all null: no cache).  Active
 // rows with a slot take their dS from the cache; the others are recomputed by the dS GEMM.
+// rl: null for log p(ids); otherwise the row loss whose gradient dlogp is, with ids and lse its
+// state's row_ids and ref.
 static int lmhead_bwd_impl(const char* what, const void* hidden, const void* weight, const int64_t* ids,
                            const float* lse, const float* dlogp, int64_t N, int32_t H, int32_t V, int64_t vocab_start,
                            int64_t chunk_rows, void* dhidden, void* dweight, int32_t dweight_dtype,
                            int32_t accumulate_dweight, void* ws, size_t ws_bytes, void* stream,
                            const int* cache_slot = nullptr, const uint16_t* cache_q = nullptr,
-                           const float* cache_m = nullptr) {
+                           const float* cache_m = nullptr, const RowLossBwd* rl = nullptr) {
   int rc = check_common(hidden, weight, ids, N, H, V, what);
   if (rc) return rc;
   IKRL_REQUIRE(dweight_dtype == IKRL_DTYPE_F32 || dweight_dtype == IKRL_DTYPE_BF16, IKRL_ERR_UNSUPPORTED,
@@ -1969,8 +2114,9 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   IKRL_REQUIRE(lse && dlogp && (dhidden || dweight), IKRL_ERR_INVALID_ARGUMENT,
                "%s: null pointer", what);
   const BwdLayout L = bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
-  IKRL_REQUIRE(ws != nullptr && ws_bytes >= L.total, IKRL_ERR_WORKSPACE,
-               "%s: workspace %zu < %zu bytes", what, ws_bytes, L.total);
+  const size_t ws_need = L.total + (rl ? row_level_bytes(N) : 0);
+  IKRL_REQUIRE(ws != nullptr && ws_bytes >= ws_need, IKRL_ERR_WORKSPACE,
+               "%s: workspace %zu < %zu bytes", what, ws_bytes, ws_need);
   IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
                "%s: workspace must be 256-byte aligned", what);
   IKRL_REQUIRE(dweight == nullptr || (reinterpret_cast<uintptr_t>(dweight) & 15) == 0, IKRL_ERR_ALIGNMENT,
@@ -2044,6 +2190,16 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     }
   }
 
+  float* level = nullptr;
+  if (rl) {
+    float* gs = reinterpret_cast<float*>(w + L.gc_off);
+    level = reinterpret_cast<float*>(w + L.total);
+    row_scale_kernel<<<(unsigned)cdiv64(Nw, 256), 256, 0, s>>>(dlogp, rl->st.row_ids, rl->st.coef, idx_c, Nw,
+                                                               rl->level, gs, level);
+    if ((rc = check_launch("row_scale_kernel"))) return rc;
+    gsrc = gs;
+  }
+
   const BwdLayout Lw = bwd_layout(Nw, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
   const int64_t chunk = std::min(L.chunk, Lw.chunk);
   // Chunks: first the cached rows [0, n_cached), then the others, so every chunk takes its dS one
@@ -2088,7 +2244,18 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       p.id_offset = vocab_start;
       p.out_bf16 = dS; p.ld_bf16 = L.lds;
       p.err = err;
-      if ((rc = launch_k1<EPI_DLOGITS, false, false>(ta, t_w_k, ta, t_w_k2, p, m_tiles, sp, s, &tds))) return rc;
+      if (rl) {
+        p.level = level + c0;
+        p.c = rl->c;
+        if ((rc = launch_k1<EPI_DTAIL, false, false>(ta, t_w_k, ta, t_w_k2, p, m_tiles, sp, s, &tds))) return rc;
+      } else {
+        if ((rc = launch_k1<EPI_DLOGITS, false, false>(ta, t_w_k, ta, t_w_k2, p, m_tiles, sp, s, &tds))) return rc;
+      }
+    }
+    if (rl) {
+      ds_entries_kernel<<<(unsigned)cdiv64(rows * rl->K, 256), 256, 0, s>>>(dlogp, rl->st.cols, rl->st.grad, rl->K,
+                                                                            idx_c, c0, rows, dS, L.lds);
+      if ((rc = check_launch("ds_entries_kernel"))) return rc;
     }
     // 2) dW (+)= dS^T h[chunk]
     if (dweight) {
@@ -2150,8 +2317,138 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   return IKRL_OK;
 }
 
+// Forward of a row loss through the LM head: entries, the GEMM with the TAIL epilogue, losses.
+static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void* weight, const int64_t* tids,
+                               const float* tlp, int64_t N, int32_t H, int32_t V, int32_t K, const RowLossParams& P,
+                               float* loss, void* state, size_t state_bytes, void* ws, size_t ws_bytes,
+                               void* stream) {
+  int rc = check_common(hidden, weight, tids, N, H, V, what);
+  if (rc) return rc;
+  if (N == 0) return clear_status_word(ws, ws_bytes, stream);
+  IKRL_REQUIRE(loss != nullptr, IKRL_ERR_INVALID_ARGUMENT, "%s: output is NULL", what);
+  IKRL_REQUIRE(state != nullptr && state_bytes >= row_state_bytes(N, K), IKRL_ERR_WORKSPACE,
+               "%s: state %zu < %zu bytes", what, state_bytes, row_state_bytes(N, K));
+  const size_t need = row_loss_fwd_bytes(N, H, V, K);
+  IKRL_REQUIRE(ws != nullptr && ws_bytes >= need, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes,
+               need);
+  IKRL_REQUIRE(((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(state)) & 255) == 0,
+               IKRL_ERR_ALIGNMENT, "%s: workspace and state must be 256-byte aligned", what);
+  cudaStream_t s = as_stream(stream);
+  const FwdLayout L = fwd_layout(N, H, V);
+  const RowState st = row_state(state, N, K);
+  char* w = reinterpret_cast<char*>(ws);
+  int* err = reinterpret_cast<int*>(w + L.err_off);
+  float* part_x = reinterpret_cast<float*>(w + L.total);
+  float* xk = reinterpret_cast<float*>(w + L.total + align256((size_t)kWideGroups * L.splits * N * 4));
+  IKRL_CUDA(cudaMemsetAsync(err, 0, sizeof(int), s));
+  CUtensorMap ta, tb, tb2;
+  if ((rc = make_tmap(&ta, hidden, H, N, H, BM, "hidden"))) return rc;
+  if ((rc = make_tmap(&tb, weight, H, V, H, BN, "weight"))) return rc;
+  if ((rc = make_tmap(&tb2, weight, H, V, H, BN / 2, "weight"))) return rc;
+  if ((rc = launch_row_entries(tids, tlp, N, K, P, st, s))) return rc;
+  GemmParams p{};
+  p.M = (int)N; p.N = V; p.K = H;
+  p.part_m = reinterpret_cast<float*>(w + L.pm_off);
+  p.part_s = reinterpret_cast<float*>(w + L.ps_off);
+  p.part_x = P.loss == ROW_XENT && P.smoothing != 0.f ? part_x : nullptr;
+  p.err = err;
+  p.c = P.c;
+  p.cols = st.cols;
+  p.n_cols = K;
+  p.xk = xk;
+  if ((rc = launch_k1<EPI_TAIL, false, false>(ta, tb, ta, tb2, p, (int)cdiv64(N, BM), L.splits, s))) return rc;
+  return launch_row_losses(p.part_m, p.part_s, p.part_x, p.part_sets, xk, N, K, P, st, loss, err, s);
+}
+
+static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void* weight, int64_t N, int32_t H,
+                               int32_t V, int32_t K, const RowLossParams& P, const void* state, size_t state_bytes,
+                               const float* dloss, int64_t chunk_rows, void* dhidden, void* dweight,
+                               int32_t dweight_dtype, int32_t accumulate_dweight, void* ws, size_t ws_bytes,
+                               void* stream) {
+  RowLossBwd rl{};
+  const bool rows = N > 0;
+  if (rows) {
+    IKRL_REQUIRE(state != nullptr && state_bytes >= row_state_bytes(N, K), IKRL_ERR_WORKSPACE,
+                 "%s: state %zu < %zu bytes", what, state_bytes, row_state_bytes(N, K));
+    IKRL_REQUIRE((reinterpret_cast<uintptr_t>(state) & 255) == 0, IKRL_ERR_ALIGNMENT,
+                 "%s: state must be 256-byte aligned", what);
+    rl.st = row_state(const_cast<void*>(state), N, K);
+  }
+  rl.K = K;
+  rl.c = P.c;
+  rl.level = P.loss == ROW_XENT ? -P.smoothing / (float)V : 0.f;
+  return lmhead_bwd_impl(what, hidden, weight, rl.st.row_ids, rl.st.ref, dloss, N, H, V, 0, chunk_rows, dhidden,
+                         dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream, nullptr, nullptr, nullptr,
+                         &rl);
+}
+
 
 extern "C" {
+
+size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int32_t K) {
+  if (N <= 0 || H <= 0 || V <= 0 || K <= 0) return 256;
+  return row_loss_fwd_bytes(N, H, V, K);
+}
+
+size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
+                                                int32_t dweight_dtype, int32_t accumulate_dweight) {
+  if (N <= 0 || H <= 0 || V <= 0) return 256;
+  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + row_level_bytes(N);
+}
+
+int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,
+                            const float* teacher_logp, int64_t N, int32_t H, int32_t V, int32_t K,
+                            const ikrl_distill_params* params, float* loss, void* state, size_t state_bytes, void* ws,
+                            size_t ws_bytes, void* stream) {
+  clear_error();
+  const char* what = "ikrl_lmhead_distill_fwd";
+  RowLossParams P;
+  int rc = distill_params(what, params, V, K, &P);
+  if (rc) return rc;
+  IKRL_REQUIRE(N <= 0 || teacher_logp, IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  return lmhead_row_loss_fwd(what, hidden, weight, teacher_ids, teacher_logp, N, H, V, K, P, loss, state, state_bytes,
+                             ws, ws_bytes, stream);
+}
+
+int ikrl_lmhead_distill_bwd(const void* hidden, const void* weight, int64_t N, int32_t H, int32_t V, int32_t K,
+                            const ikrl_distill_params* params, const void* state, size_t state_bytes,
+                            const float* dloss, int64_t chunk_rows, void* dhidden, void* dweight,
+                            int32_t dweight_dtype, int32_t accumulate_dweight, void* ws, size_t ws_bytes,
+                            void* stream) {
+  clear_error();
+  const char* what = "ikrl_lmhead_distill_bwd";
+  RowLossParams P;
+  int rc = distill_params(what, params, V, K, &P);
+  if (rc) return rc;
+  return lmhead_row_loss_bwd(what, hidden, weight, N, H, V, K, P, state, state_bytes, dloss, chunk_rows, dhidden,
+                             dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream);
+}
+
+int ikrl_lmhead_cross_entropy_fwd(const void* hidden, const void* weight, const int64_t* targets, int64_t N,
+                                  int32_t H, int32_t V, float label_smoothing, float z_loss, float* loss, void* state,
+                                  size_t state_bytes, void* ws, size_t ws_bytes, void* stream) {
+  clear_error();
+  const char* what = "ikrl_lmhead_cross_entropy_fwd";
+  RowLossParams P;
+  int rc = xent_params(what, label_smoothing, z_loss, V, &P);
+  if (rc) return rc;
+  return lmhead_row_loss_fwd(what, hidden, weight, targets, nullptr, N, H, V, 1, P, loss, state, state_bytes, ws,
+                             ws_bytes, stream);
+}
+
+int ikrl_lmhead_cross_entropy_bwd(const void* hidden, const void* weight, int64_t N, int32_t H, int32_t V,
+                                  float label_smoothing, float z_loss, const void* state, size_t state_bytes,
+                                  const float* dloss, int64_t chunk_rows, void* dhidden, void* dweight,
+                                  int32_t dweight_dtype, int32_t accumulate_dweight, void* ws, size_t ws_bytes,
+                                  void* stream) {
+  clear_error();
+  const char* what = "ikrl_lmhead_cross_entropy_bwd";
+  RowLossParams P;
+  int rc = xent_params(what, label_smoothing, z_loss, V, &P);
+  if (rc) return rc;
+  return lmhead_row_loss_bwd(what, hidden, weight, N, H, V, 1, P, state, state_bytes, dloss, chunk_rows, dhidden,
+                             dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream);
+}
 
 size_t ikrl_lmhead_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V) {
   if (N <= 0 || H <= 0 || V <= 0) return 256;

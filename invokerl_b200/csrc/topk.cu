@@ -1,0 +1,238 @@
+// The k likeliest tokens of each row of logits and their log-probs over the whole vocabulary: what
+// a teacher gives a distillation.
+//
+// One pass over the row, bound by HBM.  Beside the running logsumexp, a block keeps the columns that
+// may still be among the k largest in a buffer in shared memory: a column enters when it is above the
+// k-th largest known so far.  The first columns set that bar (the k-th largest of the threads' own
+// maxima is below the k-th largest of all), so of V columns in no particular order about
+// k (1 + ln(V / 16384)) enter and the buffer is sorted once, at the end.  Where it fills up (rising
+// rows), it is sorted there, cut to k, and the bar rises; what did not fit waits in registers.
+//
+// Order and ties are those of one 64-bit key, the value above the inverted column: larger values
+// first, of equal values the lower column.  Keys are distinct, so the result does not depend on the
+// order in which columns enter.
+#include "row_dist.cuh"
+#include "row_load.cuh"
+
+#include <cooperative_groups.h>
+
+namespace ikrl {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kTopThreads = 512;
+constexpr int kTopBuf = 2048;  // keys of the buffer: the cluster's 8 x kMaxEntries at the end
+static_assert(kTopBuf >= 8 * kMaxEntries && kTopBuf >= 2 * kMaxEntries, "top-k buffer too small");
+
+// Values in key order: NaN first, -0 as +0.
+__device__ __forceinline__ uint32_t value_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return nan_f32();
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+// Sort s[0, n) descending, n a power of two; the keys behind `have` count as 0.
+__device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
+  for (int i = have + threadIdx.x; i < n; i += kTopThreads) s[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= n; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = threadIdx.x; i < (n >> 1); i += kTopThreads) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+        const uint64_t x = s[a], y = s[b];
+        const bool down = (a & k) == 0;
+        if ((x < y) == down) {
+          s[a] = y;
+          s[b] = x;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+__device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
+
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads) logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                                  int K, float c, float inv_t,
+                                                                  float* __restrict__ logp,
+                                                                  int64_t* __restrict__ ids) {
+  constexpr int U = sizeof(T) == 2 ? 4 : 2;
+  __shared__ uint64_t s_buf[kTopBuf];
+  __shared__ float s_red[64], s_part[2][8];
+  __shared__ int s_cnt;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t r = blockIdx.x / C;
+  const RowView<T> rv(logits, ld, r, V);
+  const int per = (rv.groups + C - 1) / C;
+  const int j0 = min(rank * per, rv.groups), j1 = min(j0 + per, rv.groups);
+  if (threadIdx.x == 0) s_cnt = 0;
+  __syncthreads();
+
+  float m = -INFINITY, s = 0.f;
+  uint64_t bar = 0;  // keys at or below it are out
+  for (int jb = j0; jb < j1; jb += U * kTopThreads) {
+    Group8<T> g[U];
+    float top[U];  // each group's largest value
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * kTopThreads + threadIdx.x;
+      if (j < j1) g[u] = load_group(rv, j);
+    }
+    uint32_t mine = 0;  // the largest value_key of this thread, NaN aside (0: no column)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * kTopThreads + threadIdx.x;
+      top[u] = -INFINITY;
+      if (j >= j1) continue;
+      float x[8];
+      g[u].get(x);
+      const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      online_update(x, c, m, s);
+      mine = max(mine, value_key(mx));
+      top[u] = s == s ? mx : nan_f32();  // a NaN or +inf came by: look at every column from here on
+    }
+    if (jb == j0) {
+      // The largest bar that at least K threads' maxima reach, bit by bit.
+      uint32_t t = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = t | (1u << bit);
+        if (__syncthreads_count(mine >= cand) >= K) t = cand;
+      }
+      if (t > 0) bar = ((uint64_t)t << 32) - 1;  // values equal to it stay in
+    }
+    // Columns above the bar: bit 8 u + k of `pend`.
+    uint32_t pend = 0;
+    auto filter = [&](uint32_t among) {
+      uint32_t keep = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (((among >> (8 * u)) & 0xffu) == 0) continue;
+        const int v0 = rv.first(jb + u * kTopThreads + threadIdx.x);
+        float x[8];
+        g[u].get(x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t key = ((uint64_t)value_key(x[k]) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
+          if (((among >> (8 * u + k)) & 1u) && v0 + k >= 0 && v0 + k < V && key > bar) keep |= 1u << (8 * u + k);
+        }
+      }
+      return keep;
+    };
+    {
+      uint32_t near = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (jb + u * kTopThreads + (int)threadIdx.x < j1 && value_key(top[u]) >= (uint32_t)(bar >> 32))
+          near |= 0xffu << (8 * u);
+      if (near) pend = filter(near);
+    }
+    while (true) {
+      if (pend) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (((pend >> (8 * u)) & 0xffu) == 0) continue;
+          const int v0 = rv.first(jb + u * kTopThreads + threadIdx.x);
+          float x[8];
+          g[u].get(x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (!((pend >> (8 * u + k)) & 1u)) continue;
+            const int at = atomicAdd(&s_cnt, 1);
+            if (at < kTopBuf) {
+              s_buf[at] = ((uint64_t)value_key(x[k]) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
+              pend &= ~(1u << (8 * u + k));
+            }
+          }
+        }
+      }
+      const bool more = __syncthreads_or(pend != 0);
+      if (!more) break;
+      // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
+      sort_keys(s_buf, kTopBuf, kTopBuf);
+      bar = s_buf[K - 1];
+      if (threadIdx.x == 0) s_cnt = K;
+      if (pend) pend = filter(pend);
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  block_online_merge(c, m, s, s_red);
+  const int have = min(s_cnt, kTopBuf);
+  sort_keys(s_buf, have, pow2_at_least(max(have, K)));
+  if (C > 1) {
+    // Every block's K largest go to the first one, behind its own, and are sorted there.
+    cluster.sync();
+    uint64_t* dst = cluster.map_shared_rank(s_buf, 0);
+    if (rank > 0)
+      for (int i = threadIdx.x; i < K; i += kTopThreads) dst[rank * K + i] = s_buf[i];
+    if (threadIdx.x == 0) {
+      float* part = cluster.map_shared_rank(&s_part[0][0], 0);
+      part[rank] = m;
+      part[8 + rank] = s;
+    }
+    cluster.sync();
+    if (rank != 0) return;
+    sort_keys(s_buf, C * K, pow2_at_least(C * K));
+    m = -INFINITY;
+    s = 0.f;
+    for (int q = 0; q < C; ++q) online_merge(c, m, s, s_part[0][q], s_part[1][q]);
+  }
+  const float ls = log2f(s) * kLn2;
+  for (int i = threadIdx.x; i < K; i += kTopThreads) {
+    const uint64_t key = s_buf[i];
+    const float x = key_value((uint32_t)(key >> 32));
+    logp[r * K + i] = (x - m) * inv_t - ls;
+    ids[r * K + i] = (int64_t)(0xffffffffu - (uint32_t)key);
+  }
+}
+
+template <typename T>
+int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c, float inv_t, float* logp,
+                int64_t* ids, cudaStream_t s) {
+  const int C = row_cluster(N, V, kTopThreads);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(N * C), 1, 1);
+  cfg.blockDim = dim3(kTopThreads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IKRL_CUDA(cudaLaunchKernelEx(&cfg, logits_topk_kernel<T>, reinterpret_cast<const T*>(logits), ld, V, K, c, inv_t,
+                               logp, ids));
+  return check_launch("logits_topk_kernel");
+}
+
+}  // namespace
+}  // namespace ikrl
+
+using namespace ikrl;
+
+extern "C" int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V, int32_t K,
+                                float temperature, float* logp, int64_t* ids, void* stream) {
+  clear_error();
+  const char* what = "ikrl_logits_topk";
+  int rc = check_logits_arg(what, logits, dtype, ld, N, V);
+  if (rc) return rc;
+  IKRL_REQUIRE(K >= 1 && K <= kMaxEntries, IKRL_ERR_UNSUPPORTED, "%s: K=%d outside 1..%d", what, K, kMaxEntries);
+  IKRL_REQUIRE(K <= V, IKRL_ERR_INVALID_ARGUMENT, "%s: K=%d of V=%d columns", what, K, V);
+  const float c = (float)(1.4426950408889634 / (double)temperature);
+  const float inv_t = (float)(1.0 / (double)temperature);
+  IKRL_REQUIRE(temperature > 0.f && c > 0.f && isfinite(c), IKRL_ERR_INVALID_ARGUMENT,
+               "%s: temperature %g must be positive and finite", what, (double)temperature);
+  if (N == 0) return IKRL_OK;
+  IKRL_REQUIRE(logits && logp && ids, IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  return dtype == IKRL_DTYPE_BF16 ? launch_topk<uint16_t>(logits, ld, N, V, K, c, inv_t, logp, ids, as_stream(stream))
+                                  : launch_topk<float>(logits, ld, N, V, K, c, inv_t, logp, ids, as_stream(stream));
+}

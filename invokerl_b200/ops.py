@@ -622,3 +622,262 @@ def dpo_loss(lp, ref_lp, response_mask, rewards, beta, label_smoothing, chosen_f
     return DPOLoss.apply(x.contiguous(), ref_lp.contiguous().float(), N.as_mask(response_mask),
                          None if rewards is None else rewards.contiguous().float(), float(beta),
                          float(label_smoothing), bool(chosen_first))
+
+
+# ---------------------------------------------------------------------------------------------
+# K4: losses over token distributions (no counterpart in the reference): a teacher's top log-probs,
+# distillation from them, cross entropy; on logits in memory and through the LM head
+# ---------------------------------------------------------------------------------------------
+
+_DISTILL_KINDS = {"forward": N.IKRL_DISTILL_FORWARD, "reverse": N.IKRL_DISTILL_REVERSE, "jsd": N.IKRL_DISTILL_JSD}
+
+
+def _check_temperature(temperature: float) -> float:
+    t = float(temperature)
+    if not 1e-30 < t < 1e30:  # also refuses NaN
+        raise ValueError(f"temperature {temperature} must be positive and finite")
+    return t
+
+
+def _distill_params(kind: str, beta: float, temperature: float, tail: bool) -> N.DistillParams:
+    if kind not in _DISTILL_KINDS:
+        raise ValueError(f"distillation kind {kind!r} is not one of {sorted(_DISTILL_KINDS)}")
+    if kind != "forward" and not tail:
+        raise ValueError(f"the {kind} loss needs the tail outcome (tail=True)")
+    if kind == "jsd" and not 0.0 < beta < 1.0:
+        raise ValueError(f"beta {beta} outside (0, 1)")
+    return N.DistillParams(_DISTILL_KINDS[kind], int(bool(tail)), float(beta), _check_temperature(temperature))
+
+
+def _check_xent(label_smoothing: float, z_loss: float) -> tuple[float, float]:
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing {label_smoothing} outside [0, 1]")
+    if not abs(z_loss) < float("inf"):
+        raise ValueError(f"z_loss {z_loss} is not finite")
+    return float(label_smoothing), float(z_loss)
+
+
+def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
+    """[rows, V] view of bf16 or fp32 logits with unit column stride and rows that do not overlap."""
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"expected bfloat16 or float32 logits, got {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits of shape {tuple(logits.shape)} have no vocabulary")
+    x = logits.reshape(-1, logits.shape[-1])
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _ld(x: torch.Tensor) -> int:
+    """Row stride of a [rows, V] matrix (V where there is one row at most, whose stride says nothing)."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _targets_rows(targets: torch.Tensor, shape) -> torch.Tensor:
+    if tuple(targets.shape) != tuple(shape):
+        raise ValueError(f"targets have shape {tuple(targets.shape)}, expected {tuple(shape)}")
+    if targets.is_floating_point() or targets.dtype == torch.bool:
+        raise TypeError(f"targets must be whole numbers, got {targets.dtype}")
+    return targets.reshape(-1).to(torch.int64).contiguous()
+
+
+def _teacher_rows(teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, shape):
+    """[rows, K] int64 ids and fp32 log-probs of a teacher whose rows have `shape`."""
+    if teacher_ids.shape != teacher_log_probs.shape or tuple(teacher_ids.shape[:-1]) != tuple(shape):
+        raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_log_probs "
+                         f"{tuple(teacher_log_probs.shape)} must both be {tuple(shape)} + (K,)")
+    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
+        raise TypeError(f"teacher_ids must be whole numbers, got {teacher_ids.dtype}")
+    if not teacher_log_probs.is_floating_point():
+        raise TypeError(f"teacher_log_probs must be floating point, got {teacher_log_probs.dtype}")
+    K = teacher_ids.shape[-1]
+    if not 1 <= K <= N.MAX_ENTRIES:
+        raise ValueError(f"K = {K} teacher entries outside 1..{N.MAX_ENTRIES}")
+    return (teacher_ids.reshape(-1, K).to(torch.int64).contiguous(),
+            teacher_log_probs.detach().reshape(-1, K).to(torch.float32).contiguous())
+
+
+def _row_state(n_rows: int, K: int, device) -> torch.Tensor:
+    nbytes = int(N.lib().ikrl_row_loss_state_bytes(n_rows, K))
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The k likeliest tokens of each row of bf16 or fp32 logits [..., V]: (log_probs fp32 [..., k],
+    ids int64 [..., k]), largest first and of equal logits the lower id first, with log-probs of
+    softmax(logits / temperature) over the whole vocabulary.  k <= 256; no gradient."""
+    dev = N.require_cuda(logits)
+    x = _logits_rows(logits.detach())
+    t = _check_temperature(temperature)
+    Nr, V = x.shape
+    if not 1 <= k <= min(N.MAX_ENTRIES, V):
+        raise ValueError(f"k = {k} outside 1..{min(N.MAX_ENTRIES, V)}")
+    shape = (*logits.shape[:-1], k)
+    log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
+    ids = torch.empty(shape, dtype=torch.int64, device=dev)
+    with torch.cuda.device(dev):
+        call("ikrl_logits_topk", ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V), i32(k), f32(t),
+             ptr(log_probs), ptr(ids), N.stream_of(dev))
+    return log_probs, ids
+
+
+class LogitsRowLoss(torch.autograd.Function):
+    """A row loss on logits in memory: distillation (params) or cross entropy (smoothing, z)."""
+
+    @staticmethod
+    def forward(ctx, x, ids, teacher_lp, params, smoothing, z):
+        dev = x.device
+        Nr, V = x.shape
+        K = 1 if teacher_lp is None else ids.shape[1]
+        loss = torch.empty(Nr, dtype=torch.float32, device=dev)
+        state = _row_state(Nr, K, dev)
+        head = (ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V), ptr(ids))
+        tail = (ptr(loss), ptr(state), sz(state.numel()), N.stream_of(dev))
+        with torch.cuda.device(dev):
+            if teacher_lp is None:
+                call("ikrl_logits_cross_entropy_fwd", *head, f32(smoothing), f32(z), *tail)
+            else:
+                call("ikrl_logits_distill_fwd", *head, ptr(teacher_lp), i32(K), params, *tail)
+        ctx.save_for_backward(x, state)
+        ctx.args = (K, params, smoothing, z)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, state = ctx.saved_tensors
+        K, params, smoothing, z = ctx.args
+        Nr, V = x.shape
+        g = g.float().contiguous()
+        dx = torch.empty(Nr, V, dtype=x.dtype, device=x.device)
+        head = (ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V))
+        tail = (ptr(state), sz(state.numel()), ptr(g), ptr(dx), i64(V), N.stream_of(x.device))
+        with torch.cuda.device(x.device):
+            if params is None:
+                call("ikrl_logits_cross_entropy_bwd", *head, f32(smoothing), f32(z), *tail)
+            else:
+                call("ikrl_logits_distill_bwd", *head, i32(K), params, *tail)
+        return dx, None, None, None, None, None
+
+
+def logits_distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor,
+                   kind: str = "forward", beta: float = 0.5, temperature: float = 1.0,
+                   tail: bool = True) -> torch.Tensor:
+    """Distillation loss of each row of bf16 or fp32 logits [..., V] against a teacher's top log-probs
+    (teacher_ids, teacher_log_probs [..., K], K <= 256, in any order; fp32 [...]).
+
+    p = softmax(logits / temperature); the teacher's log-probs are taken as they are.  An entry with
+    an id below 0 or a log-prob of -inf is no entry, a repeated id counts at its first place, a row
+    without entries has loss 0, an id past the vocabulary makes its row NaN.  With `tail` the tokens
+    that are not entries form one more outcome, of teacher mass 1 - sum q (0 below 2^-20).
+    kind "forward": KL(q | p), without `tail` over the renormalised entries; "reverse": KL(p | q);
+    "jsd": beta KL(q | m) + (1 - beta) KL(p | m), m = beta q + (1 - beta) p.  The gradient goes to
+    the logits only (it reads them again: do not overwrite them in between)."""
+    params = _distill_params(kind, beta, temperature, tail)
+    N.require_cuda(logits, teacher_ids, teacher_log_probs)
+    x = _logits_rows(logits)
+    ids, lp = _teacher_rows(teacher_ids, teacher_log_probs, logits.shape[:-1])
+    return LogitsRowLoss.apply(x, ids, lp, params, 0.0, 0.0).reshape(logits.shape[:-1])
+
+
+def logits_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, label_smoothing: float = 0.0,
+                         z_loss: float = 0.0) -> torch.Tensor:
+    """Cross entropy of each row of bf16 or fp32 logits [..., V] with its target [...] (fp32 [...]):
+    (lse - x_y) + label_smoothing * (x_y - mean x) + z_loss * lse^2.  Targets of -100 give 0."""
+    label_smoothing, z_loss = _check_xent(label_smoothing, z_loss)
+    N.require_cuda(logits, targets)
+    x = _logits_rows(logits)
+    t = _targets_rows(targets, logits.shape[:-1])
+    return LogitsRowLoss.apply(x, t, None, None, label_smoothing, z_loss).reshape(logits.shape[:-1])
+
+
+class LMHeadRowLoss(torch.autograd.Function):
+    """A row loss of hidden @ weight.T without the logits in memory."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, teacher_lp, params, smoothing, z, chunk_rows):
+        dev = hidden.device
+        Nr, H = hidden.shape
+        V = weight.shape[0]
+        K = 1 if teacher_lp is None else ids.shape[1]
+        loss = torch.empty(Nr, dtype=torch.float32, device=dev)
+        state = _row_state(Nr, K, dev)
+        nbytes = int(N.lib().ikrl_lmhead_row_loss_fwd_workspace_bytes(Nr, H, V, K))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        tail = (ptr(loss), ptr(state), sz(state.numel()), ptr(ws), sz(nbytes), N.stream_of(dev))
+        with torch.cuda.device(dev):
+            if teacher_lp is None:
+                call("ikrl_lmhead_cross_entropy_fwd", ptr(hidden), ptr(weight), ptr(ids), i64(Nr), i32(H), i32(V),
+                     f32(smoothing), f32(z), *tail)
+            else:
+                call("ikrl_lmhead_distill_fwd", ptr(hidden), ptr(weight), ptr(ids), ptr(teacher_lp), i64(Nr), i32(H),
+                     i32(V), i32(K), params, *tail)
+        if _CHECK_DEVICE_STATUS:
+            lmhead_status(ws)
+        ctx.save_for_backward(hidden, weight, state)
+        ctx.args = (K, params, smoothing, z, chunk_rows)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        hidden, weight, state = ctx.saved_tensors
+        K, params, smoothing, z, chunk_rows = ctx.args
+        want_dh, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        none = (None,) * 6
+        if not (want_dh or want_dw):
+            return None, None, *none
+        dev = hidden.device
+        Nr, H = hidden.shape
+        V = weight.shape[0]
+        if chunk_rows is None:
+            chunk_rows = default_chunk_rows(Nr, V)
+        g = g.float().contiguous()
+        dh = torch.empty_like(hidden) if want_dh else None
+        dw = torch.empty_like(weight) if want_dw else None
+        nbytes = int(N.lib().ikrl_lmhead_row_loss_bwd_workspace_bytes(Nr, H, V, chunk_rows, N.IKRL_DTYPE_BF16, 0))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        head = (ptr(hidden), ptr(weight), i64(Nr), i32(H), i32(V))
+        tail = (ptr(state), sz(state.numel()), ptr(g), i64(chunk_rows), ptr(dh), ptr(dw), i32(N.IKRL_DTYPE_BF16),
+                i32(0), ptr(ws), sz(nbytes), N.stream_of(dev))
+        with torch.cuda.device(dev):
+            if params is None:
+                call("ikrl_lmhead_cross_entropy_bwd", *head, f32(smoothing), f32(z), *tail)
+            else:
+                call("ikrl_lmhead_distill_bwd", *head, i32(K), params, *tail)
+        if _CHECK_DEVICE_STATUS:
+            lmhead_status(ws)
+        return dh, dw, *none
+
+
+def _head_rows(hidden: torch.Tensor, weight: torch.Tensor):
+    """bf16 [rows, H] hidden and [V, H] weight, contiguous."""
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be [..., H] and [V, H]")
+    h = hidden.reshape(-1, hidden.shape[-1]).to(torch.bfloat16).contiguous()
+    return h, weight.to(torch.bfloat16).contiguous()
+
+
+def lmhead_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
+                   teacher_log_probs: torch.Tensor, kind: str = "forward", beta: float = 0.5,
+                   temperature: float = 1.0, tail: bool = True, chunk_rows: int | None = None) -> torch.Tensor:
+    """`logits_distill` of the logits hidden [..., H] @ weight [V, H].T, which are never in memory:
+    fp32 loss [...], gradients to hidden and weight.  `chunk_rows` as in `lmhead_logprob`."""
+    params = _distill_params(kind, beta, temperature, tail)
+    N.require_cuda(hidden, weight, teacher_ids, teacher_log_probs)
+    h, w = _head_rows(hidden, weight)
+    ids, lp = _teacher_rows(teacher_ids, teacher_log_probs, hidden.shape[:-1])
+    return LMHeadRowLoss.apply(h, w, ids, lp, params, 0.0, 0.0, chunk_rows).reshape(hidden.shape[:-1])
+
+
+def lmhead_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                         label_smoothing: float = 0.0, z_loss: float = 0.0,
+                         chunk_rows: int | None = None) -> torch.Tensor:
+    """`logits_cross_entropy` of the logits hidden [..., H] @ weight [V, H].T, which are never in
+    memory: fp32 loss [...], gradients to hidden and weight.  `chunk_rows` as in `lmhead_logprob`."""
+    label_smoothing, z_loss = _check_xent(label_smoothing, z_loss)
+    N.require_cuda(hidden, weight, targets)
+    h, w = _head_rows(hidden, weight)
+    t = _targets_rows(targets, hidden.shape[:-1])
+    return LMHeadRowLoss.apply(h, w, t, None, None, label_smoothing, z_loss, chunk_rows).reshape(hidden.shape[:-1])

@@ -96,6 +96,88 @@ class PolicyModel:
         """F.linear + -cross_entropy of one chunk (policy.py:173-191); fp32."""
         return ops.lmhead_logprob(hidden_chunk, lm_head_weight, target_chunk)
 
+    # -- losses over token distributions (additions; the reference has none) ----------------------
+
+    def _body(self, token_ids: Tensor, attention_mask: Tensor):
+        """(logits, None) under FSDP, (None, last hidden states) otherwise."""
+        ctx = (torch.autocast("cuda", dtype=self._autocast_dtype) if self._autocast_dtype
+               else contextlib.nullcontext())
+        with ctx:
+            if self._fsdp_wrapped:
+                return self.model(input_ids=token_ids, attention_mask=attention_mask).logits, None
+            return None, self.model.model(input_ids=token_ids, attention_mask=attention_mask).last_hidden_state
+
+    @staticmethod
+    def _at_next_token(rows: Tensor) -> Tensor:
+        """[B, T] row values (row t is about token t + 1) moved to the token they are about; 0 at position 0."""
+        return torch.cat([torch.zeros_like(rows[:, :1]), rows[:, :-1]], dim=1)
+
+    @torch.no_grad()
+    def topk_log_probs(self, token_ids: Tensor, attention_mask: Tensor, k: int,
+                       temperature: float = 1.0) -> tuple[Tensor, Tensor]:
+        """As a teacher: (log_probs fp32, ids int64), both [B, T, k], where position t holds the k
+        likeliest tokens given the tokens before t.  Position 0 and unattended positions hold no
+        entries (-inf, -1), which `distill_loss` skips."""
+        token_ids = token_ids.to(self.device)
+        attention_mask = attention_mask.to(self.device)
+        logits, hidden = self._body(token_ids, attention_mask)
+        B, T = token_ids.shape
+        log_probs = torch.full((B, T, k), -torch.inf, dtype=torch.float32, device=token_ids.device)
+        ids = torch.full((B, T, k), -1, dtype=torch.int64, device=token_ids.device)
+        if hidden is None:
+            if logits.dtype != torch.bfloat16:
+                logits = logits.to(torch.bfloat16)
+            lp, top = ops.logits_topk(logits, k, temperature)
+            log_probs[:, 1:], ids[:, 1:] = lp[:, :-1], top[:, :-1]
+        else:
+            # logits of at most 1 GiB of rows at a time
+            w = self.model.lm_head.weight.to(torch.bfloat16)
+            h = hidden.to(torch.bfloat16)
+            step = max(1, (1 << 30) // (2 * w.shape[0] * B))
+            for s in range(0, T - 1, step):
+                e = min(s + step, T - 1)
+                lp, top = ops.logits_topk(torch.nn.functional.linear(h[:, s:e], w), k, temperature)
+                log_probs[:, s + 1:e + 1], ids[:, s + 1:e + 1] = lp, top
+        off = ~attention_mask.bool()
+        off[:, :1] = True
+        return log_probs.masked_fill_(off[..., None], -torch.inf), ids.masked_fill_(off[..., None], -1)
+
+    def distill_loss(self, token_ids: Tensor, attention_mask: Tensor, teacher_ids: Tensor, teacher_log_probs: Tensor,
+                     kind: str = "forward", beta: float = 0.5, temperature: float = 1.0, tail: bool = True) -> Tensor:
+        """Distillation loss of each token [B, T] (fp32; `ops.lmhead_distill`) against a teacher's
+        entries [B, T, K] as `topk_log_probs` lays them out; position 0 is 0.  Weight it by the
+        response mask: tokens whose loss has no gradient cost no backward work."""
+        token_ids = token_ids.to(self.device)
+        attention_mask = attention_mask.to(self.device)
+        teacher_ids, teacher_log_probs = teacher_ids.to(self.device), teacher_log_probs.to(self.device)
+        logits, hidden = self._body(token_ids, attention_mask)
+        ids = torch.full_like(teacher_ids, -1)
+        ids[:, :-1] = teacher_ids[:, 1:]
+        lp = torch.roll(teacher_log_probs, -1, dims=1)
+        args = (ids, lp, kind, beta, temperature, tail)
+        if hidden is None:
+            rows = ops.logits_distill(logits.to(torch.bfloat16), *args)
+        else:
+            rows = ops.lmhead_distill(hidden, self.model.lm_head.weight, *args)
+        return self._at_next_token(rows)
+
+    def cross_entropy_loss(self, token_ids: Tensor, attention_mask: Tensor, label_smoothing: float = 0.0,
+                           z_loss: float = 0.0, loss_mask: Tensor | None = None) -> Tensor:
+        """Cross entropy of each token [B, T] given the tokens before it (fp32;
+        `ops.lmhead_cross_entropy`); 0 at position 0 and outside `loss_mask` (the attention mask by
+        default)."""
+        token_ids = token_ids.to(self.device)
+        attention_mask = attention_mask.to(self.device)
+        keep = attention_mask.bool() if loss_mask is None else loss_mask.to(self.device).bool()
+        logits, hidden = self._body(token_ids, attention_mask)
+        targets = torch.full_like(token_ids, -100)
+        targets[:, :-1] = torch.where(keep[:, 1:], token_ids[:, 1:], -100)
+        if hidden is None:
+            rows = ops.logits_cross_entropy(logits.to(torch.bfloat16), targets, label_smoothing, z_loss)
+        else:
+            rows = ops.lmhead_cross_entropy(hidden, self.model.lm_head.weight, targets, label_smoothing, z_loss)
+        return self._at_next_token(rows)
+
     @torch.no_grad()
     def forward_no_grad(self, token_ids: Tensor, attention_mask: Tensor) -> Tensor:
         """forward() without gradients (reference log-probs, policy.py:193-196)."""
