@@ -2203,15 +2203,23 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   const BwdLayout Lw = bwd_layout(Nw, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
   const int64_t chunk = std::min(L.chunk, Lw.chunk);
   // Chunks: first the cached rows [0, n_cached), then the others, so every chunk takes its dS one
-  // way (from the cache, or by the recompute GEMM).
+  // way (from the cache, or by the recompute GEMM).  Two such chunks need the fp32 accumulator of a
+  // bf16 dweight; where the workspace has none (the rows fit one chunk), both kinds of rows share
+  // one chunk: the cached ones are its first `cached`.
   struct Chunk {
-    int64_t c0, rows;
-    bool cached;
+    int64_t c0, rows, cached;
   };
   std::vector<Chunk> chunks;
-  for (int seg = 0; seg < 2; ++seg) {
-    const int64_t a0 = seg == 0 ? 0 : n_cached, a1 = seg == 0 ? n_cached : Nw;
-    for (int64_t c0 = a0; c0 < a1; c0 += chunk) chunks.push_back({c0, std::min<int64_t>(chunk, a1 - c0), seg == 0});
+  if (n_cached > 0 && n_cached < Nw && Nw <= chunk && dweight && dweight_dtype == IKRL_DTYPE_BF16 && !L.need_dw32) {
+    chunks.push_back({0, Nw, n_cached});
+  } else {
+    for (int seg = 0; seg < 2; ++seg) {
+      const int64_t a0 = seg == 0 ? 0 : n_cached, a1 = seg == 0 ? n_cached : Nw;
+      for (int64_t c0 = a0; c0 < a1; c0 += chunk) {
+        const int64_t n = std::min<int64_t>(chunk, a1 - c0);
+        chunks.push_back({c0, n, seg == 0 ? n : 0});
+      }
+    }
   }
   const int64_t nchunks = (int64_t)chunks.size();
   const bool use_dw32 = (dweight_dtype == IKRL_DTYPE_BF16) && nchunks > 1;
@@ -2227,29 +2235,34 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     const int m_tiles = (int)cdiv64(rows, BM);
     const uint16_t* hc = hsrc + c0 * H;
     // 1) dS = g * (onehot - softmax(h W^T)) for this chunk: from the logit cache, or recomputed
-    if (chunks[ci].cached) {
+    const int64_t from_cache = chunks[ci].cached;  // leading rows of the chunk
+    if (from_cache > 0) {
       const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
-                      (unsigned)std::min<int64_t>(rows, 65535));
+                      (unsigned)std::min<int64_t>(from_cache, 65535));
       ds_from_cache_kernel<<<grid, 256, 0, s>>>(cache_q, cache_m, L.lds, (int)cdiv64(V, 32), cache_slot, idx_c,
-                                                idsrc, lsesrc, gsrc, c0, rows, V, vocab_start, dS, L.lds);
+                                                idsrc, lsesrc, gsrc, c0, from_cache, V, vocab_start, dS, L.lds);
       if ((rc = check_launch("ds_from_cache_kernel"))) return rc;
-    } else {
+    }
+    if (from_cache < rows) {
+      const int64_t r0 = c0 + from_cache, nr = rows - from_cache;
+      uint16_t* dS_r = dS + from_cache * L.lds;
       CUtensorMap ta, tds;
-      if ((rc = make_tmap(&ta, hc, H, rows, H, BM, "hidden chunk"))) return rc;
-      if ((rc = make_store_tmap(&tds, dS, V, rows, L.lds, "dS store"))) return rc;
+      if ((rc = make_tmap(&ta, hsrc + r0 * H, H, nr, H, BM, "hidden chunk"))) return rc;
+      if ((rc = make_store_tmap(&tds, dS_r, V, nr, L.lds, "dS store"))) return rc;
       GemmParams p{};
-      p.M = (int)rows; p.N = V; p.K = H;
-      const int sp = choose_splits(m_tiles, n_vt, H);
-      p.ids = idsrc + c0; p.lse = lsesrc + c0; p.g = gsrc + c0;
+      p.M = (int)nr; p.N = V; p.K = H;
+      const int nr_tiles = (int)cdiv64(nr, BM);
+      const int sp = choose_splits(nr_tiles, n_vt, H);
+      p.ids = idsrc + r0; p.lse = lsesrc + r0; p.g = gsrc + r0;
       p.id_offset = vocab_start;
-      p.out_bf16 = dS; p.ld_bf16 = L.lds;
+      p.out_bf16 = dS_r; p.ld_bf16 = L.lds;
       p.err = err;
       if (rl) {
-        p.level = level + c0;
+        p.level = level + r0;
         p.c = rl->c;
-        if ((rc = launch_k1<EPI_DTAIL, false, false>(ta, t_w_k, ta, t_w_k2, p, m_tiles, sp, s, &tds))) return rc;
+        if ((rc = launch_k1<EPI_DTAIL, false, false>(ta, t_w_k, ta, t_w_k2, p, nr_tiles, sp, s, &tds))) return rc;
       } else {
-        if ((rc = launch_k1<EPI_DLOGITS, false, false>(ta, t_w_k, ta, t_w_k2, p, m_tiles, sp, s, &tds))) return rc;
+        if ((rc = launch_k1<EPI_DLOGITS, false, false>(ta, t_w_k, ta, t_w_k2, p, nr_tiles, sp, s, &tds))) return rc;
       }
     }
     if (rl) {
