@@ -409,28 +409,37 @@ IKRL_API int ikrl_lmhead_noalloc_status(int32_t* status_out, void* stream);
  * and the one host synchronisation of the backward outside a stream capture, chunk_rows,
  * dweight_dtype and accumulation, ikrl_lmhead_status on the workspace).  The [N, V] logits are never
  * in memory.  state: ikrl_row_loss_state_bytes(N, K), K = 1 for the cross entropy, as the forward
- * left it; dloss[N] fp32 is the upstream gradient of the row losses. */
-IKRL_API size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int32_t K);
+ * left it; dloss[N] fp32 is the upstream gradient of the row losses.
+ * cache_*: the logit cache of ikrl_lmhead_logprob_fwd_cached (sizes from ikrl_lmhead_cache_row_elems),
+ * cache_rows = 0 for none; slots go to the rows that have entries (or a target), in row order.  The
+ * backward gets what the forward filled.  Rows without entries are left out of both directions' GEMMs
+ * (above 256 rows, where gathering the others pays); up to 256 rows neither direction synchronises. */
+IKRL_API size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V);
 IKRL_API size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
                                                          int32_t dweight_dtype, int32_t accumulate_dweight);
 IKRL_API int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,
                                      const float* teacher_logp, int64_t N, int32_t H, int32_t V, int32_t K,
                                      const ikrl_distill_params* params, float* loss, void* state,
-                                     size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
+                                     size_t state_bytes, int64_t cache_rows, int32_t* cache_slot, void* cache_q,
+                                     float* cache_m, void* ws, size_t ws_bytes, void* stream);
 IKRL_API int ikrl_lmhead_distill_bwd(const void* hidden, const void* weight, int64_t N, int32_t H, int32_t V,
                                      int32_t K, const ikrl_distill_params* params, const void* state,
                                      size_t state_bytes, const float* dloss, int64_t chunk_rows, void* dhidden,
-                                     void* dweight, int32_t dweight_dtype, int32_t accumulate_dweight, void* ws,
-                                     size_t ws_bytes, void* stream);
+                                     void* dweight, int32_t dweight_dtype, int32_t accumulate_dweight,
+                                     int64_t cache_rows, const int32_t* cache_slot, const void* cache_q,
+                                     const float* cache_m, void* ws, size_t ws_bytes, void* stream);
 IKRL_API int ikrl_lmhead_cross_entropy_fwd(const void* hidden, const void* weight, const int64_t* targets,
                                            int64_t N, int32_t H, int32_t V, float label_smoothing, float z_loss,
-                                           float* loss, void* state, size_t state_bytes, void* ws,
+                                           float* loss, void* state, size_t state_bytes, int64_t cache_rows,
+                                           int32_t* cache_slot, void* cache_q, float* cache_m, void* ws,
                                            size_t ws_bytes, void* stream);
 IKRL_API int ikrl_lmhead_cross_entropy_bwd(const void* hidden, const void* weight, int64_t N, int32_t H,
                                            int32_t V, float label_smoothing, float z_loss, const void* state,
                                            size_t state_bytes, const float* dloss, int64_t chunk_rows,
                                            void* dhidden, void* dweight, int32_t dweight_dtype,
-                                           int32_t accumulate_dweight, void* ws, size_t ws_bytes, void* stream);
+                                           int32_t accumulate_dweight, int64_t cache_rows,
+                                           const int32_t* cache_slot, const void* cache_q, const float* cache_m,
+                                           void* ws, size_t ws_bytes, void* stream);
 
 /* Selects the K1 GEMM kernel for later calls in this process: CTA pairs (tcgen05 cta_group::2,
  * clusters of two; the default) or single CTAs (enable = 0).  Returns the previous setting.  The

@@ -165,29 +165,30 @@ _SIGNATURES: dict[str, tuple] = {
         ctypes.c_int,
         [_P, c_int32, c_int64, c_int64, c_int32, c_float, c_float, _P, c_size_t, _P, _P, c_int64, _P],
     ),
-    "ikrl_lmhead_row_loss_fwd_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32]),
+    "ikrl_lmhead_row_loss_fwd_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int32]),
     "ikrl_lmhead_row_loss_bwd_workspace_bytes": (
         c_size_t,
         [c_int64, c_int32, c_int32, c_int64, c_int32, c_int32],
     ),
     "ikrl_lmhead_distill_fwd": (
         ctypes.c_int,
-        [_P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, POINTER(DistillParams), _P, _P, c_size_t, _P, c_size_t,
-         _P],
+        [_P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, POINTER(DistillParams), _P, _P, c_size_t, c_int64, _P,
+         _P, _P, _P, c_size_t, _P],
     ),
     "ikrl_lmhead_distill_bwd": (
         ctypes.c_int,
         [_P, _P, c_int64, c_int32, c_int32, c_int32, POINTER(DistillParams), _P, c_size_t, _P, c_int64, _P, _P,
-         c_int32, c_int32, _P, c_size_t, _P],
+         c_int32, c_int32, c_int64, _P, _P, _P, _P, c_size_t, _P],
     ),
     "ikrl_lmhead_cross_entropy_fwd": (
         ctypes.c_int,
-        [_P, _P, _P, c_int64, c_int32, c_int32, c_float, c_float, _P, _P, c_size_t, _P, c_size_t, _P],
+        [_P, _P, _P, c_int64, c_int32, c_int32, c_float, c_float, _P, _P, c_size_t, c_int64, _P, _P, _P, _P,
+         c_size_t, _P],
     ),
     "ikrl_lmhead_cross_entropy_bwd": (
         ctypes.c_int,
         [_P, _P, c_int64, c_int32, c_int32, c_float, c_float, _P, c_size_t, _P, c_int64, _P, _P, c_int32, c_int32,
-         _P, c_size_t, _P],
+         c_int64, _P, _P, _P, _P, c_size_t, _P],
     ),
     "ikrl_lmhead_status": (ctypes.c_int, [_P, POINTER(c_int32), _P]),
     "ikrl_lmhead_cache_row_elems": (ctypes.c_int, [c_int32, POINTER(c_int64), POINTER(c_int64)]),
@@ -339,6 +340,28 @@ def stream_of(device: torch.device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class on_device:
+    """Makes the device of a call's tensors the current one while the call launches (a launch goes to
+    the current device, whatever its stream)."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+        self.prev = -1
+
+    def __enter__(self):
+        cur = torch.cuda.current_device()
+        if self.index is not None and cur != self.index:
+            self.prev = cur
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
 def dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.float32:
         return IKRL_DTYPE_F32
@@ -398,6 +421,7 @@ __all__ = [
     "ptr",
     "require_cuda",
     "stream_of",
+    "on_device",
     "dtype_code",
     "as_mask",
     "workspace",

@@ -17,6 +17,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kFwdThreads = 512;
 constexpr int kBwdThreads = 512;
+constexpr int kBwdRounds = 5;  // rounds of a backward block when there are rows enough
 
 template <typename T> constexpr int unroll_of() { return sizeof(T) == 2 ? 4 : 2; }  // 64 bytes in flight a thread
 
@@ -32,7 +33,8 @@ __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __re
                                                                    RowLossParams P, RowState st,
                                                                    float* __restrict__ loss) {
   extern __shared__ uint32_t s_map[];  // a bit per group of this block
-  __shared__ int s_col[kMaxEntries], s_raw[kMaxEntries];
+  __shared__ int s_col[kMaxEntries];
+  __shared__ __align__(16) int s_raw[kMaxEntries];
   __shared__ float s_lp[kMaxEntries], s_x[kMaxEntries], s_red[64], s_part[3][8];
   constexpr int U = unroll_of<T>();
   cg::cluster_group cluster = cg::this_cluster();
@@ -56,48 +58,43 @@ __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __re
     float* x_dst = C > 1 ? cluster.map_shared_rank(s_x, 0) : s_x;
 
     float m = -INFINITY, s = 0.f, sum = 0.f;
-    auto take = [&](const Group8<T>& g, int j) {
-      float x[8];
-      g.get(x);
-      if constexpr (SUM) {
-        if (rv.whole(j)) {
-          sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) sum += (rv.first(j) + k >= 0 && rv.first(j) + k < P.V) ? x[k] : 0.f;
-        }
-      }
-      if ((s_map[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u) {
-        int lo = 0, hi = cnt;  // first entry at or after this group
-        const int v0 = rv.first(j);
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (s_col[mid] < v0) lo = mid + 1;
-          else hi = mid;
-        }
-        for (; lo < cnt && s_col[lo] < v0 + 8; ++lo) {
-          const int rel = s_col[lo] - v0;
-          float xe = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k == rel) {
-              xe = x[k];
-              x[k] = -INFINITY;
-            }
-          x_dst[lo] = xe;
-        }
-      }
-      online_update(x, P.c, m, s);
-    };
-    int j = j0 + threadIdx.x;
-    for (; j + (U - 1) * kFwdThreads < j1; j += U * kFwdThreads) {
+    for (int jb = j0; jb < j1; jb += U * kFwdThreads) {
       Group8<T> g[U];
+      const int n = min(U, (j1 - jb + kFwdThreads - 1) / kFwdThreads);  // groups a thread, at most
 #pragma unroll
-      for (int u = 0; u < U; ++u) g[u] = load_group(rv, j + u * kFwdThreads);
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kFwdThreads + threadIdx.x;
+        if (j < j1) load_group(g[u], rv, j);
+        else g[u].fill();
+      }
 #pragma unroll
-      for (int u = 0; u < U; ++u) take(g[u], j + u * kFwdThreads);
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kFwdThreads + threadIdx.x;
+        if (j >= j1) continue;
+        const int v0 = rv.first(j);
+        if constexpr (SUM) {
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = g[u].get(k);
+          if (!rv.whole(j)) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (v0 + k < 0 || v0 + k >= P.V) x[k] = 0.f;
+          }
+          sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        }
+        if ((s_map[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u) {
+          int lo = 0, hi = cnt;  // first entry at or after this group
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_col[mid] < v0) lo = mid + 1;
+            else hi = mid;
+          }
+          for (; lo < cnt && s_col[lo] < v0 + 8; ++lo) x_dst[lo] = g[u].take(s_col[lo] - v0);
+        }
+      }
+      online_groups<T, U>(g, n, P.c, m, s);
     }
-    for (; j < j1; j += kFwdThreads) take(load_group(rv, j), j);
     block_online_merge(P.c, m, s, s_red);
     if constexpr (SUM) {
       float v[1] = {sum};
@@ -130,8 +127,8 @@ __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __re
 }
 
 // dlogits = g (coef 2^(c (x - ref)) + level) over the row, then g grad_k over its entries (written
-// by the same block behind a barrier).  A block takes U groups a thread of one row; rows without a
-// gradient are zeros and read nothing.
+// by the same block behind a barrier).  A block takes a part of one row, U groups a thread at a time;
+// rows without a gradient are zeros and read nothing.
 template <typename T>
 __global__ void __launch_bounds__(kBwdThreads) row_loss_bwd_kernel(const T* __restrict__ logits, int64_t ld, int K,
                                                                    int V, float c, float level, RowState st,
@@ -144,52 +141,63 @@ __global__ void __launch_bounds__(kBwdThreads) row_loss_bwd_kernel(const T* __re
   const RowView<T> rv(logits, ld, r, V);
   T* out = dlogits + r * ld_out;
   const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
-  const int j0 = seg * (U * kBwdThreads);
-  const float g = dloss[r];
-  const bool skip = g == 0.f || st.row_ids[r] == kRowNone;
-  const float gc = skip ? 0.f : g * st.coef[r], lv = skip ? 0.f : g * level, ref = st.ref[r];
+  const int per = (rv.groups + blocks_per_row - 1) / blocks_per_row;
+  const int j0 = min(seg * per, rv.groups), j1 = min(j0 + per, rv.groups);
+  const float g = dloss[r], ref = st.ref[r], coef = st.coef[r];
+  const bool skip = st.row_ids[r] == kRowNone || g == 0.f;
+  const float lv = skip ? 0.f : g * level;
+  // as in online_groups: one fma an exponent where c ref is finite, its rounding put into the factor
+  const bool fma_ok = fabsf(ref) < kFmaLimit;
+  const float pt = fma_ok ? ref * c : 0.f;
+  const float gc = skip ? 0.f : g * coef * (fma_ok ? exp2f(-fmaf(ref, c, -pt)) : 1.f);
 
-  Group8<T> in[U];
-  if (!skip) {
+  for (int jb = j0; jb < j1; jb += U * kBwdThreads) {
+    Group8<T> in[U];
+    if (!skip) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kBwdThreads + threadIdx.x;
+        if (j < j1) load_group(in[u], rv, j);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * kBwdThreads + threadIdx.x;
-      if (j < rv.groups) in[u] = load_group(rv, j);
-    }
-  }
+      const int j = jb + u * kBwdThreads + threadIdx.x;
+      if (j >= j1) break;
+      float d[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (!skip) {
+        if (fma_ok) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int j = j0 + u * kBwdThreads + threadIdx.x;
-    if (j >= rv.groups) break;
-    float d[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (!skip) {
-      in[u].get(d);
+          for (int k = 0; k < 8; ++k) d[k] = fmaf(gc, fast_exp2(fmaf(in[u].get(k), c, -pt)), lv);
+        } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = fmaf(gc, fast_exp2((d[k] - ref) * c), lv);
-    }
-    const int v0 = rv.first(j);
-    if (same && rv.whole(j)) {
-      if constexpr (sizeof(T) == 2) {
-        st_stream16(out + v0, make_uint4(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]),
-                                         pack_bf16x2(d[6], d[7])));
-      } else {
-        st_stream16(out + v0, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]),
-                                         __float_as_uint(d[3])));
-        st_stream16(out + v0 + 4, make_uint4(__float_as_uint(d[4]), __float_as_uint(d[5]), __float_as_uint(d[6]),
-                                             __float_as_uint(d[7])));
+          for (int k = 0; k < 8; ++k) d[k] = fmaf(gc, fast_exp2((in[u].get(k) - ref) * c), lv);
+        }
       }
-    } else {
+      const int v0 = rv.first(j);
+      if (same && rv.whole(j)) {
+        if constexpr (sizeof(T) == 2) {
+          st_stream16(out + v0, make_uint4(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]),
+                                           pack_bf16x2(d[6], d[7])));
+        } else {
+          st_stream16(out + v0, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]),
+                                           __float_as_uint(d[3])));
+          st_stream16(out + v0 + 4, make_uint4(__float_as_uint(d[4]), __float_as_uint(d[5]), __float_as_uint(d[6]),
+                                               __float_as_uint(d[7])));
+        }
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (v0 + k < 0 || v0 + k >= V) continue;
-        if constexpr (sizeof(T) == 2) out[v0 + k] = f32_to_bf16_rn(d[k]);
-        else out[v0 + k] = d[k];
+        for (int k = 0; k < 8; ++k) {
+          if (v0 + k < 0 || v0 + k >= V) continue;
+          if constexpr (sizeof(T) == 2) out[v0 + k] = f32_to_bf16_rn(d[k]);
+          else out[v0 + k] = d[k];
+        }
       }
     }
   }
   if (skip) return;
   __syncthreads();
-  const int lo = rv.first(j0), hi = lo + 8 * U * kBwdThreads;
+  const int lo = rv.first(j0), hi = rv.first(j1);
   for (int e = threadIdx.x; e < K; e += kBwdThreads) {
     const int col = st.cols[r * K + e];
     if (col == kNoEntry || col < lo || col >= hi) continue;
@@ -203,7 +211,8 @@ __global__ void __launch_bounds__(kBwdThreads) row_loss_bwd_kernel(const T* __re
 __global__ void __launch_bounds__(kMaxEntries) row_entries_kernel(const int64_t* __restrict__ tids,
                                                                   const float* __restrict__ tlp, int K, int V,
                                                                   RowState st) {
-  __shared__ int s_col[kMaxEntries], s_raw[kMaxEntries];
+  __shared__ int s_col[kMaxEntries];
+  __shared__ __align__(16) int s_raw[kMaxEntries];
   __shared__ float s_lp[kMaxEntries];
   const int64_t r = blockIdx.x;
   int cnt = 0;
@@ -215,31 +224,34 @@ __global__ void __launch_bounds__(kMaxEntries) row_entries_kernel(const int64_t*
   if (threadIdx.x == 0) st.row_ids[r] = id;
 }
 
-// Loss of each row from the GEMM's partial sums: one warp a row.
+// Loss of each row from partial sums: one warp a row.
 __global__ void __launch_bounds__(128) row_losses_kernel(const float* __restrict__ part_m,
                                                          const float* __restrict__ part_s,
                                                          const float* __restrict__ part_x, int sets,
-                                                         const float* __restrict__ xk, int64_t N, int K,
+                                                         const int* __restrict__ pos, int64_t N, int K,
                                                          RowLossParams P, RowState st, float* __restrict__ loss,
                                                          const int* __restrict__ err) {
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (r >= N) return;
   const int lane = threadIdx.x & 31;
   int64_t id = st.row_ids[r];
-  if (*err != 0) id = kRowBad;
+  if (err != nullptr && *err != 0) id = kRowBad;
   int cnt = 0;
   for (int k = lane; k < K; k += 32) cnt += st.cols[r * K + k] != kNoEntry;
   cnt = warp_sum(cnt);
   float m = -INFINITY, s = 0.f, sum = 0.f;
-  for (int q = lane; q < sets; q += 32) {
-    online_merge(P.c, m, s, part_m[(int64_t)q * N + r], part_s[(int64_t)q * N + r]);
-    if (part_x) sum += part_x[(int64_t)q * N + r];
+  if (id == kRowLive) {
+    const int64_t at = pos ? pos[r] : r;
+    for (int q = lane; q < sets; q += 32) {
+      online_merge(P.c, m, s, part_m[(int64_t)q * N + at], part_s[(int64_t)q * N + at]);
+      if (part_x) sum += part_x[(int64_t)q * N + at];
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     online_merge(P.c, m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   sum = warp_sum(sum);
-  row_loss(P, id, cnt, xk + r * K, st.grad + r * K, m, s, sum, loss + r, st.ref + r, st.coef + r, st.grad + r * K);
+  row_loss(P, id, cnt, st.xk + r * K, st.grad + r * K, m, s, sum, loss + r, st.ref + r, st.coef + r, st.grad + r * K);
 }
 
 template <typename T>
@@ -270,8 +282,11 @@ template <typename T>
 int launch_bwd(const void* logits, int64_t ld, int64_t N, int K, int V, float c, float level, const RowState& st,
                const float* dloss, void* dlogits, int64_t ld_out, cudaStream_t s, const char* what) {
   const int groups = (V + 7 + 7) / 8;
+  // Rows are cut so that a block runs a few rounds: its start (the row's scalars, then the first
+  // loads) is paid once for them, while thousands of rows still even out over the SMs.
   const int per = unroll_of<T>() * kBwdThreads;
-  const int bpr = (groups + per - 1) / per;
+  const int rounds = N >= 8 * kNumSMs ? kBwdRounds : 1;
+  const int bpr = (groups + per * rounds - 1) / (per * rounds);
   IKRL_REQUIRE(N * bpr <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need too many blocks", what,
                (long long)N, V);
   row_loss_bwd_kernel<T><<<(unsigned)(N * bpr), kBwdThreads, 0, s>>>(reinterpret_cast<const T*>(logits), ld, K, V, c,
@@ -349,10 +364,10 @@ int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, 
   return check_launch("row_entries_kernel");
 }
 
-int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const float* xk,
+int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const int* pos,
                       int64_t N, int K, const RowLossParams& p, const RowState& st, float* loss, const int* err,
                       cudaStream_t s) {
-  row_losses_kernel<<<(unsigned)((N + 3) / 4), 128, 0, s>>>(part_m, part_s, part_x, sets, xk, N, K, p, st, loss, err);
+  row_losses_kernel<<<(unsigned)((N + 3) / 4), 128, 0, s>>>(part_m, part_s, part_x, sets, pos, N, K, p, st, loss, err);
   return check_launch("row_losses_kernel");
 }
 

@@ -52,9 +52,9 @@ constexpr uint32_t kMnAtomBytes = 64 * BK * 2;  // one 64-wide MN slab of an MN-
 
 // EPI_LSE_CACHED: the forward's epilogue that also fills the logit cache (its own instantiation,
 // so the plain forward carries none of the cache's code).
-// EPI_TAIL, EPI_DTAIL: forward and backward of the row losses (row_dist.cuh).  EPI_TAIL takes each
-// row's entry columns out of the accumulator, stores their logits and keeps the running sum of the
-// others; EPI_DTAIL forms the gradient of the others.
+// EPI_TAIL, EPI_DTAIL: forward and backward of the row losses (row_dist.cuh).  EPI_TAIL leaves each
+// row's entry columns out and keeps the running sum of the others; EPI_DTAIL forms the gradient of the
+// others.  EPI_TAIL_CACHED is EPI_TAIL that fills the logit cache.
 enum Epi : int {
   EPI_LSE = 0,
   EPI_DLOGITS = 1,
@@ -62,13 +62,16 @@ enum Epi : int {
   EPI_F32 = 3,
   EPI_LSE_CACHED = 4,
   EPI_TAIL = 5,
-  EPI_DTAIL = 6
+  EPI_DTAIL = 6,
+  EPI_TAIL_CACHED = 7
 };
 constexpr bool is_lse(int epi) { return epi == EPI_LSE || epi == EPI_LSE_CACHED; }
 constexpr bool is_dlogits(int epi) { return epi == EPI_DLOGITS || epi == EPI_DTAIL; }
+constexpr bool is_tail(int epi) { return epi == EPI_TAIL || epi == EPI_TAIL_CACHED; }
+constexpr bool is_cached(int epi) { return epi == EPI_LSE_CACHED || epi == EPI_TAIL_CACHED; }
 // The epilogue whose launch rules (pacing, splits) an epilogue follows.
 constexpr int epi_kind(int epi) {
-  return (epi == EPI_LSE_CACHED || epi == EPI_TAIL) ? (int)EPI_LSE : (epi == EPI_DTAIL ? (int)EPI_DLOGITS : epi);
+  return (is_cached(epi) || is_tail(epi)) ? (int)EPI_LSE : (epi == EPI_DTAIL ? (int)EPI_DLOGITS : epi);
 }
 enum F32Mode : int { F32_STORE = 0, F32_ADD = 1, F32_ADD_TO_BF16 = 2 };
 
@@ -109,9 +112,12 @@ struct GemmParams {
   int n_mchunks;
   // Row losses (TAIL, DTAIL)
   float c;                // log2(e) / temperature
-  const int* cols;        // [M][n_cols] entry columns ascending, kNoEntry behind the last (TAIL)
+  const int* m_dev;       // rows in use, on the device (<= M), or null: all M (TAIL)
+  const int* row_idx;     // original row of each row, or null: itself (TAIL)
+  const int* cols;        // [original rows][n_cols] entry columns ascending, then kNoEntry (TAIL)
   int n_cols;
-  float* xk;              // [M][n_cols] logits at the entries (TAIL)
+  float* xk;              // [original rows][n_cols] logits at the entries, or null (TAIL)
+  int64_t cache_cap;      // TAIL_CACHED: slots; a row's slot is slot[row] (row itself with row_idx)
   float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
   const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
 };
@@ -129,6 +135,15 @@ __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, i
 
 __device__ __forceinline__ void st_global_v4(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Rows of a launch: p.M, or for the row losses the count a kernel before left on the device.
+template <int EPI>
+__device__ __forceinline__ int live_rows(const GemmParams& p) {
+  if constexpr (is_tail(EPI)) {
+    if (p.m_dev != nullptr) return min(*p.m_dev, p.M);
+  }
+  return p.M;
 }
 
 // Epilogue role (warps 2..): drain accumulator tiles from TMEM, one row per thread, and apply the
@@ -164,7 +179,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   const int c_lo = group * kCols;
   const int r = q * 32 + lane;
   const int grow = m0 + r;
-  const bool row_ok = grow < p.M;
+  const bool row_ok = grow < live_rows<EPI>(p);
   int64_t tgt = -1;
   float lse2 = 0.f, gval = 0.f;
   if constexpr (is_lse(EPI) || EPI == EPI_DLOGITS) {
@@ -173,19 +188,27 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   int cslot = -1;  // logit-cache slot of this row (LSE)
   bool cache_run = false;  // the warp's 32 rows have consecutive slots: one TMA store per block
   int cslot0 = 0;
-  if constexpr (EPI == EPI_LSE_CACHED) {
-    if (row_ok && p.slot != nullptr) cslot = p.slot[grow];
+  if constexpr (is_cached(EPI)) {
+    if constexpr (EPI == EPI_TAIL_CACHED) {
+      if (row_ok) cslot = p.row_idx != nullptr ? grow : p.slot[grow];
+      if (cslot >= p.cache_cap) cslot = -1;
+    } else if (row_ok && p.slot != nullptr) {
+      cslot = p.slot[grow];
+    }
     cslot0 = __shfl_sync(0xffffffffu, cslot, 0);
     cache_run = stage_smem != 0 && __all_sync(0xffffffffu, cslot >= 0 && cslot == cslot0 + lane);
   }
   // TAIL: the row's next entry column at or after the columns read so far
   const int* next_col = nullptr;
+  float* entry_x = nullptr;
   int next = kNoEntry, at = 0;
   float sum_x = 0.f;
   auto advance = [&]() { next = ++at < p.n_cols ? next_col[at] : kNoEntry; };
-  if constexpr (EPI == EPI_TAIL) {
+  if constexpr (is_tail(EPI)) {
     if (row_ok) {
-      next_col = p.cols + (int64_t)grow * p.n_cols;
+      const int64_t row = p.row_idx != nullptr ? p.row_idx[grow] : grow;
+      next_col = p.cols + row * p.n_cols;
+      if (p.xk != nullptr) entry_x = p.xk + row * p.n_cols;
       int hi = p.n_cols;
       const int from = t_begin * TILE_N;
       while (at < hi) {
@@ -216,6 +239,35 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   if (tgt != -100) tgt -= p.id_offset;
   float run_m = -INFINITY, run_s = 0.f, tval = 0.f;
   bool found = false;
+
+  // The numerators v of a chunk whose maximum is cm into the logit cache.
+  auto store_numerators = [&](const float* v, int col0, float cm) {
+    if (cache_run) {
+      // Consecutive slots: the 32 x 32 block goes out with one TMA store, as the dS blocks do.
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+      const uint32_t row_addr = stage_smem + (uint32_t)lane * 64u;
+      const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), pack_bf16x2(v[8 * k], v[8 * k + 1]),
+                     pack_bf16x2(v[8 * k + 2], v[8 * k + 3]), pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
+                     pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tm_store, stage_smem, col0, cslot0);
+        bulk_commit();
+      }
+    } else if (cslot >= 0) {
+      uint16_t* dst = p.cache_q + (int64_t)cslot * p.ld_cache + col0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        st_global_v4(dst + 8 * k, pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                     pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+    }
+    if (cslot >= 0) p.cache_m[(int64_t)cslot * p.n_mchunks + (col0 >> 5)] = cm;
+  };
 
   // The epilogue of one 32-column chunk of this thread's row, columns [col0, col0 + 32) of the
   // output (col0 < N; the chunk may end past N).  Warp-uniform control flow.
@@ -252,50 +304,23 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       } else {
         run_s = fmaf(cs, fast_exp2(cm - run_m), run_s);
       }
-      if constexpr (EPI == EPI_LSE_CACHED) {
-      if (cache_run) {
-        // Consecutive slots: the 32 x 32 block goes out with one TMA store, as the dS blocks do.
-        if (lane == 0) bulk_wait_read_all();
-        __syncwarp();
-        const uint32_t row_addr = stage_smem + (uint32_t)lane * 64u;
-        const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), pack_bf16x2(v[8 * k], v[8 * k + 1]),
-                       pack_bf16x2(v[8 * k + 2], v[8 * k + 3]), pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
-                       pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(tm_store, stage_smem, col0, cslot0);
-          bulk_commit();
-        }
-      } else if (cslot >= 0) {
-        uint16_t* dst = p.cache_q + (int64_t)cslot * p.ld_cache + col0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          st_global_v4(dst + 8 * k, pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                       pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
-      }
-      if (cslot >= 0) p.cache_m[(int64_t)cslot * p.n_mchunks + (col0 >> 5)] = cm;
-      }  // EPI_LSE_CACHED
-    } else if constexpr (EPI == EPI_TAIL) {
+      if constexpr (EPI == EPI_LSE_CACHED) store_numerators(v, col0, cm);
+    } else if constexpr (is_tail(EPI)) {
       if (p.part_x != nullptr) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) sum_x += i < nvalid ? v[i] : 0.f;
       }
-      // Entries in this chunk leave it: their logits to xk, -inf in their place.
+      // Entries in this chunk leave it (their logits to xk, where it is given).
       while (next < col0) advance();  // entries of other warps' columns
       while (next < col0 + nvalid) {
         const int rel = next - col0;
         float x = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i == rel) {
-            x = v[i];
-            v[i] = -INFINITY;
-          }
-        p.xk[(int64_t)grow * p.n_cols + at] = x;
+        for (int i = 0; i < 32; ++i) {
+          x += i == rel ? v[i] : 0.f;
+          v[i] = i == rel ? -INFINITY : v[i];
+        }
+        if (entry_x != nullptr) entry_x[at] = x;
         advance();
       }
       float cm = -INFINITY;
@@ -305,13 +330,17 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       const float from = cm == -INFINITY ? 0.f : cm;  // a chunk of entries only sums to 0
       float cs = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) cs += i < nvalid ? fast_exp2((v[i] - from) * p.c) : 0.f;
+      for (int i = 0; i < 32; ++i) {
+        v[i] = i < nvalid ? fast_exp2((v[i] - from) * p.c) : 0.f;
+        cs += v[i];
+      }
       if (cm > run_m) {
         run_s = fmaf(run_s, fast_exp2((run_m - cm) * p.c), cs);
         run_m = cm;
       } else {
         run_s = fmaf(cs, cm == -INFINITY ? 1.f : fast_exp2((cm - run_m) * p.c), run_s);
       }
+      if constexpr (EPI == EPI_TAIL_CACHED) store_numerators(v, col0, cm);
     } else if constexpr (is_dlogits(EPI)) {
       uint32_t w[16];
 #pragma unroll
@@ -454,7 +483,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       }
     }
   }
-  if constexpr (is_dlogits(EPI) || EPI == EPI_LSE_CACHED) {
+  if constexpr (is_dlogits(EPI) || is_cached(EPI)) {
     // Every TMA store of this warp has completed before the CTA can exit.
     if (stage_smem != 0 && lane == 0) bulk_wait_all();
     __syncwarp();
@@ -467,7 +496,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       if (found) p.part_t[grow] = tval;
     }
   }
-  if constexpr (EPI == EPI_TAIL) {
+  if constexpr (is_tail(EPI)) {
     if (row_ok && !*abort_v) {
       const int64_t o = (int64_t)(split * GROUPS + group) * p.M + grow;
       p.part_m[o] = run_m;
@@ -704,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // split and the A rows of a row-block pair through L2, and proceed in step.
   const int pair_id = blockIdx.x >> 1;
   const int npairs = gridDim.x >> 1;
-  const int m_pairs = (((p.M + BM - 1) / BM) + 1) >> 1;
+  const int m_pairs = (((live_rows<EPI>(p) + BM - 1) / BM) + 1) >> 1;
   const int nunits = m_pairs * p.splits;
   const int nk = (p.K + BK - 1) / BK;
 
@@ -899,7 +928,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const int pair_id = blockIdx.x >> 1;
   const int npairs = gridDim.x >> 1;
-  const int m_pairs = (((p.M + BM - 1) / BM) + 1) >> 1;
+  const int m_pairs = (((live_rows<EPI>(p) + BM - 1) / BM) + 1) >> 1;
   const int kspl = p.ksplits > 1 ? p.ksplits : 1;
   const int nunits = m_pairs * p.splits * kspl;
   const int nk_all = (p.K + BK - 1) / BK;
@@ -1120,7 +1149,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     // ---------------- epilogue (both CTAs, own 128 rows x 512 columns) ----------------
     const uint32_t af[2] = {smem_u32(&acc_full[0]), smem_u32(&acc_full[1])};
     const uint32_t ae[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
-    const uint32_t stage = ((is_dlogits(EPI) || EPI == EPI_LSE_CACHED) && p.ds_tma)
+    const uint32_t stage = ((is_dlogits(EPI) || is_cached(EPI)) && p.ds_tma)
                                ? smem_base + kWideStages * kWideStageBytes + (uint32_t)(warp - 2) * kDsStageBytes
                                : 0u;
     int jb = 0;
@@ -1328,7 +1357,7 @@ int launch_gemm_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorM
                      int m_tiles, cudaStream_t s) {
   GemmParams p = p_in;
   auto kern = WIDE ? lmhead_gemm_wide_kernel<EPI, A_MN, B_MN> : lmhead_gemm_pair_kernel<EPI, A_MN, B_MN>;
-  p.ds_tma = (WIDE && c != nullptr && (is_dlogits(EPI) || EPI == EPI_LSE_CACHED)) ? 1 : 0;
+  p.ds_tma = (WIDE && c != nullptr && (is_dlogits(EPI) || is_cached(EPI))) ? 1 : 0;
   const uint32_t smem_bytes = WIDE ? (p.ds_tma ? kWideDsSmemBytes : kWideSmemBytes) : kPairSmemBytes;
   IKRL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes));
   IKRL_REQUIRE(p.split_major == 1, IKRL_ERR_UNSUPPORTED, "pair kernel needs a split-major grid");
@@ -1471,7 +1500,7 @@ K1Plan plan_k1(int epi, int64_t m_tiles, int N, int K, int splits_hint, int nsm)
     pl.tiles_per_split = 1;
   } else {
     pl.tiles_per_split = (int)cdiv64(pl.n_tiles, splits_hint);
-    if (is_dlogits(epi) && pl.kind != 0 && persistent && balance_splits_enabled())
+    if ((is_dlogits(epi) || is_tail(epi)) && pl.kind != 0 && persistent && balance_splits_enabled())
       pl.tiles_per_split = balanced_tiles_per_split(m_tiles, pl.n_tiles, splits_hint, npairs);
   }
   pl.splits = (int)cdiv64(pl.n_tiles, pl.tiles_per_split);
@@ -1914,6 +1943,114 @@ __global__ void __launch_bounds__(256) ds_from_cache_kernel(
   }
 }
 
+// The same for a row loss: dS = gs q 2^(c (m - ref)) + level, with the row's scaled upstream and level
+// (row_scale_kernel).  idx null: chunk row k is row c0 + k.  Rows without a slot have no gradient.
+__global__ void __launch_bounds__(256) dtail_from_cache_kernel(
+    const uint16_t* __restrict__ cache_q, const float* __restrict__ cache_m, int64_t ld_cache, int n_mchunks,
+    const int* __restrict__ slot, const int* __restrict__ idx, const float* __restrict__ ref_c,
+    const float* __restrict__ gs_c, const float* __restrict__ level_c, float c, int64_t c0, int64_t rows, int V,
+    uint16_t* __restrict__ ds, int64_t ld_ds) {
+  const int vec = V >> 3;
+  for (int64_t k = blockIdx.y; k < rows; k += gridDim.y) {
+    const int64_t kc = c0 + k;
+    const int64_t sl = slot[idx ? idx[kc] : kc];
+    const float ref = ref_c[kc], gs = gs_c[kc], lv = level_c[kc];
+    const bool on = sl >= 0 && (gs != 0.f || lv != 0.f);
+    const uint16_t* qrow = cache_q + (on ? sl : 0) * ld_cache;
+    const float* mrow = cache_m + (on ? sl : 0) * n_mchunks;
+    uint16_t* drow = ds + k * ld_ds;
+    for (int jb = blockIdx.x * blockDim.x * kDsUnroll + threadIdx.x; jb < vec;
+         jb += gridDim.x * blockDim.x * kDsUnroll) {
+      uint4 qv[kDsUnroll];
+      float mv[kDsUnroll];
+#pragma unroll
+      for (int u = 0; u < kDsUnroll; ++u) {
+        const int jv = jb + u * (int)blockDim.x;
+        qv[u] = make_uint4(0u, 0u, 0u, 0u);
+        mv[u] = 0.f;
+        if (on && jv < vec) {
+          qv[u] = *reinterpret_cast<const uint4*>(qrow + (jv << 3));
+          mv[u] = mrow[jv >> 2];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kDsUnroll; ++u) {
+        const int jv = jb + u * (int)blockDim.x;
+        if (jv >= vec) break;
+        const float sc = on ? gs * fast_exp2((mv[u] - ref) * c) : 0.f;
+        const uint32_t w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(fmaf(bf16lo(w[e]), sc, lv), fmaf(bf16hi(w[e]), sc, lv));
+        *reinterpret_cast<uint4*>(drow + (jv << 3)) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+}
+
+// From the numbers pos[r] that cache_slot_kernel gave the rows of a row loss that are not kRowNone:
+// idx[pos[r]] = r, *count = how many, and slot[r] = pos[r] where that is below the cache's slots.
+// idx and slot may be null.
+__global__ void row_index_kernel(const int* __restrict__ pos, int64_t N, int64_t cap, int* __restrict__ idx,
+                                 int* __restrict__ slot, const int* __restrict__ counts, int n_counts,
+                                 int* __restrict__ count) {
+  const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (r == 0 && count != nullptr) {
+    int n = 0;
+    for (int b = 0; b < n_counts; ++b) n += counts[b];
+    *count = n;
+  }
+  if (r >= N) return;
+  const int k = pos[r];
+  if (idx != nullptr && k >= 0) idx[k] = (int)r;
+  if (slot != nullptr) slot[r] = k < cap ? k : -1;
+}
+
+// h_c[k] = h[idx[k]] for k < *n.
+__global__ void gather_live_rows_kernel(const uint4* __restrict__ h, const int* __restrict__ idx,
+                                        const int* __restrict__ n, int vec_per_row, uint4* __restrict__ h_c) {
+  const int64_t total = (int64_t)*n * vec_per_row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t k = i / vec_per_row;
+    const int c = (int)(i - k * vec_per_row);
+    h_c[i] = h[(int64_t)idx[k] * vec_per_row + c];
+  }
+}
+
+// A distillation's logits at the entries, xk[r][e] = h_r . w_col, one warp an entry: 32-bit sums of
+// exact products, rounded.  The GEMM's accumulators cut every partial sum to 24 bits towards zero,
+// which at K = 4096 takes 4e-6 of a logit of 12 away; the student's likely tokens are mostly among the
+// entries, so this leaves little of it (loss of an 8B-sized head against 64 bits: 1.3e-5 -> 2.5e-6).
+// A cross entropy takes its target's logit from the accumulators instead: there the likely tokens stay
+// in the tail, and target and tail are short by about the same (2e-6 against 1e-5 with only the target
+// exact).
+__global__ void __launch_bounds__(256) entry_logits_kernel(const uint4* __restrict__ h, const uint4* __restrict__ w,
+                                                           const int* __restrict__ cols, int64_t n, int K,
+                                                           int vec_per_row, float* __restrict__ xk) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (i >= n) return;
+  const int col = cols[i];
+  if (col == kNoEntry) return;
+  const uint4* a = h + i / K * vec_per_row;
+  const uint4* b = w + (int64_t)col * vec_per_row;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+  for (int v = lane; v < vec_per_row; v += 32) {
+    const uint4 x = a[v], y = b[v];
+    s0 = fmaf(bf16lo(x.x), bf16lo(y.x), s0);
+    s1 = fmaf(bf16hi(x.x), bf16hi(y.x), s1);
+    s0 = fmaf(bf16lo(x.y), bf16lo(y.y), s0);
+    s1 = fmaf(bf16hi(x.y), bf16hi(y.y), s1);
+    s0 = fmaf(bf16lo(x.z), bf16lo(y.z), s0);
+    s1 = fmaf(bf16hi(x.z), bf16hi(y.z), s1);
+    s0 = fmaf(bf16lo(x.w), bf16lo(y.w), s0);
+    s1 = fmaf(bf16hi(x.w), bf16hi(y.w), s1);
+  }
+  const float s = warp_sum(s0 + s1);
+  if (lane == 0) xk[i] = s;
+}
+
 // h_c[k] = h[idx[k]] for k < n, 16 bytes per thread.
 __global__ void gather_rows_kernel(const uint4* __restrict__ h, const int* __restrict__ idx, int64_t n, int vec_per_row,
                                    uint4* __restrict__ h_c) {
@@ -2009,13 +2146,38 @@ size_t cache_fwd_workspace_bytes(int64_t N, int H, int V) {
   return base + ((((size_t)std::max<int64_t>(1, cdiv64(N, kCompactRows)) * 4) + 255) & ~size_t(255));
 }
 
-// Workspace of a row loss: its forward's partial sums of all logits and logits at the entries stand
-// behind the forward's own, its backward's levels behind the backward's own.
+// A row loss of at most this many rows runs its GEMMs on all of them: one row pair of tiles costs
+// the same however many of its rows count, and the compaction's host synchronisation and launches
+// would cost more than they save.
+constexpr int64_t kRowLossDense = 256;
+
+// Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums
+// of all logits (up to 3 times the forward's splits, which the balance rule may take), and the
+// numbering of the rows that count with their hidden rows gathered.  Its backward's: the rows' levels
+// behind the backward's own.
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 static size_t row_level_bytes(int64_t N) { return align256((size_t)N * 4); }
-static size_t row_loss_fwd_bytes(int64_t N, int H, int V, int K) {
-  const FwdLayout L = fwd_layout(N, H, V);
-  return L.total + align256((size_t)kWideGroups * L.splits * N * 4) + align256((size_t)N * K * 4);
+struct RowLossFwdLayout {
+  size_t pm_off, ps_off, px_off, counts_off, count_off, pos_off, idx_off, hc_off, total;
+  int splits;
+  bool gather;  // the rows that count are gathered before the GEMM
+};
+static RowLossFwdLayout row_loss_fwd_layout(int64_t N, int H, int V) {
+  RowLossFwdLayout L;
+  L.splits = fwd_layout(N, H, V).splits;
+  L.gather = N > kRowLossDense;
+  const size_t part = align256((size_t)kWideGroups * 3 * L.splits * N * 4);
+  size_t o = 256;  // the error word
+  L.pm_off = o; o += part;
+  L.ps_off = o; o += part;
+  L.px_off = o; o += part;
+  L.counts_off = o; o += align256((size_t)std::max<int64_t>(1, cdiv64(N, kCompactRows)) * 4);
+  L.count_off = o; o += 256;
+  L.pos_off = o; o += align256((size_t)N * 4);
+  L.idx_off = o; o += align256((size_t)N * 4);
+  L.hc_off = o; o += L.gather ? align256((size_t)N * H * 2) : 0;
+  L.total = o;
+  return L;
 }
 
 static int lmhead_fwd_impl(const char* what, const void* hidden, const void* weight, const int64_t* ids, int64_t N, int32_t H,
@@ -2087,6 +2249,7 @@ struct RowLossBwd {
   RowState st;
   int K;
   float c, level;
+  bool all_cached;  // every row that is not kRowNone has a cache slot
 };
 
 // cache_slot / cache_q / cache_m: the logit cache a forward filled (all null: no cache).  Active
@@ -2149,7 +2312,8 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   int64_t n_cached = 0;                                      // leading compacted rows whose dS is cached
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   IKRL_CUDA(cudaStreamIsCapturing(s, &cap));
-  if (skip_zero_rows_enabled() && cap == cudaStreamCaptureStatusNone && N <= INT32_MAX) {
+  if (skip_zero_rows_enabled() && cap == cudaStreamCaptureStatusNone && N <= INT32_MAX &&
+      !(rl && N <= kRowLossDense)) {
     int* counts = reinterpret_cast<int*>(w + L.cnt_off);
     int64_t* n_act_d = reinterpret_cast<int64_t*>(w + L.nact_off);
     int* idx = reinterpret_cast<int*>(w + L.idx_off);
@@ -2209,6 +2373,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   struct Chunk {
     int64_t c0, rows, cached;
   };
+  if (rl && rl->all_cached && cache_slot != nullptr) n_cached = Nw;
   std::vector<Chunk> chunks;
   if (n_cached > 0 && n_cached < Nw && Nw <= chunk && dweight && dweight_dtype == IKRL_DTYPE_BF16 && !L.need_dw32) {
     chunks.push_back({0, Nw, n_cached});
@@ -2236,7 +2401,13 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     const uint16_t* hc = hsrc + c0 * H;
     // 1) dS = g * (onehot - softmax(h W^T)) for this chunk: from the logit cache, or recomputed
     const int64_t from_cache = chunks[ci].cached;  // leading rows of the chunk
-    if (from_cache > 0) {
+    if (from_cache > 0 && rl) {
+      const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
+                      (unsigned)std::min<int64_t>(from_cache, 65535));
+      dtail_from_cache_kernel<<<grid, 256, 0, s>>>(cache_q, cache_m, L.lds, (int)cdiv64(V, 32), cache_slot, idx_c,
+                                                   lsesrc, gsrc, level, rl->c, c0, from_cache, V, dS, L.lds);
+      if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
+    } else if (from_cache > 0) {
       const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
                       (unsigned)std::min<int64_t>(from_cache, 65535));
       ds_from_cache_kernel<<<grid, 256, 0, s>>>(cache_q, cache_m, L.lds, (int)cdiv64(V, 32), cache_slot, idx_c,
@@ -2330,77 +2501,155 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   return IKRL_OK;
 }
 
-// Forward of a row loss through the LM head: entries, the GEMM with the TAIL epilogue, losses.
+// The logit cache of a row loss: slots 0, 1, ... go to the rows that count, in row order, while there
+// are any (rows = 0: no cache).
+struct RowCacheArgs {
+  int64_t rows;
+  int* slot;
+  uint16_t* q;
+  float* m;
+};
+
+static int check_row_cache(const char* what, int64_t N, int V, const RowCacheArgs& c) {
+  IKRL_REQUIRE(c.rows >= 0, IKRL_ERR_INVALID_ARGUMENT, "%s: cache_rows %lld < 0", what, (long long)c.rows);
+  if (c.rows == 0 || N == 0) return IKRL_OK;
+  IKRL_REQUIRE(V % 8 == 0, IKRL_ERR_UNSUPPORTED, "%s: the logit cache needs V (%d) to be a multiple of 8", what, V);
+  IKRL_REQUIRE(c.slot && c.q && c.m, IKRL_ERR_INVALID_ARGUMENT, "%s: null cache pointer", what);
+  IKRL_REQUIRE((reinterpret_cast<uintptr_t>(c.q) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.m) & 3) == 0,
+               IKRL_ERR_ALIGNMENT, "%s: cache_q must be 16-byte and cache_m 4-byte aligned", what);
+  return IKRL_OK;
+}
+
+// Forward of a row loss through the LM head: the rows' entries, the rows that count gathered, the GEMM with the TAIL epilogue, the losses.
 static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void* weight, const int64_t* tids,
                                const float* tlp, int64_t N, int32_t H, int32_t V, int32_t K, const RowLossParams& P,
-                               float* loss, void* state, size_t state_bytes, void* ws, size_t ws_bytes,
-                               void* stream) {
+                               float* loss, void* state, size_t state_bytes, const RowCacheArgs& cache, void* ws,
+                               size_t ws_bytes, void* stream) {
   int rc = check_common(hidden, weight, tids, N, H, V, what);
   if (rc) return rc;
   if (N == 0) return clear_status_word(ws, ws_bytes, stream);
   IKRL_REQUIRE(loss != nullptr, IKRL_ERR_INVALID_ARGUMENT, "%s: output is NULL", what);
   IKRL_REQUIRE(state != nullptr && state_bytes >= row_state_bytes(N, K), IKRL_ERR_WORKSPACE,
                "%s: state %zu < %zu bytes", what, state_bytes, row_state_bytes(N, K));
-  const size_t need = row_loss_fwd_bytes(N, H, V, K);
-  IKRL_REQUIRE(ws != nullptr && ws_bytes >= need, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes,
-               need);
+  const RowLossFwdLayout L = row_loss_fwd_layout(N, H, V);
+  IKRL_REQUIRE(ws != nullptr && ws_bytes >= L.total, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what,
+               ws_bytes, L.total);
   IKRL_REQUIRE(((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(state)) & 255) == 0,
                IKRL_ERR_ALIGNMENT, "%s: workspace and state must be 256-byte aligned", what);
+  IKRL_REQUIRE(((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15) == 0,
+               IKRL_ERR_ALIGNMENT, "%s: hidden and weight must be 16-byte aligned", what);
+  if ((rc = check_row_cache(what, N, V, cache))) return rc;
   cudaStream_t s = as_stream(stream);
-  const FwdLayout L = fwd_layout(N, H, V);
   const RowState st = row_state(state, N, K);
   char* w = reinterpret_cast<char*>(ws);
-  int* err = reinterpret_cast<int*>(w + L.err_off);
-  float* part_x = reinterpret_cast<float*>(w + L.total);
-  float* xk = reinterpret_cast<float*>(w + L.total + align256((size_t)kWideGroups * L.splits * N * 4));
+  int* err = reinterpret_cast<int*>(w);
   IKRL_CUDA(cudaMemsetAsync(err, 0, sizeof(int), s));
-  CUtensorMap ta, tb, tb2;
-  if ((rc = make_tmap(&ta, hidden, H, N, H, BM, "hidden"))) return rc;
-  if ((rc = make_tmap(&tb, weight, H, V, H, BN, "weight"))) return rc;
-  if ((rc = make_tmap(&tb2, weight, H, V, H, BN / 2, "weight"))) return rc;
   if ((rc = launch_row_entries(tids, tlp, N, K, P, st, s))) return rc;
+  const int vpr = H / 8;
   GemmParams p{};
+  if (P.loss == ROW_XENT) {
+    p.xk = st.xk;
+  } else {
+    IKRL_REQUIRE(cdiv64(N * K, 8) <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: %lld rows of %d entries", what,
+                 (long long)N, K);
+    entry_logits_kernel<<<(unsigned)cdiv64(N * K, 8), 256, 0, s>>>(reinterpret_cast<const uint4*>(hidden),
+                                                                   reinterpret_cast<const uint4*>(weight), st.cols,
+                                                                   N * K, K, vpr, st.xk);
+    if ((rc = check_launch("entry_logits_kernel"))) return rc;
+  }
+
   p.M = (int)N; p.N = V; p.K = H;
   p.part_m = reinterpret_cast<float*>(w + L.pm_off);
   p.part_s = reinterpret_cast<float*>(w + L.ps_off);
-  p.part_x = P.loss == ROW_XENT && P.smoothing != 0.f ? part_x : nullptr;
+  p.part_x = P.loss == ROW_XENT && P.smoothing != 0.f ? reinterpret_cast<float*>(w + L.px_off) : nullptr;
   p.err = err;
   p.c = P.c;
   p.cols = st.cols;
   p.n_cols = K;
-  p.xk = xk;
-  if ((rc = launch_k1<EPI_TAIL, false, false>(ta, tb, ta, tb2, p, (int)cdiv64(N, BM), L.splits, s))) return rc;
-  return launch_row_losses(p.part_m, p.part_s, p.part_x, p.part_sets, xk, N, K, P, st, loss, err, s);
+  const void* rows_in = hidden;
+  const int* pos = nullptr;
+  const bool cached = cache.rows > 0;
+  if (L.gather || cached) {
+    int* counts = reinterpret_cast<int*>(w + L.counts_off);
+    int* count = reinterpret_cast<int*>(w + L.count_off);
+    int* posw = reinterpret_cast<int*>(w + L.pos_off);
+    int* idx = L.gather ? reinterpret_cast<int*>(w + L.idx_off) : nullptr;
+    const int nb = (int)cdiv64(N, kCompactRows);
+    cache_count_kernel<<<nb, kCompactThreads, 0, s>>>(nullptr, st.row_ids, N, counts);
+    if ((rc = check_launch("cache_count_kernel"))) return rc;
+    cache_slot_kernel<<<nb, kCompactThreads, 0, s>>>(nullptr, st.row_ids, N, counts, N, posw);
+    if ((rc = check_launch("cache_slot_kernel"))) return rc;
+    row_index_kernel<<<(unsigned)cdiv64(N, 256), 256, 0, s>>>(posw, N, cache.rows, idx, cached ? cache.slot : nullptr,
+                                                              counts, nb, count);
+    if ((rc = check_launch("row_index_kernel"))) return rc;
+    if (L.gather) {
+      uint4* hc = reinterpret_cast<uint4*>(w + L.hc_off);
+      gather_live_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(N * vpr, 256), 148ll * 16), 256, 0, s>>>(
+          reinterpret_cast<const uint4*>(hidden), idx, count, vpr, hc);
+      if ((rc = check_launch("gather_live_rows_kernel"))) return rc;
+      rows_in = hc;
+      pos = posw;
+      p.m_dev = count;
+      p.row_idx = idx;
+    }
+    if (cached) {
+      p.slot = posw;
+      p.cache_cap = cache.rows;
+      p.cache_q = cache.q;
+      p.cache_m = cache.m;
+      p.ld_cache = cdiv64(V, 64) * 64;
+      p.n_mchunks = (int)cdiv64(V, 32);
+    }
+  }
+  CUtensorMap ta, tb, tb2, tq;
+  if ((rc = make_tmap(&ta, rows_in, H, N, H, BM, "hidden"))) return rc;
+  if ((rc = make_tmap(&tb, weight, H, V, H, BN, "weight"))) return rc;
+  if ((rc = make_tmap(&tb2, weight, H, V, H, BN / 2, "weight"))) return rc;
+  const int m_tiles = (int)cdiv64(N, BM);
+  if (cached) {
+    if ((rc = make_store_tmap(&tq, cache.q, V, cache.rows, p.ld_cache, "logit cache store"))) return rc;
+    if ((rc = launch_k1<EPI_TAIL_CACHED, false, false>(ta, tb, ta, tb2, p, m_tiles, L.splits, s, &tq))) return rc;
+  } else {
+    if ((rc = launch_k1<EPI_TAIL, false, false>(ta, tb, ta, tb2, p, m_tiles, L.splits, s))) return rc;
+  }
+  return launch_row_losses(p.part_m, p.part_s, p.part_x, p.part_sets, pos, N, K, P, st, loss, err, s);
 }
 
 static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void* weight, int64_t N, int32_t H,
                                int32_t V, int32_t K, const RowLossParams& P, const void* state, size_t state_bytes,
                                const float* dloss, int64_t chunk_rows, void* dhidden, void* dweight,
-                               int32_t dweight_dtype, int32_t accumulate_dweight, void* ws, size_t ws_bytes,
-                               void* stream) {
+                               int32_t dweight_dtype, int32_t accumulate_dweight, const RowCacheArgs& cache, void* ws,
+                               size_t ws_bytes, void* stream) {
+  int rc = check_row_cache(what, N, V, cache);
+  if (rc) return rc;
   RowLossBwd rl{};
-  const bool rows = N > 0;
-  if (rows) {
+  if (N > 0) {
     IKRL_REQUIRE(state != nullptr && state_bytes >= row_state_bytes(N, K), IKRL_ERR_WORKSPACE,
                  "%s: state %zu < %zu bytes", what, state_bytes, row_state_bytes(N, K));
     IKRL_REQUIRE((reinterpret_cast<uintptr_t>(state) & 255) == 0, IKRL_ERR_ALIGNMENT,
                  "%s: state must be 256-byte aligned", what);
+    const size_t need = ikrl_lmhead_row_loss_bwd_workspace_bytes(N, H, V, chunk_rows, dweight_dtype,
+                                                                 accumulate_dweight);
+    IKRL_REQUIRE(ws != nullptr && ws_bytes >= need, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what,
+                 ws_bytes, need);
     rl.st = row_state(const_cast<void*>(state), N, K);
   }
   rl.K = K;
   rl.c = P.c;
   rl.level = P.loss == ROW_XENT ? -P.smoothing / (float)V : 0.f;
+  rl.all_cached = cache.rows >= N;
+  const bool cached = cache.rows > 0;
   return lmhead_bwd_impl(what, hidden, weight, rl.st.row_ids, rl.st.ref, dloss, N, H, V, 0, chunk_rows, dhidden,
-                         dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream, nullptr, nullptr, nullptr,
-                         &rl);
+                         dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream,
+                         cached ? cache.slot : nullptr, cached ? cache.q : nullptr, cached ? cache.m : nullptr, &rl);
 }
 
 
 extern "C" {
 
-size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int32_t K) {
-  if (N <= 0 || H <= 0 || V <= 0 || K <= 0) return 256;
-  return row_loss_fwd_bytes(N, H, V, K);
+size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V) {
+  if (N <= 0 || H <= 0 || V <= 0) return 256;
+  return row_loss_fwd_layout(N, H, V).total;
 }
 
 size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
@@ -2411,7 +2660,8 @@ size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V,
 
 int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,
                             const float* teacher_logp, int64_t N, int32_t H, int32_t V, int32_t K,
-                            const ikrl_distill_params* params, float* loss, void* state, size_t state_bytes, void* ws,
+                            const ikrl_distill_params* params, float* loss, void* state, size_t state_bytes,
+                            int64_t cache_rows, int32_t* cache_slot, void* cache_q, float* cache_m, void* ws,
                             size_t ws_bytes, void* stream) {
   clear_error();
   const char* what = "ikrl_lmhead_distill_fwd";
@@ -2420,47 +2670,58 @@ int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_
   if (rc) return rc;
   IKRL_REQUIRE(N <= 0 || teacher_logp, IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   return lmhead_row_loss_fwd(what, hidden, weight, teacher_ids, teacher_logp, N, H, V, K, P, loss, state, state_bytes,
-                             ws, ws_bytes, stream);
+                             {cache_rows, cache_slot, reinterpret_cast<uint16_t*>(cache_q), cache_m}, ws, ws_bytes,
+                             stream);
 }
 
 int ikrl_lmhead_distill_bwd(const void* hidden, const void* weight, int64_t N, int32_t H, int32_t V, int32_t K,
                             const ikrl_distill_params* params, const void* state, size_t state_bytes,
                             const float* dloss, int64_t chunk_rows, void* dhidden, void* dweight,
-                            int32_t dweight_dtype, int32_t accumulate_dweight, void* ws, size_t ws_bytes,
-                            void* stream) {
+                            int32_t dweight_dtype, int32_t accumulate_dweight, int64_t cache_rows,
+                            const int32_t* cache_slot, const void* cache_q, const float* cache_m, void* ws,
+                            size_t ws_bytes, void* stream) {
   clear_error();
   const char* what = "ikrl_lmhead_distill_bwd";
   RowLossParams P;
   int rc = distill_params(what, params, V, K, &P);
   if (rc) return rc;
   return lmhead_row_loss_bwd(what, hidden, weight, N, H, V, K, P, state, state_bytes, dloss, chunk_rows, dhidden,
-                             dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream);
+                             dweight, dweight_dtype, accumulate_dweight,
+                             {cache_rows, const_cast<int32_t*>(cache_slot),
+                              reinterpret_cast<uint16_t*>(const_cast<void*>(cache_q)), const_cast<float*>(cache_m)},
+                             ws, ws_bytes, stream);
 }
 
 int ikrl_lmhead_cross_entropy_fwd(const void* hidden, const void* weight, const int64_t* targets, int64_t N,
                                   int32_t H, int32_t V, float label_smoothing, float z_loss, float* loss, void* state,
-                                  size_t state_bytes, void* ws, size_t ws_bytes, void* stream) {
+                                  size_t state_bytes, int64_t cache_rows, int32_t* cache_slot, void* cache_q,
+                                  float* cache_m, void* ws, size_t ws_bytes, void* stream) {
   clear_error();
   const char* what = "ikrl_lmhead_cross_entropy_fwd";
   RowLossParams P;
   int rc = xent_params(what, label_smoothing, z_loss, V, &P);
   if (rc) return rc;
-  return lmhead_row_loss_fwd(what, hidden, weight, targets, nullptr, N, H, V, 1, P, loss, state, state_bytes, ws,
-                             ws_bytes, stream);
+  return lmhead_row_loss_fwd(what, hidden, weight, targets, nullptr, N, H, V, 1, P, loss, state, state_bytes,
+                             {cache_rows, cache_slot, reinterpret_cast<uint16_t*>(cache_q), cache_m}, ws, ws_bytes,
+                             stream);
 }
 
 int ikrl_lmhead_cross_entropy_bwd(const void* hidden, const void* weight, int64_t N, int32_t H, int32_t V,
                                   float label_smoothing, float z_loss, const void* state, size_t state_bytes,
                                   const float* dloss, int64_t chunk_rows, void* dhidden, void* dweight,
-                                  int32_t dweight_dtype, int32_t accumulate_dweight, void* ws, size_t ws_bytes,
-                                  void* stream) {
+                                  int32_t dweight_dtype, int32_t accumulate_dweight, int64_t cache_rows,
+                                  const int32_t* cache_slot, const void* cache_q, const float* cache_m, void* ws,
+                                  size_t ws_bytes, void* stream) {
   clear_error();
   const char* what = "ikrl_lmhead_cross_entropy_bwd";
   RowLossParams P;
   int rc = xent_params(what, label_smoothing, z_loss, V, &P);
   if (rc) return rc;
   return lmhead_row_loss_bwd(what, hidden, weight, N, H, V, 1, P, state, state_bytes, dloss, chunk_rows, dhidden,
-                             dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream);
+                             dweight, dweight_dtype, accumulate_dweight,
+                             {cache_rows, const_cast<int32_t*>(cache_slot),
+                              reinterpret_cast<uint16_t*>(const_cast<void*>(cache_q)), const_cast<float*>(cache_m)},
+                             ws, ws_bytes, stream);
 }
 
 size_t ikrl_lmhead_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V) {

@@ -52,11 +52,13 @@ struct RowState {
   float* coef;       // [N]
   int* cols;         // [N][K] entry columns ascending, then kNoEntry
   float* grad;       // [N][K] gradient at them (until the loss is formed: the teacher's log-probs)
+  float* xk;         // [N][K] logits at them (forward only)
+  float* part;       // [3][N] tail maximum and sum, sum of all logits (forward on logits only)
 };
 
 inline size_t row_state_bytes(int64_t N, int K) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
-  return al((size_t)N * 8) + 2 * al((size_t)N * 4) + 2 * al((size_t)N * K * 4);
+  return al((size_t)N * 8) + 2 * al((size_t)N * 4) + 3 * al((size_t)N * K * 4) + al((size_t)N * 12);
 }
 
 inline RowState row_state(void* base, int64_t N, int K) {
@@ -67,7 +69,9 @@ inline RowState row_state(void* base, int64_t N, int K) {
   s.ref = reinterpret_cast<float*>(p); p += al((size_t)N * 4);
   s.coef = reinterpret_cast<float*>(p); p += al((size_t)N * 4);
   s.cols = reinterpret_cast<int*>(p); p += al((size_t)N * K * 4);
-  s.grad = reinterpret_cast<float*>(p);
+  s.grad = reinterpret_cast<float*>(p); p += al((size_t)N * K * 4);
+  s.xk = reinterpret_cast<float*>(p); p += al((size_t)N * K * 4);
+  s.part = reinterpret_cast<float*>(p);
   return s;
 }
 
@@ -82,8 +86,9 @@ int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossP
 int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, const RowLossParams& p,
                        const RowState& st, cudaStream_t s);
 // part_m / part_s / part_x: [sets][N] tail maxima, sums of 2^(c (x - max)), plain sums of all logits
-// (part_x only for ROW_XENT); xk: [N][K] logits at the entries; err: the GEMM's error word.
-int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const float* xk,
+// (part_x null without label smoothing); pos: the place of each row in them, or null: itself; err: an
+// error word that makes every loss NaN, or null.
+int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const int* pos,
                       int64_t N, int K, const RowLossParams& p, const RowState& st, float* loss, const int* err,
                       cudaStream_t s);
 
@@ -94,8 +99,8 @@ __device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); 
 // One row's entries, by a block of at least kMaxEntries threads: columns ascending into s_col
 // (kNoEntry behind the last) and the teacher's log-probs beside them into s_lp.  An entry counts
 // when its id is >= 0 and its log-prob is not -inf, and a repeated id at its first place only.
-// s_raw: K scratch words.  Returns the row's id; cnt = entries that count.  Every entry counts the
-// smaller columns for its rank (K comparisons a thread), so the order never depends on timing.
+// s_raw: kMaxEntries scratch words, 16-byte aligned.  Returns the row's id; cnt = entries that count.  Every entry counts the
+// smaller columns for its rank, so the order never depends on timing.
 __device__ __forceinline__ int64_t row_entries(const int64_t* __restrict__ tids, const float* __restrict__ tlp, int K,
                                                int V, int* s_col, float* s_lp, int* s_raw, int& cnt) {
   if (tlp == nullptr) {  // one target
@@ -123,19 +128,33 @@ __device__ __forceinline__ int64_t row_entries(const int64_t* __restrict__ tids,
     s_col[e] = kNoEntry;
     s_lp[e] = 0.f;
   }
+  for (int i = K + e; i < ((K + 3) & ~3); i += blockDim.x) s_raw[i] = kNoEntry;  // whole vectors below
   const bool any_bad = __syncthreads_or(bad);
+  // One sweep: an earlier equal column makes this entry a repeat, smaller columns make its rank.
   bool repeat = false;
-  if (col != kNoEntry)
-    for (int j = 0; j < e; ++j) repeat |= s_raw[j] == col;
-  __syncthreads();
-  if (repeat) {
-    s_raw[e] = kNoEntry;
-    col = kNoEntry;
+  int rank = 0;
+  if (col != kNoEntry) {
+    const int4* v = reinterpret_cast<const int4*>(s_raw);
+#pragma unroll 4
+    for (int q = 0; q < (K + 3) / 4; ++q) {
+      const int4 o = v[q];
+      rank += (o.x < col) + (o.y < col) + (o.z < col) + (o.w < col);
+      repeat |= (o.x == col && 4 * q < e) | (o.y == col && 4 * q + 1 < e) | (o.z == col && 4 * q + 2 < e) |
+                (o.w == col && 4 * q + 3 < e);
+    }
+  }
+  if (__syncthreads_or(repeat)) {  // repeats leave the table, and the ranks are counted again
+    if (repeat) {
+      s_raw[e] = kNoEntry;
+      col = kNoEntry;
+    }
+    __syncthreads();
+    rank = 0;
+    if (col != kNoEntry)
+      for (int j = 0; j < K; ++j) rank += s_raw[j] < col;
   }
   cnt = __syncthreads_count(col != kNoEntry);
   if (col != kNoEntry) {
-    int rank = 0;
-    for (int j = 0; j < K; ++j) rank += s_raw[j] < col;
     s_col[rank] = col;
     s_lp[rank] = lp;
   }

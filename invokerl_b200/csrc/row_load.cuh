@@ -25,23 +25,50 @@ template <typename T>
 struct Group8;
 template <>
 struct Group8<uint16_t> {
-  uint4 v;
-  __device__ __forceinline__ void get(float (&x)[8]) const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[2 * k] = bf16lo(w[k]);
-      x[2 * k + 1] = bf16hi(w[k]);
-    }
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int k) const { return (k & 1) ? bf16hi(w[k >> 1]) : bf16lo(w[k >> 1]); }
+  // The largest value, NaN aside (-inf when there is no other).
+  __device__ __forceinline__ float max() const {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
   }
+  // Value `rel` of the group, which becomes -inf.
+  __device__ __forceinline__ float take(int rel) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k == rel) {
+        x = get(k);
+        w[k >> 1] = (k & 1) ? ((w[k >> 1] & 0xffffu) | 0xff800000u) : ((w[k >> 1] & 0xffff0000u) | 0xff80u);
+      }
+    return x;
+  }
+  __device__ __forceinline__ void load(const uint16_t* p);
+  __device__ __forceinline__ void fill() { w[0] = w[1] = w[2] = w[3] = 0xff80ff80u; }
 };
 template <>
 struct Group8<float> {
-  uint4 v, u;
-  __device__ __forceinline__ void get(float (&x)[8]) const {
-    const uint32_t w[8] = {v.x, v.y, v.z, v.w, u.x, u.y, u.z, u.w};
+  uint32_t w[8];
+  __device__ __forceinline__ float get(int k) const { return __uint_as_float(w[k]); }
+  __device__ __forceinline__ float max() const {
+    return fmaxf(fmaxf(fmaxf(fmaxf(get(0), get(1)), fmaxf(get(2), get(3))),
+                       fmaxf(fmaxf(get(4), get(5)), fmaxf(get(6), get(7)))), -INFINITY);
+  }
+  __device__ __forceinline__ float take(int rel) {
+    float x = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(w[k]);
+    for (int k = 0; k < 8; ++k)
+      if (k == rel) {
+        x = get(k);
+        w[k] = 0xff800000u;
+      }
+    return x;
+  }
+  __device__ __forceinline__ void load(const float* p);
+  __device__ __forceinline__ void fill() {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = 0xff800000u;
   }
 };
 
@@ -56,57 +83,80 @@ __device__ __forceinline__ void st_stream16(void* p, uint4 v) {
                : "memory");
 }
 
-// Group j of the row; columns outside the row read as -inf.
-__device__ __forceinline__ Group8<uint16_t> load_group(const RowView<uint16_t>& rv, int j) {
-  Group8<uint16_t> g;
-  const int v0 = rv.first(j);
-  if (rv.whole(j)) {
-    g.v = ld_stream16(rv.row + v0);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int a = v0 + 2 * k, b = a + 1;
-      const uint32_t lo = (a >= 0 && a < rv.V) ? rv.row[a] : 0xff80u;
-      const uint32_t hi = (b >= 0 && b < rv.V) ? rv.row[b] : 0xff80u;
-      w[k] = lo | (hi << 16);
-    }
-    g.v = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  return g;
+__device__ __forceinline__ void Group8<uint16_t>::load(const uint16_t* p) {
+  const uint4 v = ld_stream16(p);
+  w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
 }
-__device__ __forceinline__ Group8<float> load_group(const RowView<float>& rv, int j) {
-  Group8<float> g;
-  const int v0 = rv.first(j);
-  if (rv.whole(j)) {
-    g.v = ld_stream16(rv.row + v0);
-    g.u = ld_stream16(rv.row + v0 + 4);
-  } else {
-    uint32_t w[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int a = v0 + k;
-      w[k] = (a >= 0 && a < rv.V) ? __float_as_uint(rv.row[a]) : 0xff800000u;
-    }
-    g.v = make_uint4(w[0], w[1], w[2], w[3]);
-    g.u = make_uint4(w[4], w[5], w[6], w[7]);
-  }
-  return g;
+__device__ __forceinline__ void Group8<float>::load(const float* p) {
+  const uint4 v = ld_stream16(p), u = ld_stream16(p + 4);
+  w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  w[4] = u.x; w[5] = u.y; w[6] = u.z; w[7] = u.w;
 }
 
-// Running (m, s) over eight more values: m the maximum, s the sum of 2^(c (x - m)).  The difference
-// is taken before the product: c x may pass the range of fp32 where a mask holds the type's lowest
-// value, x - m does not.  While nothing but -inf was seen the sum is taken from 0, which leaves it
-// 0; NaN and +inf make it NaN.
-__device__ __forceinline__ void online_update(const float (&x)[8], float c, float& m, float& s) {
-  const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+// Group j of the row; columns outside the row read as -inf.
+template <typename T>
+__device__ __forceinline__ void load_group(Group8<T>& g, const RowView<T>& rv, int j) {
+  const int v0 = rv.first(j);
+  if (rv.whole(j)) {
+    g.load(rv.row + v0);
+    return;
+  }
+  g.fill();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int a = v0 + k;
+    if (a < 0 || a >= rv.V) continue;
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t b = rv.row[a];
+      g.w[k >> 1] = (k & 1) ? ((g.w[k >> 1] & 0xffffu) | (b << 16)) : ((g.w[k >> 1] & 0xffff0000u) | b);
+    } else {
+      g.w[k] = __float_as_uint(rv.row[a]);
+    }
+  }
+}
+
+// Where |m| is below this, c m is finite and exponents are formed with one fma.
+constexpr float kFmaLimit = 1e37f;
+
+// Running (m, s) over U more groups (the first `n` of them): m the maximum, s the sum of 2^(c (x - m)).
+// One maximum and one rescaling serve all of them; then a value costs its unpacking, an fma, an
+// exponential and an addition.  The fma takes c x from the rounded c m, and what that rounding
+// leaves is multiplied out once per call, so the sum stands relative to m itself.
+//
+// A mask may hold the type's lowest value: there c x passes the range of fp32, so the difference
+// x - m is taken first.  While nothing but -inf was seen the sum is taken from 0, which leaves it 0;
+// NaN and +inf make it NaN.
+template <typename T, int U>
+__device__ __forceinline__ void online_groups(const Group8<T> (&g)[U], int n, float c, float& m, float& s) {
+  float mx = g[0].max();
+#pragma unroll
+  for (int u = 1; u < U; ++u)
+    if (u < n) mx = fmaxf(mx, g[u].max());
   if (mx > m) {
     s *= fast_exp2((m - mx) * c);
     m = mx;
   }
-  const float from = m == -INFINITY ? 0.f : m;
+  if (fabsf(m) < kFmaLimit) {
+    const float pt = m * c;
+    float b = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) s += fast_exp2((x[k] - from) * c);
+    for (int u = 0; u < U; ++u) {
+      if (u >= n) break;
+      float e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = fast_exp2(fmaf(g[u].get(k), c, -pt));
+      b += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    }
+    s = fmaf(b, fast_exp2(-fmaf(m, c, -pt)), s);
+  } else {
+    const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= n) break;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += fast_exp2((g[u].get(k) - from) * c);
+    }
+  }
 }
 
 __device__ __forceinline__ void online_merge(float c, float& m, float& s, float m2, float s2) {

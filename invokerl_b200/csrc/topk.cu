@@ -1,12 +1,14 @@
 // The k likeliest tokens of each row of logits and their log-probs over the whole vocabulary: what
 // a teacher gives a distillation.
 //
-// One pass over the row, bound by HBM.  Beside the running logsumexp, a block keeps the columns that
-// may still be among the k largest in a buffer in shared memory: a column enters when it is above the
-// k-th largest known so far.  The first columns set that bar (the k-th largest of the threads' own
-// maxima is below the k-th largest of all), so of V columns in no particular order about
-// k (1 + ln(V / 16384)) enter and the buffer is sorted once, at the end.  Where it fills up (rising
-// rows), it is sorted there, cut to k, and the bar rises; what did not fit waits in registers.
+// One pass over the row, bound by HBM.  Beside the running logsumexp, a block notes the groups of
+// eight columns whose maximum reaches a bar, a lower bound of the k-th largest value: the k-th largest
+// of the threads' own maxima so far, found bit by bit with block-wide counts and raised after 1, 2,
+// 4, 8, ... rounds.  With 512 threads that bound is nearly the k-th largest itself, so of V columns in
+// no particular order about k (1 + log2(V / 16384)) are noted.  The noted groups are read again (from
+// L2), their columns above the bar go to a buffer of keys, and the buffer is sorted.  Where a list
+// fills up (rising rows, many equal values) it is worked off, and the keys are cut to the k largest,
+// which raises the bar to the k-th key itself.
 //
 // Order and ties are those of one 64-bit key, the value above the inverted column: larger values
 // first, of equal values the lower column.  Keys are distinct, so the result does not depend on the
@@ -23,6 +25,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kTopThreads = 512;
 constexpr int kTopBuf = 2048;  // keys of the buffer: the cluster's 8 x kMaxEntries at the end
+constexpr int kTopList = 4096;  // noted groups
 static_assert(kTopBuf >= 8 * kMaxEntries && kTopBuf >= 2 * kMaxEntries, "top-k buffer too small");
 
 // Values in key order: NaN first, -0 as +0.
@@ -59,111 +62,131 @@ __device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
 template <typename T>
-__global__ void __launch_bounds__(kTopThreads) logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int V,
-                                                                  int K, float c, float inv_t,
-                                                                  float* __restrict__ logp,
-                                                                  int64_t* __restrict__ ids) {
+__global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                                     int K, float c, float inv_t,
+                                                                     float* __restrict__ logp,
+                                                                     int64_t* __restrict__ ids) {
   constexpr int U = sizeof(T) == 2 ? 4 : 2;
+  constexpr int kRound = U * kTopThreads;
+  static_assert(kTopList >= 2 * kRound, "the list holds a round behind its limit");
   __shared__ uint64_t s_buf[kTopBuf];
+  __shared__ int s_list[kTopList];
   __shared__ float s_red[64], s_part[2][8];
-  __shared__ int s_cnt;
+  __shared__ int s_cnt, s_noted;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t r = blockIdx.x / C;
   const RowView<T> rv(logits, ld, r, V);
   const int per = (rv.groups + C - 1) / C;
   const int j0 = min(rank * per, rv.groups), j1 = min(j0 + per, rv.groups);
-  if (threadIdx.x == 0) s_cnt = 0;
+  if (threadIdx.x == 0) s_cnt = s_noted = 0;
   __syncthreads();
 
   float m = -INFINITY, s = 0.f;
-  uint64_t bar = 0;  // keys at or below it are out
-  for (int jb = j0; jb < j1; jb += U * kTopThreads) {
-    Group8<T> g[U];
-    float top[U];  // each group's largest value
+  uint32_t mine = 0;  // the largest value_key this thread saw, NaN aside (0: no column)
+  uint64_t bar = 0;   // keys at or below it are out
+  float bar_value = -INFINITY;
+
+  // Columns of the noted groups above the bar into the buffer.
+  auto work_off = [&]() {
+    __syncthreads();
+    const int n = s_noted;
+    for (int b = 0; b < n; b += kTopThreads) {
+      Group8<T> g;
+      int v0 = 0;
+      uint32_t pend = 0;
+      auto key_of = [&](int k) {
+        return ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
+      };
+      if (b + (int)threadIdx.x < n) {
+        const int j = s_list[b + threadIdx.x];
+        load_group(g, rv, j);
+        v0 = rv.first(j);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * kTopThreads + threadIdx.x;
-      if (j < j1) g[u] = load_group(rv, j);
-    }
-    uint32_t mine = 0;  // the largest value_key of this thread, NaN aside (0: no column)
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * kTopThreads + threadIdx.x;
-      top[u] = -INFINITY;
-      if (j >= j1) continue;
-      float x[8];
-      g[u].get(x);
-      const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      online_update(x, c, m, s);
-      mine = max(mine, value_key(mx));
-      top[u] = s == s ? mx : nan_f32();  // a NaN or +inf came by: look at every column from here on
-    }
-    if (jb == j0) {
-      // The largest bar that at least K threads' maxima reach, bit by bit.
-      uint32_t t = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t cand = t | (1u << bit);
-        if (__syncthreads_count(mine >= cand) >= K) t = cand;
+        for (int k = 0; k < 8; ++k)
+          if (v0 + k >= 0 && v0 + k < V && key_of(k) > bar) pend |= 1u << k;
       }
-      if (t > 0) bar = ((uint64_t)t << 32) - 1;  // values equal to it stay in
-    }
-    // Columns above the bar: bit 8 u + k of `pend`.
-    uint32_t pend = 0;
-    auto filter = [&](uint32_t among) {
-      uint32_t keep = 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (((among >> (8 * u)) & 0xffu) == 0) continue;
-        const int v0 = rv.first(jb + u * kTopThreads + threadIdx.x);
-        float x[8];
-        g[u].get(x);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t key = ((uint64_t)value_key(x[k]) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
-          if (((among >> (8 * u + k)) & 1u) && v0 + k >= 0 && v0 + k < V && key > bar) keep |= 1u << (8 * u + k);
-        }
-      }
-      return keep;
-    };
-    {
-      uint32_t near = 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (jb + u * kTopThreads + (int)threadIdx.x < j1 && value_key(top[u]) >= (uint32_t)(bar >> 32))
-          near |= 0xffu << (8 * u);
-      if (near) pend = filter(near);
-    }
-    while (true) {
-      if (pend) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (((pend >> (8 * u)) & 0xffu) == 0) continue;
-          const int v0 = rv.first(jb + u * kTopThreads + threadIdx.x);
-          float x[8];
-          g[u].get(x);
+      while (true) {
+        if (pend) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            if (!((pend >> (8 * u + k)) & 1u)) continue;
+            if (!((pend >> k) & 1u)) continue;
             const int at = atomicAdd(&s_cnt, 1);
             if (at < kTopBuf) {
-              s_buf[at] = ((uint64_t)value_key(x[k]) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
-              pend &= ~(1u << (8 * u + k));
+              s_buf[at] = key_of(k);
+              pend &= ~(1u << k);
             }
           }
         }
+        if (!__syncthreads_or(pend != 0)) break;
+        // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
+        sort_keys(s_buf, kTopBuf, kTopBuf);
+        bar = s_buf[K - 1];
+        bar_value = key_value((uint32_t)(bar >> 32));
+        if (threadIdx.x == 0) s_cnt = K;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (((pend >> k) & 1u) && key_of(k) <= bar) pend &= ~(1u << k);
+        __syncthreads();
       }
-      const bool more = __syncthreads_or(pend != 0);
-      if (!more) break;
-      // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
-      sort_keys(s_buf, kTopBuf, kTopBuf);
-      bar = s_buf[K - 1];
-      if (threadIdx.x == 0) s_cnt = K;
-      if (pend) pend = filter(pend);
-      __syncthreads();
     }
+    __syncthreads();
+    if (threadIdx.x == 0) s_noted = 0;
+    __syncthreads();
+  };
+
+  int round = 0;
+  for (int jb = j0; jb < j1; jb += kRound, ++round) {
+    Group8<T> g[U];
+    const int n = min(U, (j1 - jb + kTopThreads - 1) / kTopThreads);  // groups a thread, at most
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * kTopThreads + threadIdx.x;
+      if (j < j1) load_group(g[u], rv, j);
+      else g[u].fill();
+    }
+    online_groups<T, U>(g, n, c, m, s);
+    float top[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) top[u] = g[u].max();
+    if ((round & (round + 1)) == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kTopThreads + threadIdx.x;
+        if (j < j1) mine = max(mine, value_key(top[u]));
+      }
+      // The largest bar, to 16 bits of the key, that at least K threads' maxima reach.
+      uint32_t t = 0;
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t cand = t | (1u << bit);
+        if (__syncthreads_count(mine >= cand) >= K) t = cand;
+      }
+      const uint64_t found = t > 0 ? ((uint64_t)t << 32) - 1 : 0;  // values equal to it stay in
+      if (found > bar) {
+        bar = found;
+        bar_value = key_value(t);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kTopThreads + threadIdx.x;
+        if (j < j1) mine = max(mine, value_key(top[u]));
+      }
+    }
+    // Note the groups that reach the bar; all of them once a NaN or +inf came by (s is NaN then).
+    bool full = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * kTopThreads + threadIdx.x;
+      if (j < j1 && (!(top[u] < bar_value) || s != s)) {
+        const int at = atomicAdd(&s_noted, 1);
+        s_list[at] = j;
+        full |= at >= kTopList - kRound - 1;
+      }
+    }
+    if (__syncthreads_or(full)) work_off();
   }
-  __syncthreads();
+  work_off();
   block_online_merge(c, m, s, s_red);
   const int have = min(s_cnt, kTopBuf);
   sort_keys(s_buf, have, pow2_at_least(max(have, K)));

@@ -716,7 +716,7 @@ def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple
     shape = (*logits.shape[:-1], k)
     log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
     ids = torch.empty(shape, dtype=torch.int64, device=dev)
-    with torch.cuda.device(dev):
+    with N.on_device(dev):
         call("ikrl_logits_topk", ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V), i32(k), f32(t),
              ptr(log_probs), ptr(ids), N.stream_of(dev))
     return log_probs, ids
@@ -734,7 +734,7 @@ class LogitsRowLoss(torch.autograd.Function):
         state = _row_state(Nr, K, dev)
         head = (ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V), ptr(ids))
         tail = (ptr(loss), ptr(state), sz(state.numel()), N.stream_of(dev))
-        with torch.cuda.device(dev):
+        with N.on_device(dev):
             if teacher_lp is None:
                 call("ikrl_logits_cross_entropy_fwd", *head, f32(smoothing), f32(z), *tail)
             else:
@@ -753,7 +753,7 @@ class LogitsRowLoss(torch.autograd.Function):
         dx = torch.empty(Nr, V, dtype=x.dtype, device=x.device)
         head = (ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V))
         tail = (ptr(state), sz(state.numel()), ptr(g), ptr(dx), i64(V), N.stream_of(x.device))
-        with torch.cuda.device(x.device):
+        with N.on_device(x.device):
             if params is None:
                 call("ikrl_logits_cross_entropy_bwd", *head, f32(smoothing), f32(z), *tail)
             else:
@@ -792,21 +792,44 @@ def logits_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, label_smoo
     return LogitsRowLoss.apply(x, t, None, None, label_smoothing, z_loss).reshape(logits.shape[:-1])
 
 
+# A head call of up to this many rows keeps all of them in the logit cache (a few dozen MB) without
+# asking how much memory is free.
+_ROW_CACHE_SMALL = 256
+
+
+def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> LogitCache | None:
+    """Logit cache of a row loss's forward under the policy of `set_logit_cache`, or None."""
+    if _LOGIT_CACHE["mode"] == "off" or V % 8 or n_rows == 0 or torch.cuda.is_current_stream_capturing():
+        return None
+    rows = n_rows if n_rows <= _ROW_CACHE_SMALL else logit_cache_rows(n_rows, H, V, device, n_rows, chunk_rows)
+    return LogitCache(n_rows, V, rows, device) if rows > 0 else None
+
+
+def _cache_args(cache: LogitCache | None):
+    if cache is None:
+        return i64(0), None, None, None
+    return i64(cache.rows), ptr(cache.slot), ptr(cache.q), ptr(cache.m)
+
+
 class LMHeadRowLoss(torch.autograd.Function):
-    """A row loss of hidden @ weight.T without the logits in memory."""
+    """A row loss of hidden @ weight.T without the logits in memory.  As `LMHeadLogProb`, it may keep
+    the rows' softmax numerators between forward and backward (`set_logit_cache`)."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, ids, teacher_lp, params, smoothing, z, chunk_rows):
+    def forward(ctx, hidden, weight, ids, teacher_lp, params, smoothing, z, chunk_rows, grad_mode):
         dev = hidden.device
         Nr, H = hidden.shape
         V = weight.shape[0]
         K = 1 if teacher_lp is None else ids.shape[1]
         loss = torch.empty(Nr, dtype=torch.float32, device=dev)
         state = _row_state(Nr, K, dev)
-        nbytes = int(N.lib().ikrl_lmhead_row_loss_fwd_workspace_bytes(Nr, H, V, K))
+        cache = None
+        if grad_mode and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
+            cache = _row_cache(Nr, H, V, dev, chunk_rows)
+        nbytes = int(N.lib().ikrl_lmhead_row_loss_fwd_workspace_bytes(Nr, H, V))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        tail = (ptr(loss), ptr(state), sz(state.numel()), ptr(ws), sz(nbytes), N.stream_of(dev))
-        with torch.cuda.device(dev):
+        tail = (ptr(loss), ptr(state), sz(state.numel()), *_cache_args(cache), ptr(ws), sz(nbytes), N.stream_of(dev))
+        with N.on_device(dev):
             if teacher_lp is None:
                 call("ikrl_lmhead_cross_entropy_fwd", ptr(hidden), ptr(weight), ptr(ids), i64(Nr), i32(H), i32(V),
                      f32(smoothing), f32(z), *tail)
@@ -817,6 +840,7 @@ class LMHeadRowLoss(torch.autograd.Function):
             lmhead_status(ws)
         ctx.save_for_backward(hidden, weight, state)
         ctx.args = (K, params, smoothing, z, chunk_rows)
+        ctx.cache = cache
         return loss
 
     @staticmethod
@@ -825,7 +849,8 @@ class LMHeadRowLoss(torch.autograd.Function):
         hidden, weight, state = ctx.saved_tensors
         K, params, smoothing, z, chunk_rows = ctx.args
         want_dh, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        none = (None,) * 6
+        cache, ctx.cache = ctx.cache, None  # a second backward recomputes the logits
+        none = (None,) * 7
         if not (want_dh or want_dw):
             return None, None, *none
         dev = hidden.device
@@ -840,8 +865,8 @@ class LMHeadRowLoss(torch.autograd.Function):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         head = (ptr(hidden), ptr(weight), i64(Nr), i32(H), i32(V))
         tail = (ptr(state), sz(state.numel()), ptr(g), i64(chunk_rows), ptr(dh), ptr(dw), i32(N.IKRL_DTYPE_BF16),
-                i32(0), ptr(ws), sz(nbytes), N.stream_of(dev))
-        with torch.cuda.device(dev):
+                i32(0), *_cache_args(cache), ptr(ws), sz(nbytes), N.stream_of(dev))
+        with N.on_device(dev):
             if params is None:
                 call("ikrl_lmhead_cross_entropy_bwd", *head, f32(smoothing), f32(z), *tail)
             else:
@@ -868,7 +893,8 @@ def lmhead_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
     N.require_cuda(hidden, weight, teacher_ids, teacher_log_probs)
     h, w = _head_rows(hidden, weight)
     ids, lp = _teacher_rows(teacher_ids, teacher_log_probs, hidden.shape[:-1])
-    return LMHeadRowLoss.apply(h, w, ids, lp, params, 0.0, 0.0, chunk_rows).reshape(hidden.shape[:-1])
+    return LMHeadRowLoss.apply(h, w, ids, lp, params, 0.0, 0.0, chunk_rows,
+                               torch.is_grad_enabled()).reshape(hidden.shape[:-1])
 
 
 def lmhead_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
@@ -880,4 +906,5 @@ def lmhead_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     N.require_cuda(hidden, weight, targets)
     h, w = _head_rows(hidden, weight)
     t = _targets_rows(targets, hidden.shape[:-1])
-    return LMHeadRowLoss.apply(h, w, t, None, None, label_smoothing, z_loss, chunk_rows).reshape(hidden.shape[:-1])
+    return LMHeadRowLoss.apply(h, w, t, None, None, label_smoothing, z_loss, chunk_rows,
+                               torch.is_grad_enabled()).reshape(hidden.shape[:-1])

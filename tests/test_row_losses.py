@@ -176,23 +176,28 @@ def test_c_entries_refuse_before_any_cuda_call(lib):
         with pytest.raises(N.IkrlError, match=msg):
             N.call("ikrl_logits_topk", p, N.i32(1), N.i64(9), N.i64(2), N.i32(9), N.i32(k), N.f32(1), p, p, None)
 
-    def head(n=4, H=64, K=3, nbytes=1 << 24, state_bytes=1 << 20, ws=p):
-        N.call("ikrl_lmhead_distill_fwd", p, p, p, p, N.i64(n), N.i32(H), N.i32(100), N.i32(K), params(), p, p,
-               N.sz(state_bytes), ws, N.sz(nbytes), None)
+    def head(n=4, H=64, K=3, nbytes=1 << 24, state_bytes=1 << 20, ws=p, V=100, cache=0, q=p):
+        N.call("ikrl_lmhead_distill_fwd", p, p, p, p, N.i64(n), N.i32(H), N.i32(V), N.i32(K), params(), p, p,
+               N.sz(state_bytes), N.i64(cache), p, p, q, ws, N.sz(nbytes), None)
 
     for kw, msg in [(dict(H=12), "multiple of 8"), (dict(n=-1), "bad sizes"), (dict(nbytes=256), "workspace"),
-                    (dict(state_bytes=64), "state"), (dict(ws=N.c_void_p(264)), "aligned"), (dict(K=300), "K=300")]:
+                    (dict(state_bytes=64), "state"), (dict(ws=N.c_void_p(264)), "aligned"), (dict(K=300), "K=300"),
+                    (dict(cache=-1), "cache_rows"), (dict(cache=4, V=101), "multiple of 8"),
+                    (dict(cache=4, V=104, q=None), "null cache"), (dict(cache=4, V=104, q=N.c_void_p(258)), "aligned")]:
         with pytest.raises(N.IkrlError, match=msg):
             head(**kw)
     with pytest.raises(N.IkrlError, match="bf16 dweight"):
         N.call("ikrl_lmhead_cross_entropy_bwd", p, p, N.i64(4), N.i32(64), N.i32(100), N.f32(0), N.f32(0), p,
-               N.sz(1 << 20), p, N.i64(0), p, p, N.i32(N.IKRL_DTYPE_BF16), N.i32(1), p, N.sz(1 << 24), None)
+               N.sz(1 << 20), p, N.i64(0), p, p, N.i32(N.IKRL_DTYPE_BF16), N.i32(1), N.i64(0), None, None, None, p,
+               N.sz(1 << 24), None)
 
 
 def test_workspace_sizes_grow_with_their_parts(lib):
     s = lib.ikrl_row_loss_state_bytes
-    assert s(0, 5) == 256 and s(100, 64) >= 100 * (8 + 4 + 4 + 64 * 8)
+    assert s(0, 5) == 256 and s(100, 64) >= 100 * (8 + 4 + 4 + 64 * 12 + 12)
     f = lib.ikrl_lmhead_row_loss_fwd_workspace_bytes
-    assert f(1000, 1024, 5000, 64) >= lib.ikrl_lmhead_fwd_workspace_bytes(1000, 1024, 5000) + 1000 * 64 * 4
+    # three sets of partial sums, the rows that count gathered (above 256 rows)
+    assert f(1000, 1024, 5000) >= lib.ikrl_lmhead_fwd_workspace_bytes(1000, 1024, 5000) + 1000 * 1024 * 2
+    assert f(256, 1024, 5000) < f(257, 1024, 5000) - 256 * 1024 * 2
     b = lib.ikrl_lmhead_row_loss_bwd_workspace_bytes
     assert b(1000, 1024, 5000, 0, 1, 0) >= lib.ikrl_lmhead_bwd_workspace_bytes(1000, 1024, 5000, 0, 1, 0) + 4000

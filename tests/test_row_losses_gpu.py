@@ -388,10 +388,14 @@ def make_head(n, H, V, K, seed, w_std=None):
     return h.to(torch.bfloat16), w, ids, lp.float(), up
 
 
-def check_head(h, w, up, got, rows_fn, scale_fn, K, span):
+def check_head(h, w, up, got, rows_fn, scale_fn, K, span, roundings=1):
     """(loss, dh, dw) against 64 bits.  A logit errs by at most H half-steps of fp32 of its terms'
-    magnitudes (delta); dS is rounded to bf16 once (2^-8) from p, q that err by 4 delta; the second
-    products add V (or n) half-steps; the outputs are rounded to bf16."""
+    magnitudes (delta); dS is rounded to bf16 once (2^-8 of itself) from p, q that err by 4 delta; the
+    second products add V (or n) half-steps; the outputs are rounded to bf16.
+
+    roundings=2, dS from the logit cache: dS = coef q + level with q rounded to bf16, so the sum errs by
+    2^-8 of coef q, before the level is taken off.  With smoothing coef q (about g p) and level (g e / V)
+    cancel where p is near e / V, so this rounding is 2^-8 of A, which holds g p, and not of dS."""
     loss, dh, dw = (t.detach().double().cpu() for t in got)
     hd, wd = h.double(), w.double()
     n, H = h.shape
@@ -402,7 +406,7 @@ def check_head(h, w, up, got, rows_fn, scale_fn, K, span):
     tol = fp32_tol(V, K, span) * (1 + span)
     check_loss(loss, want, tol + 2 * delta * (2 + span))
     A = scale_fn(x)
-    unit = 2 ** -8 * ds.abs() + (4 * delta + tol) * A
+    unit = 2 ** -8 * ds.abs() + (4 * delta + tol + (roundings - 1) * 2 ** -8) * A
     for g, ref, e in ((dh, ds @ wd, unit @ wd.abs() + V * EPS32 * (ds.abs() @ wd.abs())),
                       (dw, ds.t() @ hd, unit.t() @ hd.abs() + n * EPS32 * (ds.abs().t() @ hd.abs()))):
         err = (g - ref).abs()
@@ -411,7 +415,7 @@ def check_head(h, w, up, got, rows_fn, scale_fn, K, span):
     # and the whole: independent roundings of 2^-8 at most leave far less than 2^-8 of the norm
     for g, ref in ((dh, ds @ wd), (dw, ds.t() @ hd)):
         if float(ref.norm()) > 0:
-            assert float((g - ref).norm() / ref.norm()) <= 2 ** -7 + 8 * delta
+            assert float((g - ref).norm() / ref.norm()) <= (1 + roundings) * 2 ** -8 + 8 * delta
 
 
 def run_head(f, h, w, up, *args, **kw):
@@ -470,6 +474,46 @@ def test_head_under_each_kernel_choice(knobs):
     span = span_of(h.double() @ w.double().t(), ids, lp, 1.0)
     check_head(h, w, up, got, lambda y: distill_rows(y, ids, lp, "jsd"), lambda x: grad_scale(x, ids, lp, up), 12,
                span)
+
+
+@pytest.mark.parametrize("loss", ["jsd", "xent"])
+@pytest.mark.parametrize("n,H,V,slots", [(200, 1024, 2056, 200), (3, 64, 40, 3), (600, 1024, 1000, 600),
+                                         (600, 1024, 1000, 250), (600, 256, 1000, 1)])
+def test_head_with_the_logit_cache(n, H, V, slots, loss, monkeypatch):
+    """dS from stored numerators: all rows in the cache, some, one; rows without entries hold no slot; a
+    second backward, without the cache, agrees within the roundings; the kernel choices share it."""
+    h, w, ids, lp, up = make_head(n, H, V, 9, n + V + slots)
+    t = ids[:, 0].clone()
+    if n > 5:
+        ids[1::3] = -1
+        t[1::3] = -100
+    asked = []
+    monkeypatch.setattr(ops, "logit_cache_rows", lambda *a: asked.append(a) or slots)
+    if loss == "jsd":
+        f, args, kw = ops.lmhead_distill, (ids, lp), dict(kind="jsd", temperature=1.3)
+        rows = lambda y: distill_rows(y, ids, lp, "jsd", 0.5, 1.3)  # noqa: E731
+        scale = lambda x: grad_scale(x, ids, lp, up, 1.3)  # noqa: E731
+        span = span_of(h.double() @ w.double().t(), ids, lp, 1.3)
+    else:
+        f, args, kw = ops.lmhead_cross_entropy, (t,), dict(label_smoothing=0.1)
+        rows = lambda y: xent_rows(y, t, 0.1)  # noqa: E731
+        x = h.double() @ w.double().t()
+        span = float((x.amax(1) - x.amin(1)).max())
+
+        def scale(x):
+            p = torch.softmax(x, 1)
+            return up.double().abs()[:, None] * (p + 0.1 / V).scatter(1, t.clamp(min=0)[:, None], 1.0)
+
+    for knobs in ({}, dict(wide=0), dict(wide=1), dict(cta_pairs=0), dict(skip_zero_rows=0)):
+        with N.tuning(**knobs):
+            check_head(h, w, up, run_head(f, h, w, up, *args, **kw), rows, scale, 9, span, roundings=2)
+    assert bool(asked) == (n > 256)
+    hd, wd = h.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    out = f(hd, wd, *[a.to(DEV) for a in args], **kw)
+    first = torch.autograd.grad(out, (hd, wd), up.to(DEV), retain_graph=True)
+    again = torch.autograd.grad(out, (hd, wd), up.to(DEV))
+    for g1, g2 in zip(first, again):
+        assert float((g1.float() - g2.float()).norm()) <= 4 * 2 ** -8 * float(g2.float().norm())
 
 
 def test_head_in_chunks_one_sided_and_bad_rows():
