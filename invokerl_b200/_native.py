@@ -340,6 +340,12 @@ def stream_of(device: torch.device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def stream_handle(device: torch.device) -> int:
+    """The current stream of `device` as a plain integer, without building a Stream object."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 class on_device:
     """Makes the device of a call's tensors the current one while the call launches (a launch goes to
     the current device, whatever its stream)."""
@@ -421,6 +427,7 @@ __all__ = [
     "ptr",
     "require_cuda",
     "stream_of",
+    "stream_handle",
     "on_device",
     "dtype_code",
     "as_mask",

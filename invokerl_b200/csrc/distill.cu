@@ -17,211 +17,339 @@ namespace cg = cooperative_groups;
 
 constexpr int kFwdThreads = 512;
 constexpr int kBwdThreads = 512;
-constexpr int kBwdRounds = 5;  // rounds of a backward block when there are rows enough
+constexpr int kBwdRounds = 2;  // rounds of a backward block
 
 template <typename T> constexpr int unroll_of() { return sizeof(T) == 2 ? 4 : 2; }  // 64 bytes in flight a thread
 
-// One row per cluster of blocks (one block when there are rows enough).  Each block finds the
-// row's entries, marks the groups of eight columns that hold one in a bitmap, and runs once over
-// its groups: a group without an entry goes to the running (maximum, sum) as it is; from the others
-// the entries are taken out first (their logits go to the first block), so what is summed is the
-// tail.  The first block joins the blocks' sums and one of its warps forms the loss.
+// Words of the bitmap of n groups, up to a whole round of the block.
+__host__ __device__ __forceinline__ int map_words(int n) {
+  return (n + kFwdThreads - 1) / kFwdThreads * (kFwdThreads / 32);
+}
+
+// A row's entries in a forward block: their columns ascending, a bit for each whole group of the part
+// that holds one (bit j - a), and where their logits go.
+struct RowEntries {
+  const int* col;
+  int cnt;
+  const uint32_t* map;
+  float* x;
+};
+
+template <typename T>
+__device__ __forceinline__ void mark_entry(const RowPart<T>& p, int col, uint32_t* map) {
+  const int j = p.group_of(col);
+  if (j >= p.a && j < p.b) atomicOr(&map[(j - p.a) >> 5], 1u << ((j - p.a) & 31));
+}
+
+// First U groups a thread of a part: issued ahead of the work on the entries.
+template <typename T, int U>
+__device__ __forceinline__ void load_round(Group8<T> (&g)[U], const RowPart<T>& p, int jb) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kFwdThreads + (int)threadIdx.x));
+}
+template <typename T, int U>
+__device__ __forceinline__ bool whole_round(const RowPart<T>& p, int jb) {
+  return jb + U * kFwdThreads <= p.b;
+}
+
+// Running sums of a part by a block: m, s over the tail and, with SUM, the sum of all logits.
+//
+// The loop over the part leaves out the groups that hold entries: their bits are one shared word a
+// warp and group, zero most of the time.  Those groups are taken one a thread, by the thread of their
+// first entry, and so are the groups that reach past the row.  g holds the first round, if whole.
+template <typename T, int U, bool SUM>
+__device__ __forceinline__ void sum_part(Group8<T> (&g)[U], const RowPart<T>& p, const RowEntries& e, float c, float& m,
+                                         float& s, float& sum) {
+  const int tid = (int)threadIdx.x;
+  int mine = -1, first = 0;
+  if (tid < e.cnt) {
+    const int j = p.group_of(e.col[tid]);
+    if (j >= p.j0 && j < p.j1 && (tid == 0 || p.group_of(e.col[tid - 1]) != j)) {
+      mine = j;
+      first = tid;
+    }
+  }
+  // The block's last two threads take the edges that hold no entry.
+  const int ej = p.edge(kFwdThreads - 1 - tid);
+  if (ej >= 0) {
+    bool holds = false;
+    for (int k = 0; k < e.cnt; ++k) holds |= p.group_of(e.col[k]) == ej;
+    if (!holds) {
+      mine = ej;
+      first = e.cnt;
+    }
+  }
+  if (mine >= 0) {
+    Group8<T> h[1];
+    load_group(h[0], p.rv, mine);
+    const int v0 = p.rv.first(mine);
+    if constexpr (SUM) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v0 + k >= 0 && v0 + k < p.rv.V) sum += h[0].get(k);
+    }
+    for (; first < e.cnt && e.col[first] < v0 + 8; ++first) e.x[first] = h[0].take(e.col[first] - v0);
+    online_groups<T, 1>(h, c, m, s);
+  }
+
+  int jb = p.a;
+  const uint32_t* word = e.map + (tid >> 5);
+  const uint32_t bit = 1u << (tid & 31);
+  for (; whole_round<T, U>(p, jb); jb += U * kFwdThreads) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t wd = word[u * (kFwdThreads / 32)];
+      if constexpr (SUM) {
+        uint64_t t = add2(add2(g[u].get2(0), g[u].get2(1)), add2(g[u].get2(2), g[u].get2(3)));
+        float lo, hi;
+        unpack2(t, lo, hi);
+        sum += (wd & bit) ? 0.f : lo + hi;
+      }
+      if (wd != 0 && (wd & bit)) g[u].fill();
+    }
+    word += U * (kFwdThreads / 32);
+    online_groups<T, U>(g, c, m, s);
+    if (whole_round<T, U>(p, jb + U * kFwdThreads)) load_round<T, U>(g, p, jb + U * kFwdThreads);
+  }
+  for (; jb < p.b; jb += kFwdThreads) {  // what is left, a group a thread at a time
+    const int j = jb + tid;
+    Group8<T> h[1];
+    h[0].fill();
+    if (j < p.b && !(*word & bit)) {
+      h[0].load(p.at(j));
+      if constexpr (SUM) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += h[0].get(k);
+      }
+    }
+    word += kFwdThreads / 32;
+    online_groups<T, 1>(h, c, m, s);
+  }
+}
+
+// Few rows: one launch.  A cluster of blocks shares a row (one block when it is short); each finds the
+// row's entries and sums its part, the first block joins the parts and one of its warps forms the loss.
 template <typename T, bool SUM>
 __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __restrict__ logits, int64_t ld,
                                                                    const int64_t* __restrict__ tids,
                                                                    const float* __restrict__ tlp, int K,
                                                                    RowLossParams P, RowState st,
                                                                    float* __restrict__ loss) {
-  extern __shared__ uint32_t s_map[];  // a bit per group of this block
+  extern __shared__ uint32_t s_map[];
   __shared__ int s_col[kMaxEntries];
   __shared__ __align__(16) int s_raw[kMaxEntries];
-  __shared__ float s_lp[kMaxEntries], s_x[kMaxEntries], s_red[64], s_part[3][8];
+  __shared__ float s_lp[kMaxEntries], s_x[kMaxEntries], s_red[64], s_part[3][kMaxParts];
   constexpr int U = unroll_of<T>();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t r = blockIdx.x / C;
-  const RowView<T> rv(logits, ld, r, P.V);
-  const int per = (rv.groups + C - 1) / C;
-  const int j0 = min(rank * per, rv.groups), j1 = min(j0 + per, rv.groups);
+  const RowPart<T> p(logits, ld, r, P.V, rank, C);
+  Group8<T> g[U];
+  if (whole_round<T, U>(p, p.a)) load_round<T, U>(g, p, p.a);
 
+  for (int i = threadIdx.x; i < map_words(p.b - p.a); i += kFwdThreads) s_map[i] = 0u;
   int cnt = 0;
   const int64_t id = row_entries(tids + r * K, tlp ? tlp + r * K : nullptr, K, P.V, s_col, s_lp, s_raw, cnt);
-  if (id == kRowLive) {
-    for (int i = threadIdx.x; i < (per + 31) / 32; i += kFwdThreads) s_map[i] = 0u;
-    __syncthreads();
-    if (threadIdx.x < cnt) {
-      const int j = (s_col[threadIdx.x] + rv.shift) >> 3;
-      if (j >= j0 && j < j1) atomicOr(&s_map[(j - j0) >> 5], 1u << ((j - j0) & 31));
-    }
-    if (C > 1) cluster.sync();  // the first block's s_x and s_part exist before others write them
-    else __syncthreads();
-    float* x_dst = C > 1 ? cluster.map_shared_rank(s_x, 0) : s_x;
+  if (threadIdx.x < cnt) mark_entry(p, s_col[threadIdx.x], s_map);
+  if (C > 1) cluster.sync();  // the first block's s_x and s_part exist before others write them
+  else __syncthreads();
+  const RowEntries e{s_col, cnt, s_map, C > 1 ? cluster.map_shared_rank(s_x, 0) : s_x};
 
-    float m = -INFINITY, s = 0.f, sum = 0.f;
-    for (int jb = j0; jb < j1; jb += U * kFwdThreads) {
-      Group8<T> g[U];
-      const int n = min(U, (j1 - jb + kFwdThreads - 1) / kFwdThreads);  // groups a thread, at most
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * kFwdThreads + threadIdx.x;
-        if (j < j1) load_group(g[u], rv, j);
-        else g[u].fill();
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * kFwdThreads + threadIdx.x;
-        if (j >= j1) continue;
-        const int v0 = rv.first(j);
-        if constexpr (SUM) {
-          float x[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = g[u].get(k);
-          if (!rv.whole(j)) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (v0 + k < 0 || v0 + k >= P.V) x[k] = 0.f;
-          }
-          sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-        }
-        if ((s_map[(j - j0) >> 5] >> ((j - j0) & 31)) & 1u) {
-          int lo = 0, hi = cnt;  // first entry at or after this group
-          while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_col[mid] < v0) lo = mid + 1;
-            else hi = mid;
-          }
-          for (; lo < cnt && s_col[lo] < v0 + 8; ++lo) x_dst[lo] = g[u].take(s_col[lo] - v0);
-        }
-      }
-      online_groups<T, U>(g, n, P.c, m, s);
-    }
-    block_online_merge(P.c, m, s, s_red);
-    if constexpr (SUM) {
-      float v[1] = {sum};
-      __syncthreads();
-      block_sum<float, 1>(v, s_red);
-      sum = v[0];
-    }
-    if (threadIdx.x == 0) {
-      float* part = C > 1 ? cluster.map_shared_rank(&s_part[0][0], 0) : &s_part[0][0];
-      part[rank] = m;
-      part[8 + rank] = s;
-      part[16 + rank] = sum;
-    }
-    if (C > 1) cluster.sync();
-    else __syncthreads();
+  float m = -INFINITY, s = 0.f, sum = 0.f;
+  sum_part<T, U, SUM>(g, p, e, P.c, m, s, sum);
+  block_online_merge(P.c, m, s, s_red);
+  if constexpr (SUM) {
+    float v[1] = {sum};
+    __syncthreads();
+    block_sum<float, 1>(v, s_red);
+    sum = v[0];
   }
+  if (threadIdx.x == 0) {
+    float* part = C > 1 ? cluster.map_shared_rank(&s_part[0][0], 0) : &s_part[0][0];
+    part[rank] = m;
+    part[kMaxParts + rank] = s;
+    part[2 * kMaxParts + rank] = sum;
+  }
+  if (C > 1) cluster.sync();
+  else __syncthreads();
   if (rank != 0) return;
   if (threadIdx.x < K) st.cols[r * K + threadIdx.x] = s_col[threadIdx.x];
   if (threadIdx.x == 0) st.row_ids[r] = id;
   if (threadIdx.x < 32) {
-    float m = -INFINITY, s = 0.f, sum = 0.f;
-    if (id == kRowLive) {
-      for (int q = 0; q < C; ++q) {
-        online_merge(P.c, m, s, s_part[0][q], s_part[1][q]);
-        sum += s_part[2][q];
-      }
+    m = -INFINITY;
+    s = sum = 0.f;
+    for (int q = 0; q < C; ++q) {
+      online_merge(P.c, m, s, s_part[0][q], s_part[1][q]);
+      sum += s_part[2][q];
     }
     row_loss(P, id, cnt, s_x, s_lp, m, s, sum, loss + r, st.ref + r, st.coef + r, st.grad + r * K);
   }
 }
 
-// dlogits = g (coef 2^(c (x - ref)) + level) over the row, then g grad_k over its entries (written
-// by the same block behind a barrier).  A block takes a part of one row, U groups a thread at a time;
-// rows without a gradient are zeros and read nothing.
+// Many rows: the sums between row_entries_kernel and row_losses_kernel, one block a part of a row.
+// Rows without entries are not read.
+template <typename T, bool SUM, int U, int MINB>
+__global__ void __launch_bounds__(kFwdThreads, MINB) row_sums_kernel(const T* __restrict__ logits, int64_t ld,
+                                                                     int segs, int K, float c, int V, RowState st,
+                                                                     int64_t N) {
+  extern __shared__ uint32_t s_map[];
+  __shared__ int s_cols[kMaxEntries];
+  __shared__ float s_red[64], s_sum[32];
+  const int64_t r = blockIdx.x / segs;
+  const int seg = (int)(blockIdx.x - r * segs);
+  const RowPart<T> p(logits, ld, r, V, seg, segs);
+  Group8<T> g[U];
+  if (whole_round<T, U>(p, p.a)) load_round<T, U>(g, p, p.a);  // a row that is not live costs this read
+  const int64_t id = st.row_ids[r];
+  const int col = threadIdx.x < K ? st.cols[r * K + threadIdx.x] : kNoEntry;
+  for (int i = threadIdx.x; i < map_words(p.b - p.a); i += kFwdThreads) s_map[i] = 0u;
+  if (threadIdx.x < K) s_cols[threadIdx.x] = col;
+  if (id != kRowLive) return;
+  __syncthreads();
+  if (col != kNoEntry) mark_entry(p, col, s_map);
+  const int cnt = __syncthreads_count(col != kNoEntry);
+  float m = -INFINITY, s = 0.f, sum = 0.f;
+  sum_part<T, U, SUM>(g, p, RowEntries{s_cols, cnt, s_map, st.xk + r * K}, c, m, s, sum);
+  if constexpr (SUM) {
+    sum = warp_sum(sum);
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
+  }
+  block_online_merge(c, m, s, s_red);
+  if (threadIdx.x < 32) {
+    if constexpr (SUM) sum = warp_sum(threadIdx.x < kFwdThreads / 32 ? s_sum[threadIdx.x] : 0.f);
+    if (threadIdx.x == 0) {
+      st.part[(int64_t)seg * N + r] = m;
+      st.part[((int64_t)kMaxParts + seg) * N + r] = s;
+      if constexpr (SUM) st.part[((int64_t)2 * kMaxParts + seg) * N + r] = sum;
+    }
+  }
+}
+
+// One group of the gradient.
 template <typename T>
-__global__ void __launch_bounds__(kBwdThreads) row_loss_bwd_kernel(const T* __restrict__ logits, int64_t ld, int K,
-                                                                   int V, float c, float level, RowState st,
-                                                                   const float* __restrict__ dloss,
-                                                                   T* __restrict__ dlogits, int64_t ld_out,
-                                                                   int blocks_per_row) {
-  constexpr int U = unroll_of<T>();
-  const int64_t r = blockIdx.x / blocks_per_row;
-  const int seg = (int)(blockIdx.x - r * blocks_per_row);
-  const RowView<T> rv(logits, ld, r, V);
+__device__ __forceinline__ void store_group(T* __restrict__ out, const float (&d)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    st_stream16(out, make_uint4(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]),
+                                pack_bf16x2(d[6], d[7])));
+  } else {
+    st_stream16(out, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]),
+                                __float_as_uint(d[3])));
+    st_stream16(out + 4, make_uint4(__float_as_uint(d[4]), __float_as_uint(d[5]), __float_as_uint(d[6]),
+                                    __float_as_uint(d[7])));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_value(T* out, float d) {
+  if constexpr (sizeof(T) == 2) *out = f32_to_bf16_rn(d);
+  else *out = d;
+}
+
+// dlogits = g (coef 2^(c (x - ref)) + level) over the row, then g grad_k over its entries (written
+// by the same block behind a barrier).  One block a part of a row; rows without a gradient are zeros
+// and read nothing.
+template <typename T, int U, int MINB>
+__global__ void __launch_bounds__(kBwdThreads, MINB) row_loss_bwd_kernel(const T* __restrict__ logits, int64_t ld,
+                                                                         int K, int V, float c, float level,
+                                                                         RowState st, const float* __restrict__ dloss,
+                                                                         T* __restrict__ dlogits, int64_t ld_out,
+                                                                         int segs) {
+  const int64_t r = blockIdx.x / segs;
+  const int seg = (int)(blockIdx.x - r * segs);
+  const RowPart<T> p(logits, ld, r, V, seg, segs);
   T* out = dlogits + r * ld_out;
-  const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
-  const int per = (rv.groups + blocks_per_row - 1) / blocks_per_row;
-  const int j0 = min(seg * per, rv.groups), j1 = min(j0 + per, rv.groups);
   const float g = dloss[r], ref = st.ref[r], coef = st.coef[r];
   const bool skip = st.row_ids[r] == kRowNone || g == 0.f;
+  const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (reinterpret_cast<uintptr_t>(p.rv.row) & 15);
+  if (skip && same) {
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j = p.a + (int)threadIdx.x; j < p.b; j += kBwdThreads) store_group<T>(out + p.rv.first(j), zero);
+    const int j = p.edge(threadIdx.x);
+    if (j >= 0)
+      for (int v = max(p.rv.first(j), 0); v < min(p.rv.first(j) + 8, V); ++v) store_value<T>(out + v, 0.f);
+    return;
+  }
   const float lv = skip ? 0.f : g * level;
   // as in online_groups: one fma an exponent where c ref is finite, its rounding put into the factor
   const bool fma_ok = fabsf(ref) < kFmaLimit;
   const float pt = fma_ok ? ref * c : 0.f;
   const float gc = skip ? 0.f : g * coef * (fma_ok ? exp2f(-fmaf(ref, c, -pt)) : 1.f);
-
-  for (int jb = j0; jb < j1; jb += U * kBwdThreads) {
-    Group8<T> in[U];
-    if (!skip) {
+  if (fma_ok && same) {
+    const uint64_t c2 = pack2(c, c), npt2 = pack2(-pt, -pt), gc2 = pack2(gc, gc), lv2 = pack2(lv, lv);
+    for (int jb = p.a; jb < p.b; jb += U * kBwdThreads) {
+      Group8<T> in[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = jb + u * kBwdThreads + threadIdx.x;
-        if (j < j1) load_group(in[u], rv, j);
+        const int j = jb + u * kBwdThreads + (int)threadIdx.x;
+        if (j < p.b) in[u].load(p.rv.row + p.rv.first(j));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kBwdThreads + (int)threadIdx.x;
+        if (j >= p.b) break;
+        float d[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          unpack2(fma2(gc2, exp2x2(fma2(in[u].get2(k), c2, npt2)), lv2), d[2 * k], d[2 * k + 1]);
+        store_group<T>(out + p.rv.first(j), d);
       }
     }
+    const int j = p.edge(threadIdx.x);
+    if (j >= 0) {
+      Group8<T> e;
+      load_group(e, p.rv, j);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * kBwdThreads + threadIdx.x;
-      if (j >= j1) break;
-      float d[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < 8; ++k) {
+        const int v = p.rv.first(j) + k;
+        if (v >= 0 && v < V) store_value<T>(out + v, fmaf(gc, fast_exp2(fmaf(e.get(k), c, -pt)), lv));
+      }
+    }
+  } else {
+    // outputs placed unlike the inputs, or a tail that holds nothing or the type's lowest values
+    const int lo = max(p.rv.first(p.j0), 0), hi = min(p.rv.first(p.j1), V);
+    for (int v = lo + (int)threadIdx.x; v < hi; v += kBwdThreads) {
+      float d = 0.f;
       if (!skip) {
-        if (fma_ok) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) d[k] = fmaf(gc, fast_exp2(fmaf(in[u].get(k), c, -pt)), lv);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) d[k] = fmaf(gc, fast_exp2((in[u].get(k) - ref) * c), lv);
-        }
+        float x;
+        if constexpr (sizeof(T) == 2) x = bf16_to_f32(p.rv.row[v]);
+        else x = p.rv.row[v];
+        d = fmaf(g * coef, fast_exp2((x - ref) * c), lv);
       }
-      const int v0 = rv.first(j);
-      if (same && rv.whole(j)) {
-        if constexpr (sizeof(T) == 2) {
-          st_stream16(out + v0, make_uint4(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]),
-                                           pack_bf16x2(d[6], d[7])));
-        } else {
-          st_stream16(out + v0, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]),
-                                           __float_as_uint(d[3])));
-          st_stream16(out + v0 + 4, make_uint4(__float_as_uint(d[4]), __float_as_uint(d[5]), __float_as_uint(d[6]),
-                                               __float_as_uint(d[7])));
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (v0 + k < 0 || v0 + k >= V) continue;
-          if constexpr (sizeof(T) == 2) out[v0 + k] = f32_to_bf16_rn(d[k]);
-          else out[v0 + k] = d[k];
-        }
-      }
+      store_value<T>(out + v, d);
     }
   }
   if (skip) return;
   __syncthreads();
-  const int lo = rv.first(j0), hi = rv.first(j1);
+  const int lo = p.rv.first(p.j0), hi = p.rv.first(p.j1);
   for (int e = threadIdx.x; e < K; e += kBwdThreads) {
     const int col = st.cols[r * K + e];
     if (col == kNoEntry || col < lo || col >= hi) continue;
-    const float d = g * st.grad[r * K + e];
-    if constexpr (sizeof(T) == 2) out[col] = f32_to_bf16_rn(d);
-    else out[col] = d;
+    store_value<T>(out + col, g * st.grad[r * K + e]);
   }
 }
 
-// Entries of each row before the LM head's GEMM: one block a row.
-__global__ void __launch_bounds__(kMaxEntries) row_entries_kernel(const int64_t* __restrict__ tids,
-                                                                  const float* __restrict__ tlp, int K, int V,
-                                                                  RowState st) {
+// Entries of each row: one block of at least K threads a row, or one thread for a single target.
+__global__ void row_entries_kernel(const int64_t* __restrict__ tids, const float* __restrict__ tlp, int K, int V,
+                                   RowState st) {
   __shared__ int s_col[kMaxEntries];
   __shared__ __align__(16) int s_raw[kMaxEntries];
   __shared__ float s_lp[kMaxEntries];
   const int64_t r = blockIdx.x;
   int cnt = 0;
-  const int64_t id = row_entries(tids + r * K, tlp ? tlp + r * K : nullptr, K, V, s_col, s_lp, s_raw, cnt);
+  const int64_t id = row_entries(tids + r * K, tlp + r * K, K, V, s_col, s_lp, s_raw, cnt);
   if (threadIdx.x < K) {
     st.cols[r * K + threadIdx.x] = s_col[threadIdx.x];
     st.grad[r * K + threadIdx.x] = s_lp[threadIdx.x];
   }
   if (threadIdx.x == 0) st.row_ids[r] = id;
+}
+
+__global__ void row_targets_kernel(const int64_t* __restrict__ targets, int64_t N, int V, RowState st) {
+  const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= N) return;
+  const int64_t t = targets[r];
+  const bool ok = t >= 0 && t < V;
+  st.cols[r] = ok ? (int)t : kNoEntry;
+  st.row_ids[r] = ok ? kRowLive : (t == -100 ? kRowNone : kRowBad);
 }
 
 // Loss of each row from partial sums: one warp a row.
@@ -254,44 +382,73 @@ __global__ void __launch_bounds__(128) row_losses_kernel(const float* __restrict
   row_loss(P, id, cnt, st.xk + r * K, st.grad + r * K, m, s, sum, loss + r, st.ref + r, st.coef + r, st.grad + r * K);
 }
 
+// Rows up to which a forward is one launch with clusters sharing rows; above, three launches with
+// resident blocks.  At 64 rows of 151936 columns both take about as long.
+constexpr int64_t kFusedRows = 64;
+
 template <typename T>
 int launch_fwd(const void* logits, int64_t ld, const int64_t* tids, const float* tlp, int64_t N, int K,
                const RowLossParams& P, const RowState& st, float* loss, cudaStream_t s) {
-  const int C = row_cluster(N, P.V, kFwdThreads);
-  const int groups = (P.V + 7 + 7) / 8;
-  const size_t smem = (size_t)(((groups + C - 1) / C + 31) / 32) * 4;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(N * C), 1, 1);
-  cfg.blockDim = dim3(kFwdThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   const bool sum = P.loss == ROW_XENT && P.smoothing != 0.f;
-  auto kern = sum ? row_loss_fwd_kernel<T, true> : row_loss_fwd_kernel<T, false>;
-  IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, reinterpret_cast<const T*>(logits), ld, tids, tlp, K, P, st, loss));
-  return check_launch("row_loss_fwd_kernel");
+  const int groups = (P.V + 7 + 7) / 8;
+  const T* x = reinterpret_cast<const T*>(logits);
+  if (N <= kFusedRows) {
+    const int C = row_cluster(N, P.V, kFwdThreads);
+    const size_t smem = (size_t)map_words((groups + C - 1) / C) * 4;
+    auto kern = sum ? row_loss_fwd_kernel<T, true> : row_loss_fwd_kernel<T, false>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(N * C), 1, 1);
+    cfg.blockDim = dim3(kFwdThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, x, ld, tids, tlp, K, P, st, loss));
+    return check_launch("row_loss_fwd_kernel");
+  }
+  int rc = launch_row_entries(tids, tlp, N, K, P, st, s);
+  if (rc) return rc;
+  // Parts of a row.  Three blocks share an SM's 44 GB/s (per ns, of 6.5 TB/s), and a part costs a block
+  // about 2.8 us beside its bytes (4096 rows of 151936 bf16 columns: 218, 258, 316, 420 us in 1, 2, 4, 8
+  // parts), so rows are cut only where the blocks would not come out even otherwise.
+  constexpr int U = unroll_of<T>();
+  const int64_t resident = 3 * kNumSMs;
+  const double row_us = (double)P.V * sizeof(T) * 3.0 / 44e3;
+  int segs = 1;
+  double best = 0.0;
+  for (int q = 1; q <= kMaxParts && (q == 1 || groups / q >= kFwdThreads * U); q *= 2) {
+    const double us = (double)((N * q + resident - 1) / resident) * (row_us / q + 2.8);
+    if (q == 1 || us < best) {
+      best = us;
+      segs = q;
+    }
+  }
+  IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "N=%lld rows of V=%d need too many blocks",
+               (long long)N, P.V);
+  const size_t smem = (size_t)map_words((groups + segs - 1) / segs) * 4;
+  auto kern = sum ? row_sums_kernel<T, true, U, 3> : row_sums_kernel<T, false, U, 3>;
+  kern<<<(unsigned)(N * segs), kFwdThreads, smem, s>>>(x, ld, segs, K, P.c, P.V, st, N);
+  if ((rc = check_launch("row_sums_kernel"))) return rc;
+  const float* part = st.part;
+  return launch_row_losses(part, part + (int64_t)kMaxParts * N, sum ? part + (int64_t)2 * kMaxParts * N : nullptr,
+                           segs, nullptr, N, K, P, st, loss, nullptr, s);
 }
 
 template <typename T>
 int launch_bwd(const void* logits, int64_t ld, int64_t N, int K, int V, float c, float level, const RowState& st,
                const float* dloss, void* dlogits, int64_t ld_out, cudaStream_t s, const char* what) {
   const int groups = (V + 7 + 7) / 8;
-  // Rows are cut so that a block runs a few rounds: its start (the row's scalars, then the first
-  // loads) is paid once for them, while thousands of rows still even out over the SMs.
-  const int per = unroll_of<T>() * kBwdThreads;
-  const int rounds = N >= 8 * kNumSMs ? kBwdRounds : 1;
-  const int bpr = (groups + per * rounds - 1) / (per * rounds);
-  IKRL_REQUIRE(N * bpr <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need too many blocks", what,
+  constexpr int U = unroll_of<T>();
+  const int segs = std::max(1, groups / (kBwdThreads * U * kBwdRounds));
+  IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need too many blocks", what,
                (long long)N, V);
-  row_loss_bwd_kernel<T><<<(unsigned)(N * bpr), kBwdThreads, 0, s>>>(reinterpret_cast<const T*>(logits), ld, K, V, c,
-                                                                     level, st, dloss, reinterpret_cast<T*>(dlogits),
-                                                                     ld_out, bpr);
+  row_loss_bwd_kernel<T, U, 3><<<(unsigned)(N * segs), kBwdThreads, 0, s>>>(
+      reinterpret_cast<const T*>(logits), ld, K, V, c, level, st, dloss, reinterpret_cast<T*>(dlogits), ld_out, segs);
   return check_launch("row_loss_bwd_kernel");
 }
 
@@ -360,7 +517,11 @@ int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossP
 
 int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, const RowLossParams& p,
                        const RowState& st, cudaStream_t s) {
-  row_entries_kernel<<<(unsigned)N, kMaxEntries, 0, s>>>(tids, tlp, K, p.V, st);
+  if (tlp == nullptr) {
+    row_targets_kernel<<<(unsigned)((N + 255) / 256), 256, 0, s>>>(tids, N, p.V, st);
+    return check_launch("row_targets_kernel");
+  }
+  row_entries_kernel<<<(unsigned)N, (unsigned)((K + 31) / 32 * 32), 0, s>>>(tids, tlp, K, p.V, st);
   return check_launch("row_entries_kernel");
 }
 

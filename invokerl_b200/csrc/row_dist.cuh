@@ -19,6 +19,7 @@ namespace ikrl {
 
 constexpr int kMaxEntries = 256;           // entries a row may have
 constexpr int kMaxVocab = 1 << 21;         // columns of the kernels on logits
+constexpr int kMaxParts = 8;               // parts a row of logits may be cut into
 constexpr int kNoEntry = 0x7fffffff;       // pads a row's sorted entry columns
 constexpr double kTailEps = 1.0 / (1 << 20);
 
@@ -53,12 +54,14 @@ struct RowState {
   int* cols;         // [N][K] entry columns ascending, then kNoEntry
   float* grad;       // [N][K] gradient at them (until the loss is formed: the teacher's log-probs)
   float* xk;         // [N][K] logits at them (forward only)
-  float* part;       // [3][N] tail maximum and sum, sum of all logits (forward on logits only)
+  float* part;       // [3][kMaxParts][N] tail maxima and sums, sums of all logits, per part of a row
+                     //     (forward on logits only)
 };
 
 inline size_t row_state_bytes(int64_t N, int K) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
-  return al((size_t)N * 8) + 2 * al((size_t)N * 4) + 3 * al((size_t)N * K * 4) + al((size_t)N * 12);
+  return al((size_t)N * 8) + 2 * al((size_t)N * 4) + 3 * al((size_t)N * K * 4) +
+         al((size_t)N * 12 * kMaxParts);
 }
 
 inline RowState row_state(void* base, int64_t N, int K) {
@@ -96,7 +99,7 @@ int launch_row_losses(const float* part_m, const float* part_s, const float* par
 
 __device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); }
 
-// One row's entries, by a block of at least kMaxEntries threads: columns ascending into s_col
+// One row's entries, by a block of at least K threads: columns ascending into s_col
 // (kNoEntry behind the last) and the teacher's log-probs beside them into s_lp.  An entry counts
 // when its id is >= 0 and its log-prob is not -inf, and a repeated id at its first place only.
 // s_raw: kMaxEntries scratch words, 16-byte aligned.  Returns the row's id; cnt = entries that count.  Every entry counts the

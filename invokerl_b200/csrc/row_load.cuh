@@ -21,12 +21,61 @@ struct RowView {
   __device__ __forceinline__ bool whole(int j) const { return first(j) >= 0 && first(j) + 8 <= V; }
 };
 
+// One part of a row of logits: part `seg` of `segs`, in groups of eight columns.
+template <typename T>
+struct RowPart {
+  RowView<T> rv;
+  int j0, j1;  // its groups
+  int a, b;    // those of them that lie wholly inside the row
+  __device__ __forceinline__ RowPart(const T* base, int64_t ld, int64_t r, int V, int seg, int segs)
+      : rv(base, ld, r, V) {
+    const int per = (rv.groups + segs - 1) / segs;
+    j0 = min(seg * per, rv.groups);
+    j1 = min(j0 + per, rv.groups);
+    a = max(j0, rv.shift > 0 ? 1 : 0);
+    b = max(a, min(j1, (V + rv.shift) >> 3));
+  }
+  __device__ __forceinline__ int group_of(int col) const { return (col + rv.shift) >> 3; }
+  __device__ __forceinline__ const T* at(int j) const { return rv.row + rv.first(j); }
+  // Edge t (0, 1): the group at the front or the back of the part that reaches past the row, or -1.
+  __device__ __forceinline__ int edge(int t) const {
+    return (t == 0 && a > j0) ? j0 : (t == 1 && b < j1 && j1 - 1 >= a) ? j1 - 1 : -1;
+  }
+};
+
+// Two fp32 values in one 64-bit register, and the instructions that work on both at once.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+// 2^v of both.
+__device__ __forceinline__ uint64_t exp2x2(uint64_t v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  return pack2(fast_exp2(lo), fast_exp2(hi));
+}
+
 template <typename T>
 struct Group8;
 template <>
 struct Group8<uint16_t> {
   uint32_t w[4];
   __device__ __forceinline__ float get(int k) const { return (k & 1) ? bf16hi(w[k >> 1]) : bf16lo(w[k >> 1]); }
+  __device__ __forceinline__ uint64_t get2(int k) const { return pack2(bf16lo(w[k]), bf16hi(w[k])); }
   // The largest value, NaN aside (-inf when there is no other).
   __device__ __forceinline__ float max() const {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
@@ -51,6 +100,7 @@ template <>
 struct Group8<float> {
   uint32_t w[8];
   __device__ __forceinline__ float get(int k) const { return __uint_as_float(w[k]); }
+  __device__ __forceinline__ uint64_t get2(int k) const { return pack2(get(2 * k), get(2 * k + 1)); }
   __device__ __forceinline__ float max() const {
     return fmaxf(fmaxf(fmaxf(fmaxf(get(0), get(1)), fmaxf(get(2), get(3))),
                        fmaxf(fmaxf(get(4), get(5)), fmaxf(get(6), get(7)))), -INFINITY);
@@ -118,45 +168,55 @@ __device__ __forceinline__ void load_group(Group8<T>& g, const RowView<T>& rv, i
 // Where |m| is below this, c m is finite and exponents are formed with one fma.
 constexpr float kFmaLimit = 1e37f;
 
-// Running (m, s) over U more groups (the first `n` of them): m the maximum, s the sum of 2^(c (x - m)).
-// One maximum and one rescaling serve all of them; then a value costs its unpacking, an fma, an
-// exponential and an addition.  The fma takes c x from the rounded c m, and what that rounding
-// leaves is multiplied out once per call, so the sum stands relative to m itself.
+// Running (m, s) over U more groups: m the maximum, s the sum of 2^(c (x - m)).  One maximum and one
+// rescaling serve all of them; then two values cost two unpackings, a packed fma, two exponentials and
+// a packed addition.  The fma takes c x from the rounded c m, and what that rounding leaves is
+// multiplied out once per call, so the sum stands relative to m itself.
 //
 // A mask may hold the type's lowest value: there c x passes the range of fp32, so the difference
 // x - m is taken first.  While nothing but -inf was seen the sum is taken from 0, which leaves it 0;
 // NaN and +inf make it NaN.
+// top[u]: the groups' own maxima, NaN aside.
 template <typename T, int U>
-__device__ __forceinline__ void online_groups(const Group8<T> (&g)[U], int n, float c, float& m, float& s) {
-  float mx = g[0].max();
+__device__ __forceinline__ void online_groups(const Group8<T> (&g)[U], float c, float& m, float& s, float (&top)[U]) {
 #pragma unroll
-  for (int u = 1; u < U; ++u)
-    if (u < n) mx = fmaxf(mx, g[u].max());
+  for (int u = 0; u < U; ++u) top[u] = g[u].max();
+  float mx = top[0];
+#pragma unroll
+  for (int u = 1; u < U; ++u) mx = fmaxf(mx, top[u]);
   if (mx > m) {
     s *= fast_exp2((m - mx) * c);
     m = mx;
   }
   if (fabsf(m) < kFmaLimit) {
     const float pt = m * c;
-    float b = 0.f;
+    const uint64_t c2 = pack2(c, c), npt2 = pack2(-pt, -pt);
+    uint64_t b0 = 0, b1 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (u >= n) break;
-      float e[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = fast_exp2(fmaf(g[u].get(k), c, -pt));
-      b += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      for (int k = 0; k < 4; k += 2) {
+        b0 = add2(b0, exp2x2(fma2(g[u].get2(k), c2, npt2)));
+        b1 = add2(b1, exp2x2(fma2(g[u].get2(k + 1), c2, npt2)));
+      }
     }
-    s = fmaf(b, fast_exp2(-fmaf(m, c, -pt)), s);
+    float lo, hi;
+    unpack2(add2(b0, b1), lo, hi);
+    s = fmaf(lo + hi, fast_exp2(-fmaf(m, c, -pt)), s);
   } else {
     const float from = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (u >= n) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += fast_exp2((g[u].get(k) - from) * c);
     }
   }
+}
+
+template <typename T, int U>
+__device__ __forceinline__ void online_groups(const Group8<T> (&g)[U], float c, float& m, float& s) {
+  float top[U];
+  online_groups<T, U>(g, c, m, s, top);
 }
 
 __device__ __forceinline__ void online_merge(float c, float& m, float& s, float m2, float s2) {

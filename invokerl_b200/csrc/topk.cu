@@ -61,12 +61,11 @@ __device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
 
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
-template <typename T>
-__global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int V,
-                                                                     int K, float c, float inv_t,
-                                                                     float* __restrict__ logp,
-                                                                     int64_t* __restrict__ ids) {
-  constexpr int U = sizeof(T) == 2 ? 4 : 2;
+template <typename T, int U, int MINB>
+__global__ void __launch_bounds__(kTopThreads, MINB) logits_topk_kernel(const T* __restrict__ logits, int64_t ld,
+                                                                        int V, int K, float c, float inv_t,
+                                                                        float* __restrict__ logp,
+                                                                        int64_t* __restrict__ ids) {
   constexpr int kRound = U * kTopThreads;
   static_assert(kTopList >= 2 * kRound, "the list holds a round behind its limit");
   __shared__ uint64_t s_buf[kTopBuf];
@@ -76,15 +75,13 @@ __global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t r = blockIdx.x / C;
-  const RowView<T> rv(logits, ld, r, V);
-  const int per = (rv.groups + C - 1) / C;
-  const int j0 = min(rank * per, rv.groups), j1 = min(j0 + per, rv.groups);
-  if (threadIdx.x == 0) s_cnt = s_noted = 0;
-  __syncthreads();
+  const int tid = (int)threadIdx.x;
+  const RowPart<T> p(logits, ld, r, V, rank, C);
 
   float m = -INFINITY, s = 0.f;
-  uint32_t mine = 0;  // the largest value_key this thread saw, NaN aside (0: no column)
-  uint64_t bar = 0;   // keys at or below it are out
+  float mine = -INFINITY;  // the largest value of this thread, NaN aside
+  bool any = false;        // this thread had a column
+  uint64_t bar = 0;        // keys at or below it are out
   float bar_value = -INFINITY;
 
   // Columns of the noted groups above the bar into the buffer.
@@ -98,10 +95,10 @@ __global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __
       auto key_of = [&](int k) {
         return ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
       };
-      if (b + (int)threadIdx.x < n) {
-        const int j = s_list[b + threadIdx.x];
-        load_group(g, rv, j);
-        v0 = rv.first(j);
+      if (b + tid < n) {
+        const int j = s_list[b + tid];
+        load_group(g, p.rv, j);
+        v0 = p.rv.first(j);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (v0 + k >= 0 && v0 + k < V && key_of(k) > bar) pend |= 1u << k;
@@ -123,7 +120,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __
         sort_keys(s_buf, kTopBuf, kTopBuf);
         bar = s_buf[K - 1];
         bar_value = key_value((uint32_t)(bar >> 32));
-        if (threadIdx.x == 0) s_cnt = K;
+        if (tid == 0) s_cnt = K;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (((pend >> k) & 1u) && key_of(k) <= bar) pend &= ~(1u << k);
@@ -131,60 +128,86 @@ __global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __
       }
     }
     __syncthreads();
-    if (threadIdx.x == 0) s_noted = 0;
+    if (tid == 0) s_noted = 0;
     __syncthreads();
   };
+  // Raise the bar to the largest value (16 bits of its key) that at least K threads' maxima reach.
+  auto raise_bar = [&]() {
+    const uint32_t key = any ? value_key(mine) : 0u;
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t cand = t | (1u << bit);
+      if (__syncthreads_count(key >= cand) >= K) t = cand;
+    }
+    const uint64_t found = t > 0 ? ((uint64_t)t << 32) - 1 : 0;  // values equal to it stay in
+    if (found > bar) {
+      bar = found;
+      bar_value = key_value(t);
+    }
+  };
+  // Note a group that reaches the bar; any group once a NaN or +inf came by (s is NaN then).  Returns
+  // whether the list is near its end.
+  auto note = [&](float top, int j) {
+    if (top < bar_value && s == s) return false;
+    const int at = atomicAdd(&s_noted, 1);
+    if (at < kTopList) s_list[at] = j;
+    return at >= kTopList - kRound - 1;
+  };
 
-  int round = 0;
-  for (int jb = j0; jb < j1; jb += kRound, ++round) {
-    Group8<T> g[U];
-    const int n = min(U, (j1 - jb + kTopThreads - 1) / kTopThreads);  // groups a thread, at most
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * kTopThreads + threadIdx.x;
-      if (j < j1) load_group(g[u], rv, j);
-      else g[u].fill();
-    }
-    online_groups<T, U>(g, n, c, m, s);
-    float top[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) top[u] = g[u].max();
-    if ((round & (round + 1)) == 0) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * kTopThreads + threadIdx.x;
-        if (j < j1) mine = max(mine, value_key(top[u]));
-      }
-      // The largest bar, to 16 bits of the key, that at least K threads' maxima reach.
-      uint32_t t = 0;
-      for (int bit = 31; bit >= 16; --bit) {
-        const uint32_t cand = t | (1u << bit);
-        if (__syncthreads_count(mine >= cand) >= K) t = cand;
-      }
-      const uint64_t found = t > 0 ? ((uint64_t)t << 32) - 1 : 0;  // values equal to it stay in
-      if (found > bar) {
-        bar = found;
-        bar_value = key_value(t);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * kTopThreads + threadIdx.x;
-        if (j < j1) mine = max(mine, value_key(top[u]));
-      }
-    }
-    // Note the groups that reach the bar; all of them once a NaN or +inf came by (s is NaN then).
+  // The first sweep assumes that the list holds every noted group, and has no barrier but those of the
+  // bar (after rounds 1, 3, 7, 15, ...).  Where it did not (rising rows, many equal values), a second
+  // sweep looks after every round and works the list off in between.
+  for (bool careful = false;; careful = true) {
+    if (tid == 0) s_cnt = s_noted = 0;
+    m = -INFINITY;
+    s = 0.f;
+    __syncthreads();
     bool full = false;
+    int round = 0, next_bar = 0;
+    int jb = p.a;
+    for (; jb + kRound <= p.b; jb += kRound, ++round) {
+      Group8<T> g[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * kTopThreads + threadIdx.x;
-      if (j < j1 && (!(top[u] < bar_value) || s != s)) {
-        const int at = atomicAdd(&s_noted, 1);
-        s_list[at] = j;
-        full |= at >= kTopList - kRound - 1;
+      for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kTopThreads + tid));
+      float top[U];
+      online_groups<T, U>(g, c, m, s, top);
+      any = true;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mine = fmaxf(mine, top[u]);
+      if (round == next_bar) {
+        raise_bar();
+        next_bar = 2 * next_bar + 2;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        full |= note(top[u], jb + u * kTopThreads + tid);
+      if (careful && __syncthreads_or(full)) {
+        work_off();
+        full = false;
       }
     }
-    if (__syncthreads_or(full)) work_off();
+    // what is left, a group a thread at a time: whole groups, then those that reach past the row
+    auto single = [&](int j) {
+      Group8<T> h[1];
+      float top[1] = {-INFINITY};
+      if (j >= 0) {
+        load_group(h[0], p.rv, j);
+        online_groups<T, 1>(h, c, m, s, top);
+        any = true;
+        mine = fmaxf(mine, top[0]);
+      }
+      if (round++ == 0) raise_bar();
+      if (j >= 0) full |= note(top[0], j);
+      if (careful && __syncthreads_or(full)) {
+        work_off();
+        full = false;
+      }
+    };
+    for (; jb < p.b; jb += kTopThreads) single(jb + tid < p.b ? jb + tid : -1);
+    if (p.a > p.j0 || p.b < p.j1) single(p.edge(kTopThreads - 1 - tid));
+    __syncthreads();
+    if (careful || s_noted <= kTopList) break;
+    __syncthreads();  // s_noted is read before it is cleared
   }
   work_off();
   block_online_merge(c, m, s, s_red);
@@ -232,7 +255,8 @@ int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  IKRL_CUDA(cudaLaunchKernelEx(&cfg, logits_topk_kernel<T>, reinterpret_cast<const T*>(logits), ld, V, K, c, inv_t,
+  auto kern = logits_topk_kernel<T, sizeof(T) == 2 ? 4 : 2, 2>;
+  IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, reinterpret_cast<const T*>(logits), ld, V, K, c, inv_t,
                                logp, ids));
   return check_launch("logits_topk_kernel");
 }

@@ -658,12 +658,13 @@ def _check_xent(label_smoothing: float, z_loss: float) -> tuple[float, float]:
 
 
 def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
-    """[rows, V] view of bf16 or fp32 logits with unit column stride and rows that do not overlap."""
+    """[rows, V] view of bf16 or fp32 logits with unit column stride and rows that do not overlap (the
+    tensor itself where it is one: every view is one more node for autograd)."""
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"expected bfloat16 or float32 logits, got {logits.dtype}")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits of shape {tuple(logits.shape)} have no vocabulary")
-    x = logits.reshape(-1, logits.shape[-1])
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()
     return x
@@ -675,8 +676,10 @@ def _ld(x: torch.Tensor) -> int:
 
 
 def _targets_rows(targets: torch.Tensor, shape) -> torch.Tensor:
-    if tuple(targets.shape) != tuple(shape):
+    if targets.shape != shape:
         raise ValueError(f"targets have shape {tuple(targets.shape)}, expected {tuple(shape)}")
+    if targets.dtype == torch.int64 and targets.dim() == 1 and targets.is_contiguous():
+        return targets
     if targets.is_floating_point() or targets.dtype == torch.bool:
         raise TypeError(f"targets must be whole numbers, got {targets.dtype}")
     return targets.reshape(-1).to(torch.int64).contiguous()
@@ -684,23 +687,33 @@ def _targets_rows(targets: torch.Tensor, shape) -> torch.Tensor:
 
 def _teacher_rows(teacher_ids: torch.Tensor, teacher_log_probs: torch.Tensor, shape):
     """[rows, K] int64 ids and fp32 log-probs of a teacher whose rows have `shape`."""
-    if teacher_ids.shape != teacher_log_probs.shape or tuple(teacher_ids.shape[:-1]) != tuple(shape):
+    if teacher_ids.shape != teacher_log_probs.shape or teacher_ids.shape[:-1] != shape:
         raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_log_probs "
                          f"{tuple(teacher_log_probs.shape)} must both be {tuple(shape)} + (K,)")
-    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
-        raise TypeError(f"teacher_ids must be whole numbers, got {teacher_ids.dtype}")
-    if not teacher_log_probs.is_floating_point():
-        raise TypeError(f"teacher_log_probs must be floating point, got {teacher_log_probs.dtype}")
     K = teacher_ids.shape[-1]
     if not 1 <= K <= N.MAX_ENTRIES:
         raise ValueError(f"K = {K} teacher entries outside 1..{N.MAX_ENTRIES}")
-    return (teacher_ids.reshape(-1, K).to(torch.int64).contiguous(),
-            teacher_log_probs.detach().reshape(-1, K).to(torch.float32).contiguous())
+    lp = teacher_log_probs.detach() if teacher_log_probs.requires_grad else teacher_log_probs
+    if (teacher_ids.dtype == torch.int64 and lp.dtype == torch.float32 and lp.dim() == 2
+            and teacher_ids.is_contiguous() and lp.is_contiguous()):
+        return teacher_ids, lp
+    if teacher_ids.is_floating_point() or teacher_ids.dtype == torch.bool:
+        raise TypeError(f"teacher_ids must be whole numbers, got {teacher_ids.dtype}")
+    if not lp.is_floating_point():
+        raise TypeError(f"teacher_log_probs must be floating point, got {lp.dtype}")
+    return teacher_ids.reshape(-1, K).to(torch.int64).contiguous(), lp.reshape(-1, K).to(torch.float32).contiguous()
+
+
+def _like_rows(loss: torch.Tensor, shape) -> torch.Tensor:
+    return loss if loss.shape == shape else loss.reshape(shape)
 
 
 def _row_state(n_rows: int, K: int, device) -> torch.Tensor:
-    nbytes = int(N.lib().ikrl_row_loss_state_bytes(n_rows, K))
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return torch.empty(N.lib().ikrl_row_loss_state_bytes(n_rows, K), dtype=torch.uint8, device=device)
+
+
+# The calls below pass plain integers (the argument types are declared): a small call's time is mostly
+# this side's.
 
 
 def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -717,8 +730,8 @@ def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple
     log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
     ids = torch.empty(shape, dtype=torch.int64, device=dev)
     with N.on_device(dev):
-        call("ikrl_logits_topk", ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V), i32(k), f32(t),
-             ptr(log_probs), ptr(ids), N.stream_of(dev))
+        call("ikrl_logits_topk", x.data_ptr(), N.dtype_code(x), _ld(x), Nr, V, k, t, log_probs.data_ptr(),
+             ids.data_ptr(), N.stream_handle(dev))
     return log_probs, ids
 
 
@@ -732,13 +745,13 @@ class LogitsRowLoss(torch.autograd.Function):
         K = 1 if teacher_lp is None else ids.shape[1]
         loss = torch.empty(Nr, dtype=torch.float32, device=dev)
         state = _row_state(Nr, K, dev)
-        head = (ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V), ptr(ids))
-        tail = (ptr(loss), ptr(state), sz(state.numel()), N.stream_of(dev))
+        head = (x.data_ptr(), N.dtype_code(x), _ld(x), Nr, V, ids.data_ptr())
+        tail = (loss.data_ptr(), state.data_ptr(), state.numel(), N.stream_handle(dev))
         with N.on_device(dev):
             if teacher_lp is None:
-                call("ikrl_logits_cross_entropy_fwd", *head, f32(smoothing), f32(z), *tail)
+                call("ikrl_logits_cross_entropy_fwd", *head, smoothing, z, *tail)
             else:
-                call("ikrl_logits_distill_fwd", *head, ptr(teacher_lp), i32(K), params, *tail)
+                call("ikrl_logits_distill_fwd", *head, teacher_lp.data_ptr(), K, params, *tail)
         ctx.save_for_backward(x, state)
         ctx.args = (K, params, smoothing, z)
         return loss
@@ -749,15 +762,17 @@ class LogitsRowLoss(torch.autograd.Function):
         x, state = ctx.saved_tensors
         K, params, smoothing, z = ctx.args
         Nr, V = x.shape
-        g = g.float().contiguous()
-        dx = torch.empty(Nr, V, dtype=x.dtype, device=x.device)
-        head = (ptr(x), i32(N.dtype_code(x)), i64(_ld(x)), i64(Nr), i32(V))
-        tail = (ptr(state), sz(state.numel()), ptr(g), ptr(dx), i64(V), N.stream_of(x.device))
-        with N.on_device(x.device):
+        dev = x.device
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
+        dx = torch.empty((Nr, V), dtype=x.dtype, device=dev)
+        head = (x.data_ptr(), N.dtype_code(x), _ld(x), Nr, V)
+        tail = (state.data_ptr(), state.numel(), g.data_ptr(), dx.data_ptr(), V, N.stream_handle(dev))
+        with N.on_device(dev):
             if params is None:
-                call("ikrl_logits_cross_entropy_bwd", *head, f32(smoothing), f32(z), *tail)
+                call("ikrl_logits_cross_entropy_bwd", *head, smoothing, z, *tail)
             else:
-                call("ikrl_logits_distill_bwd", *head, i32(K), params, *tail)
+                call("ikrl_logits_distill_bwd", *head, K, params, *tail)
         return dx, None, None, None, None, None
 
 
@@ -778,7 +793,7 @@ def logits_distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_
     N.require_cuda(logits, teacher_ids, teacher_log_probs)
     x = _logits_rows(logits)
     ids, lp = _teacher_rows(teacher_ids, teacher_log_probs, logits.shape[:-1])
-    return LogitsRowLoss.apply(x, ids, lp, params, 0.0, 0.0).reshape(logits.shape[:-1])
+    return _like_rows(LogitsRowLoss.apply(x, ids, lp, params, 0.0, 0.0), logits.shape[:-1])
 
 
 def logits_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, label_smoothing: float = 0.0,
@@ -789,7 +804,7 @@ def logits_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, label_smoo
     N.require_cuda(logits, targets)
     x = _logits_rows(logits)
     t = _targets_rows(targets, logits.shape[:-1])
-    return LogitsRowLoss.apply(x, t, None, None, label_smoothing, z_loss).reshape(logits.shape[:-1])
+    return _like_rows(LogitsRowLoss.apply(x, t, None, None, label_smoothing, z_loss), logits.shape[:-1])
 
 
 # A head call of up to this many rows keeps all of them in the logit cache (a few dozen MB) without
@@ -807,8 +822,8 @@ def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> L
 
 def _cache_args(cache: LogitCache | None):
     if cache is None:
-        return i64(0), None, None, None
-    return i64(cache.rows), ptr(cache.slot), ptr(cache.q), ptr(cache.m)
+        return 0, None, None, None
+    return cache.rows, cache.slot.data_ptr(), cache.q.data_ptr(), cache.m.data_ptr()
 
 
 class LMHeadRowLoss(torch.autograd.Function):
@@ -826,16 +841,16 @@ class LMHeadRowLoss(torch.autograd.Function):
         cache = None
         if grad_mode and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
             cache = _row_cache(Nr, H, V, dev, chunk_rows)
-        nbytes = int(N.lib().ikrl_lmhead_row_loss_fwd_workspace_bytes(Nr, H, V))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        tail = (ptr(loss), ptr(state), sz(state.numel()), *_cache_args(cache), ptr(ws), sz(nbytes), N.stream_of(dev))
+        ws = torch.empty(N.lib().ikrl_lmhead_row_loss_fwd_workspace_bytes(Nr, H, V), dtype=torch.uint8, device=dev)
+        tail = (loss.data_ptr(), state.data_ptr(), state.numel(), *_cache_args(cache), ws.data_ptr(), ws.numel(),
+                N.stream_handle(dev))
         with N.on_device(dev):
             if teacher_lp is None:
-                call("ikrl_lmhead_cross_entropy_fwd", ptr(hidden), ptr(weight), ptr(ids), i64(Nr), i32(H), i32(V),
-                     f32(smoothing), f32(z), *tail)
+                call("ikrl_lmhead_cross_entropy_fwd", hidden.data_ptr(), weight.data_ptr(), ids.data_ptr(), Nr, H, V,
+                     smoothing, z, *tail)
             else:
-                call("ikrl_lmhead_distill_fwd", ptr(hidden), ptr(weight), ptr(ids), ptr(teacher_lp), i64(Nr), i32(H),
-                     i32(V), i32(K), params, *tail)
+                call("ikrl_lmhead_distill_fwd", hidden.data_ptr(), weight.data_ptr(), ids.data_ptr(),
+                     teacher_lp.data_ptr(), Nr, H, V, K, params, *tail)
         if _CHECK_DEVICE_STATUS:
             lmhead_status(ws)
         ctx.save_for_backward(hidden, weight, state)
@@ -858,19 +873,21 @@ class LMHeadRowLoss(torch.autograd.Function):
         V = weight.shape[0]
         if chunk_rows is None:
             chunk_rows = default_chunk_rows(Nr, V)
-        g = g.float().contiguous()
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
         dh = torch.empty_like(hidden) if want_dh else None
         dw = torch.empty_like(weight) if want_dw else None
-        nbytes = int(N.lib().ikrl_lmhead_row_loss_bwd_workspace_bytes(Nr, H, V, chunk_rows, N.IKRL_DTYPE_BF16, 0))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        head = (ptr(hidden), ptr(weight), i64(Nr), i32(H), i32(V))
-        tail = (ptr(state), sz(state.numel()), ptr(g), i64(chunk_rows), ptr(dh), ptr(dw), i32(N.IKRL_DTYPE_BF16),
-                i32(0), *_cache_args(cache), ptr(ws), sz(nbytes), N.stream_of(dev))
+        ws = torch.empty(N.lib().ikrl_lmhead_row_loss_bwd_workspace_bytes(Nr, H, V, chunk_rows, N.IKRL_DTYPE_BF16, 0),
+                         dtype=torch.uint8, device=dev)
+        head = (hidden.data_ptr(), weight.data_ptr(), Nr, H, V)
+        tail = (state.data_ptr(), state.numel(), g.data_ptr(), chunk_rows, dh.data_ptr() if want_dh else None,
+                dw.data_ptr() if want_dw else None, N.IKRL_DTYPE_BF16, 0, *_cache_args(cache), ws.data_ptr(),
+                ws.numel(), N.stream_handle(dev))
         with N.on_device(dev):
             if params is None:
-                call("ikrl_lmhead_cross_entropy_bwd", *head, f32(smoothing), f32(z), *tail)
+                call("ikrl_lmhead_cross_entropy_bwd", *head, smoothing, z, *tail)
             else:
-                call("ikrl_lmhead_distill_bwd", *head, i32(K), params, *tail)
+                call("ikrl_lmhead_distill_bwd", *head, K, params, *tail)
         if _CHECK_DEVICE_STATUS:
             lmhead_status(ws)
         return dh, dw, *none
@@ -880,8 +897,8 @@ def _head_rows(hidden: torch.Tensor, weight: torch.Tensor):
     """bf16 [rows, H] hidden and [V, H] weight, contiguous."""
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be [..., H] and [V, H]")
-    h = hidden.reshape(-1, hidden.shape[-1]).to(torch.bfloat16).contiguous()
-    return h, weight.to(torch.bfloat16).contiguous()
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+    return h.to(torch.bfloat16).contiguous(), weight.to(torch.bfloat16).contiguous()
 
 
 def lmhead_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
@@ -893,8 +910,8 @@ def lmhead_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
     N.require_cuda(hidden, weight, teacher_ids, teacher_log_probs)
     h, w = _head_rows(hidden, weight)
     ids, lp = _teacher_rows(teacher_ids, teacher_log_probs, hidden.shape[:-1])
-    return LMHeadRowLoss.apply(h, w, ids, lp, params, 0.0, 0.0, chunk_rows,
-                               torch.is_grad_enabled()).reshape(hidden.shape[:-1])
+    loss = LMHeadRowLoss.apply(h, w, ids, lp, params, 0.0, 0.0, chunk_rows, torch.is_grad_enabled())
+    return _like_rows(loss, hidden.shape[:-1])
 
 
 def lmhead_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
@@ -906,5 +923,5 @@ def lmhead_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     N.require_cuda(hidden, weight, targets)
     h, w = _head_rows(hidden, weight)
     t = _targets_rows(targets, hidden.shape[:-1])
-    return LMHeadRowLoss.apply(h, w, t, None, None, label_smoothing, z_loss, chunk_rows,
-                               torch.is_grad_enabled()).reshape(hidden.shape[:-1])
+    loss = LMHeadRowLoss.apply(h, w, t, None, None, label_smoothing, z_loss, chunk_rows, torch.is_grad_enabled())
+    return _like_rows(loss, hidden.shape[:-1])
