@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kBwdThreads, MINB) row_loss_bwd_kernel(const T
 
 // Entries of each row: one block of at least K threads a row, or one thread for a single target.
 __global__ void row_entries_kernel(const int64_t* __restrict__ tids, const float* __restrict__ tlp, int K, int V,
-                                   RowState st) {
+                                   RowState st, int* __restrict__ clear) {
   __shared__ int s_col[kMaxEntries];
   __shared__ __align__(16) int s_raw[kMaxEntries];
   __shared__ float s_lp[kMaxEntries];
@@ -341,10 +341,13 @@ __global__ void row_entries_kernel(const int64_t* __restrict__ tids, const float
     st.grad[r * K + threadIdx.x] = s_lp[threadIdx.x];
   }
   if (threadIdx.x == 0) st.row_ids[r] = id;
+  if (r == 0 && threadIdx.x == 0 && clear != nullptr) *clear = 0;
 }
 
-__global__ void row_targets_kernel(const int64_t* __restrict__ targets, int64_t N, int V, RowState st) {
+__global__ void row_targets_kernel(const int64_t* __restrict__ targets, int64_t N, int V, RowState st,
+                                   int* __restrict__ clear) {
   const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (r == 0 && clear != nullptr) *clear = 0;
   if (r >= N) return;
   const int64_t t = targets[r];
   const bool ok = t >= 0 && t < V;
@@ -352,25 +355,26 @@ __global__ void row_targets_kernel(const int64_t* __restrict__ targets, int64_t 
   st.row_ids[r] = ok ? kRowLive : (t == -100 ? kRowNone : kRowBad);
 }
 
-// Loss of each row from partial sums: one warp a row.
+// Loss of each row from partial sums: WARPS warps a row (they share its partial sums; the first forms the
+// loss), four warps a block.
+template <int WARPS>
 __global__ void __launch_bounds__(128) row_losses_kernel(const float* __restrict__ part_m,
                                                          const float* __restrict__ part_s,
                                                          const float* __restrict__ part_x, int sets,
                                                          const int* __restrict__ pos, int64_t N, int K,
                                                          RowLossParams P, RowState st, float* __restrict__ loss,
                                                          const int* __restrict__ err) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  static_assert(WARPS == 1 || WARPS == 4, "a block's four warps take four rows or one");
+  __shared__ float s_part[3][4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * (4 / WARPS) + (WARPS == 1 ? warp : 0);
   if (r >= N) return;
-  const int lane = threadIdx.x & 31;
   int64_t id = st.row_ids[r];
   if (err != nullptr && *err != 0) id = kRowBad;
-  int cnt = 0;
-  for (int k = lane; k < K; k += 32) cnt += st.cols[r * K + k] != kNoEntry;
-  cnt = warp_sum(cnt);
   float m = -INFINITY, s = 0.f, sum = 0.f;
   if (id == kRowLive) {
     const int64_t at = pos ? pos[r] : r;
-    for (int q = lane; q < sets; q += 32) {
+    for (int q = WARPS == 1 ? lane : (int)threadIdx.x; q < sets; q += 32 * WARPS) {
       online_merge(P.c, m, s, part_m[(int64_t)q * N + at], part_s[(int64_t)q * N + at]);
       if (part_x) sum += part_x[(int64_t)q * N + at];
     }
@@ -379,6 +383,25 @@ __global__ void __launch_bounds__(128) row_losses_kernel(const float* __restrict
   for (int o = 16; o > 0; o >>= 1)
     online_merge(P.c, m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   sum = warp_sum(sum);
+  if constexpr (WARPS == 4) {
+    if (lane == 0) {
+      s_part[0][warp] = m;
+      s_part[1][warp] = s;
+      s_part[2][warp] = sum;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    m = -INFINITY;
+    s = sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      online_merge(P.c, m, s, s_part[0][w], s_part[1][w]);
+      sum += s_part[2][w];
+    }
+  }
+  int cnt = 0;
+  for (int k = lane; k < K; k += 32) cnt += st.cols[r * K + k] != kNoEntry;
+  cnt = warp_sum(cnt);
   row_loss(P, id, cnt, st.xk + r * K, st.grad + r * K, m, s, sum, loss + r, st.ref + r, st.coef + r, st.grad + r * K);
 }
 
@@ -516,19 +539,24 @@ int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossP
 }
 
 int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, const RowLossParams& p,
-                       const RowState& st, cudaStream_t s) {
+                       const RowState& st, cudaStream_t s, int* clear) {
   if (tlp == nullptr) {
-    row_targets_kernel<<<(unsigned)((N + 255) / 256), 256, 0, s>>>(tids, N, p.V, st);
+    row_targets_kernel<<<(unsigned)((N + 255) / 256), 256, 0, s>>>(tids, N, p.V, st, clear);
     return check_launch("row_targets_kernel");
   }
-  row_entries_kernel<<<(unsigned)N, (unsigned)((K + 31) / 32 * 32), 0, s>>>(tids, tlp, K, p.V, st);
+  row_entries_kernel<<<(unsigned)N, (unsigned)((K + 31) / 32 * 32), 0, s>>>(tids, tlp, K, p.V, st, clear);
   return check_launch("row_entries_kernel");
 }
 
 int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const int* pos,
                       int64_t N, int K, const RowLossParams& p, const RowState& st, float* loss, const int* err,
                       cudaStream_t s) {
-  row_losses_kernel<<<(unsigned)((N + 3) / 4), 128, 0, s>>>(part_m, part_s, part_x, sets, pos, N, K, p, st, loss, err);
+  // Few rows come with many sets (a GEMM of one row tile cuts the columns as fine as it can).
+  if (sets > 64 && N <= 4 * kNumSMs)
+    row_losses_kernel<4><<<(unsigned)N, 128, 0, s>>>(part_m, part_s, part_x, sets, pos, N, K, p, st, loss, err);
+  else
+    row_losses_kernel<1><<<(unsigned)((N + 3) / 4), 128, 0, s>>>(part_m, part_s, part_x, sets, pos, N, K, p, st, loss,
+                                                                 err);
   return check_launch("row_losses_kernel");
 }
 

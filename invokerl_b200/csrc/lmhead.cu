@@ -54,7 +54,9 @@ constexpr uint32_t kMnAtomBytes = 64 * BK * 2;  // one 64-wide MN slab of an MN-
 // so the plain forward carries none of the cache's code).
 // EPI_TAIL, EPI_DTAIL: forward and backward of the row losses (row_dist.cuh).  EPI_TAIL leaves each
 // row's entry columns out and keeps the running sum of the others; EPI_DTAIL forms the gradient of the
-// others.  EPI_TAIL_CACHED is EPI_TAIL that fills the logit cache.
+// others.  EPI_TAIL_CACHED is EPI_TAIL that fills the logit cache.  EPI_STORE_TMA is EPI_STORE_BF16 whose
+// blocks leave through TMA stores (the wide kernel only): for short reductions, where writing the output
+// is most of the work.
 enum Epi : int {
   EPI_LSE = 0,
   EPI_DLOGITS = 1,
@@ -63,15 +65,21 @@ enum Epi : int {
   EPI_LSE_CACHED = 4,
   EPI_TAIL = 5,
   EPI_DTAIL = 6,
-  EPI_TAIL_CACHED = 7
+  EPI_TAIL_CACHED = 7,
+  EPI_STORE_TMA = 8
 };
 constexpr bool is_lse(int epi) { return epi == EPI_LSE || epi == EPI_LSE_CACHED; }
 constexpr bool is_dlogits(int epi) { return epi == EPI_DLOGITS || epi == EPI_DTAIL; }
 constexpr bool is_tail(int epi) { return epi == EPI_TAIL || epi == EPI_TAIL_CACHED; }
 constexpr bool is_cached(int epi) { return epi == EPI_LSE_CACHED || epi == EPI_TAIL_CACHED; }
+// Epilogues of the wide kernel that stage 32 x 32 bf16 blocks in shared memory for TMA stores.
+constexpr bool is_staged(int epi) { return is_dlogits(epi) || is_cached(epi) || epi == EPI_STORE_TMA; }
 // The epilogue whose launch rules (pacing, splits) an epilogue follows.
 constexpr int epi_kind(int epi) {
-  return (is_cached(epi) || is_tail(epi)) ? (int)EPI_LSE : (epi == EPI_DTAIL ? (int)EPI_DLOGITS : epi);
+  return (is_cached(epi) || is_tail(epi)) ? (int)EPI_LSE
+         : epi == EPI_DTAIL               ? (int)EPI_DLOGITS
+         : epi == EPI_STORE_TMA           ? (int)EPI_STORE_BF16
+                                          : epi;
 }
 enum F32Mode : int { F32_STORE = 0, F32_ADD = 1, F32_ADD_TO_BF16 = 2 };
 
@@ -190,7 +198,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   int cslot0 = 0;
   if constexpr (is_cached(EPI)) {
     if constexpr (EPI == EPI_TAIL_CACHED) {
-      if (row_ok) cslot = p.row_idx != nullptr ? grow : p.slot[grow];
+      if (row_ok) cslot = (p.row_idx != nullptr || p.slot == nullptr) ? grow : p.slot[grow];
       if (cslot >= p.cache_cap) cslot = -1;
     } else if (row_ok && p.slot != nullptr) {
       cslot = p.slot[grow];
@@ -378,6 +386,22 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
         for (int k = 0; k < 4; ++k)
           if (8 * k < nvalid) st_global_v4(dst + 8 * k, w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
       }
+    } else if constexpr (EPI == EPI_STORE_TMA) {
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+      const uint32_t row_addr = stage_smem + (uint32_t)lane * 64u;
+      const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), pack_bf16x2(v[8 * k], v[8 * k + 1]),
+                     pack_bf16x2(v[8 * k + 2], v[8 * k + 3]), pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
+                     pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tm_store, stage_smem, col0, m0 + q * 32);
+        bulk_commit();
+      }
     } else if constexpr (EPI == EPI_STORE_BF16) {
       if (row_ok) {
         uint32_t w[16];
@@ -483,7 +507,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       }
     }
   }
-  if constexpr (is_dlogits(EPI) || is_cached(EPI)) {
+  if constexpr (is_staged(EPI)) {
     // Every TMA store of this warp has completed before the CTA can exit.
     if (stage_smem != 0 && lane == 0) bulk_wait_all();
     __syncwarp();
@@ -1149,7 +1173,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     // ---------------- epilogue (both CTAs, own 128 rows x 512 columns) ----------------
     const uint32_t af[2] = {smem_u32(&acc_full[0]), smem_u32(&acc_full[1])};
     const uint32_t ae[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
-    const uint32_t stage = ((is_dlogits(EPI) || is_cached(EPI)) && p.ds_tma)
+    const uint32_t stage = (is_staged(EPI) && p.ds_tma)
                                ? smem_base + kWideStages * kWideStageBytes + (uint32_t)(warp - 2) * kDsStageBytes
                                : 0u;
     int jb = 0;
@@ -1357,7 +1381,7 @@ int launch_gemm_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorM
                      int m_tiles, cudaStream_t s) {
   GemmParams p = p_in;
   auto kern = WIDE ? lmhead_gemm_wide_kernel<EPI, A_MN, B_MN> : lmhead_gemm_pair_kernel<EPI, A_MN, B_MN>;
-  p.ds_tma = (WIDE && c != nullptr && (is_dlogits(EPI) || is_cached(EPI))) ? 1 : 0;
+  p.ds_tma = (WIDE && c != nullptr && is_staged(EPI)) ? 1 : 0;
   const uint32_t smem_bytes = WIDE ? (p.ds_tma ? kWideDsSmemBytes : kWideSmemBytes) : kPairSmemBytes;
   IKRL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes));
   IKRL_REQUIRE(p.split_major == 1, IKRL_ERR_UNSUPPORTED, "pair kernel needs a split-major grid");
@@ -1380,7 +1404,7 @@ int launch_gemm_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorM
     int rc = pace_array(&p.lockstep);
     if (rc) return rc;
     IKRL_CUDA(cudaMemsetAsync(p.lockstep, 0, sizeof(unsigned) * (size_t)npairs, s));
-    p.pace_kb = (int)tuning((EPI == EPI_F32 || EPI == EPI_STORE_BF16) ? IKRL_TUNE_PACE_KB_LONG : IKRL_TUNE_PACE_KB);
+    p.pace_kb = (int)tuning((EPI == EPI_F32 || epi_kind(EPI) == EPI_STORE_BF16) ? IKRL_TUNE_PACE_KB_LONG : IKRL_TUNE_PACE_KB);
     p.pace_lag = (int)tuning(IKRL_TUNE_PACE_LAG);
   }
   cudaLaunchConfig_t cfg = {};
@@ -1480,7 +1504,10 @@ struct K1Plan {
 
 K1Plan plan_k1(int epi, int64_t m_tiles, int N, int K, int splits_hint, int nsm) {
   K1Plan pl{};
-  pl.kind = !use_pairs() ? 0 : (use_wide(K) ? 2 : 1);
+  // A row loss of at most 128 rows takes single CTAs: a pair's MMAs would run 256 rows for it, half of
+  // them empty (96 rows x 1024 against 151936 columns: 104 us in 256 x 512 pair tiles, 62 us so).
+  pl.kind = !use_pairs() || ((is_tail(epi) || epi == EPI_DTAIL) && m_tiles == 1) ? 0 : (use_wide(K) ? 2 : 1);
+  if (epi == EPI_STORE_TMA) pl.kind = 2;
   const bool persistent = persistent_pairs();
   const int64_t npairs = std::max(1, nsm / 2);
   if (epi == EPI_STORE_BF16 && pl.kind == 2 && splits_hint <= 0 && persistent && balance_splits_enabled() &&
@@ -1500,6 +1527,8 @@ K1Plan plan_k1(int epi, int64_t m_tiles, int N, int K, int splits_hint, int nsm)
     pl.tiles_per_split = 1;
   } else {
     pl.tiles_per_split = (int)cdiv64(pl.n_tiles, splits_hint);
+    if (pl.kind == 0 && m_tiles == 1 && (is_tail(epi) || epi == EPI_DTAIL))
+      pl.tiles_per_split = (int)cdiv64(pl.n_tiles, nsm);  // one CTA an SM, one round
     if ((is_dlogits(epi) || is_tail(epi)) && pl.kind != 0 && persistent && balance_splits_enabled())
       pl.tiles_per_split = balanced_tiles_per_split(m_tiles, pl.n_tiles, splits_hint, npairs);
   }
@@ -1555,6 +1584,7 @@ int dh_split_k(int64_t m_tiles, int H, int V, int64_t rows, int64_t part_elems, 
 __global__ void splitk_sum_kernel(const float4* __restrict__ part, int64_t n4, int ks, uint2* __restrict__ out) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
     float4 a = part[i];
+#pragma unroll 8
     for (int s = 1; s < ks; ++s) {
       const float4 b = part[(int64_t)s * n4 + i];
       a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
@@ -1593,8 +1623,9 @@ int launch_k1(const CUtensorMap& a_single, const CUtensorMap& b_single, const CU
     }
   }
   if (kind == 2) return launch_gemm_pair<EPI, A_MN, B_MN, true>(a_pair, b_pair, c_store, p, m_tiles, s);
-  if (kind == 1) return launch_gemm_pair<EPI, A_MN, B_MN, false>(a_pair, b_pair, nullptr, p, m_tiles, s);
-  return launch_gemm<EPI, A_MN, B_MN>(a_single, b_single, p, m_tiles, s);
+  if constexpr (EPI == EPI_STORE_TMA) return IKRL_ERR_UNSUPPORTED;  // plan_k1 gives it the wide kernel
+  else if (kind == 1) return launch_gemm_pair<EPI, A_MN, B_MN, false>(a_pair, b_pair, nullptr, p, m_tiles, s);
+  else return launch_gemm<EPI, A_MN, B_MN>(a_single, b_single, p, m_tiles, s);
 }
 
 int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1943,46 +1974,55 @@ __global__ void __launch_bounds__(256) ds_from_cache_kernel(
   }
 }
 
-// The same for a row loss: dS = gs q 2^(c (m - ref)) + level, with the row's scaled upstream and level
-// (row_scale_kernel).  idx null: chunk row k is row c0 + k.  Rows without a slot have no gradient.
+// The same for a row loss: dS = g (coef q 2^(c (m - ref)) + level), then g grad at the row's entries,
+// written behind a barrier by the block that holds their columns.  slot null: row r has slot r; idx null:
+// chunk row k is row c0 + k.  Rows without a gradient (or a slot) are zeros.
 __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
     const uint16_t* __restrict__ cache_q, const float* __restrict__ cache_m, int64_t ld_cache, int n_mchunks,
-    const int* __restrict__ slot, const int* __restrict__ idx, const float* __restrict__ ref_c,
-    const float* __restrict__ gs_c, const float* __restrict__ level_c, float c, int64_t c0, int64_t rows, int V,
-    uint16_t* __restrict__ ds, int64_t ld_ds) {
+    const int* __restrict__ slot, const int* __restrict__ idx, const float* __restrict__ dloss,
+    const int64_t* __restrict__ row_ids, const float* __restrict__ refs, const float* __restrict__ coefs,
+    const int* __restrict__ cols, const float* __restrict__ grads, int K, float level, float c, int64_t c0,
+    int64_t rows, int V, uint16_t* __restrict__ ds, int64_t ld_ds) {
   const int vec = V >> 3;
+  const int jb = blockIdx.x * blockDim.x * kDsUnroll + threadIdx.x;  // gridDim.x covers the columns
   for (int64_t k = blockIdx.y; k < rows; k += gridDim.y) {
-    const int64_t kc = c0 + k;
-    const int64_t sl = slot[idx ? idx[kc] : kc];
-    const float ref = ref_c[kc], gs = gs_c[kc], lv = level_c[kc];
-    const bool on = sl >= 0 && (gs != 0.f || lv != 0.f);
+    const int64_t r = idx ? idx[c0 + k] : c0 + k;
+    const int64_t sl = slot ? slot[r] : r;
+    const float g = dloss[r], ref = refs[r], coef = coefs[r];
+    const bool on = sl >= 0 && g != 0.f && row_ids[r] != kRowNone;
+    const float gs = g * coef, lv = on ? g * level : 0.f;
     const uint16_t* qrow = cache_q + (on ? sl : 0) * ld_cache;
     const float* mrow = cache_m + (on ? sl : 0) * n_mchunks;
     uint16_t* drow = ds + k * ld_ds;
-    for (int jb = blockIdx.x * blockDim.x * kDsUnroll + threadIdx.x; jb < vec;
-         jb += gridDim.x * blockDim.x * kDsUnroll) {
-      uint4 qv[kDsUnroll];
-      float mv[kDsUnroll];
+    uint4 qv[kDsUnroll];
+    float mv[kDsUnroll];
 #pragma unroll
-      for (int u = 0; u < kDsUnroll; ++u) {
-        const int jv = jb + u * (int)blockDim.x;
-        qv[u] = make_uint4(0u, 0u, 0u, 0u);
-        mv[u] = 0.f;
-        if (on && jv < vec) {
-          qv[u] = *reinterpret_cast<const uint4*>(qrow + (jv << 3));
-          mv[u] = mrow[jv >> 2];
-        }
+    for (int u = 0; u < kDsUnroll; ++u) {
+      const int jv = jb + u * (int)blockDim.x;
+      qv[u] = make_uint4(0u, 0u, 0u, 0u);
+      mv[u] = 0.f;
+      if (on && jv < vec) {
+        qv[u] = *reinterpret_cast<const uint4*>(qrow + (jv << 3));
+        mv[u] = mrow[jv >> 2];
       }
+    }
 #pragma unroll
-      for (int u = 0; u < kDsUnroll; ++u) {
-        const int jv = jb + u * (int)blockDim.x;
-        if (jv >= vec) break;
-        const float sc = on ? gs * fast_exp2((mv[u] - ref) * c) : 0.f;
-        const uint32_t w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
-        uint32_t o[4];
+    for (int u = 0; u < kDsUnroll; ++u) {
+      const int jv = jb + u * (int)blockDim.x;
+      if (jv >= vec) break;
+      const float sc = on ? gs * fast_exp2((mv[u] - ref) * c) : 0.f;
+      const uint32_t w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
+      uint32_t o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(fmaf(bf16lo(w[e]), sc, lv), fmaf(bf16hi(w[e]), sc, lv));
-        *reinterpret_cast<uint4*>(drow + (jv << 3)) = make_uint4(o[0], o[1], o[2], o[3]);
+      for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(fmaf(bf16lo(w[e]), sc, lv), fmaf(bf16hi(w[e]), sc, lv));
+      *reinterpret_cast<uint4*>(drow + (jv << 3)) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    __syncthreads();
+    if (on) {
+      const int lo = (int)(blockIdx.x * blockDim.x * kDsUnroll) << 3, hi = lo + ((int)blockDim.x * kDsUnroll << 3);
+      for (int e = threadIdx.x; e < K; e += blockDim.x) {
+        const int col = cols[r * K + e];
+        if (col != kNoEntry && col >= lo && col < hi) drow[col] = f32_to_bf16_rn(g * grads[r * K + e]);
       }
     }
   }
@@ -2153,10 +2193,8 @@ constexpr int64_t kRowLossDense = 256;
 
 // Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums
 // of all logits (up to 3 times the forward's splits, which the balance rule may take), and the
-// numbering of the rows that count with their hidden rows gathered.  Its backward's: the rows' levels
-// behind the backward's own.
+// numbering of the rows that count with their hidden rows gathered.
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-static size_t row_level_bytes(int64_t N) { return align256((size_t)N * 4); }
 struct RowLossFwdLayout {
   size_t pm_off, ps_off, px_off, counts_off, count_off, pos_off, idx_off, hc_off, total;
   int splits;
@@ -2243,6 +2281,28 @@ static int lmhead_fwd_impl(const char* what, const void* hidden, const void* wei
 }
 
 
+// A dW over fewer rows than this is mostly its output: it takes the wide kernel with TMA stores.
+constexpr int64_t kShortDw = 1024;
+
+// K ranges of a dH of one row pair: as many as keep every pair busy (dh_split_k stops at 16, which leaves
+// more than half of them idle at H = 1024), each at least 16 K blocks, as far as the partials fit.
+static int64_t few_rows_part_elems(int64_t N, int H) {
+  return (cdiv64(kNumSMs / 2, cdiv64(H, WN)) + 1) * std::min<int64_t>(N, kRowLossDense) * H;
+}
+static int few_rows_split_k(int H, int V, int64_t rows, int64_t part_elems, int nsm) {
+  if (tuning(IKRL_TUNE_DH_SPLIT_K) >= 0 || !use_pairs() || !use_wide(V) || !persistent_pairs()) return 1;
+  const int64_t pairs = std::max(1, nsm / 2), tiles = cdiv64(H, WN);
+  int64_t ks = std::min(pairs / tiles, cdiv64(V, BK) / 16);
+  ks = std::min(ks, part_elems / (rows * H));
+  return (int)std::max<int64_t>(1, ks);
+}
+
+// Workspace of a row loss's backward behind the backward's own: the partials of a dH of few rows, then the
+// rows' levels.
+static size_t row_loss_bwd_extra(int64_t N, int H) {
+  return (N <= kRowLossDense ? align256((size_t)few_rows_part_elems(N, H) * 4) : 0) + align256((size_t)N * 4);
+}
+
 // A row loss (row_dist.cuh) behind the LM head's backward: the state its forward left, and its level
 // (the constant part of the gradient).
 struct RowLossBwd {
@@ -2250,6 +2310,9 @@ struct RowLossBwd {
   int K;
   float c, level;
   bool all_cached;  // every row that is not kRowNone has a cache slot
+  bool identity;    // row r has slot r
+  float* part;      // fp32 partials of a dH of few rows
+  int64_t part_elems;
 };
 
 // cache_slot / cache_q / cache_m: the logit cache a forward filled (all null: no cache).  Active
@@ -2277,7 +2340,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   IKRL_REQUIRE(lse && dlogp && (dhidden || dweight), IKRL_ERR_INVALID_ARGUMENT,
                "%s: null pointer", what);
   const BwdLayout L = bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
-  const size_t ws_need = L.total + (rl ? row_level_bytes(N) : 0);
+  const size_t ws_need = L.total + (rl ? row_loss_bwd_extra(N, H) : 0);
   IKRL_REQUIRE(ws != nullptr && ws_bytes >= ws_need, IKRL_ERR_WORKSPACE,
                "%s: workspace %zu < %zu bytes", what, ws_bytes, ws_need);
   IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
@@ -2355,9 +2418,9 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   }
 
   float* level = nullptr;
-  if (rl) {
+  if (rl && !(rl->all_cached && cache_slot != nullptr)) {  // what the dS epilogue multiplies and adds
     float* gs = reinterpret_cast<float*>(w + L.gc_off);
-    level = reinterpret_cast<float*>(w + L.total);
+    level = reinterpret_cast<float*>(w + L.total + row_loss_bwd_extra(N, H) - align256((size_t)N * 4));
     row_scale_kernel<<<(unsigned)cdiv64(Nw, 256), 256, 0, s>>>(dlogp, rl->st.row_ids, rl->st.coef, idx_c, Nw,
                                                                rl->level, gs, level);
     if ((rc = check_launch("row_scale_kernel"))) return rc;
@@ -2404,8 +2467,10 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     if (from_cache > 0 && rl) {
       const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
                       (unsigned)std::min<int64_t>(from_cache, 65535));
-      dtail_from_cache_kernel<<<grid, 256, 0, s>>>(cache_q, cache_m, L.lds, (int)cdiv64(V, 32), cache_slot, idx_c,
-                                                   lsesrc, gsrc, level, rl->c, c0, from_cache, V, dS, L.lds);
+      dtail_from_cache_kernel<<<grid, 256, 0, s>>>(
+          cache_q, cache_m, L.lds, (int)cdiv64(V, 32), rl->identity ? nullptr : cache_slot, idx_c, dlogp,
+          rl->st.row_ids, rl->st.ref, rl->st.coef, rl->st.cols, rl->st.grad, rl->K, rl->level, rl->c, c0, from_cache, V,
+          dS, L.lds);
       if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
     } else if (from_cache > 0) {
       const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
@@ -2436,9 +2501,11 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
         if ((rc = launch_k1<EPI_DLOGITS, false, false>(ta, t_w_k, ta, t_w_k2, p, nr_tiles, sp, s, &tds))) return rc;
       }
     }
-    if (rl) {
-      ds_entries_kernel<<<(unsigned)cdiv64(rows * rl->K, 256), 256, 0, s>>>(dlogp, rl->st.cols, rl->st.grad, rl->K,
-                                                                            idx_c, c0, rows, dS, L.lds);
+    if (rl && from_cache < rows) {
+      const int64_t n = rows - from_cache;
+      ds_entries_kernel<<<(unsigned)cdiv64(n * rl->K, 256), 256, 0, s>>>(dlogp, rl->st.cols, rl->st.grad, rl->K, idx_c,
+                                                                         c0 + from_cache, n, dS + from_cache * L.lds,
+                                                                         L.lds);
       if ((rc = check_launch("ds_entries_kernel"))) return rc;
     }
     // 2) dW (+)= dS^T h[chunk]
@@ -2451,7 +2518,12 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       p.err = err;
       const int v_tiles = (int)cdiv64(V, BM);
       const bool last = ci == nchunks - 1;
-      if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32) {
+      if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32 && rl && rows < kShortDw && use_pairs() &&
+          tuning(IKRL_TUNE_WIDE) != 0) {
+        CUtensorMap tc;
+        if ((rc = make_store_tmap(&tc, dweight, H, V, H, "dW store"))) return rc;
+        if ((rc = launch_k1<EPI_STORE_TMA, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s, &tc))) return rc;
+      } else if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32) {
         p.out_bf16 = reinterpret_cast<uint16_t*>(dweight); p.ld_bf16 = H;
         if ((rc = launch_k1<EPI_STORE_BF16, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s))) return rc;
       } else {
@@ -2474,9 +2546,16 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       GemmParams p{};
       p.M = (int)rows; p.N = H; p.K = V;
       p.err = err;
-      const int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm);
+      int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm);
+      float* part = reinterpret_cast<float*>(w + L.part_off);
+      if (rl && rows <= kRowLossDense) {
+        const int few = few_rows_split_k(H, V, rows, rl->part_elems, nsm);
+        if (few > ks) {
+          ks = few;
+          part = rl->part;
+        }
+      }
       if (ks > 1) {
-        float* part = reinterpret_cast<float*>(w + L.part_off);
         p.out_f32 = part; p.ld_f32 = H; p.f32_mode = F32_STORE;
         p.ksplits = ks; p.ks_stride = rows * H;
         if ((rc = launch_k1<EPI_F32, false, true>(ta, t_w_mn, ta, t_w_mn, p, m_tiles, 0, s))) return rc;
@@ -2543,8 +2622,7 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   const RowState st = row_state(state, N, K);
   char* w = reinterpret_cast<char*>(ws);
   int* err = reinterpret_cast<int*>(w);
-  IKRL_CUDA(cudaMemsetAsync(err, 0, sizeof(int), s));
-  if ((rc = launch_row_entries(tids, tlp, N, K, P, st, s))) return rc;
+  if ((rc = launch_row_entries(tids, tlp, N, K, P, st, s, err))) return rc;
   const int vpr = H / 8;
   GemmParams p{};
   if (P.loss == ROW_XENT) {
@@ -2569,7 +2647,9 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   const void* rows_in = hidden;
   const int* pos = nullptr;
   const bool cached = cache.rows > 0;
-  if (L.gather || cached) {
+  // Without gathering and with a slot for every row, row r takes slot r: nothing to number.
+  const bool identity = cached && !L.gather && cache.rows >= N;
+  if (L.gather || (cached && !identity)) {
     int* counts = reinterpret_cast<int*>(w + L.counts_off);
     int* count = reinterpret_cast<int*>(w + L.count_off);
     int* posw = reinterpret_cast<int*>(w + L.pos_off);
@@ -2592,14 +2672,14 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
       p.m_dev = count;
       p.row_idx = idx;
     }
-    if (cached) {
-      p.slot = posw;
-      p.cache_cap = cache.rows;
-      p.cache_q = cache.q;
-      p.cache_m = cache.m;
-      p.ld_cache = cdiv64(V, 64) * 64;
-      p.n_mchunks = (int)cdiv64(V, 32);
-    }
+    p.slot = posw;
+  }
+  if (cached) {
+    p.cache_cap = cache.rows;
+    p.cache_q = cache.q;
+    p.cache_m = cache.m;
+    p.ld_cache = cdiv64(V, 64) * 64;
+    p.n_mchunks = (int)cdiv64(V, 32);
   }
   CUtensorMap ta, tb, tb2, tq;
   if ((rc = make_tmap(&ta, rows_in, H, N, H, BM, "hidden"))) return rc;
@@ -2638,6 +2718,12 @@ static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void*
   rl.c = P.c;
   rl.level = P.loss == ROW_XENT ? -P.smoothing / (float)V : 0.f;
   rl.all_cached = cache.rows >= N;
+  rl.identity = rl.all_cached && N <= kRowLossDense;  // as the forward that filled the cache
+  if (N > 0 && N <= kRowLossDense) {
+    rl.part_elems = few_rows_part_elems(N, H);
+    rl.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) +
+                                       bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total);
+  }
   const bool cached = cache.rows > 0;
   return lmhead_bwd_impl(what, hidden, weight, rl.st.row_ids, rl.st.ref, dloss, N, H, V, 0, chunk_rows, dhidden,
                          dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream,
@@ -2655,7 +2741,7 @@ size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V)
 size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
                                                 int32_t dweight_dtype, int32_t accumulate_dweight) {
   if (N <= 0 || H <= 0 || V <= 0) return 256;
-  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + row_level_bytes(N);
+  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + row_loss_bwd_extra(N, H);
 }
 
 int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,

@@ -85,9 +85,10 @@ int distill_params(const char* what, const ikrl_distill_params* d, int V, int K,
 int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossParams* out);
 
 // The LM head's use of the two kernels in distill.cu: entries before its GEMM, losses after it.
-// tids / tlp: the teacher's [N][K], or targets with K = 1 and tlp null (ROW_XENT).
+// tids / tlp: the teacher's [N][K], or targets with K = 1 and tlp null (ROW_XENT); clear: a word to
+// zero, or null.
 int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, const RowLossParams& p,
-                       const RowState& st, cudaStream_t s);
+                       const RowState& st, cudaStream_t s, int* clear = nullptr);
 // part_m / part_s / part_x: [sets][N] tail maxima, sums of 2^(c (x - max)), plain sums of all logits
 // (part_x null without label smoothing); pos: the place of each row in them, or null: itself; err: an
 // error word that makes every loss NaN, or null.

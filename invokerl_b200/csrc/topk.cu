@@ -39,13 +39,41 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// Sort s[0, n) descending, n a power of two; the keys behind `have` count as 0.
+// Sort s[0, n) descending, n a power of two; the keys behind `have` count as 0.  Bitonic: up to one key a
+// thread, the exchanges inside a warp are shuffles and only those between warps go through memory.
 __device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
-  for (int i = have + threadIdx.x; i < n; i += kTopThreads) s[i] = 0;
+  const int t = (int)threadIdx.x;
+  if (n <= kTopThreads) {
+    uint64_t x = t < have ? s[t] : 0;
+    for (int k = 2; k <= n; k <<= 1) {
+      const bool down = (t & k) == 0;
+      int j = k >> 1;
+      for (; j >= 32; j >>= 1) {
+        __syncthreads();
+        if (t < n) s[t] = x;
+        __syncthreads();
+        if (t < n) {
+          const uint64_t y = s[t ^ j];
+          if (((t & j) == 0) == down ? x < y : x > y) x = y;
+        }
+      }
+      if ((t & ~31) < n) {  // whole warps
+        for (; j > 0; j >>= 1) {
+          const uint64_t y = __shfl_xor_sync(0xffffffffu, x, j);
+          if (((t & j) == 0) == down ? x < y : x > y) x = y;
+        }
+      }
+    }
+    __syncthreads();
+    if (t < n) s[t] = x;
+    __syncthreads();
+    return;
+  }
+  for (int i = have + t; i < n; i += kTopThreads) s[i] = 0;
   __syncthreads();
   for (int k = 2; k <= n; k <<= 1) {
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < (n >> 1); i += kTopThreads) {
+      for (int i = t; i < (n >> 1); i += kTopThreads) {
         const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
         const uint64_t x = s[a], y = s[b];
         const bool down = (a & k) == 0;
@@ -147,8 +175,9 @@ __global__ void __launch_bounds__(kTopThreads, MINB) logits_topk_kernel(const T*
   };
   // Note a group that reaches the bar; any group once a NaN or +inf came by (s is NaN then).  Returns
   // whether the list is near its end.
+  auto below = [&](float top) { return top < bar_value && s == s; };
   auto note = [&](float top, int j) {
-    if (top < bar_value && s == s) return false;
+    if (below(top)) return false;
     const int at = atomicAdd(&s_noted, 1);
     if (at < kTopList) s_list[at] = j;
     return at >= kTopList - kRound - 1;
@@ -172,15 +201,18 @@ __global__ void __launch_bounds__(kTopThreads, MINB) logits_topk_kernel(const T*
       float top[U];
       online_groups<T, U>(g, c, m, s, top);
       any = true;
+      float mx = top[0];
 #pragma unroll
-      for (int u = 0; u < U; ++u) mine = fmaxf(mine, top[u]);
+      for (int u = 1; u < U; ++u) mx = fmaxf(mx, top[u]);
+      mine = fmaxf(mine, mx);
       if (round == next_bar) {
         raise_bar();
         next_bar = 2 * next_bar + 2;
       }
+      if (!below(mx)) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        full |= note(top[u], jb + u * kTopThreads + tid);
+        for (int u = 0; u < U; ++u) full |= note(top[u], jb + u * kTopThreads + tid);
+      }
       if (careful && __syncthreads_or(full)) {
         work_off();
         full = false;
@@ -255,7 +287,7 @@ int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kern = logits_topk_kernel<T, sizeof(T) == 2 ? 4 : 2, 2>;
+  auto kern = logits_topk_kernel<T, sizeof(T) == 2 ? 4 : 2, sizeof(T) == 2 ? 3 : 2>;
   IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, reinterpret_cast<const T*>(logits), ld, V, K, c, inv_t,
                                logp, ids));
   return check_launch("logits_topk_kernel");
