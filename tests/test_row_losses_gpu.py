@@ -489,6 +489,7 @@ def test_head_with_the_logit_cache(n, H, V, slots, loss, monkeypatch):
         t[1::3] = -100
     asked = []
     monkeypatch.setattr(ops, "logit_cache_rows", lambda *a: asked.append(a) or slots)
+    monkeypatch.setattr(ops, "_ROW_CACHE_MIN_HIDDEN", 1)
     if loss == "jsd":
         f, args, kw = ops.lmhead_distill, (ids, lp), dict(kind="jsd", temperature=1.3)
         rows = lambda y: distill_rows(y, ids, lp, "jsd", 0.5, 1.3)  # noqa: E731
