@@ -410,8 +410,8 @@ IKRL_API int ikrl_lmhead_noalloc_status(int32_t* status_out, void* stream);
  * dweight_dtype and accumulation, ikrl_lmhead_status on the workspace).  The [N, V] logits are never
  * in memory.  state: ikrl_row_loss_state_bytes(N, K), K = 1 for the cross entropy, as the forward
  * left it; dloss[N] fp32 is the upstream gradient of the row losses.
- * cache_*: the logit cache of ikrl_lmhead_logprob_fwd_cached (sizes from ikrl_lmhead_cache_row_elems),
- * cache_rows = 0 for none; slots go to the rows that have entries (or a target), in row order.  The
+ * cache_*: a logit cache as ikrl_lmhead_logprob_fwd_cached has it (sizes from
+ * ikrl_lmhead_cache_row_elems; its 16-bit numerators are fp16 here), cache_rows = 0 for none; slots go to the rows that have entries (or a target), in row order.  The
  * backward gets what the forward filled.  Rows without entries are left out of both directions' GEMMs
  * (above 256 rows, where gathering the others pays); up to 256 rows neither direction synchronises. */
 IKRL_API size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V);

@@ -25,6 +25,8 @@
 #include "row_dist.cuh"
 #include "sm100.cuh"
 
+#include <cuda_fp16.h>
+
 #include <atomic>
 #include <mutex>
 #include <vector>
@@ -248,7 +250,18 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   float run_m = -INFINITY, run_s = 0.f, tval = 0.f;
   bool found = false;
 
-  // The numerators v of a chunk whose maximum is cm into the logit cache.
+  // The numerators v of a chunk whose maximum is cm into the logit cache.  They are at most 1: a row
+  // loss keeps them in fp16, whose 11 bits leave the one rounding of dS to bf16 (in bf16 the two
+  // together took dH and dW from 1.4 to 1.55 times the error of a single final rounding); what lies
+  // below 2^-14 of its chunk's maximum loses bits that the sums over the vocabulary do not see.
+  auto pack16 = [](float lo, float hi) -> uint32_t {
+    if constexpr (EPI == EPI_TAIL_CACHED) {
+      const __half2 h = __floats2half2_rn(lo, hi);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      return pack_bf16x2(lo, hi);
+    }
+  };
   auto store_numerators = [&](const float* v, int col0, float cm) {
     if (cache_run) {
       // Consecutive slots: the 32 x 32 block goes out with one TMA store, as the dS blocks do.
@@ -258,9 +271,9 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), pack_bf16x2(v[8 * k], v[8 * k + 1]),
-                     pack_bf16x2(v[8 * k + 2], v[8 * k + 3]), pack_bf16x2(v[8 * k + 4], v[8 * k + 5]),
-                     pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+        st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), pack16(v[8 * k], v[8 * k + 1]),
+                     pack16(v[8 * k + 2], v[8 * k + 3]), pack16(v[8 * k + 4], v[8 * k + 5]),
+                     pack16(v[8 * k + 6], v[8 * k + 7]));
       fence_async_shared();
       __syncwarp();
       if (lane == 0) {
@@ -271,8 +284,8 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       uint16_t* dst = p.cache_q + (int64_t)cslot * p.ld_cache + col0;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        st_global_v4(dst + 8 * k, pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                     pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+        st_global_v4(dst + 8 * k, pack16(v[8 * k], v[8 * k + 1]), pack16(v[8 * k + 2], v[8 * k + 3]),
+                     pack16(v[8 * k + 4], v[8 * k + 5]), pack16(v[8 * k + 6], v[8 * k + 7]));
     }
     if (cslot >= 0) p.cache_m[(int64_t)cslot * p.n_mchunks + (col0 >> 5)] = cm;
   };
@@ -2014,7 +2027,10 @@ __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
       const uint32_t w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
       uint32_t o[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(fmaf(bf16lo(w[e]), sc, lv), fmaf(bf16hi(w[e]), sc, lv));
+      for (int e = 0; e < 4; ++e) {
+        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        o[e] = pack_bf16x2(fmaf(q.x, sc, lv), fmaf(q.y, sc, lv));
+      }
       *reinterpret_cast<uint4*>(drow + (jv << 3)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
     __syncthreads();
