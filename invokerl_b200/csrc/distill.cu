@@ -436,21 +436,9 @@ int launch_fwd(const void* logits, int64_t ld, const int64_t* tids, const float*
   }
   int rc = launch_row_entries(tids, tlp, N, K, P, st, s);
   if (rc) return rc;
-  // Parts of a row.  Three blocks share an SM's 44 GB/s (per ns, of 6.5 TB/s), and a part costs a block
-  // about 2.8 us beside its bytes (4096 rows of 151936 bf16 columns: 218, 258, 316, 420 us in 1, 2, 4, 8
-  // parts), so rows are cut only where the blocks would not come out even otherwise.
   constexpr int U = unroll_of<T>();
-  const int64_t resident = 3 * kNumSMs;
-  const double row_us = (double)P.V * sizeof(T) * 3.0 / 44e3;
-  int segs = 1;
-  double best = 0.0;
-  for (int q = 1; q <= kMaxParts && (q == 1 || groups / q >= kFwdThreads * U); q *= 2) {
-    const double us = (double)((N * q + resident - 1) / resident) * (row_us / q + 2.8);
-    if (q == 1 || us < best) {
-      best = us;
-      segs = q;
-    }
-  }
+  static_assert(kMaxRowParts <= kMaxParts, "the state holds a sum for every part");
+  const int segs = row_parts(N, P.V, sizeof(T), kFwdThreads * U);
   IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "N=%lld rows of V=%d need too many blocks",
                (long long)N, P.V);
   const size_t smem = (size_t)map_words((groups + segs - 1) / segs) * 4;

@@ -3,12 +3,13 @@
 //
 // One pass over the row, bound by HBM.  Beside the running logsumexp, a block notes the groups of
 // eight columns whose maximum reaches a bar, a lower bound of the k-th largest value: the k-th largest
-// of the threads' own maxima so far, found bit by bit with block-wide counts and raised after 1, 2,
-// 4, 8, ... rounds.  With 512 threads that bound is nearly the k-th largest itself, so of V columns in
-// no particular order about k (1 + log2(V / 16384)) are noted.  The noted groups are read again (from
-// L2), their columns above the bar go to a buffer of keys, and the buffer is sorted.  Where a list
-// fills up (rising rows, many equal values) it is worked off, and the keys are cut to the k largest,
-// which raises the bar to the k-th key itself.
+// of the threads' own maxima so far, found bit by bit with block-wide counts and raised after 1, 3,
+// 7, 15, ... rounds of 16384 columns.  With 512 threads that bound is nearly the k-th largest itself,
+// so of V columns in no particular order about k (1 + log2(V / 16384)) groups are noted.  They are read
+// again (from L2), their columns above the last bar go to a buffer of keys, and the buffer is sorted.
+// Where a list does not hold the noted groups (rising rows, many equal values) the row is swept again,
+// working the list off on the way and cutting the keys to the k largest, which raises the bar to the
+// k-th key itself.
 //
 // Order and ties are those of one 64-bit key, the value above the inverted column: larger values
 // first, of equal values the lower column.  Keys are distinct, so the result does not depend on the
@@ -89,168 +90,208 @@ __device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
 
 __device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
-template <typename T, int U, int MINB>
-__global__ void __launch_bounds__(kTopThreads, MINB) logits_topk_kernel(const T* __restrict__ logits, int64_t ld,
-                                                                        int V, int K, float c, float inv_t,
-                                                                        float* __restrict__ logp,
-                                                                        int64_t* __restrict__ ids) {
-  constexpr int kRound = U * kTopThreads;
-  static_assert(kTopList >= 2 * kRound, "the list holds a round behind its limit");
-  __shared__ uint64_t s_buf[kTopBuf];
-  __shared__ int s_list[kTopList];
-  __shared__ float s_red[64], s_part[2][8];
-  __shared__ int s_cnt, s_noted;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t r = blockIdx.x / C;
-  const int tid = (int)threadIdx.x;
-  const RowPart<T> p(logits, ld, r, V, rank, C);
-
-  float m = -INFINITY, s = 0.f;
-  float mine = -INFINITY;  // the largest value of this thread, NaN aside
-  bool any = false;        // this thread had a column
-  uint64_t bar = 0;        // keys at or below it are out
-  float bar_value = -INFINITY;
-
-  // Columns of the noted groups above the bar into the buffer.
-  auto work_off = [&]() {
-    __syncthreads();
-    const int n = s_noted;
-    for (int b = 0; b < n; b += kTopThreads) {
-      Group8<T> g;
-      int v0 = 0;
-      uint32_t pend = 0;
-      auto key_of = [&](int k) {
-        return ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
-      };
-      if (b + tid < n) {
-        const int j = s_list[b + tid];
-        load_group(g, p.rv, j);
-        v0 = p.rv.first(j);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (v0 + k >= 0 && v0 + k < V && key_of(k) > bar) pend |= 1u << k;
-      }
-      while (true) {
-        if (pend) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (!((pend >> k) & 1u)) continue;
-            const int at = atomicAdd(&s_cnt, 1);
-            if (at < kTopBuf) {
-              s_buf[at] = key_of(k);
-              pend &= ~(1u << k);
-            }
-          }
-        }
-        if (!__syncthreads_or(pend != 0)) break;
-        // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
-        sort_keys(s_buf, kTopBuf, kTopBuf);
-        bar = s_buf[K - 1];
-        bar_value = key_value((uint32_t)(bar >> 32));
-        if (tid == 0) s_cnt = K;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (((pend >> k) & 1u) && key_of(k) <= bar) pend &= ~(1u << k);
-        __syncthreads();
-      }
-    }
-    __syncthreads();
-    if (tid == 0) s_noted = 0;
-    __syncthreads();
-  };
-  // Raise the bar to the largest value (16 bits of its key) that at least K threads' maxima reach.
-  auto raise_bar = [&]() {
-    const uint32_t key = any ? value_key(mine) : 0u;
+// The lower bound that decides which groups are noted.
+struct Bar {
+  uint64_t key = 0;  // keys at or below it are out
+  float value = -INFINITY;
+  // To the largest value (16 bits of its key) that at least K threads' maxima reach.
+  __device__ __forceinline__ void raise(bool any, float mine, int K) {
+    const uint32_t key_mine = any ? value_key(mine) : 0u;
     uint32_t t = 0;
     for (int bit = 31; bit >= 16; --bit) {
       const uint32_t cand = t | (1u << bit);
-      if (__syncthreads_count(key >= cand) >= K) t = cand;
+      if (__syncthreads_count(key_mine >= cand) >= K) t = cand;
     }
     const uint64_t found = t > 0 ? ((uint64_t)t << 32) - 1 : 0;  // values equal to it stay in
-    if (found > bar) {
-      bar = found;
-      bar_value = key_value(t);
+    if (found > key) {
+      key = found;
+      value = key_value(t);
     }
-  };
-  // Note a group that reaches the bar; any group once a NaN or +inf came by (s is NaN then).  Returns
-  // whether the list is near its end.
-  auto below = [&](float top) { return top < bar_value && s == s; };
-  auto note = [&](float top, int j) {
-    if (below(top)) return false;
-    const int at = atomicAdd(&s_noted, 1);
-    if (at < kTopList) s_list[at] = j;
-    return at >= kTopList - kRound - 1;
-  };
+  }
+};
 
-  // The first sweep assumes that the list holds every noted group, and has no barrier but those of the
-  // bar (after rounds 1, 3, 7, 15, ...).  Where it did not (rising rows, many equal values), a second
-  // sweep looks after every round and works the list off in between.
+// One sweep of a block over its part: the running sums, the bar, and note(top, j, s) for each group
+// (whose maximum is top), then end_round() by all threads.
+template <typename T, int U, typename Note, typename End>
+__device__ __forceinline__ void sweep_part(const RowPart<T>& p, int K, float c, float& m, float& s, Bar& bar,
+                                           Note note, End end_round) {
+  constexpr int kRound = U * kTopThreads;
+  const int tid = (int)threadIdx.x;
+  float mine = -INFINITY;  // the largest value of this thread, NaN aside
+  bool any = false;        // this thread had a column
+  m = -INFINITY;
+  s = 0.f;
+  int round = 0, next_bar = 0;
+  int jb = p.a;
+  for (; jb + kRound <= p.b; jb += kRound, ++round) {
+    Group8<T> g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kTopThreads + tid));
+    float top[U];
+    online_groups<T, U>(g, c, m, s, top);
+    any = true;
+    float mx = top[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, top[u]);
+    mine = fmaxf(mine, mx);
+    if (round == next_bar) {
+      bar.raise(any, mine, K);
+      next_bar = 2 * next_bar + 2;
+    }
+    // any group counts once a NaN or +inf came by (s is NaN then)
+    if (!(mx < bar.value && s == s)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (!(top[u] < bar.value && s == s)) note(jb + u * kTopThreads + tid);
+    }
+    end_round();
+  }
+  // what is left, a group a thread at a time: whole groups, then those that reach past the row
+  auto single = [&](int j) {
+    Group8<T> h[1];
+    float top[1] = {-INFINITY};
+    if (j >= 0) {
+      load_group(h[0], p.rv, j);
+      online_groups<T, 1>(h, c, m, s, top);
+      any = true;
+      mine = fmaxf(mine, top[0]);
+    }
+    if (round++ == 0) bar.raise(any, mine, K);
+    if (j >= 0 && !(top[0] < bar.value && s == s)) note(j);
+    end_round();
+  };
+  for (; jb < p.b; jb += kTopThreads) single(jb + tid < p.b ? jb + tid : -1);
+  if (p.a > p.j0 || p.b < p.j1) single(p.edge(kTopThreads - 1 - tid));
+}
+
+// Columns of the groups list[0, n) above the bar into the buffer of keys (s_cnt of them).
+template <typename T>
+__device__ __forceinline__ void absorb(const RowView<T>& rv, const int* list, int n, int K, Bar& bar, uint64_t* s_buf,
+                                       int* s_cnt) {
+  const int tid = (int)threadIdx.x;
+  for (int b = 0; b < n; b += kTopThreads) {
+    Group8<T> g;
+    int v0 = 0;
+    uint32_t pend = 0;
+    auto key_of = [&](int k) {
+      return ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
+    };
+    if (b + tid < n) {
+      const int j = list[b + tid];
+      load_group(g, rv, j);
+      v0 = rv.first(j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v0 + k >= 0 && v0 + k < rv.V && key_of(k) > bar.key) pend |= 1u << k;
+    }
+    while (true) {
+      if (pend) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (!((pend >> k) & 1u)) continue;
+          const int at = atomicAdd(s_cnt, 1);
+          if (at < kTopBuf) {
+            s_buf[at] = key_of(k);
+            pend &= ~(1u << k);
+          }
+        }
+      }
+      if (!__syncthreads_or(pend != 0)) break;
+      // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
+      sort_keys(s_buf, kTopBuf, kTopBuf);
+      bar.key = s_buf[K - 1];
+      bar.value = key_value((uint32_t)(bar.key >> 32));
+      if (tid == 0) *s_cnt = K;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (((pend >> k) & 1u) && key_of(k) <= bar.key) pend &= ~(1u << k);
+      __syncthreads();
+    }
+  }
+}
+
+struct TopShared {
+  uint64_t buf[kTopBuf];
+  int list[kTopList];
+  float red[64];
+  int cnt, noted;
+};
+
+// A block's part of a row: its sums and, at the front of sh.buf, its K largest keys (0 behind the last).
+// The first sweep assumes that the list holds every noted group and has no barrier but those of the bar;
+// where it did not, a second one looks after every round and works the list off in between.
+template <typename T, int U>
+__device__ __forceinline__ void part_topk(const RowPart<T>& p, int K, float c, float& m, float& s, TopShared& sh) {
+  constexpr int kRound = U * kTopThreads;
+  static_assert(kTopList >= 2 * kRound, "the list holds a round behind its limit");
+  const int tid = (int)threadIdx.x;
+  Bar bar;
+  auto work_off = [&]() {
+    __syncthreads();
+    absorb(p.rv, sh.list, sh.noted, K, bar, sh.buf, &sh.cnt);
+    __syncthreads();
+    if (tid == 0) sh.noted = 0;
+    __syncthreads();
+  };
   for (bool careful = false;; careful = true) {
-    if (tid == 0) s_cnt = s_noted = 0;
-    m = -INFINITY;
-    s = 0.f;
+    if (tid == 0) sh.cnt = sh.noted = 0;
     __syncthreads();
     bool full = false;
-    int round = 0, next_bar = 0;
-    int jb = p.a;
-    for (; jb + kRound <= p.b; jb += kRound, ++round) {
-      Group8<T> g[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kTopThreads + tid));
-      float top[U];
-      online_groups<T, U>(g, c, m, s, top);
-      any = true;
-      float mx = top[0];
-#pragma unroll
-      for (int u = 1; u < U; ++u) mx = fmaxf(mx, top[u]);
-      mine = fmaxf(mine, mx);
-      if (round == next_bar) {
-        raise_bar();
-        next_bar = 2 * next_bar + 2;
-      }
-      if (!below(mx)) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) full |= note(top[u], jb + u * kTopThreads + tid);
-      }
-      if (careful && __syncthreads_or(full)) {
-        work_off();
-        full = false;
-      }
-    }
-    // what is left, a group a thread at a time: whole groups, then those that reach past the row
-    auto single = [&](int j) {
-      Group8<T> h[1];
-      float top[1] = {-INFINITY};
-      if (j >= 0) {
-        load_group(h[0], p.rv, j);
-        online_groups<T, 1>(h, c, m, s, top);
-        any = true;
-        mine = fmaxf(mine, top[0]);
-      }
-      if (round++ == 0) raise_bar();
-      if (j >= 0) full |= note(top[0], j);
-      if (careful && __syncthreads_or(full)) {
-        work_off();
-        full = false;
-      }
-    };
-    for (; jb < p.b; jb += kTopThreads) single(jb + tid < p.b ? jb + tid : -1);
-    if (p.a > p.j0 || p.b < p.j1) single(p.edge(kTopThreads - 1 - tid));
+    sweep_part<T, U>(
+        p, K, c, m, s, bar,
+        [&](int j) {
+          const int at = atomicAdd(&sh.noted, 1);
+          if (at < kTopList) sh.list[at] = j;
+          full |= at >= kTopList - kRound - 1;
+        },
+        [&]() {
+          if (careful && __syncthreads_or(full)) {
+            work_off();
+            full = false;
+          }
+        });
     __syncthreads();
-    if (careful || s_noted <= kTopList) break;
-    __syncthreads();  // s_noted is read before it is cleared
+    if (careful || sh.noted <= kTopList) break;
+    __syncthreads();  // noted is read before it is cleared
   }
   work_off();
-  block_online_merge(c, m, s, s_red);
-  const int have = min(s_cnt, kTopBuf);
-  sort_keys(s_buf, have, pow2_at_least(max(have, K)));
+  block_online_merge(c, m, s, sh.red);
+  const int have = min(sh.cnt, kTopBuf);
+  sort_keys(sh.buf, have, pow2_at_least(max(have, K)));
+}
+
+// The K largest keys of a row as its output.
+__device__ __forceinline__ void write_topk(const uint64_t* keys, int K, float m, float s, float inv_t,
+                                           float* __restrict__ logp, int64_t* __restrict__ ids) {
+  const float ls = log2f(s) * kLn2;
+  for (int i = threadIdx.x; i < K; i += kTopThreads) {
+    const uint64_t key = keys[i];
+    const float x = key_value((uint32_t)(key >> 32));
+    logp[i] = (x - m) * inv_t - ls;
+    ids[i] = (int64_t)(0xffffffffu - (uint32_t)key);
+  }
+}
+
+// Few rows: one launch, a cluster of blocks a row (one block when it is short).
+template <typename T, int U>
+__global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                                     int K, float c, float inv_t,
+                                                                     float* __restrict__ logp,
+                                                                     int64_t* __restrict__ ids) {
+  __shared__ TopShared sh;
+  __shared__ float s_part[2][8];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t r = blockIdx.x / C;
+  const RowPart<T> p(logits, ld, r, V, rank, C);
+  float m, s;
+  part_topk<T, U>(p, K, c, m, s, sh);
   if (C > 1) {
     // Every block's K largest go to the first one, behind its own, and are sorted there.
     cluster.sync();
-    uint64_t* dst = cluster.map_shared_rank(s_buf, 0);
+    uint64_t* dst = cluster.map_shared_rank(sh.buf, 0);
     if (rank > 0)
-      for (int i = threadIdx.x; i < K; i += kTopThreads) dst[rank * K + i] = s_buf[i];
+      for (int i = threadIdx.x; i < K; i += kTopThreads) dst[rank * K + i] = sh.buf[i];
     if (threadIdx.x == 0) {
       float* part = cluster.map_shared_rank(&s_part[0][0], 0);
       part[rank] = m;
@@ -258,23 +299,122 @@ __global__ void __launch_bounds__(kTopThreads, MINB) logits_topk_kernel(const T*
     }
     cluster.sync();
     if (rank != 0) return;
-    sort_keys(s_buf, C * K, pow2_at_least(C * K));
+    sort_keys(sh.buf, C * K, pow2_at_least(C * K));
     m = -INFINITY;
     s = 0.f;
     for (int q = 0; q < C; ++q) online_merge(c, m, s, s_part[0][q], s_part[1][q]);
   }
-  const float ls = log2f(s) * kLn2;
-  for (int i = threadIdx.x; i < K; i += kTopThreads) {
-    const uint64_t key = s_buf[i];
-    const float x = key_value((uint32_t)(key >> 32));
-    logp[r * K + i] = (x - m) * inv_t - ls;
-    ids[r * K + i] = (int64_t)(0xffffffffu - (uint32_t)key);
+  write_topk(sh.buf, K, m, s, inv_t, logp + r * K, ids + r * K);
+}
+
+// Many rows: two launches.  The first sweeps parts of rows and leaves, per part, its sums, its bar and the
+// groups it noted; blocks end with the sweep, so the memory never waits for a sort.  The second picks each
+// row's K largest out of the noted groups, all rows at once.
+struct TopNotes {
+  int* list;      // [N parts][kNoteCap]
+  int* count;     // [N parts] noted groups; above kNoteCap: some are missing, the row is swept again
+  uint64_t* bar;  // [N parts]
+  float* part;    // [2][N parts] maxima and sums
+};
+constexpr int kNoteCap = 2048;
+
+inline size_t top_notes_bytes(int64_t parts) {
+  auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
+  return al((size_t)parts * kNoteCap * 4) + al((size_t)parts * 4) + 2 * al((size_t)parts * 8);
+}
+inline TopNotes top_notes(void* ws, int64_t parts) {
+  auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
+  char* p = reinterpret_cast<char*>(ws);
+  TopNotes t;
+  t.list = reinterpret_cast<int*>(p); p += al((size_t)parts * kNoteCap * 4);
+  t.count = reinterpret_cast<int*>(p); p += al((size_t)parts * 4);
+  t.bar = reinterpret_cast<uint64_t*>(p); p += al((size_t)parts * 8);
+  t.part = reinterpret_cast<float*>(p);
+  return t;
+}
+
+template <typename T, int U, int MINB>
+__global__ void __launch_bounds__(kTopThreads, MINB) topk_note_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                                      int K, int segs, float c, int64_t parts,
+                                                                      TopNotes notes) {
+  __shared__ float s_red[64];
+  __shared__ int s_noted;
+  const int64_t q = blockIdx.x, r = q / segs;
+  const RowPart<T> p(logits, ld, r, V, (int)(q - r * segs), segs);
+  if (threadIdx.x == 0) s_noted = 0;
+  __syncthreads();
+  Bar bar;
+  float m, s;
+  int* list = notes.list + q * kNoteCap;
+  sweep_part<T, U>(
+      p, K, c, m, s, bar,
+      [&](int j) {
+        const int at = atomicAdd(&s_noted, 1);
+        if (at < kNoteCap) list[at] = j;
+      },
+      []() {});
+  block_online_merge(c, m, s, s_red);  // its barrier also closes s_noted
+  if (threadIdx.x == 0) {
+    notes.count[q] = s_noted;
+    notes.bar[q] = bar.key;
+    notes.part[q] = m;
+    notes.part[parts + q] = s;
   }
+}
+
+template <typename T, int U>
+__global__ void __launch_bounds__(kTopThreads, 2) topk_select_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                                     int K, int segs, float c, float inv_t,
+                                                                     int64_t parts, TopNotes notes,
+                                                                     float* __restrict__ logp,
+                                                                     int64_t* __restrict__ ids) {
+  __shared__ TopShared sh;
+  const int64_t r = blockIdx.x, q0 = r * segs;
+  float m = -INFINITY, s = 0.f;
+  Bar bar;
+  bool missing = false;
+  for (int q = 0; q < segs; ++q) {
+    online_merge(c, m, s, notes.part[q0 + q], notes.part[parts + q0 + q]);
+    bar.key = max(bar.key, notes.bar[q0 + q]);  // each is below the K-th largest of its part
+    missing |= notes.count[q0 + q] > kNoteCap;
+  }
+  const RowPart<T> p(logits, ld, r, V, 0, 1);
+  if (missing) {
+    part_topk<T, U>(p, K, c, m, s, sh);
+  } else {
+    if (threadIdx.x == 0) sh.cnt = 0;
+    __syncthreads();
+    for (int q = 0; q < segs; ++q)
+      absorb(p.rv, notes.list + (q0 + q) * kNoteCap, notes.count[q0 + q], K, bar, sh.buf, &sh.cnt);
+    __syncthreads();
+    const int have = min(sh.cnt, kTopBuf);
+    sort_keys(sh.buf, have, pow2_at_least(max(have, K)));
+  }
+  write_topk(sh.buf, K, m, s, inv_t, logp + r * K, ids + r * K);
+}
+
+template <typename T> constexpr int top_unroll() { return sizeof(T) == 2 ? 4 : 2; }
+constexpr int64_t kTopFew = 2 * kNumSMs;  // rows up to which one launch with clusters takes them
+
+int top_parts(int64_t N, int V, int dtype) {
+  return dtype == IKRL_DTYPE_BF16 ? row_parts(N, V, 2, kTopThreads * top_unroll<uint16_t>())
+                                  : row_parts(N, V, 4, kTopThreads * top_unroll<float>());
 }
 
 template <typename T>
 int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c, float inv_t, float* logp,
-                int64_t* ids, cudaStream_t s) {
+                int64_t* ids, void* ws, int segs, cudaStream_t s) {
+  constexpr int U = top_unroll<T>();
+  const T* x = reinterpret_cast<const T*>(logits);
+  if (N > kTopFew) {
+    const int64_t parts = N * segs;
+    const TopNotes notes = top_notes(ws, parts);
+    topk_note_kernel<T, U, 3><<<(unsigned)parts, kTopThreads, 0, s>>>(x, ld, V, K, segs, c, parts, notes);
+    int rc = check_launch("topk_note_kernel");
+    if (rc) return rc;
+    topk_select_kernel<T, U><<<(unsigned)N, kTopThreads, 0, s>>>(x, ld, V, K, segs, c, inv_t, parts, notes, logp, ids);
+    return check_launch("topk_select_kernel");
+  }
   const int C = row_cluster(N, V, kTopThreads);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(N * C), 1, 1);
@@ -287,9 +427,8 @@ int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kern = logits_topk_kernel<T, sizeof(T) == 2 ? 4 : 2, sizeof(T) == 2 ? 3 : 2>;
-  IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, reinterpret_cast<const T*>(logits), ld, V, K, c, inv_t,
-                               logp, ids));
+  auto kern = logits_topk_kernel<T, U>;
+  IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, x, ld, V, K, c, inv_t, logp, ids));
   return check_launch("logits_topk_kernel");
 }
 
@@ -298,8 +437,15 @@ int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c
 
 using namespace ikrl;
 
-extern "C" int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V, int32_t K,
-                                float temperature, float* logp, int64_t* ids, void* stream) {
+extern "C" {
+
+size_t ikrl_logits_topk_workspace_bytes(int32_t dtype, int64_t N, int32_t V) {
+  if (N <= kTopFew || V <= 0) return 0;
+  return top_notes_bytes(N * top_parts(N, V, dtype));
+}
+
+int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V, int32_t K,
+                     float temperature, float* logp, int64_t* ids, void* ws, size_t ws_bytes, void* stream) {
   clear_error();
   const char* what = "ikrl_logits_topk";
   int rc = check_logits_arg(what, logits, dtype, ld, N, V);
@@ -312,6 +458,20 @@ extern "C" int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, i
                "%s: temperature %g must be positive and finite", what, (double)temperature);
   if (N == 0) return IKRL_OK;
   IKRL_REQUIRE(logits && logp && ids, IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  return dtype == IKRL_DTYPE_BF16 ? launch_topk<uint16_t>(logits, ld, N, V, K, c, inv_t, logp, ids, as_stream(stream))
-                                  : launch_topk<float>(logits, ld, N, V, K, c, inv_t, logp, ids, as_stream(stream));
+  int segs = 1;
+  if (N > kTopFew) {
+    segs = top_parts(N, V, dtype);
+    IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need too many blocks", what,
+                 (long long)N, V);
+    const size_t need = top_notes_bytes(N * segs);
+    IKRL_REQUIRE(ws != nullptr && ws_bytes >= need, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes,
+                 need);
+    IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
+                 "%s: workspace must be 256-byte aligned", what);
+  }
+  return dtype == IKRL_DTYPE_BF16
+             ? launch_topk<uint16_t>(logits, ld, N, V, K, c, inv_t, logp, ids, ws, segs, as_stream(stream))
+             : launch_topk<float>(logits, ld, N, V, K, c, inv_t, logp, ids, ws, segs, as_stream(stream));
 }
+
+}  // extern "C"

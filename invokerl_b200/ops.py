@@ -736,9 +736,12 @@ def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple
     shape = (*logits.shape[:-1], k)
     log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
     ids = torch.empty(shape, dtype=torch.int64, device=dev)
+    code = N.dtype_code(x)
+    nbytes = N.lib().ikrl_logits_topk_workspace_bytes(code, Nr, V)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with N.on_device(dev):
-        call("ikrl_logits_topk", x.data_ptr(), N.dtype_code(x), _ld(x), Nr, V, k, t, log_probs.data_ptr(),
-             ids.data_ptr(), N.stream_handle(dev))
+        call("ikrl_logits_topk", x.data_ptr(), code, _ld(x), Nr, V, k, t, log_probs.data_ptr(), ids.data_ptr(),
+             ws.data_ptr() if nbytes else None, nbytes, N.stream_handle(dev))
     return log_probs, ids
 
 
