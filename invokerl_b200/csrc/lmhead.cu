@@ -1561,7 +1561,9 @@ constexpr int64_t kSplitKPartElems = 128ll << 20;
 // order.  ks minimises the busiest pair's work plus the partials' HBM write and read (in units of
 // one full-vocabulary 256 x 256 tile), and is taken when that beats the undivided choice of
 // plan_k1 (256 x 512, or 256 x 256 pairs) by 5%.  1 = no split.
-int dh_split_k(int64_t m_tiles, int H, int V, int64_t rows, int64_t part_elems, int nsm) {
+// many: weigh K ranges for launches of more than two rounds of units too (the row losses' rule; 5461 rows x
+// 4096 are 176 units, 2.4 rounds of the pairs: two ranges took 2% off the whole step).
+int dh_split_k(int64_t m_tiles, int H, int V, int64_t rows, int64_t part_elems, int nsm, bool many = false) {
   const int64_t forced = tuning(IKRL_TUNE_DH_SPLIT_K);
   if (forced == 0 || forced == 1) return 1;
   if (!use_pairs() || !use_wide(V) || !persistent_pairs()) return 1;
@@ -1575,7 +1577,7 @@ int dh_split_k(int64_t m_tiles, int H, int V, int64_t rows, int64_t part_elems, 
   const int64_t P = std::max(1, nsm / 2);
   const int64_t m_pairs = (m_tiles + 1) / 2;
   const int64_t U = m_pairs * cdiv64(H, WN);
-  if (U >= 2 * P) return 1;
+  if (U >= (many ? 8 : 2) * P) return 1;
   const double tile_s = 2.0 * BN * BN * (double)V / (1.4e15 / (double)P);  // one tile on one pair
   const double elem_s = 8.0 / 6.0e12;                                       // fp32 written and read
   auto cost = [&](int64_t ks) {
@@ -2562,7 +2564,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       GemmParams p{};
       p.M = (int)rows; p.N = H; p.K = V;
       p.err = err;
-      int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm);
+      int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm, rl != nullptr);
       float* part = reinterpret_cast<float*>(w + L.part_off);
       if (rl && rows <= kRowLossDense) {
         const int few = few_rows_split_k(H, V, rows, rl->part_elems, nsm);

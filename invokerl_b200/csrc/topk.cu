@@ -110,8 +110,9 @@ struct Bar {
   }
 };
 
-// One sweep of a block over its part: the running sums, the bar, and note(top, j, s) for each group
-// (whose maximum is top), then end_round() by all threads.
+// One sweep of a block over its part: the running sums, the bar, and note(j, top) for each group whose
+// maximum `top` reaches it (NaN: the group may hold a NaN), then end_round() by all threads.  The bar is
+// raised once more at the end: what it then leaves of the noted groups is little more than K columns.
 template <typename T, int U, typename Note, typename End>
 __device__ __forceinline__ void sweep_part(const RowPart<T>& p, int K, float c, float& m, float& s, Bar& bar,
                                            Note note, End end_round) {
@@ -142,7 +143,7 @@ __device__ __forceinline__ void sweep_part(const RowPart<T>& p, int K, float c, 
     if (!(mx < bar.value && s == s)) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (!(top[u] < bar.value && s == s)) note(jb + u * kTopThreads + tid);
+        if (!(top[u] < bar.value && s == s)) note(jb + u * kTopThreads + tid, s == s ? top[u] : nan_f32());
     }
     end_round();
   }
@@ -157,11 +158,12 @@ __device__ __forceinline__ void sweep_part(const RowPart<T>& p, int K, float c, 
       mine = fmaxf(mine, top[0]);
     }
     if (round++ == 0) bar.raise(any, mine, K);
-    if (j >= 0 && !(top[0] < bar.value && s == s)) note(j);
+    if (j >= 0 && !(top[0] < bar.value && s == s)) note(j, s == s ? top[0] : nan_f32());
     end_round();
   };
   for (; jb < p.b; jb += kTopThreads) single(jb + tid < p.b ? jb + tid : -1);
   if (p.a > p.j0 || p.b < p.j1) single(p.edge(kTopThreads - 1 - tid));
+  if (round > 2) bar.raise(any, mine, K);
 }
 
 // Columns of the groups list[0, n) above the bar into the buffer of keys (s_cnt of them).
@@ -214,14 +216,16 @@ struct TopShared {
   uint64_t buf[kTopBuf];
   int list[kTopList];
   float red[64];
+  float m, s;
   int cnt, noted;
 };
 
-// A block's part of a row: its sums and, at the front of sh.buf, its K largest keys (0 behind the last).
-// The first sweep assumes that the list holds every noted group and has no barrier but those of the bar;
+// A block's part of a row: its sums and, in sh.buf, keys (their number is returned, at most `limit`) that
+// hold its K largest, in no order.  The first sweep assumes that the list holds every noted group and has no barrier but those of the bar;
 // where it did not, a second one looks after every round and works the list off in between.
 template <typename T, int U>
-__device__ __forceinline__ void part_topk(const RowPart<T>& p, int K, float c, float& m, float& s, TopShared& sh) {
+__device__ __forceinline__ int part_topk(const RowPart<T>& p, int K, float c, int limit, float& m, float& s,
+                                         TopShared& sh) {
   constexpr int kRound = U * kTopThreads;
   static_assert(kTopList >= 2 * kRound, "the list holds a round behind its limit");
   const int tid = (int)threadIdx.x;
@@ -239,7 +243,7 @@ __device__ __forceinline__ void part_topk(const RowPart<T>& p, int K, float c, f
     bool full = false;
     sweep_part<T, U>(
         p, K, c, m, s, bar,
-        [&](int j) {
+        [&](int j, float) {
           const int at = atomicAdd(&sh.noted, 1);
           if (at < kTopList) sh.list[at] = j;
           full |= at >= kTopList - kRound - 1;
@@ -256,19 +260,33 @@ __device__ __forceinline__ void part_topk(const RowPart<T>& p, int K, float c, f
   }
   work_off();
   block_online_merge(c, m, s, sh.red);
+  if (tid == 0) {  // one thread's rounding for all: which thread writes an output depends on timing
+    sh.m = m;
+    sh.s = s;
+  }
+  __syncthreads();
+  m = sh.m;
+  s = sh.s;
   const int have = min(sh.cnt, kTopBuf);
-  sort_keys(sh.buf, have, pow2_at_least(max(have, K)));
+  if (have <= limit) return have;
+  sort_keys(sh.buf, have, pow2_at_least(have));
+  return K;
 }
 
-// The K largest keys of a row as its output.
-__device__ __forceinline__ void write_topk(const uint64_t* keys, int K, float m, float s, float inv_t,
+// The K largest of n keys (n >= K) as a row's output: a key's place is the number of keys above it.
+template <int THREADS>
+__device__ __forceinline__ void write_topk(const uint64_t* keys, int n, int K, float m, float s, float inv_t,
                                            float* __restrict__ logp, int64_t* __restrict__ ids) {
   const float ls = log2f(s) * kLn2;
-  for (int i = threadIdx.x; i < K; i += kTopThreads) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
     const uint64_t key = keys[i];
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) place += keys[j] > key;
+    if (place >= K) continue;
     const float x = key_value((uint32_t)(key >> 32));
-    logp[i] = (x - m) * inv_t - ls;
-    ids[i] = (int64_t)(0xffffffffu - (uint32_t)key);
+    logp[place] = (x - m) * inv_t - ls;
+    ids[place] = (int64_t)(0xffffffffu - (uint32_t)key);
   }
 }
 
@@ -284,34 +302,44 @@ __global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t r = blockIdx.x / C;
   const RowPart<T> p(logits, ld, r, V, rank, C);
+  __shared__ int s_have[8];
   float m, s;
-  part_topk<T, U>(p, K, c, m, s, sh);
+  int have = part_topk<T, U>(p, K, c, kTopBuf / C, m, s, sh);
   if (C > 1) {
-    // Every block's K largest go to the first one, behind its own, and are sorted there.
+    // Every block's keys go to the first one, behind those of the blocks before it.
     cluster.sync();
-    uint64_t* dst = cluster.map_shared_rank(sh.buf, 0);
-    if (rank > 0)
-      for (int i = threadIdx.x; i < K; i += kTopThreads) dst[rank * K + i] = sh.buf[i];
+    if (threadIdx.x < C) cluster.map_shared_rank(s_have, threadIdx.x)[rank] = have;
     if (threadIdx.x == 0) {
       float* part = cluster.map_shared_rank(&s_part[0][0], 0);
       part[rank] = m;
       part[8 + rank] = s;
     }
     cluster.sync();
+    int before = 0, total = 0;
+    for (int q = 0; q < C; ++q) {
+      before += q < rank ? s_have[q] : 0;
+      total += s_have[q];
+    }
+    if (rank > 0) {
+      uint64_t* dst = cluster.map_shared_rank(sh.buf, 0);
+      for (int i = threadIdx.x; i < have; i += kTopThreads) dst[before + i] = sh.buf[i];
+    }
+    cluster.sync();
     if (rank != 0) return;
-    sort_keys(sh.buf, C * K, pow2_at_least(C * K));
+    have = total;
     m = -INFINITY;
     s = 0.f;
     for (int q = 0; q < C; ++q) online_merge(c, m, s, s_part[0][q], s_part[1][q]);
   }
-  write_topk(sh.buf, K, m, s, inv_t, logp + r * K, ids + r * K);
+  write_topk<kTopThreads>(sh.buf, have, K, m, s, inv_t, logp + r * K, ids + r * K);
 }
 
-// Many rows: two launches.  The first sweeps parts of rows and leaves, per part, its sums, its bar and the
-// groups it noted; blocks end with the sweep, so the memory never waits for a sort.  The second picks each
-// row's K largest out of the noted groups, all rows at once.
+// Many rows.  One launch sweeps parts of rows and leaves, per part, its sums, its bar and the groups it
+// noted; blocks end with the sweep, so the memory never waits for a choice.  The next picks each row's K
+// largest out of the noted groups, all rows at once, and a last one takes the rows (hardly any) whose
+// lists did not hold them.
 struct TopNotes {
-  int* list;      // [N parts][kNoteCap]
+  int2* list;     // [N parts][kNoteCap] group and its maximum
   int* count;     // [N parts] noted groups; above kNoteCap: some are missing, the row is swept again
   uint64_t* bar;  // [N parts]
   float* part;    // [2][N parts] maxima and sums
@@ -320,13 +348,13 @@ constexpr int kNoteCap = 2048;
 
 inline size_t top_notes_bytes(int64_t parts) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
-  return al((size_t)parts * kNoteCap * 4) + al((size_t)parts * 4) + 2 * al((size_t)parts * 8);
+  return al((size_t)parts * kNoteCap * 8) + al((size_t)parts * 4) + 2 * al((size_t)parts * 8);
 }
 inline TopNotes top_notes(void* ws, int64_t parts) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   char* p = reinterpret_cast<char*>(ws);
   TopNotes t;
-  t.list = reinterpret_cast<int*>(p); p += al((size_t)parts * kNoteCap * 4);
+  t.list = reinterpret_cast<int2*>(p); p += al((size_t)parts * kNoteCap * 8);
   t.count = reinterpret_cast<int*>(p); p += al((size_t)parts * 4);
   t.bar = reinterpret_cast<uint64_t*>(p); p += al((size_t)parts * 8);
   t.part = reinterpret_cast<float*>(p);
@@ -345,12 +373,12 @@ __global__ void __launch_bounds__(kTopThreads, MINB) topk_note_kernel(const T* _
   __syncthreads();
   Bar bar;
   float m, s;
-  int* list = notes.list + q * kNoteCap;
+  int2* list = notes.list + q * kNoteCap;
   sweep_part<T, U>(
       p, K, c, m, s, bar,
-      [&](int j) {
+      [&](int j, float top) {
         const int at = atomicAdd(&s_noted, 1);
-        if (at < kNoteCap) list[at] = j;
+        if (at < kNoteCap) list[at] = make_int2(j, __float_as_int(top));
       },
       []() {});
   block_online_merge(c, m, s, s_red);  // its barrier also closes s_noted
@@ -362,35 +390,79 @@ __global__ void __launch_bounds__(kTopThreads, MINB) topk_note_kernel(const T* _
   }
 }
 
-template <typename T, int U>
-__global__ void __launch_bounds__(kTopThreads, 2) topk_select_kernel(const T* __restrict__ logits, int64_t ld, int V,
+// A row's K largest out of its noted groups.  Rows with missing groups, or with more columns above the bar
+// than the buffer holds, are left to topk_again_kernel: their first part's count says so.
+constexpr int kSelectThreads = 256;
+constexpr int kSelectBuf = 2048;
+template <typename T>
+__global__ void __launch_bounds__(kSelectThreads) topk_select_kernel(const T* __restrict__ logits, int64_t ld, int V,
                                                                      int K, int segs, float c, float inv_t,
                                                                      int64_t parts, TopNotes notes,
                                                                      float* __restrict__ logp,
                                                                      int64_t* __restrict__ ids) {
-  __shared__ TopShared sh;
+  __shared__ uint64_t s_buf[kSelectBuf];
+  __shared__ int s_cnt;
   const int64_t r = blockIdx.x, q0 = r * segs;
+  if (threadIdx.x == 0) s_cnt = 0;
   float m = -INFINITY, s = 0.f;
-  Bar bar;
+  uint64_t bar = 0;
   bool missing = false;
   for (int q = 0; q < segs; ++q) {
     online_merge(c, m, s, notes.part[q0 + q], notes.part[parts + q0 + q]);
-    bar.key = max(bar.key, notes.bar[q0 + q]);  // each is below the K-th largest of its part
+    bar = max(bar, notes.bar[q0 + q]);  // each is below the K-th largest of its part
     missing |= notes.count[q0 + q] > kNoteCap;
   }
-  const RowPart<T> p(logits, ld, r, V, 0, 1);
   if (missing) {
-    part_topk<T, U>(p, K, c, m, s, sh);
-  } else {
-    if (threadIdx.x == 0) sh.cnt = 0;
-    __syncthreads();
-    for (int q = 0; q < segs; ++q)
-      absorb(p.rv, notes.list + (q0 + q) * kNoteCap, notes.count[q0 + q], K, bar, sh.buf, &sh.cnt);
-    __syncthreads();
-    const int have = min(sh.cnt, kTopBuf);
-    sort_keys(sh.buf, have, pow2_at_least(max(have, K)));
+    if (threadIdx.x == 0) notes.count[q0] = kNoteCap + 1;
+    return;
   }
-  write_topk(sh.buf, K, m, s, inv_t, logp + r * K, ids + r * K);
+  __syncthreads();
+  const RowView<T> rv(logits, ld, r, V);
+  for (int q = 0; q < segs; ++q) {
+    const int n = notes.count[q0 + q];
+    for (int i = threadIdx.x; i < n; i += kSelectThreads) {
+      const int2 note = notes.list[(q0 + q) * kNoteCap + i];
+      const float top = __int_as_float(note.y);
+      if (top == top && value_key(top) < (uint32_t)(bar >> 32)) continue;  // nothing in it above the bar
+      Group8<T> g;
+      load_group(g, rv, note.x);
+      const int v0 = rv.first(note.x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint64_t key = ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
+        if (v0 + k < 0 || v0 + k >= V || key <= bar) continue;
+        const int at = atomicAdd(&s_cnt, 1);
+        if (at < kSelectBuf) s_buf[at] = key;
+      }
+    }
+  }
+  __syncthreads();
+  const int have = s_cnt;
+  if (have > kSelectBuf) {
+    if (threadIdx.x == 0) notes.count[q0] = kNoteCap + 1;
+    return;
+  }
+  write_topk<kSelectThreads>(s_buf, have, K, m, s, inv_t, logp + r * K, ids + r * K);
+}
+
+template <typename T, int U>
+__global__ void __launch_bounds__(kTopThreads, 2) topk_again_kernel(const T* __restrict__ logits, int64_t ld, int64_t N,
+                                                                    int V, int K, int segs, float c, float inv_t,
+                                                                    TopNotes notes, float* __restrict__ logp,
+                                                                    int64_t* __restrict__ ids) {
+  __shared__ TopShared sh;
+  bool any = false;
+  for (int64_t r = blockIdx.x + (int64_t)threadIdx.x * gridDim.x; r < N; r += (int64_t)gridDim.x * kTopThreads)
+    any |= notes.count[r * segs] > kNoteCap;
+  if (!__syncthreads_or(any)) return;
+  for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
+    if (notes.count[r * segs] <= kNoteCap) continue;
+    float m, s;
+    const RowPart<T> p(logits, ld, r, V, 0, 1);
+    const int have = part_topk<T, U>(p, K, c, kTopBuf, m, s, sh);
+    write_topk<kTopThreads>(sh.buf, have, K, m, s, inv_t, logp + r * K, ids + r * K);
+    __syncthreads();
+  }
 }
 
 template <typename T> constexpr int top_unroll() { return sizeof(T) == 2 ? 4 : 2; }
@@ -412,8 +484,10 @@ int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c
     topk_note_kernel<T, U, 3><<<(unsigned)parts, kTopThreads, 0, s>>>(x, ld, V, K, segs, c, parts, notes);
     int rc = check_launch("topk_note_kernel");
     if (rc) return rc;
-    topk_select_kernel<T, U><<<(unsigned)N, kTopThreads, 0, s>>>(x, ld, V, K, segs, c, inv_t, parts, notes, logp, ids);
-    return check_launch("topk_select_kernel");
+    topk_select_kernel<T><<<(unsigned)N, kSelectThreads, 0, s>>>(x, ld, V, K, segs, c, inv_t, parts, notes, logp, ids);
+    if ((rc = check_launch("topk_select_kernel"))) return rc;
+    topk_again_kernel<T, U><<<2 * kNumSMs, kTopThreads, 0, s>>>(x, ld, N, V, K, segs, c, inv_t, notes, logp, ids);
+    return check_launch("topk_again_kernel");
   }
   const int C = row_cluster(N, V, kTopThreads);
   cudaLaunchConfig_t cfg = {};
@@ -461,6 +535,7 @@ int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, i
   int segs = 1;
   if (N > kTopFew) {
     segs = top_parts(N, V, dtype);
+    while (segs * K > kSelectBuf / 2) segs /= 2;  // each part may leave a little more than K keys
     IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need too many blocks", what,
                  (long long)N, V);
     const size_t need = top_notes_bytes(N * segs);

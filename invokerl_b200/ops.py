@@ -728,7 +728,7 @@ def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple
     ids int64 [..., k]), largest first and of equal logits the lower id first, with log-probs of
     softmax(logits / temperature) over the whole vocabulary.  k <= 256; no gradient."""
     dev = N.require_cuda(logits)
-    x = _logits_rows(logits.detach())
+    x = _logits_rows(logits)
     t = _check_temperature(temperature)
     Nr, V = x.shape
     if not 1 <= k <= min(N.MAX_ENTRIES, V):

@@ -670,3 +670,13 @@ def test_teacher_and_student_policies():
     for fsdp, t in ((False, tol), (True, coarse)):
         assert float((losses[fsdp][0][:, 1:].cpu() - want).abs().max()) <= t
         assert float((losses[fsdp][1][:, 1:].cpu() - want_ce).abs().max()) <= t
+
+
+@pytest.mark.parametrize("n,V,k", [(2, 40000, 50), (40, 1500, 12), (400, 20000, 200)])
+def test_topk_repeats_bit_for_bit(n, V, k):
+    """Ids and log-probs do not depend on the order in which columns reach the buffer."""
+    x = torch.randn(n, V, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).to(DEV)
+    lp, ids = ops.logits_topk(x, k, 1.3)
+    for _ in range(5):
+        lp2, ids2 = ops.logits_topk(x, k, 1.3)
+        assert torch.equal(lp, lp2) and torch.equal(ids, ids2)
