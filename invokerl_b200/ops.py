@@ -817,8 +817,8 @@ def logits_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, label_smoo
     return _like_rows(LogitsRowLoss.apply(x, t, None, None, label_smoothing, z_loss), logits.shape[:-1])
 
 
-# A head call of up to this many rows keeps all of them in the logit cache (a few dozen MB) without
-# asking how much memory is free.
+# A head call of up to this many rows keeps all of them in the logit cache, where that takes at most
+# 256 MB, without asking how much memory is free.
 _ROW_CACHE_SMALL = 256
 # The row losses' cache pays from this H on: at 1024 the forward and backward of 16,384 rows, two thirds
 # with targets, took 10.3 ms with it and 11.2 ms without.
@@ -847,7 +847,7 @@ def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> L
     """Logit cache of a row loss's forward under the policy of `set_logit_cache`, or None."""
     if _LOGIT_CACHE["mode"] == "off" or V % 8 or n_rows == 0 or torch.cuda.is_current_stream_capturing():
         return None
-    if n_rows <= _ROW_CACHE_SMALL:
+    if n_rows <= _ROW_CACHE_SMALL and n_rows * V <= 1 << 27:
         return LogitCache(n_rows, V, n_rows, device)
     if H < _ROW_CACHE_MIN_HIDDEN:
         return None

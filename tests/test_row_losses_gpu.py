@@ -255,9 +255,67 @@ def test_losses_on_strided_and_unaligned_logits(dtype):
         flat = (view.reshape(-1, V).cpu(), ids.reshape(-1, 9).cpu(), lp.reshape(-1, 9).cpu(), up.reshape(-1).cpu())
         loss2, d2 = run_distill(flat[0].contiguous(), *flat[1:], kind="jsd")
         # the same arithmetic on other groups of eight: equal up to the order of the sums
-        assert float((loss.reshape(-1) - loss2).abs().max()) <= fp32_tol(V, 9, 20) * 20
+        assert float((loss.detach().reshape(-1) - loss2).abs().max()) <= fp32_tol(V, 9, 20) * 20
         want, dw = loss_and_grad(lambda y: distill_rows(y, flat[1], flat[2], "jsd"), flat[0], flat[3])
         check_grad(d.reshape(-1, V), dw, dtype, grad_scale(*flat), fp32_tol(V, 9, 20))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,ld,off", [(5, 1001, 1040, 0), (70, 1000, 1001, 1), (3, 2049, 2056, 7), (66, 9, 9, 5)])
+def test_losses_on_a_matrix_with_a_row_stride(n, V, ld, off, dtype):
+    """2-D views are taken as they are: rows of any alignment, gradients (dense) aligned otherwise."""
+    x, ids, lp, up = make_rows(n, V, 7, dtype, n + ld)
+    buf = torch.full((n * ld + 16,), 77.0, dtype=dtype, device=DEV)
+    view = buf[off:off + n * ld].view(n, ld)[:, :V]
+    view.copy_(x)
+    xd = view.detach().requires_grad_(True)
+    assert xd.stride(0) == ld
+    t = ids[:, 0]
+    for loss, rows in ((ops.logits_distill(xd, ids.to(DEV), lp.to(DEV), "reverse"),
+                        lambda y: distill_rows(y, ids, lp, "reverse")),
+                       (ops.logits_cross_entropy(xd, t.to(DEV)), lambda y: xent_rows(y, t))):
+        d, = torch.autograd.grad(loss, xd, up.to(DEV))
+        want, dw = loss_and_grad(rows, x, up)
+        span = span_of(x, ids, lp, 1.0)
+        tol = fp32_tol(V, 7, span)
+        check_loss(loss.detach(), want, tol * (1 + span))
+        check_grad(d, dw, dtype, grad_scale(x, ids, lp, up) + up.double().abs()[:, None] * torch.softmax(x.double(), 1),
+                   tol * (1 + span))
+
+
+@pytest.mark.parametrize("n", [3, 80])  # one launch, and three
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_bad_logits_stay_in_their_row(n, bad):
+    x, ids, lp, up = make_rows(n, 3000, 5, torch.float32, 17)
+    ok = torch.arange(n) != 1
+    clean = run_distill(x, ids, lp, up, kind="jsd")
+    for col in (int(ids[1, 2]), [c for c in range(3000) if c not in ids[1].tolist()][1234]):
+        y = x.clone()
+        y[1, col] = bad
+        loss, d = run_distill(y, ids, lp, up, kind="jsd")
+        assert bool(loss[1].isnan()) and bool(d[1].isnan().any())
+        assert torch.equal(loss[ok], clean[0][ok]) and torch.equal(d[ok], clean[1][ok])
+        xd = y.to(DEV).requires_grad_(True)
+        ce = ops.logits_cross_entropy(xd, ids[:, 0].to(DEV), 0.1)
+        assert bool(ce[1].isnan()) and bool(ce[ok].isfinite().all())
+
+
+def test_other_types_of_entries_and_no_grad():
+    x, ids, lp, up = make_rows(4, 300, 6, torch.float32, 18)
+    want, _ = run_distill(x, ids, lp, up)
+    coarse = lp.to(torch.bfloat16)
+    want_coarse, _ = run_distill(x, ids, coarse.float(), up)
+    with torch.no_grad():
+        xd = x.to(DEV)
+        assert torch.equal(ops.logits_distill(xd, ids.to(DEV), lp.to(DEV)), want)
+        assert torch.equal(ops.logits_distill(xd, ids.to(DEV, torch.int32), lp.to(DEV, torch.float64)), want)
+        got = ops.logits_distill(xd, ids.to(DEV).t().contiguous().t(), coarse.to(DEV))
+        assert torch.equal(got, want_coarse)
+        ce = ops.logits_cross_entropy(xd, ids[:, 0].to(DEV, torch.int32))
+        assert torch.equal(ce, ops.logits_cross_entropy(xd, ids[:, 0].to(DEV)))
+    lpg = lp.to(DEV).requires_grad_(True)  # a teacher's log-probs are constants
+    loss = ops.logits_distill(x.to(DEV).requires_grad_(True), ids.to(DEV), lpg)
+    assert torch.autograd.grad(loss.sum(), lpg, allow_unused=True) == (None,)
 
 
 def check_xent(x, t, up, smoothing, z):
@@ -540,6 +598,50 @@ def test_head_in_chunks_one_sided_and_bad_rows():
     got = run_head(ops.lmhead_distill, h, w, up, ids, lp)
     assert bool(got[0][7].isnan()) and int(got[0].isnan().sum()) == 1
     assert bool(got[1].isfinite().all()) and bool(got[2].isfinite().all())
+
+
+def test_head_cache_in_chunks(monkeypatch):
+    h, w, ids, lp, up = make_head(600, 256, 1000, 6, 24)
+    monkeypatch.setattr(ops, "_ROW_CACHE_MIN_HIDDEN", 1)
+    for slots in (600, 300):
+        monkeypatch.setattr(ops, "logit_cache_rows", lambda *a: slots)
+        span = span_of(h.double() @ w.double().t(), ids, lp, 1.0)
+        got = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="reverse", chunk_rows=256)
+        check_head(h, w, up, got, lambda y: distill_rows(y, ids, lp, "reverse"),
+                   lambda x: grad_scale(x, ids, lp, up), 6, span, cached=True)
+
+
+@pytest.mark.parametrize("n", [60, 400])
+def test_head_c_entry_accumulates_an_fp32_dweight(n):
+    """dW added to what is there, in fp32; dH left out; nothing written behind the outputs."""
+    H, V = 128, 600
+    h, w, ids, _, up = make_head(n, H, V, 1, 25)
+    hd, wd, t, upd = h.to(DEV), w.to(DEV), ids[:, 0].contiguous().to(DEV), up.to(DEV)
+    dev = torch.device(DEV)
+    lib, s = N.lib(), N.stream_of(dev)
+    state = ops._row_state(n, 1, dev)
+    loss = torch.full((n + 3,), 7.0, device=DEV)
+    ws = torch.empty(lib.ikrl_lmhead_row_loss_fwd_workspace_bytes(n, H, V), dtype=torch.uint8, device=DEV)
+    none = (N.i64(0), None, None, None)
+    N.call("ikrl_lmhead_cross_entropy_fwd", N.ptr(hd), N.ptr(wd), N.ptr(t), N.i64(n), N.i32(H), N.i32(V), N.f32(0.1),
+           N.f32(0), N.ptr(loss), N.ptr(state), N.sz(state.numel()), *none, N.ptr(ws), N.sz(ws.numel()), s)
+    base = torch.randn(V + 2, H, generator=torch.Generator().manual_seed(1)).to(DEV)
+    acc = base.clone()
+    wb = torch.empty(lib.ikrl_lmhead_row_loss_bwd_workspace_bytes(n, H, V, 0, N.IKRL_DTYPE_F32, 1), dtype=torch.uint8,
+                     device=DEV)
+    for _ in range(2):
+        N.call("ikrl_lmhead_cross_entropy_bwd", N.ptr(hd), N.ptr(wd), N.i64(n), N.i32(H), N.i32(V), N.f32(0.1),
+               N.f32(0), N.ptr(state), N.sz(state.numel()), N.ptr(upd), N.i64(0), None, N.ptr(acc),
+               N.i32(N.IKRL_DTYPE_F32), N.i32(1), *none, N.ptr(wb), N.sz(wb.numel()), s)
+    assert bool((loss[n:] == 7).all()) and torch.equal(acc[V:], base[V:])
+    x = h.double() @ w.double().t()
+    _, ds = loss_and_grad(lambda y: xent_rows(y, ids[:, 0], 0.1), x, up)
+    want = 2 * (ds.t() @ h.double())
+    got = (acc[:V] - base[:V]).double().cpu()
+    # dS rounded to bf16, fp32 sums of n terms and two additions to values of about 1
+    lim = 2 * (2 ** -8 + 8 * n * EPS32) * (ds.abs().t() @ h.double().abs()) + 1e-3 * (ds.abs().t() @ h.double().abs()) \
+        + 4 * EPS32 * (base[:V].double().cpu().abs() + want.abs())
+    assert bool(((got - want).abs() <= lim).all())
 
 
 def test_head_fp32_weight_and_3d_hidden():
