@@ -269,9 +269,9 @@ __global__ void __launch_bounds__(kBwdThreads, MINB) row_loss_bwd_kernel(const T
     return;
   }
   const float lv = skip ? 0.f : g * level;
-  // as in online_groups: one fma an exponent where c ref is finite, its rounding put into the factor
-  const bool fma_ok = fabsf(ref) < kFmaLimit;
-  const float pt = fma_ok ? ref * c : 0.f;
+  // as in online_groups: one fma an exponent where c ref is small enough, its rounding put into the factor
+  const float pt = ref * c;
+  const bool fma_ok = fabsf(pt) < kFmaLimit;
   const float gc = skip ? 0.f : g * coef * (fma_ok ? exp2f(-fmaf(ref, c, -pt)) : 1.f);
   if (fma_ok && same) {
     const uint64_t c2 = pack2(c, c), npt2 = pack2(-pt, -pt), gc2 = pack2(gc, gc), lv2 = pack2(lv, lv);
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kBwdThreads, MINB) row_loss_bwd_kernel(const T
       }
     }
   } else {
-    // outputs placed unlike the inputs, or a tail that holds nothing or the type's lowest values
+    // outputs placed unlike the inputs, or a tail that holds nothing or nothing but masks
     const int lo = max(p.rv.first(p.j0), 0), hi = min(p.rv.first(p.j1), V);
     for (int v = lo + (int)threadIdx.x; v < hi; v += kBwdThreads) {
       float d = 0.f;

@@ -103,8 +103,8 @@ __device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); 
 // One row's entries, by a block of at least K threads: columns ascending into s_col
 // (kNoEntry behind the last) and the teacher's log-probs beside them into s_lp.  An entry counts
 // when its id is >= 0 and its log-prob is not -inf, and a repeated id at its first place only.
-// s_raw: kMaxEntries scratch words, 16-byte aligned.  Returns the row's id; cnt = entries that count.  Every entry counts the
-// smaller columns for its rank, so the order never depends on timing.
+// s_raw: kMaxEntries scratch words, 16-byte aligned.  Returns the row's id; cnt = entries that count.
+// Every entry counts the smaller columns for its rank, so the order never depends on timing.
 __device__ __forceinline__ int64_t row_entries(const int64_t* __restrict__ tids, const float* __restrict__ tlp, int K,
                                                int V, int* s_col, float* s_lp, int* s_raw, int& cnt) {
   if (tlp == nullptr) {  // one target

@@ -165,16 +165,16 @@ __device__ __forceinline__ void load_group(Group8<T>& g, const RowView<T>& rv, i
   }
 }
 
-// Where |m| is below this, c m is finite and exponents are formed with one fma.
-constexpr float kFmaLimit = 1e37f;
+// Below this size of c m its rounding is at most half of one log2 unit, and exponents are formed with one
+// fma from the rounded value.  (At -1e30, a common mask, the rounding alone would be 10^22 units.)
+constexpr float kFmaLimit = 1e7f;
 
 // Running (m, s) over U more groups: m the maximum, s the sum of 2^(c (x - m)).  One maximum and one
 // rescaling serve all of them; then two values cost two unpackings, a packed fma, two exponentials and
 // a packed addition.  The fma takes c x from the rounded c m, and what that rounding leaves is
 // multiplied out once per call, so the sum stands relative to m itself.
 //
-// A mask may hold the type's lowest value: there c x passes the range of fp32, so the difference
-// x - m is taken first.  While nothing but -inf was seen the sum is taken from 0, which leaves it 0;
+// A mask may hold -1e30 or the type's lowest value: there the difference x - m is taken first.  While nothing but -inf was seen the sum is taken from 0, which leaves it 0;
 // NaN and +inf make it NaN.
 // top[u]: the groups' own maxima, NaN aside.
 template <typename T, int U>
@@ -188,8 +188,8 @@ __device__ __forceinline__ void online_groups(const Group8<T> (&g)[U], float c, 
     s *= fast_exp2((m - mx) * c);
     m = mx;
   }
-  if (fabsf(m) < kFmaLimit) {
-    const float pt = m * c;
+  const float pt = m * c;
+  if (fabsf(pt) < kFmaLimit) {
     const uint64_t c2 = pack2(c, c), npt2 = pack2(-pt, -pt);
     uint64_t b0 = 0, b1 = 0;
 #pragma unroll

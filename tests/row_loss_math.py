@@ -29,6 +29,9 @@ def distill_rows(x, ids, lp, kind="forward", beta=0.5, temperature=1.0, tail=Tru
     x = x.double() if x.dtype != torch.float64 else x
     use = entry_mask(ids, lp)
     V = x.shape[1]
+    # Taken off before anything else: a row of -1e30 would swallow the logarithms of its sums.
+    top = x.detach().amax(1)
+    top = torch.where(top.isfinite(), top, 0.0)
     for r in range(x.shape[0]):
         cols, l = ids[r][use[r]], lp[r][use[r]].double()
         if len(cols) == 0:
@@ -37,7 +40,7 @@ def distill_rows(x, ids, lp, kind="forward", beta=0.5, temperature=1.0, tail=Tru
         if int(cols.max()) >= V:
             out.append(x[r].sum() * math.nan)
             continue
-        logp = torch.log_softmax(x[r] / temperature, 0)
+        logp = torch.log_softmax((x[r] - top[r]) / temperature, 0)
         q, lpk = l.exp(), logp[cols]
         if not tail:
             l = l - q.sum().log()
@@ -46,11 +49,16 @@ def distill_rows(x, ids, lp, kind="forward", beta=0.5, temperature=1.0, tail=Tru
             rest = torch.ones(V, dtype=torch.bool, device=x.device)
             rest[cols] = False
             left = 1.0 - q.sum()
-            lpk = torch.cat([lpk, torch.logsumexp(logp[rest], 0)[None]])
+            # from the tail's own maximum: beside a mask of -1e30 even 64 bits lose the logarithm of the sum
+            z = (x[r] - top[r]) / temperature
+            mx = z[rest].detach().max()
+            mx = mx if mx > -math.inf else torch.zeros_like(mx)
+            log_pt = torch.logsumexp(z[rest] - mx, 0) + (mx - torch.logsumexp(z, 0))
+            lpk = torch.cat([lpk, log_pt[None]])
             q = torch.cat([q, torch.where(left >= TAIL_EPS, left, 0.0)[None]])
             l = torch.cat([l, left.clamp(min=TAIL_EPS).log()[None]])
-        # outcomes the student excludes (-inf) have no part in p log p, and no gradient
-        on = lpk > -math.inf
+        # outcomes the student excludes (p is 0, in 64 bits) have no part in p log p, and no gradient
+        on = lpk.exp() > 0
         if kind == "forward":
             on |= q > 0
             out.append((q[on] * (l[on] - lpk[on])).sum())
@@ -76,12 +84,46 @@ def xent_rows(x, targets, label_smoothing=0.0, z_loss=0.0):
         elif not 0 <= t < x.shape[1]:
             out.append(x[r].sum() * math.nan)
         else:
-            lse = torch.logsumexp(x[r], 0)
-            v = lse - x[r, t] + z_loss * lse ** 2
+            top = x[r].detach().max()
+            top = top if bool(top.isfinite()) else torch.zeros_like(top)
+            rel = torch.logsumexp(x[r] - top, 0)
+            v = rel - (x[r, t] - top) + z_loss * (rel + top) ** 2
             if label_smoothing:
                 v = v + label_smoothing * (x[r, t] - x[r].mean())
             out.append(v)
     return torch.stack(out) if out else x.new_zeros(0)
+
+
+def loss_size(x, ids, lp, kind="forward", beta=0.5, temperature=1.0, tail=True):
+    """Per row, the sum of the magnitudes its loss is formed from: each outcome's weight times the logarithms
+    beside it.  An entry at a masked column (log p = -1e9, say) makes a forward loss of that size, whose
+    fp32 terms are off by half steps of that size; in the other losses such an outcome weighs nothing."""
+    V = x.shape[1]
+    logp = torch.log_softmax(x.detach().double() / temperature, 1)
+    use = entry_mask(ids, lp) & (ids < V)
+    out = torch.ones(x.shape[0], dtype=torch.float64)
+    for r in range(x.shape[0]):
+        cols, l = ids[r][use[r]], lp[r][use[r]].double()
+        if len(cols) == 0 or not bool(logp[r].isfinite().any()):
+            continue
+        lpk, q = logp[r, cols], l.exp()
+        rest = torch.ones(V, dtype=torch.bool)
+        rest[cols] = False
+        if tail and bool(rest.any()):
+            left = max(float(1 - q.sum()), TAIL_EPS)
+            lpk = torch.cat([lpk, torch.logsumexp(logp[r, rest], 0)[None]])
+            l = torch.cat([l, torch.tensor([math.log(left)], dtype=torch.float64)])
+            q = l.exp()
+        p = lpk.exp()
+        lpa = lpk.abs().nan_to_num(posinf=0.0)
+        if kind == "forward":
+            out[r] += float((q * (l.abs() + lpa)).sum())
+        elif kind == "reverse":
+            out[r] += float(torch.where(p > 0, p * (l.abs() + lpa), 0.0).sum())
+        else:
+            lm = (beta * q + (1 - beta) * p).log().abs()
+            out[r] += float((q * (l.abs() + lm) + torch.where(p > 0, p * (lpa + lm), 0.0)).sum())
+    return out
 
 
 def loss_and_grad(fn, x, upstream):
@@ -101,14 +143,15 @@ def fp32_tol(V: int, K: int, span: float) -> float:
 
 
 def check_loss(got, want, tol):
-    """tol: relative to 1 + the loss's own terms, which are at most of the order of its log-probs."""
+    """tol: an absolute bound, for all rows or for each."""
     got, want = got.double().cpu(), want.cpu()
     assert torch.equal(got.isnan(), want.isnan())
     inf = want.isinf()
     assert torch.equal(got[inf], want[inf])
     ok = ~(inf | want.isnan())
     err = (got[ok] - want[ok]).abs()
-    assert bool((err <= tol).all()), (float(err.max()), tol)
+    tol = torch.as_tensor(tol, dtype=torch.float64).expand(want.shape)[ok]
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
 
 
 def check_grad(got, want, dtype, scale, tol, ref_err=0.0):

@@ -9,7 +9,7 @@ import torch
 from invokerl_b200 import _native as N
 from invokerl_b200 import ops
 from row_loss_math import (EPS32, check_grad, check_loss, distill_rows, fp32_tol, grad_scale, half_step,
-                           loss_and_grad, xent_rows)
+                           loss_and_grad, loss_size, xent_rows)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -137,7 +137,7 @@ def check_distill(x, ids, lp, up, kind="forward", tail=True, temperature=1.0, be
     want, dw = loss_and_grad(lambda y: distill_rows(y, ids, lp, kind, beta, temperature, tail), x, up)
     span = span_of(x, ids, lp, temperature)
     tol = fp32_tol(x.shape[1], ids.shape[1], span)
-    check_loss(loss, want, tol * (1 + span))
+    check_loss(loss, want, tol * loss_size(x, ids, lp, kind, beta, temperature, tail))
     check_grad(d, dw, x.dtype, grad_scale(x, ids, lp, up, temperature), tol)
     return loss, d
 
@@ -182,12 +182,12 @@ def test_distill_entry_rules(kind, tail, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["reverse", "jsd", "forward"])
-@pytest.mark.parametrize("hole", ["inf", "lowest"])
+@pytest.mark.parametrize("hole", ["inf", "lowest", -1e4, -1e9, -1e30])
 def test_distill_masked_columns(kind, hole, dtype):
     """Columns masked in the student (-inf, or the type's lowest value), whole vectors of them, a row
     that keeps its entries only."""
     x, ids, lp, up = make_rows(4, 3001, 8, dtype, 6)
-    low = -math.inf if hole == "inf" else torch.finfo(dtype).min
+    low = {"inf": -math.inf, "lowest": torch.finfo(dtype).min}.get(hole, hole)
     keep = torch.zeros(4, 3001, dtype=torch.bool).scatter_(1, ids, True)
     x[0, 64:2500] = torch.where(keep[0, 64:2500], x[0, 64:2500], low)
     x[1] = torch.where(keep[1], x[1], low)
@@ -198,12 +198,29 @@ def test_distill_masked_columns(kind, hole, dtype):
     check_distill(x, ids, lp, up, kind)
 
 
+@pytest.mark.parametrize("n", [3, 80])  # one launch, and three
+@pytest.mark.parametrize("low", [-1e9, -1e30, torch.finfo(torch.float32).min])
+def test_losses_where_everything_is_masked(low, n):
+    """Rows of one value, however low: a uniform softmax; and masks behind which whole vectors lie before
+    the first other value comes."""
+    x, ids, lp, up = make_rows(n, 9000, 8, torch.float32, 19)
+    x[0] = low
+    x[1, :8800] = low
+    x[2] = low
+    x[2, ids[2]] = 1.0
+    for kind in ("forward", "reverse", "jsd"):
+        check_distill(x, ids, lp, up, kind)
+    check_xent(x, ids[:, 0], up, 0.0, 0.0)
+    check_topk(x.to(DEV), 60)
+
+
 @pytest.mark.parametrize("kind,tail", KINDS)
-def test_distill_all_mass_on_the_entries(kind, tail):
-    """Nothing left for the tail: every other column is -inf, and the teacher's mass is 1."""
+@pytest.mark.parametrize("low", [-math.inf, -1e30, torch.finfo(torch.float32).min])
+def test_distill_all_mass_on_the_entries(low, kind, tail):
+    """Nothing left for the tail: every other column is masked, and the teacher's mass is 1."""
     x, ids, lp, up = make_rows(3, 200, 6, torch.float32, 7)
     keep = torch.zeros(3, 200, dtype=torch.bool).scatter_(1, ids, True)
-    x = torch.where(keep, x, -math.inf)
+    x = torch.where(keep, x, low)
     lp = torch.log_softmax(lp, 1)
     loss, d = run_distill(x, ids, lp, up, kind=kind, tail=tail)
     want, _ = loss_and_grad(lambda y: distill_rows(y, ids, lp, kind, 0.5, 1.0, tail), x, up)
