@@ -734,8 +734,8 @@ def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple
     if not 1 <= k <= min(N.MAX_ENTRIES, V):
         raise ValueError(f"k = {k} outside 1..{min(N.MAX_ENTRIES, V)}")
     shape = (*logits.shape[:-1], k)
-    log_probs = torch.empty(shape, dtype=torch.float32, device=dev)
-    ids = torch.empty(shape, dtype=torch.int64, device=dev)
+    log_probs = x.new_empty(shape, dtype=torch.float32)
+    ids = x.new_empty(shape, dtype=torch.int64)
     code = N.dtype_code(x)
     nbytes = N.lib().ikrl_logits_topk_workspace_bytes(code, Nr, V)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
@@ -753,7 +753,7 @@ class LogitsRowLoss(torch.autograd.Function):
         dev = x.device
         Nr, V = x.shape
         K = 1 if teacher_lp is None else ids.shape[1]
-        loss = torch.empty(Nr, dtype=torch.float32, device=dev)
+        loss = x.new_empty(Nr, dtype=torch.float32)
         state = _row_state(Nr, K, dev)
         head = (x.data_ptr(), N.dtype_code(x), _ld(x), Nr, V, ids.data_ptr())
         tail = (loss.data_ptr(), state.data_ptr(), state.numel(), N.stream_handle(dev))
@@ -775,7 +775,7 @@ class LogitsRowLoss(torch.autograd.Function):
         dev = x.device
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
-        dx = torch.empty((Nr, V), dtype=x.dtype, device=dev)
+        dx = x.new_empty((Nr, V))
         head = (x.data_ptr(), N.dtype_code(x), _ld(x), Nr, V)
         tail = (state.data_ptr(), state.numel(), g.data_ptr(), dx.data_ptr(), V, N.stream_handle(dev))
         with N.on_device(dev):
@@ -876,7 +876,7 @@ class LMHeadRowLoss(torch.autograd.Function):
         Nr, H = hidden.shape
         V = weight.shape[0]
         K = 1 if teacher_lp is None else ids.shape[1]
-        loss = torch.empty(Nr, dtype=torch.float32, device=dev)
+        loss = hidden.new_empty(Nr, dtype=torch.float32)
         state = _row_state(Nr, K, dev)
         cache = None
         if grad_mode and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
