@@ -131,6 +131,7 @@ struct GemmParams {
   int64_t cache_cap;      // TAIL_CACHED: slots; a row's slot is slot[row] (row itself with row_idx)
   float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
   const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
+  uint16_t* out_lo;       // what rounding to out_bf16 leaves, itself rounded, or null (DTAIL)
 };
 
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err) {
@@ -368,8 +369,9 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         if constexpr (EPI == EPI_DTAIL) {
-          w[i >> 1] = pack_bf16x2(fmaf(gval, fast_exp2(fmaf(v[i], p.c, -lse2)), level),
-                                  fmaf(gval, fast_exp2(fmaf(v[i + 1], p.c, -lse2)), level));
+          v[i] = fmaf(gval, fast_exp2(fmaf(v[i], p.c, -lse2)), level);
+          v[i + 1] = fmaf(gval, fast_exp2(fmaf(v[i + 1], p.c, -lse2)), level);
+          w[i >> 1] = pack_bf16x2(v[i], v[i + 1]);
           continue;
         }
         const float p0 = fast_exp2(fmaf(v[i], kLog2e, -lse2));
@@ -377,6 +379,22 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
         const float d0 = gval * (((int64_t)(col0 + i) == tgt ? 1.f : 0.f) - p0);
         const float d1 = gval * (((int64_t)(col0 + i + 1) == tgt ? 1.f : 0.f) - p1);
         w[i >> 1] = pack_bf16x2(d0, d1);
+      }
+      if constexpr (EPI == EPI_DTAIL) {
+        if (p.out_lo != nullptr && row_ok) {
+          uint16_t* lo = p.out_lo + (int64_t)grow * p.ld_bf16 + col0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (8 * k >= nvalid) break;
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 8 * k + 2 * e;
+              o[e] = pack_bf16x2(v[i] - bf16lo(w[i >> 1]), v[i + 1] - bf16hi(w[i >> 1]));
+            }
+            st_global_v4(lo + 8 * k, o[0], o[1], o[2], o[3]);
+          }
+        }
       }
       if (stage_smem != 0) {
         // One TMA store per 32 x 32 block: row `lane` goes to the staging tile with its 16-byte
@@ -2013,7 +2031,9 @@ __global__ void __launch_bounds__(256) ds_from_cache_kernel(
 
 // The same for a row loss: dS = g (coef q 2^(c (m - ref)) + level), then g grad at the row's entries,
 // written behind a barrier by the block that holds their columns.  slot null: row r has slot r; idx null:
-// chunk row k is row c0 + k.  Rows without a gradient (or a slot) are zeros.
+// chunk row k is row c0 + k.  Rows without a gradient (or a slot) are zeros.  TWO: dS in two terms, what the
+// rounding to bf16 leaves (rounded itself) `rows` rows below.
+template <bool TWO>
 __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
     const uint16_t* __restrict__ cache_q, const float* __restrict__ cache_m, int64_t ld_cache, int n_mchunks,
     const int* __restrict__ slot, const int* __restrict__ idx, const float* __restrict__ dloss,
@@ -2031,6 +2051,7 @@ __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
     const uint16_t* qrow = cache_q + (on ? sl : 0) * ld_cache;
     const float* mrow = cache_m + (on ? sl : 0) * n_mchunks;
     uint16_t* drow = ds + k * ld_ds;
+    uint16_t* lrow = ds + (rows + k) * ld_ds;
     uint4 qv[kDsUnroll];
     float mv[kDsUnroll];
 #pragma unroll
@@ -2049,20 +2070,26 @@ __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
       if (jv >= vec) break;
       const float sc = on ? gs * fast_exp2((mv[u] - ref) * c) : 0.f;
       const uint32_t w[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
-      uint32_t o[4];
+      uint32_t o[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-        o[e] = pack_bf16x2(fmaf(q.x, sc, lv), fmaf(q.y, sc, lv));
+        const float d0 = fmaf(q.x, sc, lv), d1 = fmaf(q.y, sc, lv);
+        o[e] = pack_bf16x2(d0, d1);
+        if constexpr (TWO) lo[e] = pack_bf16x2(d0 - bf16lo(o[e]), d1 - bf16hi(o[e]));
       }
       *reinterpret_cast<uint4*>(drow + (jv << 3)) = make_uint4(o[0], o[1], o[2], o[3]);
+      if constexpr (TWO) *reinterpret_cast<uint4*>(lrow + (jv << 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     __syncthreads();
     if (on) {
       const int lo = (int)(blockIdx.x * blockDim.x * kDsUnroll) << 3, hi = lo + ((int)blockDim.x * kDsUnroll << 3);
       for (int e = threadIdx.x; e < K; e += blockDim.x) {
         const int col = cols[r * K + e];
-        if (col != kNoEntry && col >= lo && col < hi) drow[col] = f32_to_bf16_rn(g * grads[r * K + e]);
+        if (col == kNoEntry || col < lo || col >= hi) continue;
+        const float d = g * grads[r * K + e];
+        drow[col] = f32_to_bf16_rn(d);
+        if constexpr (TWO) lrow[col] = f32_to_bf16_rn(d - bf16_to_f32(drow[col]));
       }
     }
   }
@@ -2169,10 +2196,11 @@ __global__ void row_scale_kernel(const float* __restrict__ dloss, const int64_t*
 }
 
 // Row losses, backward: the gradient at the entries of chunk rows [c0, c0 + rows) goes over what the
-// dS epilogue wrote there.  One block of threads per 256 entries.
+// dS epilogue wrote there.  One block of threads per 256 entries.  two: the second term too, `rows` rows
+// below the first.
 __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __restrict__ cols,
                                   const float* __restrict__ grad, int K, const int* __restrict__ idx, int64_t c0,
-                                  int64_t rows, uint16_t* __restrict__ ds, int64_t ld_ds) {
+                                  int64_t rows, uint16_t* __restrict__ ds, int64_t ld_ds, bool two) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= rows * K) return;
   const int64_t k = i / K;
@@ -2181,7 +2209,46 @@ __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __
   const int col = cols[r * K + e];
   if (col == kNoEntry) return;
   const float g = dloss[r];
-  ds[k * ld_ds + col] = g != 0.f ? f32_to_bf16_rn(g * grad[r * K + e]) : (uint16_t)0;
+  const float d = g != 0.f ? g * grad[r * K + e] : 0.f;
+  const uint16_t hi = f32_to_bf16_rn(d);
+  ds[k * ld_ds + col] = hi;
+  if (two) ds[(rows + k) * ld_ds + col] = f32_to_bf16_rn(d - bf16_to_f32(hi));
+}
+
+// The hidden rows twice, one under the other: the dW operand beside a dS of two terms.
+__global__ void stack_rows_kernel(const uint4* __restrict__ h, int64_t n, uint4* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+    out[i] = out[n + i] = h[i];
+}
+
+// dH of a dS of two terms: out = bf16(sum over K ranges of the partials of row r and of row rows + r).
+// n4: float4 groups of the rows of one term, sets = 2 ks of them.  The sets are few groups long, so a group's
+// sum is four threads' work, a quarter of the sets each, joined in a fixed order: at 74 sets of 96 x 1024 one
+// thread's chain of loads took 19 us.
+constexpr int kTermSumGroups = 64;
+__global__ void __launch_bounds__(4 * kTermSumGroups) two_term_sum_kernel(const float4* __restrict__ part, int64_t n4,
+                                                                          int sets, uint2* __restrict__ out) {
+  __shared__ float4 sums[3][kTermSumGroups];
+  const int t = threadIdx.x % kTermSumGroups, quarter = threadIdx.x / kTermSumGroups;
+  const int64_t i = (int64_t)blockIdx.x * kTermSumGroups + t;
+  const int s0 = sets * quarter / 4, s1 = sets * (quarter + 1) / 4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (i < n4) {
+#pragma unroll 8
+    for (int s = s0; s < s1; ++s) {
+      const float4 b = part[(int64_t)s * n4 + i];
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+  }
+  if (quarter > 0) sums[quarter - 1][t] = a;
+  __syncthreads();
+  if (quarter > 0 || i >= n4) return;
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    const float4 b = sums[q][t];
+    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+  }
+  out[i] = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
 }
 
 // Row skipping is on unless IKRL_TUNE_SKIP_ZERO_ROWS = 0.
@@ -2228,7 +2295,7 @@ size_t cache_fwd_workspace_bytes(int64_t N, int H, int V) {
 
 // A row loss of at most this many rows runs its GEMMs on all of them: one row pair of tiles costs
 // the same however many of its rows count, and the compaction's host synchronisation and launches
-// would cost more than they save.
+// would cost more than they save.  Its backward is lmhead_row_loss_bwd_few.
 constexpr int64_t kRowLossDense = 256;
 
 // Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums
@@ -2324,23 +2391,35 @@ static int lmhead_fwd_impl(const char* what, const void* hidden, const void* wei
 // A dW over fewer rows than this is mostly its output: it takes the wide kernel with TMA stores.
 constexpr int64_t kShortDw = 1024;
 
-// K ranges of a dH of one row pair: as many as keep every pair busy (dh_split_k stops at 16, which leaves
-// more than half of them idle at H = 1024), each at least 16 K blocks, as far as the partials fit.
-static int64_t few_rows_part_elems(int64_t N, int H) {
-  return (cdiv64(kNumSMs / 2, cdiv64(H, WN)) + 1) * std::min<int64_t>(N, kRowLossDense) * H;
-}
-static int few_rows_split_k(int H, int V, int64_t rows, int64_t part_elems, int nsm) {
-  if (tuning(IKRL_TUNE_DH_SPLIT_K) >= 0 || !use_pairs() || !use_wide(V) || !persistent_pairs()) return 1;
-  const int64_t pairs = std::max(1, nsm / 2), tiles = cdiv64(H, WN);
-  int64_t ks = std::min(pairs / tiles, cdiv64(V, BK) / 16);
-  ks = std::min(ks, part_elems / (rows * H));
-  return (int)std::max<int64_t>(1, ks);
+static int check_dweight_kind(const char* what, int32_t dweight_dtype, int32_t accumulate_dweight) {
+  IKRL_REQUIRE(dweight_dtype == IKRL_DTYPE_F32 || dweight_dtype == IKRL_DTYPE_BF16, IKRL_ERR_UNSUPPORTED,
+               "%s: dweight dtype %d unsupported", what, dweight_dtype);
+  IKRL_REQUIRE(!(accumulate_dweight && dweight_dtype == IKRL_DTYPE_BF16), IKRL_ERR_UNSUPPORTED,
+               "%s: accumulating into a bf16 dweight is not supported; use fp32", what);
+  return IKRL_OK;
 }
 
-// Workspace of a row loss's backward behind the backward's own: the partials of a dH of few rows, then the
-// rows' levels.
-static size_t row_loss_bwd_extra(int64_t N, int H) {
-  return (N <= kRowLossDense ? align256((size_t)few_rows_part_elems(N, H) * 4) : 0) + align256((size_t)N * 4);
+static int check_grad_alignment(const char* what, const void* dhidden, const void* dweight) {
+  IKRL_REQUIRE(dweight == nullptr || (reinterpret_cast<uintptr_t>(dweight) & 15) == 0, IKRL_ERR_ALIGNMENT,
+               "%s: dweight must be 16-byte aligned", what);
+  IKRL_REQUIRE(dhidden == nullptr || (reinterpret_cast<uintptr_t>(dhidden) & 15) == 0, IKRL_ERR_ALIGNMENT,
+               "%s: dhidden must be 16-byte aligned", what);
+  return IKRL_OK;
+}
+
+// A bf16 dW of few rows: mostly its output, which leaves through TMA stores of the wide
+// kernel, where that may run.
+static int launch_short_dw(const CUtensorMap& ta, const CUtensorMap& tb, GemmParams& p, void* dweight,
+                           cudaStream_t s) {
+  const int v_tiles = (int)cdiv64(p.M, BM);
+  if (use_pairs() && tuning(IKRL_TUNE_WIDE) != 0) {
+    CUtensorMap tc;
+    const int rc = make_store_tmap(&tc, dweight, p.N, p.M, p.N, "dW store", 64);
+    if (rc) return rc;
+    return launch_k1<EPI_STORE_TMA, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s, &tc);
+  }
+  p.out_bf16 = reinterpret_cast<uint16_t*>(dweight); p.ld_bf16 = p.N;
+  return launch_k1<EPI_STORE_BF16, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s);
 }
 
 // A row loss (row_dist.cuh) behind the LM head's backward: the state its forward left, and its level
@@ -2350,9 +2429,6 @@ struct RowLossBwd {
   int K;
   float c, level;
   bool all_cached;  // every row that is not kRowNone has a cache slot
-  bool identity;    // row r has slot r
-  float* part;      // fp32 partials of a dH of few rows
-  int64_t part_elems;
 };
 
 // cache_slot / cache_q / cache_m: the logit cache a forward filled (all null: no cache).  Active
@@ -2367,10 +2443,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
                            const float* cache_m = nullptr, const RowLossBwd* rl = nullptr) {
   int rc = check_common(hidden, weight, ids, N, H, V, what);
   if (rc) return rc;
-  IKRL_REQUIRE(dweight_dtype == IKRL_DTYPE_F32 || dweight_dtype == IKRL_DTYPE_BF16, IKRL_ERR_UNSUPPORTED,
-               "%s: dweight dtype %d unsupported", what, dweight_dtype);
-  IKRL_REQUIRE(!(accumulate_dweight && dweight_dtype == IKRL_DTYPE_BF16), IKRL_ERR_UNSUPPORTED,
-               "%s: accumulating into a bf16 dweight is not supported; use fp32", what);
+  if ((rc = check_dweight_kind(what, dweight_dtype, accumulate_dweight))) return rc;
   if (N == 0) {  // no rows: dW is zero, or left as it is when accumulating
     if (dweight && !accumulate_dweight)
       IKRL_CUDA(cudaMemsetAsync(dweight, 0, (size_t)V * H * (dweight_dtype == IKRL_DTYPE_F32 ? 4 : 2),
@@ -2380,15 +2453,12 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   IKRL_REQUIRE(lse && dlogp && (dhidden || dweight), IKRL_ERR_INVALID_ARGUMENT,
                "%s: null pointer", what);
   const BwdLayout L = bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
-  const size_t ws_need = L.total + (rl ? row_loss_bwd_extra(N, H) : 0);
+  const size_t ws_need = L.total + (rl ? align256((size_t)N * 4) : 0);
   IKRL_REQUIRE(ws != nullptr && ws_bytes >= ws_need, IKRL_ERR_WORKSPACE,
                "%s: workspace %zu < %zu bytes", what, ws_bytes, ws_need);
   IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
                "%s: workspace must be 256-byte aligned", what);
-  IKRL_REQUIRE(dweight == nullptr || (reinterpret_cast<uintptr_t>(dweight) & 15) == 0, IKRL_ERR_ALIGNMENT,
-               "%s: dweight must be 16-byte aligned", what);
-  IKRL_REQUIRE(dhidden == nullptr || (reinterpret_cast<uintptr_t>(dhidden) & 15) == 0, IKRL_ERR_ALIGNMENT,
-               "%s: dhidden must be 16-byte aligned", what);
+  if ((rc = check_grad_alignment(what, dhidden, dweight))) return rc;
   cudaStream_t s = as_stream(stream);
   char* w = reinterpret_cast<char*>(ws);
   int* err = reinterpret_cast<int*>(w + L.err_off);
@@ -2415,8 +2485,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   int64_t n_cached = 0;                                      // leading compacted rows whose dS is cached
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   IKRL_CUDA(cudaStreamIsCapturing(s, &cap));
-  if (skip_zero_rows_enabled() && cap == cudaStreamCaptureStatusNone && N <= INT32_MAX &&
-      !(rl && N <= kRowLossDense)) {
+  if (skip_zero_rows_enabled() && cap == cudaStreamCaptureStatusNone && N <= INT32_MAX) {
     int* counts = reinterpret_cast<int*>(w + L.cnt_off);
     int64_t* n_act_d = reinterpret_cast<int64_t*>(w + L.nact_off);
     int* idx = reinterpret_cast<int*>(w + L.idx_off);
@@ -2460,7 +2529,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   float* level = nullptr;
   if (rl && !(rl->all_cached && cache_slot != nullptr)) {  // what the dS epilogue multiplies and adds
     float* gs = reinterpret_cast<float*>(w + L.gc_off);
-    level = reinterpret_cast<float*>(w + L.total + row_loss_bwd_extra(N, H) - align256((size_t)N * 4));
+    level = reinterpret_cast<float*>(w + L.total);
     row_scale_kernel<<<(unsigned)cdiv64(Nw, 256), 256, 0, s>>>(dlogp, rl->st.row_ids, rl->st.coef, idx_c, Nw,
                                                                rl->level, gs, level);
     if ((rc = check_launch("row_scale_kernel"))) return rc;
@@ -2507,8 +2576,8 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     if (from_cache > 0 && rl) {
       const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
                       (unsigned)std::min<int64_t>(from_cache, 65535));
-      dtail_from_cache_kernel<<<grid, 256, 0, s>>>(
-          cache_q, cache_m, L.lds, (int)cdiv64(V, 32), rl->identity ? nullptr : cache_slot, idx_c, dlogp,
+      dtail_from_cache_kernel<false><<<grid, 256, 0, s>>>(
+          cache_q, cache_m, L.lds, (int)cdiv64(V, 32), cache_slot, idx_c, dlogp,
           rl->st.row_ids, rl->st.ref, rl->st.coef, rl->st.cols, rl->st.grad, rl->K, rl->level, rl->c, c0, from_cache, V,
           dS, L.lds);
       if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
@@ -2545,7 +2614,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       const int64_t n = rows - from_cache;
       ds_entries_kernel<<<(unsigned)cdiv64(n * rl->K, 256), 256, 0, s>>>(dlogp, rl->st.cols, rl->st.grad, rl->K, idx_c,
                                                                          c0 + from_cache, n, dS + from_cache * L.lds,
-                                                                         L.lds);
+                                                                         L.lds, false);
       if ((rc = check_launch("ds_entries_kernel"))) return rc;
     }
     // 2) dW (+)= dS^T h[chunk]
@@ -2558,11 +2627,8 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       p.err = err;
       const int v_tiles = (int)cdiv64(V, BM);
       const bool last = ci == nchunks - 1;
-      if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32 && rl && rows < kShortDw && use_pairs() &&
-          tuning(IKRL_TUNE_WIDE) != 0) {
-        CUtensorMap tc;
-        if ((rc = make_store_tmap(&tc, dweight, H, V, H, "dW store", 64))) return rc;
-        if ((rc = launch_k1<EPI_STORE_TMA, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s, &tc))) return rc;
+      if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32 && rl && rows < kShortDw) {
+        if ((rc = launch_short_dw(ta, tb, p, dweight, s))) return rc;
       } else if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32) {
         p.out_bf16 = reinterpret_cast<uint16_t*>(dweight); p.ld_bf16 = H;
         if ((rc = launch_k1<EPI_STORE_BF16, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s))) return rc;
@@ -2586,16 +2652,9 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       GemmParams p{};
       p.M = (int)rows; p.N = H; p.K = V;
       p.err = err;
-      int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm, rl != nullptr);
-      float* part = reinterpret_cast<float*>(w + L.part_off);
-      if (rl && rows <= kRowLossDense) {
-        const int few = few_rows_split_k(H, V, rows, rl->part_elems, nsm);
-        if (few > ks) {
-          ks = few;
-          part = rl->part;
-        }
-      }
+      const int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm, rl != nullptr);
       if (ks > 1) {
+        float* part = reinterpret_cast<float*>(w + L.part_off);
         p.out_f32 = part; p.ld_f32 = H; p.f32_mode = F32_STORE;
         p.ksplits = ks; p.ks_stride = rows * H;
         if ((rc = launch_k1<EPI_F32, false, true>(ta, t_w_mn, ta, t_w_mn, p, m_tiles, 0, s))) return rc;
@@ -2686,14 +2745,13 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   p.n_cols = K;
   const void* rows_in = hidden;
   const int* pos = nullptr;
-  const bool cached = cache.rows > 0;
-  // Without gathering and with a slot for every row, row r takes slot r: nothing to number.
-  const bool identity = cached && !L.gather && cache.rows >= N;
-  if (L.gather || (cached && !identity)) {
+  // Without gathering a cache is used when it holds every row, and row r takes slot r: nothing to number.
+  const bool cached = L.gather ? cache.rows > 0 : cache.rows >= N;
+  if (L.gather) {
     int* counts = reinterpret_cast<int*>(w + L.counts_off);
     int* count = reinterpret_cast<int*>(w + L.count_off);
     int* posw = reinterpret_cast<int*>(w + L.pos_off);
-    int* idx = L.gather ? reinterpret_cast<int*>(w + L.idx_off) : nullptr;
+    int* idx = reinterpret_cast<int*>(w + L.idx_off);
     const int nb = (int)cdiv64(N, kCompactRows);
     cache_count_kernel<<<nb, kCompactThreads, 0, s>>>(nullptr, st.row_ids, N, counts);
     if ((rc = check_launch("cache_count_kernel"))) return rc;
@@ -2702,16 +2760,14 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
     row_index_kernel<<<(unsigned)cdiv64(N, 256), 256, 0, s>>>(posw, N, cache.rows, idx, cached ? cache.slot : nullptr,
                                                               counts, nb, count);
     if ((rc = check_launch("row_index_kernel"))) return rc;
-    if (L.gather) {
-      uint4* hc = reinterpret_cast<uint4*>(w + L.hc_off);
-      gather_live_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(N * vpr, 256), 148ll * 16), 256, 0, s>>>(
-          reinterpret_cast<const uint4*>(hidden), idx, count, vpr, hc);
-      if ((rc = check_launch("gather_live_rows_kernel"))) return rc;
-      rows_in = hc;
-      pos = posw;
-      p.m_dev = count;
-      p.row_idx = idx;
-    }
+    uint4* hc = reinterpret_cast<uint4*>(w + L.hc_off);
+    gather_live_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(N * vpr, 256), 148ll * 16), 256, 0, s>>>(
+        reinterpret_cast<const uint4*>(hidden), idx, count, vpr, hc);
+    if ((rc = check_launch("gather_live_rows_kernel"))) return rc;
+    rows_in = hc;
+    pos = posw;
+    p.m_dev = count;
+    p.row_idx = idx;
     p.slot = posw;
   }
   if (cached) {
@@ -2733,6 +2789,124 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
     if ((rc = launch_k1<EPI_TAIL, false, false>(ta, tb, ta, tb2, p, m_tiles, L.splits, s))) return rc;
   }
   return launch_row_losses(p.part_m, p.part_s, p.part_x, p.part_sets, pos, N, K, P, st, loss, err, s);
+}
+
+// Backward of a row loss of few rows (N <= kRowLossDense), all of them in one chunk, without the
+// compaction and its host synchronisation.  dS is held in two terms, hi = bf16(d) and lo = bf16(d - hi),
+// stacked as 2N rows: dW = [hi; lo]^T [h; h], dH = hi W + lo W.  With few rows a sum over the rows averages
+// little of dS's rounding away, and one term alone would leave dW with up to twice the error that its own
+// rounding to bf16 has; the second term costs K blocks of a dW that is bound by writing [V, H], and rows of a
+// tile of dH that N <= 128 left empty.
+struct FewLayout {
+  size_t ds_off, h_off, gs_off, level_off, part_off, total;
+  int64_t lds, part_sets;
+};
+static FewLayout few_layout(int64_t N, int H, int V) {
+  FewLayout L;
+  L.lds = cdiv64(V, 64) * 64;
+  L.part_sets = std::max<int64_t>(1, kNumSMs / 2 / (cdiv64(H, WN) * cdiv64(2 * N, 2 * BM)));
+  size_t o = 256;  // the error word
+  L.ds_off = o; o += align256((size_t)2 * N * L.lds * 2);
+  L.h_off = o; o += align256((size_t)2 * N * H * 2);
+  L.gs_off = o; o += align256((size_t)N * 4);
+  L.level_off = o; o += align256((size_t)N * 4);
+  L.part_off = o; o += align256((size_t)L.part_sets * 2 * N * H * 4);
+  L.total = o;
+  return L;
+}
+
+// dweight's checks; the workspace is the caller's to check.
+static int lmhead_row_loss_bwd_few(const char* what, const void* hidden, const void* weight, const float* dloss,
+                                   int64_t N, int H, int V, const RowLossBwd& rl, void* dhidden, void* dweight,
+                                   int32_t dweight_dtype, int32_t accumulate_dweight, const RowCacheArgs& cache,
+                                   void* ws, void* stream) {
+  int rc = check_common(hidden, weight, rl.st.row_ids, N, H, V, what);
+  if (rc) return rc;
+  if ((rc = check_dweight_kind(what, dweight_dtype, accumulate_dweight))) return rc;
+  if ((rc = check_grad_alignment(what, dhidden, dweight))) return rc;
+  IKRL_REQUIRE(dloss && (dhidden || dweight), IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
+               "%s: workspace must be 256-byte aligned", what);
+  cudaStream_t s = as_stream(stream);
+  const FewLayout L = few_layout(N, H, V);
+  char* w = reinterpret_cast<char*>(ws);
+  int* err = reinterpret_cast<int*>(w);
+  uint16_t* ds = reinterpret_cast<uint16_t*>(w + L.ds_off);
+  IKRL_CUDA(cudaMemsetAsync(err, 0, sizeof(int), s));
+  // 1) dS, from the forward's numerators or by the GEMM again
+  if (cache.rows >= N) {
+    const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)), (unsigned)N);
+    dtail_from_cache_kernel<true><<<grid, 256, 0, s>>>(cache.q, cache.m, L.lds, (int)cdiv64(V, 32), nullptr, nullptr,
+                                                       dloss, rl.st.row_ids, rl.st.ref, rl.st.coef, rl.st.cols,
+                                                       rl.st.grad, rl.K, rl.level, rl.c, 0, N, V, ds, L.lds);
+    if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
+  } else {
+    float* gs = reinterpret_cast<float*>(w + L.gs_off);
+    float* level = reinterpret_cast<float*>(w + L.level_off);
+    row_scale_kernel<<<(unsigned)cdiv64(N, 256), 256, 0, s>>>(dloss, rl.st.row_ids, rl.st.coef, nullptr, N, rl.level,
+                                                              gs, level);
+    if ((rc = check_launch("row_scale_kernel"))) return rc;
+    CUtensorMap ta, tb, tb2, tds;
+    if ((rc = make_tmap(&ta, hidden, H, N, H, BM, "hidden"))) return rc;
+    if ((rc = make_tmap(&tb, weight, H, V, H, BN, "weight"))) return rc;
+    if ((rc = make_tmap(&tb2, weight, H, V, H, BN / 2, "weight"))) return rc;
+    if ((rc = make_store_tmap(&tds, ds, V, N, L.lds, "dS store"))) return rc;
+    GemmParams p{};
+    p.M = (int)N; p.N = V; p.K = H;
+    p.ids = rl.st.row_ids; p.lse = rl.st.ref; p.g = gs; p.level = level; p.c = rl.c;
+    p.out_bf16 = ds; p.ld_bf16 = L.lds; p.out_lo = ds + N * L.lds;
+    p.err = err;
+    const int m_tiles = (int)cdiv64(N, BM);
+    const int sp = choose_splits(m_tiles, (int)cdiv64(V, BN), H);
+    if ((rc = launch_k1<EPI_DTAIL, false, false>(ta, tb, ta, tb2, p, m_tiles, sp, s, &tds))) return rc;
+    ds_entries_kernel<<<(unsigned)cdiv64(N * rl.K, 256), 256, 0, s>>>(dloss, rl.st.cols, rl.st.grad, rl.K, nullptr, 0,
+                                                                      N, ds, L.lds, true);
+    if ((rc = check_launch("ds_entries_kernel"))) return rc;
+  }
+  // 2) dW (+)= [hi; lo]^T [h; h]
+  if (dweight) {
+    uint4* h2 = reinterpret_cast<uint4*>(w + L.h_off);
+    const int64_t n = N * H / 8;
+    stack_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(n, 256), 148ll * 8), 256, 0, s>>>(
+        reinterpret_cast<const uint4*>(hidden), n, h2);
+    if ((rc = check_launch("stack_rows_kernel"))) return rc;
+    CUtensorMap ta, tb;
+    if ((rc = make_tmap(&ta, ds, V, 2 * N, L.lds, 64, "dS^T"))) return rc;
+    if ((rc = make_tmap(&tb, h2, H, 2 * N, H, 64, "hidden^T"))) return rc;
+    GemmParams p{};
+    p.M = V; p.N = H; p.K = (int)(2 * N);
+    p.err = err;
+    if (dweight_dtype == IKRL_DTYPE_BF16) {
+      if ((rc = launch_short_dw(ta, tb, p, dweight, s))) return rc;
+    } else {
+      p.out_f32 = reinterpret_cast<float*>(dweight); p.ld_f32 = H;
+      p.f32_mode = accumulate_dweight ? F32_ADD : F32_STORE;
+      if ((rc = launch_k1<EPI_F32, true, true>(ta, tb, ta, tb, p, (int)cdiv64(V, BM), 0, s))) return rc;
+    }
+  }
+  // 3) dH = hi W + lo W: K ranges as many as keep every pair busy, each at least 16 K blocks (the rule for
+  // more rows stops at 16 ranges, which leaves more than half of the pairs idle at H = 1024)
+  if (dhidden) {
+    const int64_t rows = 2 * N;
+    CUtensorMap ta, tb;
+    if ((rc = make_tmap(&ta, ds, V, rows, L.lds, BM, "dS"))) return rc;
+    if ((rc = make_tmap(&tb, weight, H, V, H, 64, "weight^T"))) return rc;
+    int64_t ks = 1;
+    if (tuning(IKRL_TUNE_DH_SPLIT_K) < 0 && use_pairs() && use_wide(V) && persistent_pairs())
+      ks = std::max<int64_t>(1, std::min(L.part_sets, cdiv64(V, BK) / 16));
+    float* part = reinterpret_cast<float*>(w + L.part_off);
+    GemmParams p{};
+    p.M = (int)rows; p.N = H; p.K = V;
+    p.err = err;
+    p.out_f32 = part; p.ld_f32 = H; p.f32_mode = F32_STORE;
+    if (ks > 1) { p.ksplits = (int)ks; p.ks_stride = rows * H; }
+    if ((rc = launch_k1<EPI_F32, false, true>(ta, tb, ta, tb, p, (int)cdiv64(rows, BM), 0, s))) return rc;
+    const int64_t n4 = N * H / 4;
+    two_term_sum_kernel<<<(unsigned)cdiv64(n4, kTermSumGroups), 4 * kTermSumGroups, 0, s>>>(
+        reinterpret_cast<const float4*>(part), n4, 2 * (int)ks, reinterpret_cast<uint2*>(dhidden));
+    if ((rc = check_launch("two_term_sum_kernel"))) return rc;
+  }
+  return IKRL_OK;
 }
 
 static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void* weight, int64_t N, int32_t H,
@@ -2758,12 +2932,9 @@ static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void*
   rl.c = P.c;
   rl.level = P.loss == ROW_XENT ? -P.smoothing / (float)V : 0.f;
   rl.all_cached = cache.rows >= N;
-  rl.identity = rl.all_cached && N <= kRowLossDense;  // as the forward that filled the cache
-  if (N > 0 && N <= kRowLossDense) {
-    rl.part_elems = few_rows_part_elems(N, H);
-    rl.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) +
-                                       bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total);
-  }
+  if (N > 0 && N <= kRowLossDense)
+    return lmhead_row_loss_bwd_few(what, hidden, weight, dloss, N, H, V, rl, dhidden, dweight, dweight_dtype,
+                                   accumulate_dweight, cache, ws, stream);
   const bool cached = cache.rows > 0;
   return lmhead_bwd_impl(what, hidden, weight, rl.st.row_ids, rl.st.ref, dloss, N, H, V, 0, chunk_rows, dhidden,
                          dweight, dweight_dtype, accumulate_dweight, ws, ws_bytes, stream,
@@ -2781,7 +2952,8 @@ size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V)
 size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
                                                 int32_t dweight_dtype, int32_t accumulate_dweight) {
   if (N <= 0 || H <= 0 || V <= 0) return 256;
-  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + row_loss_bwd_extra(N, H);
+  if (N <= kRowLossDense) return few_layout(N, H, V).total;
+  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + align256((size_t)N * 4);
 }
 
 int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,

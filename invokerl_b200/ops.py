@@ -847,8 +847,8 @@ def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> L
     """Logit cache of a row loss's forward under the policy of `set_logit_cache`, or None."""
     if _LOGIT_CACHE["mode"] == "off" or V % 8 or n_rows == 0 or torch.cuda.is_current_stream_capturing():
         return None
-    if n_rows <= _ROW_CACHE_SMALL and n_rows * V <= 1 << 27:
-        return LogitCache(n_rows, V, n_rows, device)
+    if n_rows <= _ROW_CACHE_SMALL:  # a cache of so few rows holds all of them or none
+        return LogitCache(n_rows, V, n_rows, device) if n_rows * V <= 1 << 27 else None
     if H < _ROW_CACHE_MIN_HIDDEN:
         return None
     rows = logit_cache_rows(n_rows, H, V, device, n_rows, chunk_rows, _ROW_CACHE_MIN_HIDDEN, _free_bytes(device))
