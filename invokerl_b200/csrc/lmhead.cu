@@ -252,6 +252,23 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   float run_m = -INFINITY, run_s = 0.f, tval = 0.f;
   bool found = false;
 
+  // A 32 x 32 block of 16-bit values leaves with one TMA store: row `lane` goes to the staging tile with
+  // its 16-byte chunks in the 64-byte swizzled order; the tensor map clips rows and columns past its edges.
+  auto store_block = [&](const uint32_t (&w)[16], int col, int row) {
+    if (lane == 0) bulk_wait_read_all();  // the previous block's store has read the tile
+    __syncwarp();
+    const uint32_t row_addr = stage_smem + (uint32_t)lane * 64u;
+    const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    fence_async_shared();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(tm_store, stage_smem, col, row);
+      bulk_commit();
+    }
+  };
   // The numerators v of a chunk whose maximum is cm into the logit cache.  They are at most 1: a row
   // loss keeps them in fp16, whose 11 bits leave the one rounding of dS to bf16 (in bf16 the two
   // together took dH and dW from 1.4 to 1.55 times the error of a single final rounding); what lies
@@ -265,29 +282,16 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
     }
   };
   auto store_numerators = [&](const float* v, int col0, float cm) {
-    if (cache_run) {
-      // Consecutive slots: the 32 x 32 block goes out with one TMA store, as the dS blocks do.
-      if (lane == 0) bulk_wait_read_all();
-      __syncwarp();
-      const uint32_t row_addr = stage_smem + (uint32_t)lane * 64u;
-      const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
+    uint32_t w[16];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), pack16(v[8 * k], v[8 * k + 1]),
-                     pack16(v[8 * k + 2], v[8 * k + 3]), pack16(v[8 * k + 4], v[8 * k + 5]),
-                     pack16(v[8 * k + 6], v[8 * k + 7]));
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(tm_store, stage_smem, col0, cslot0);
-        bulk_commit();
-      }
+    for (int i = 0; i < 32; i += 2) w[i >> 1] = pack16(v[i], v[i + 1]);
+    if (cache_run) {
+      store_block(w, col0, cslot0);  // consecutive slots
     } else if (cslot >= 0) {
       uint16_t* dst = p.cache_q + (int64_t)cslot * p.ld_cache + col0;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        st_global_v4(dst + 8 * k, pack16(v[8 * k], v[8 * k + 1]), pack16(v[8 * k + 2], v[8 * k + 3]),
-                     pack16(v[8 * k + 4], v[8 * k + 5]), pack16(v[8 * k + 6], v[8 * k + 7]));
+        st_global_v4(dst + 8 * k, w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
     }
     if (cslot >= 0) p.cache_m[(int64_t)cslot * p.n_mchunks + (col0 >> 5)] = cm;
   };
@@ -397,21 +401,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
         }
       }
       if (stage_smem != 0) {
-        // One TMA store per 32 x 32 block: row `lane` goes to the staging tile with its 16-byte
-        // chunks in the 64-byte swizzled order; the tensor map clips rows >= M and columns >= N.
-        if (lane == 0) bulk_wait_read_all();  // the previous block's store has read the tile
-        __syncwarp();
-        const uint32_t row_addr = stage_smem + (uint32_t)lane * 64u;
-        const uint32_t sw = ((uint32_t)lane >> 1) & 3u;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          st_shared_v4(row_addr + ((((uint32_t)k) ^ sw) << 4), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(tm_store, stage_smem, col0, m0 + q * 32);
-          bulk_commit();
-        }
+        store_block(w, col0, m0 + q * 32);
       } else if (row_ok) {
         uint16_t* dst = p.out_bf16 + (int64_t)grow * p.ld_bf16 + col0;
 #pragma unroll
@@ -419,26 +409,10 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
           if (8 * k < nvalid) st_global_v4(dst + 8 * k, w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
       }
     } else if constexpr (EPI == EPI_STORE_TMA) {
-      // Two chunks make one 32 x 64 block: rows of 128 bytes, in the 128-byte swizzled order.
-      const uint32_t half = ((uint32_t)col0 >> 5) & 1u;
-      if (half == 0) {
-        if (lane == 0) bulk_wait_read_all();  // the block before has left the tile
-        __syncwarp();
-      }
-      const uint32_t row_addr = stage_smem + (uint32_t)lane * 128u;
+      uint32_t w[16];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        st_shared_v4(row_addr + (((half * 4u + (uint32_t)k) ^ ((uint32_t)lane & 7u)) << 4),
-                     pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                     pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
-      if (half == 1 || col0 + 32 >= p.N) {
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(tm_store, stage_smem, col0 & ~63, m0 + q * 32);
-          bulk_commit();
-        }
-      }
+      for (int i = 0; i < 32; i += 2) w[i >> 1] = pack_bf16x2(v[i], v[i + 1]);
+      store_block(w, col0, m0 + q * 32);
     } else if constexpr (EPI == EPI_STORE_BF16) {
       if (row_ok) {
         uint32_t w[16];
@@ -977,21 +951,13 @@ constexpr uint32_t kWideSmemBytes = kWideStages * kWideStageBytes + 1024;
 // DLOGITS adds one 32 x 32 bf16 staging tile per epilogue warp for the TMA stores of dS.
 constexpr uint32_t kWideDsSmemBytes = kWideSmemBytes + kWideEpiWarps * kDsStageBytes;
 static_assert(kWideDsSmemBytes <= 232448 - 256, "wide DLOGITS kernel exceeds the shared memory of a CTA");
-// EPI_STORE_TMA reduces over few K blocks and writes much, and what bounds it is the rows that TMA stores
-// take apart: it trades a ring stage for staging tiles of 64 columns, 128-byte rows (dW of 96 rows x 1024,
-// 311 MB: 93 us with 64-byte rows, 161 us with stores from registers).
-constexpr int wide_stages(int epi) { return epi == EPI_STORE_TMA ? kWideStages - 1 : kWideStages; }
-constexpr uint32_t wide_staging(int epi) { return epi == EPI_STORE_TMA ? 2 * kDsStageBytes : kDsStageBytes; }
-static_assert((kWideStages - 1) * kWideStageBytes + kWideEpiWarps * 2 * kDsStageBytes + 1024 <= kWideDsSmemBytes,
-              "the wider staging tiles fit the stage given up");
 
 template <int EPI, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kWideThreads, 1)
     lmhead_gemm_wide_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                             const __grid_constant__ CUtensorMap tmC, const GemmParams p) {
-  constexpr int kSt = wide_stages(EPI);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[kSt], empty_bar[kSt], acc_full[2], acc_empty[2], drain_bar;
+  __shared__ __align__(8) uint64_t full_bar[kWideStages], empty_bar[kWideStages], acc_full[2], acc_empty[2], drain_bar;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
 
@@ -1017,7 +983,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSt; ++s) {
+    for (int s = 0; s < kWideStages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
@@ -1095,15 +1061,15 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                   tma_load_2d_pair_hint(bh + c * kMnAtomBytes, &tmB, fb_leader, nb + 64 * c, k0, pol_b);
               }
             }
-            if (++stage == kSt) { stage = 0; phase ^= 1u; }
+            if (++stage == kWideStages) { stage = 0; phase ^= 1u; }
           }
         }
       }
       if (p.lockstep != nullptr && rank == 0) st_relaxed_u32(p.lockstep + pair_id, kPaceDone);
       if (ok) {
-        for (int s = 0; s < kSt; ++s) {
+        for (int s = 0; s < kWideStages; ++s) {
           if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_v, p.err, kErrTimeoutProducer)) break;
-          if (++stage == kSt) { stage = 0; phase ^= 1u; }
+          if (++stage == kWideStages) { stage = 0; phase ^= 1u; }
         }
       } else {
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
@@ -1149,7 +1115,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           tc_fence_after();
           // The first half of the accumulator is free: run its MMAs over the K blocks already
           // staged while the epilogue still drains the second half.
-          const int look = min(kSt, nk);
+          const int look = min(kWideStages, nk);
           {
             int st = stage;
             uint32_t ph = phase;
@@ -1157,7 +1123,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
               if (!mbar_wait(smem_u32(&full_bar[st]), ph, abort_v, p.err, kErrTimeoutMma)) { ok = false; break; }
               tc_fence_after();
               issue_half(st, kb, 0);
-              if (++st == kSt) { st = 0; ph ^= 1u; }
+              if (++st == kWideStages) { st = 0; ph ^= 1u; }
             }
           }
           if (!ok) break;
@@ -1175,19 +1141,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           for (int kb = 0; kb < look; ++kb) {
             issue_half(stage, kb, 1);
             release_stage(stage);
-            if (++stage == kSt) { stage = 0; phase ^= 1u; }
+            if (++stage == kWideStages) { stage = 0; phase ^= 1u; }
           }
           // The last `tail` K blocks run first-half-first: the first half is final while the
           // second half's last MMAs still run, so the epilogue drains it and releases it for the
           // next tile without idling the tensor pipe.
-          const int tail = min(min(p.split_tail, kSt), nk - look);
+          const int tail = min(min(p.split_tail, kWideStages), nk - look);
           for (int kb = look; kb < nk - tail; ++kb) {
             if (!mbar_wait(smem_u32(&full_bar[stage]), phase, abort_v, p.err, kErrTimeoutMma)) { ok = false; break; }
             tc_fence_after();
             issue_half(stage, kb, 0);
             issue_half(stage, kb, 1);
             release_stage(stage);
-            if (++stage == kSt) { stage = 0; phase ^= 1u; }
+            if (++stage == kWideStages) { stage = 0; phase ^= 1u; }
           }
           if (!ok) break;
           if (tail > 0) {
@@ -1197,14 +1163,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
               if (!mbar_wait(smem_u32(&full_bar[st]), ph, abort_v, p.err, kErrTimeoutMma)) { ok = false; break; }
               tc_fence_after();
               issue_half(st, kb, 0);
-              if (++st == kSt) { st = 0; ph ^= 1u; }
+              if (++st == kWideStages) { st = 0; ph ^= 1u; }
             }
             if (!ok) break;
             commit_full(0);
             for (int kb = nk - tail; kb < nk; ++kb) {
               issue_half(stage, kb, 1);
               release_stage(stage);
-              if (++stage == kSt) { stage = 0; phase ^= 1u; }
+              if (++stage == kWideStages) { stage = 0; phase ^= 1u; }
             }
           } else if (look < nk) {
             commit_full(0);
@@ -1222,7 +1188,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const uint32_t af[2] = {smem_u32(&acc_full[0]), smem_u32(&acc_full[1])};
     const uint32_t ae[2] = {mapa_shared(smem_u32(&acc_empty[0]), 0), mapa_shared(smem_u32(&acc_empty[1]), 0)};
     const uint32_t stage = (is_staged(EPI) && p.ds_tma)
-                               ? smem_base + kSt * kWideStageBytes + (uint32_t)(warp - 2) * wide_staging(EPI)
+                               ? smem_base + kWideStages * kWideStageBytes + (uint32_t)(warp - 2) * kDsStageBytes
                                : 0u;
     int jb = 0;
     for (int u = pair_id; u < nunits; u += npairs) {
@@ -1366,9 +1332,7 @@ int make_tmap(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, 
 // Tensor map for the wide kernel's TMA stores of dS: bf16 [outer, inner] with row stride `ld`
 // elements, 32 x 32 boxes (64-byte rows) in the 64-byte swizzled shared-memory layout.  Stores clip
 // at the inner and outer extents.
-// cols = 64: 32 x 64 boxes (128-byte rows) in the 128-byte swizzled layout.
-int make_store_tmap(CUtensorMap* m, void* base, uint64_t inner, uint64_t outer, uint64_t ld, const char* what,
-                    uint32_t cols = 32) {
+int make_store_tmap(CUtensorMap* m, void* base, uint64_t inner, uint64_t outer, uint64_t ld, const char* what) {
   EncodeTiledFn fn = encode_fn();
   IKRL_REQUIRE(fn != nullptr, IKRL_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
   IKRL_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, IKRL_ERR_ALIGNMENT,
@@ -1377,10 +1341,10 @@ int make_store_tmap(CUtensorMap* m, void* base, uint64_t inner, uint64_t outer, 
                (unsigned long long)ld);
   const cuuint64_t dims[2] = {inner, outer};
   const cuuint64_t strides[1] = {ld * 2};
-  const cuuint32_t box[2] = {cols, 32};
+  const cuuint32_t box[2] = {32, 32};
   const cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   IKRL_REQUIRE(r == CUDA_SUCCESS, IKRL_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
   return IKRL_OK;
 }
@@ -2407,14 +2371,15 @@ static int check_grad_alignment(const char* what, const void* dhidden, const voi
   return IKRL_OK;
 }
 
-// A bf16 dW of few rows: mostly its output, which leaves through TMA stores of the wide
-// kernel, where that may run.
+// A bf16 dW of few rows: mostly its output, which leaves through TMA stores of the wide kernel, where that
+// may run (two terms of 96 rows x 1024 for 151936 columns, 311 MB: 100 us; a plain fill of as much takes 88 us,
+// and one term with stores from registers took 161 us).
 static int launch_short_dw(const CUtensorMap& ta, const CUtensorMap& tb, GemmParams& p, void* dweight,
                            cudaStream_t s) {
   const int v_tiles = (int)cdiv64(p.M, BM);
   if (use_pairs() && tuning(IKRL_TUNE_WIDE) != 0) {
     CUtensorMap tc;
-    const int rc = make_store_tmap(&tc, dweight, p.N, p.M, p.N, "dW store", 64);
+    const int rc = make_store_tmap(&tc, dweight, p.N, p.M, p.N, "dW store");
     if (rc) return rc;
     return launch_k1<EPI_STORE_TMA, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s, &tc);
   }
@@ -2698,7 +2663,8 @@ static int check_row_cache(const char* what, int64_t N, int V, const RowCacheArg
   return IKRL_OK;
 }
 
-// Forward of a row loss through the LM head: the rows' entries, the rows that count gathered, the GEMM with the TAIL epilogue, the losses.
+// Forward of a row loss through the LM head: the rows' entries, the rows that count gathered, the GEMM with
+// the TAIL epilogue, the losses.
 static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void* weight, const int64_t* tids,
                                const float* tlp, int64_t N, int32_t H, int32_t V, int32_t K, const RowLossParams& P,
                                float* loss, void* state, size_t state_bytes, const RowCacheArgs& cache, void* ws,
