@@ -290,12 +290,9 @@ typedef struct {
 
 /* A teacher's top log-probs: the K largest logits of each row (1 <= K <= 256, K <= V), largest first,
  * of equal ones the lower column first, NaN before all: ids int64 [N][K] and logp fp32 [N][K] =
- * log softmax(x / temperature) over the whole row.  logits as below; the workspace (256-byte aligned)
- * may be NULL where its size is 0 (few rows). */
-IKRL_API size_t ikrl_logits_topk_workspace_bytes(int32_t dtype, int64_t N, int32_t V);
+ * log softmax(x / temperature) over the whole row.  logits as below. */
 IKRL_API int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V, int32_t K,
-                              float temperature, float* logp, int64_t* ids, void* ws, size_t ws_bytes,
-                              void* stream);
+                              float temperature, float* logp, int64_t* ids, void* stream);
 
 /* Bytes of the row state a forward writes and its backward reads (256-byte aligned, caller-owned):
  * K entries a row, K = 1 for a cross entropy. */

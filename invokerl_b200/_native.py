@@ -145,10 +145,9 @@ _SIGNATURES: dict[str, tuple] = {
         [_P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int64, _P, _P, c_int32, c_int32, _P, c_size_t, _P],
     ),
     "ikrl_row_loss_state_bytes": (c_size_t, [c_int64, c_int32]),
-    "ikrl_logits_topk_workspace_bytes": (c_size_t, [c_int32, c_int64, c_int32]),
     "ikrl_logits_topk": (
         ctypes.c_int,
-        [_P, c_int32, c_int64, c_int64, c_int32, c_int32, c_float, _P, _P, _P, c_size_t, _P],
+        [_P, c_int32, c_int64, c_int64, c_int32, c_int32, c_float, _P, _P, _P],
     ),
     "ikrl_logits_distill_fwd": (
         ctypes.c_int,

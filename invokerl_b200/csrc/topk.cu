@@ -1,15 +1,13 @@
 // The k likeliest tokens of each row of logits and their log-probs over the whole vocabulary: what
 // a teacher gives a distillation.
 //
-// One pass over the row, bound by HBM.  Beside the running logsumexp, a block notes the groups of
-// eight columns whose maximum reaches a bar, a lower bound of the k-th largest value: the k-th largest
-// of the threads' own maxima so far, found bit by bit with block-wide counts and raised after 1, 3,
-// 7, 15, ... rounds of 16384 columns.  With 512 threads that bound is nearly the k-th largest itself,
-// so of V columns in no particular order about k (1 + log2(V / 16384)) groups are noted.  They are read
-// again (from L2), their columns above the last bar go to a buffer of keys, and the buffer is sorted.
-// Where a list does not hold the noted groups (rising rows, many equal values) the row is swept again,
-// working the list off on the way and cutting the keys to the k largest, which raises the bar to the
-// k-th key itself.
+// One pass over the row, bound by HBM.  Beside the running logsumexp a thread keeps the largest value of
+// each of its rounds (U groups of eight columns) in shared memory.  Behind up to kTopRounds rounds a bar is
+// set, a lower bound of the K-th largest value: the K-th largest of the threads' own maxima (of 512, so it
+// is nearly the K-th largest itself: in a random order 512 ln(512 / (512 - K)) columns reach it).  The rounds
+// whose maximum reaches the bar are read again, from L2, and their columns above it go to a buffer of keys.
+// Where the buffer fills (many equal values) it is sorted and cut to its K largest, which raises the bar
+// to the K-th key itself.
 //
 // Order and ties are those of one 64-bit key, the value above the inverted column: larger values
 // first, of equal values the lower column.  Keys are distinct, so the result does not depend on the
@@ -24,10 +22,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kTopThreads = 512;
-constexpr int kTopBuf = 2048;  // keys of the buffer: the cluster's 8 x kMaxEntries at the end
-constexpr int kTopList = 4096;  // noted groups
-static_assert(kTopBuf >= 8 * kMaxEntries && kTopBuf >= 2 * kMaxEntries, "top-k buffer too small");
+constexpr int kTopThreads = 512;  // threads that sweep
+constexpr int kTopBuf = 2048;     // keys of the buffer
+constexpr int kTopRounds = 12;    // rounds between two bars
+constexpr int kTopList = 1024;    // rounds to be read again at a time
+static_assert(kTopBuf >= 8 * kMaxEntries, "the buffer holds K keys of each block of a cluster");
+static_assert(kTopRounds * kTopThreads < 0xfffe, "list entries are 16 bits");
 
 // Values in key order: NaN first, -0 as +0.
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -39,455 +39,516 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   if (k == 0xffffffffu) return nan_f32();
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+__device__ __forceinline__ uint16_t key16(float x) { return (uint16_t)(value_key(x) >> 16); }
 
-// Sort s[0, n) descending, n a power of two; the keys behind `have` count as 0.  Bitonic: up to one key a
-// thread, the exchanges inside a warp are shuffles and only those between warps go through memory.
-__device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
-  const int t = (int)threadIdx.x;
-  if (n <= kTopThreads) {
-    uint64_t x = t < have ? s[t] : 0;
-    for (int k = 2; k <= n; k <<= 1) {
-      const bool down = (t & k) == 0;
-      int j = k >> 1;
-      for (; j >= 32; j >>= 1) {
-        __syncthreads();
-        if (t < n) s[t] = x;
-        __syncthreads();
-        if (t < n) {
-          const uint64_t y = s[t ^ j];
-          if (((t & j) == 0) == down ? x < y : x > y) x = y;
-        }
-      }
-      if ((t & ~31) < n) {  // whole warps
-        for (; j > 0; j >>= 1) {
-          const uint64_t y = __shfl_xor_sync(0xffffffffu, x, j);
-          if (((t & j) == 0) == down ? x < y : x > y) x = y;
-        }
-      }
-    }
-    __syncthreads();
-    if (t < n) s[t] = x;
-    __syncthreads();
-    return;
+__device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// N threads from thread FROM of the block on that choose keys together, with barrier ID.
+template <int FROM, int N_, int ID>
+struct Team {
+  static constexpr int N = N_;
+  static __device__ __forceinline__ int tid() { return (int)threadIdx.x - FROM; }
+  static __device__ __forceinline__ void sync() {
+    asm volatile("barrier.cta.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
   }
-  for (int i = have + t; i < n; i += kTopThreads) s[i] = 0;
-  __syncthreads();
+  static __device__ __forceinline__ bool any(bool x) {
+    int r;
+    asm volatile(
+        "{\n.reg .pred a, b;\nsetp.ne.s32 a, %1, 0;\nbarrier.cta.red.or.pred b, %2, %3, a;\n"
+        "selp.s32 %0, 1, 0, b;\n}"
+        : "=r"(r)
+        : "r"((int)x), "n"(ID), "n"(N)
+        : "memory");
+    return r != 0;
+  }
+};
+
+// Sort s[0, n) descending (bitonic), n a power of two; the keys behind `have` count as 0.
+template <typename Tm>
+__device__ __forceinline__ void sort_keys(uint64_t* s, int have, int n) {
+  for (int i = have + Tm::tid(); i < n; i += Tm::N) s[i] = 0;
+  Tm::sync();
   for (int k = 2; k <= n; k <<= 1) {
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = t; i < (n >> 1); i += kTopThreads) {
+      for (int i = Tm::tid(); i < (n >> 1); i += Tm::N) {
         const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
         const uint64_t x = s[a], y = s[b];
-        const bool down = (a & k) == 0;
-        if ((x < y) == down) {
+        if ((x < y) == ((a & k) == 0)) {
           s[a] = y;
           s[b] = x;
         }
       }
-      __syncthreads();
+      // pairs up to 32 apart lie in the 64 keys that a warp exchanges
+      if (j > 32 || (j == 1 && (k >= 64 || k == n))) Tm::sync();
+      else __syncwarp();
     }
   }
 }
 
-__device__ __forceinline__ int pow2_at_least(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
-
-// The lower bound that decides which groups are noted.
-struct Bar {
-  uint64_t key = 0;  // keys at or below it are out
-  float value = -INFINITY;
-  // To the largest value (16 bits of its key) that at least K threads' maxima reach.
-  __device__ __forceinline__ void raise(bool any, float mine, int K) {
-    const uint32_t key_mine = any ? value_key(mine) : 0u;
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t cand = t | (1u << bit);
-      if (__syncthreads_count(key_mine >= cand) >= K) t = cand;
-    }
-    const uint64_t found = t > 0 ? ((uint64_t)t << 32) - 1 : 0;  // values equal to it stay in
-    if (found > key) {
-      key = found;
-      value = key_value(t);
-    }
-  }
-};
-
-// One sweep of a block over its part: the running sums, the bar, and note(j, top) for each group whose
-// maximum `top` reaches it (NaN: the group may hold a NaN), then end_round() by all threads.  The bar is
-// raised once more at the end: what it then leaves of the noted groups is little more than K columns.
-template <typename T, int U, typename Note, typename End>
-__device__ __forceinline__ void sweep_part(const RowPart<T>& p, int K, float c, float& m, float& s, Bar& bar,
-                                           Note note, End end_round) {
-  constexpr int kRound = U * kTopThreads;
-  const int tid = (int)threadIdx.x;
-  float mine = -INFINITY;  // the largest value of this thread, NaN aside
-  bool any = false;        // this thread had a column
-  m = -INFINITY;
-  s = 0.f;
-  int round = 0, next_bar = 0;
-  int jb = p.a;
-  for (; jb + kRound <= p.b; jb += kRound, ++round) {
-    Group8<T> g[U];
+// The largest t that at least K of a warp's 16-bit values v[N] of each lane reach: bit by bit behind the
+// bits that all of them share.  At least K values.
+template <int N>
+__device__ __forceinline__ uint32_t kth_of_warp(const uint32_t (&v)[N], int K) {
+  uint32_t any = 0, all = 0xffffu;
 #pragma unroll
-    for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kTopThreads + tid));
-    float top[U];
-    online_groups<T, U>(g, c, m, s, top);
-    any = true;
-    float mx = top[0];
+  for (int i = 0; i < N; ++i) {
+    any |= v[i];
+    all &= v[i];
+  }
+  any = __reduce_or_sync(0xffffffffu, any);
+  all = __reduce_and_sync(0xffffffffu, all);
+  uint32_t bit = any ^ all;  // of these the highest
+  bit = bit ? 1u << (31 - __clz(bit)) : 0u;
+  uint32_t t = bit ? all & ~(2 * bit - 1) : all;
+  for (; bit; bit >>= 1) {
+    const uint32_t cand = t | bit;
+    int cnt = 0;
 #pragma unroll
-    for (int u = 1; u < U; ++u) mx = fmaxf(mx, top[u]);
-    mine = fmaxf(mine, mx);
-    if (round == next_bar) {
-      bar.raise(any, mine, K);
-      next_bar = 2 * next_bar + 2;
-    }
-    // any group counts once a NaN or +inf came by (s is NaN then)
-    if (!(mx < bar.value && s == s)) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (!(top[u] < bar.value && s == s)) note(jb + u * kTopThreads + tid, s == s ? top[u] : nan_f32());
-    }
-    end_round();
+    for (int i = 0; i < N; ++i) cnt += v[i] >= cand;
+    if (__reduce_add_sync(0xffffffffu, cnt) >= K) t = cand;
   }
-  // what is left, a group a thread at a time: whole groups, then those that reach past the row
-  auto single = [&](int j) {
-    Group8<T> h[1];
-    float top[1] = {-INFINITY};
-    if (j >= 0) {
-      load_group(h[0], p.rv, j);
-      online_groups<T, 1>(h, c, m, s, top);
-      any = true;
-      mine = fmaxf(mine, top[0]);
-    }
-    if (round++ == 0) bar.raise(any, mine, K);
-    if (j >= 0 && !(top[0] < bar.value && s == s)) note(j, s == s ? top[0] : nan_f32());
-    end_round();
-  };
-  for (; jb < p.b; jb += kTopThreads) single(jb + tid < p.b ? jb + tid : -1);
-  if (p.a > p.j0 || p.b < p.j1) single(p.edge(kTopThreads - 1 - tid));
-  if (round > 2) bar.raise(any, mine, K);
-}
-
-// Columns of the groups list[0, n) above the bar into the buffer of keys (s_cnt of them).
-template <typename T>
-__device__ __forceinline__ void absorb(const RowView<T>& rv, const int* list, int n, int K, Bar& bar, uint64_t* s_buf,
-                                       int* s_cnt) {
-  const int tid = (int)threadIdx.x;
-  for (int b = 0; b < n; b += kTopThreads) {
-    Group8<T> g;
-    int v0 = 0;
-    uint32_t pend = 0;
-    auto key_of = [&](int k) {
-      return ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
-    };
-    if (b + tid < n) {
-      const int j = list[b + tid];
-      load_group(g, rv, j);
-      v0 = rv.first(j);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (v0 + k >= 0 && v0 + k < rv.V && key_of(k) > bar.key) pend |= 1u << k;
-    }
-    while (true) {
-      if (pend) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (!((pend >> k) & 1u)) continue;
-          const int at = atomicAdd(s_cnt, 1);
-          if (at < kTopBuf) {
-            s_buf[at] = key_of(k);
-            pend &= ~(1u << k);
-          }
-        }
-      }
-      if (!__syncthreads_or(pend != 0)) break;
-      // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
-      sort_keys(s_buf, kTopBuf, kTopBuf);
-      bar.key = s_buf[K - 1];
-      bar.value = key_value((uint32_t)(bar.key >> 32));
-      if (tid == 0) *s_cnt = K;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (((pend >> k) & 1u) && key_of(k) <= bar.key) pend &= ~(1u << k);
-      __syncthreads();
-    }
-  }
-}
-
-struct TopShared {
-  uint64_t buf[kTopBuf];
-  int list[kTopList];
-  float red[64];
-  float m, s;
-  int cnt, noted;
-};
-
-// A block's part of a row: its sums and, in sh.buf, keys (their number is returned, at most `limit`) that
-// hold its K largest, in no order.  The first sweep assumes that the list holds every noted group and has no barrier but those of the bar;
-// where it did not, a second one looks after every round and works the list off in between.
-template <typename T, int U>
-__device__ __forceinline__ int part_topk(const RowPart<T>& p, int K, float c, int limit, float& m, float& s,
-                                         TopShared& sh) {
-  constexpr int kRound = U * kTopThreads;
-  static_assert(kTopList >= 2 * kRound, "the list holds a round behind its limit");
-  const int tid = (int)threadIdx.x;
-  Bar bar;
-  auto work_off = [&]() {
-    __syncthreads();
-    absorb(p.rv, sh.list, sh.noted, K, bar, sh.buf, &sh.cnt);
-    __syncthreads();
-    if (tid == 0) sh.noted = 0;
-    __syncthreads();
-  };
-  for (bool careful = false;; careful = true) {
-    if (tid == 0) sh.cnt = sh.noted = 0;
-    __syncthreads();
-    bool full = false;
-    sweep_part<T, U>(
-        p, K, c, m, s, bar,
-        [&](int j, float) {
-          const int at = atomicAdd(&sh.noted, 1);
-          if (at < kTopList) sh.list[at] = j;
-          full |= at >= kTopList - kRound - 1;
-        },
-        [&]() {
-          if (careful && __syncthreads_or(full)) {
-            work_off();
-            full = false;
-          }
-        });
-    __syncthreads();
-    if (careful || sh.noted <= kTopList) break;
-    __syncthreads();  // noted is read before it is cleared
-  }
-  work_off();
-  block_online_merge(c, m, s, sh.red);
-  if (tid == 0) {  // one thread's rounding for all: which thread writes an output depends on timing
-    sh.m = m;
-    sh.s = s;
-  }
-  __syncthreads();
-  m = sh.m;
-  s = sh.s;
-  const int have = min(sh.cnt, kTopBuf);
-  if (have <= limit) return have;
-  sort_keys(sh.buf, have, pow2_at_least(have));
-  return K;
-}
-
-// The K largest of n keys (n >= K) as a row's output: a key's place is the number of keys above it.
-template <int THREADS>
-__device__ __forceinline__ void write_topk(const uint64_t* keys, int n, int K, float m, float s, float inv_t,
-                                           float* __restrict__ logp, int64_t* __restrict__ ids) {
-  const float ls = log2f(s) * kLn2;
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t key = keys[i];
-    int place = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) place += keys[j] > key;
-    if (place >= K) continue;
-    const float x = key_value((uint32_t)(key >> 32));
-    logp[place] = (x - m) * inv_t - ls;
-    ids[place] = (int64_t)(0xffffffffu - (uint32_t)key);
-  }
-}
-
-// Few rows: one launch, a cluster of blocks a row (one block when it is short).
-template <typename T, int U>
-__global__ void __launch_bounds__(kTopThreads, 2) logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int V,
-                                                                     int K, float c, float inv_t,
-                                                                     float* __restrict__ logp,
-                                                                     int64_t* __restrict__ ids) {
-  __shared__ TopShared sh;
-  __shared__ float s_part[2][8];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t r = blockIdx.x / C;
-  const RowPart<T> p(logits, ld, r, V, rank, C);
-  __shared__ int s_have[8];
-  float m, s;
-  int have = part_topk<T, U>(p, K, c, kTopBuf / C, m, s, sh);
-  if (C > 1) {
-    // Every block's keys go to the first one, behind those of the blocks before it.
-    cluster.sync();
-    if (threadIdx.x < C) cluster.map_shared_rank(s_have, threadIdx.x)[rank] = have;
-    if (threadIdx.x == 0) {
-      float* part = cluster.map_shared_rank(&s_part[0][0], 0);
-      part[rank] = m;
-      part[8 + rank] = s;
-    }
-    cluster.sync();
-    int before = 0, total = 0;
-    for (int q = 0; q < C; ++q) {
-      before += q < rank ? s_have[q] : 0;
-      total += s_have[q];
-    }
-    if (rank > 0) {
-      uint64_t* dst = cluster.map_shared_rank(sh.buf, 0);
-      for (int i = threadIdx.x; i < have; i += kTopThreads) dst[before + i] = sh.buf[i];
-    }
-    cluster.sync();
-    if (rank != 0) return;
-    have = total;
-    m = -INFINITY;
-    s = 0.f;
-    for (int q = 0; q < C; ++q) online_merge(c, m, s, s_part[0][q], s_part[1][q]);
-  }
-  write_topk<kTopThreads>(sh.buf, have, K, m, s, inv_t, logp + r * K, ids + r * K);
-}
-
-// Many rows.  One launch sweeps parts of rows and leaves, per part, its sums, its bar and the groups it
-// noted; blocks end with the sweep, so the memory never waits for a choice.  The next picks each row's K
-// largest out of the noted groups, all rows at once, and a last one takes the rows (hardly any) whose
-// lists did not hold them.
-struct TopNotes {
-  int2* list;     // [N parts][kNoteCap] group and its maximum
-  int* count;     // [N parts] noted groups; above kNoteCap: some are missing, the row is swept again
-  uint64_t* bar;  // [N parts]
-  float* part;    // [2][N parts] maxima and sums
-};
-constexpr int kNoteCap = 2048;
-
-inline size_t top_notes_bytes(int64_t parts) {
-  auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
-  return al((size_t)parts * kNoteCap * 8) + al((size_t)parts * 4) + 2 * al((size_t)parts * 8);
-}
-inline TopNotes top_notes(void* ws, int64_t parts) {
-  auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
-  char* p = reinterpret_cast<char*>(ws);
-  TopNotes t;
-  t.list = reinterpret_cast<int2*>(p); p += al((size_t)parts * kNoteCap * 8);
-  t.count = reinterpret_cast<int*>(p); p += al((size_t)parts * 4);
-  t.bar = reinterpret_cast<uint64_t*>(p); p += al((size_t)parts * 8);
-  t.part = reinterpret_cast<float*>(p);
   return t;
 }
 
-template <typename T, int U, int MINB>
-__global__ void __launch_bounds__(kTopThreads, MINB) topk_note_kernel(const T* __restrict__ logits, int64_t ld, int V,
-                                                                      int K, int segs, float c, int64_t parts,
-                                                                      TopNotes notes) {
-  __shared__ float s_red[64];
-  __shared__ int s_noted;
-  const int64_t q = blockIdx.x, r = q / segs;
-  const RowPart<T> p(logits, ld, r, V, (int)(q - r * segs), segs);
-  if (threadIdx.x == 0) s_noted = 0;
-  __syncthreads();
-  Bar bar;
-  float m, s;
-  int2* list = notes.list + q * kNoteCap;
-  sweep_part<T, U>(
-      p, K, c, m, s, bar,
-      [&](int j, float top) {
-        const int at = atomicAdd(&s_noted, 1);
-        if (at < kNoteCap) list[at] = make_int2(j, __float_as_int(top));
-      },
-      []() {});
-  block_online_merge(c, m, s, s_red);  // its barrier also closes s_noted
-  if (threadIdx.x == 0) {
-    notes.count[q] = s_noted;
-    notes.bar[q] = bar.key;
-    notes.part[q] = m;
-    notes.part[parts + q] = s;
-  }
-}
+// What a sweep leaves of up to kTopRounds rounds.
+struct TopSweep {
+  uint16_t top[kTopRounds * kTopThreads];  // key16 of each round's maximum; NaN once one (or +inf) came by
+  uint16_t mine[kTopThreads];              // key16 of the threads' maxima so far in this row
+  float m[kTopThreads / 32], s[kTopThreads / 32];
+};
 
-// A row's K largest out of its noted groups.  Rows with missing groups, or with more columns above the bar
-// than the buffer holds, are left to topk_again_kernel: their first part's count says so.
-constexpr int kSelectThreads = 256;
-constexpr int kSelectBuf = 2048;
-template <typename T>
-__global__ void __launch_bounds__(kSelectThreads) topk_select_kernel(const T* __restrict__ logits, int64_t ld, int V,
-                                                                     int K, int segs, float c, float inv_t,
-                                                                     int64_t parts, TopNotes notes,
-                                                                     float* __restrict__ logp,
-                                                                     int64_t* __restrict__ ids) {
-  __shared__ uint64_t s_buf[kSelectBuf];
-  __shared__ int s_cnt;
-  const int64_t r = blockIdx.x, q0 = r * segs;
-  if (threadIdx.x == 0) s_cnt = 0;
-  float m = -INFINITY, s = 0.f;
-  uint64_t bar = 0;
-  bool missing = false;
-  for (int q = 0; q < segs; ++q) {
-    online_merge(c, m, s, notes.part[q0 + q], notes.part[parts + q0 + q]);
-    bar = max(bar, notes.bar[q0 + q]);  // each is below the K-th largest of its part
-    missing |= notes.count[q0 + q] > kNoteCap;
-  }
-  if (missing) {
-    if (threadIdx.x == 0) notes.count[q0] = kNoteCap + 1;
-    return;
-  }
-  __syncthreads();
-  const RowView<T> rv(logits, ld, r, V);
-  for (int q = 0; q < segs; ++q) {
-    const int n = notes.count[q0 + q];
-    for (int i = threadIdx.x; i < n; i += kSelectThreads) {
-      const int2 note = notes.list[(q0 + q) * kNoteCap + i];
-      const float top = __int_as_float(note.y);
-      if (top == top && value_key(top) < (uint32_t)(bar >> 32)) continue;  // nothing in it above the bar
-      Group8<T> g;
-      load_group(g, rv, note.x);
-      const int v0 = rv.first(note.x);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint64_t key = ((uint64_t)value_key(g.get(k)) << 32) | (0xffffffffu - (uint32_t)(v0 + k));
-        if (v0 + k < 0 || v0 + k >= V || key <= bar) continue;
-        const int at = atomicAdd(&s_cnt, 1);
-        if (at < kSelectBuf) s_buf[at] = key;
-      }
+template <typename Tm>
+struct TopKeys {
+  uint64_t key[kTopBuf];
+  uint16_t list[kTopList + 8 * Tm::N];  // round * kTopThreads + thread, or 0xfffe + t for edge t
+  int cnt, listed;
+  uint32_t kth;
+};
+
+// The lower bound that decides which columns come into question.
+struct Bar {
+  uint64_t key = 0;  // keys at or below it are out
+  float value = -INFINITY;
+  __device__ __forceinline__ void raise(uint64_t to, float v) {
+    if (to > key) {
+      key = to;
+      value = v;
     }
   }
-  __syncthreads();
-  const int have = s_cnt;
-  if (have > kSelectBuf) {
-    if (threadIdx.x == 0) notes.count[q0] = kNoteCap + 1;
-    return;
-  }
-  write_topk<kSelectThreads>(s_buf, have, K, m, s, inv_t, logp + r * K, ids + r * K);
+};
+
+// One round: the running sums, and its largest value.  done(u): see online_groups.
+template <typename T, int U, typename Done>
+__device__ __forceinline__ uint16_t sweep_round(Group8<T> (&g)[U], float c, float& m, float& s, float& mine,
+                                                Done done) {
+  float top[U];
+  online_groups<T, U>(g, c, m, s, top, done);
+  float mx = top[0];
+#pragma unroll
+  for (int u = 1; u < U; ++u) mx = fmaxf(mx, top[u]);
+  mine = fmaxf(mine, mx);
+  return s == s ? key16(mx) : (uint16_t)0xffff;
 }
 
+// Groups that reach past the row (p.edge), by the last two of the threads that sweep.
+template <typename T>
+__device__ __forceinline__ void sweep_edge(const RowPart<T>& p, float c, float& m, float& s, float& mine) {
+  const int j = p.edge(kTopThreads - 1 - (int)threadIdx.x);
+  if (j < 0) return;
+  Group8<T> g[1];
+  load_group(g[0], p.rv, j);
+  float top[1];
+  online_groups<T, 1>(g, c, m, s, top, [](int) {});
+  mine = fmaxf(mine, top[0]);
+}
+
+template <int N>
+__device__ __forceinline__ void warp_online_merge(float c, float& m, float& s) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1)
+    online_merge(c, m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+}
+
+// Word i of w, without memory.
+template <int N>
+__device__ __forceinline__ uint32_t pick(const uint32_t (&w)[N], int i) {
+  uint32_t x = w[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) x = i == k ? w[k] : x;
+  return x;
+}
+
+// Columns above the bar of the n listed rounds into the buffer of keys, a round a thread.  start: first group
+// of round 0.
+template <typename Tm, typename T, int U>
+__device__ __forceinline__ void absorb(const RowPart<T>& p, int start, int n, int K, Bar& bar, TopKeys<Tm>& keys) {
+  constexpr int W = sizeof(T) == 2 ? 4 : 8;  // words of a group
+  const int tid = Tm::tid();
+  for (int b = 0; b < n; b += Tm::N) {
+    uint32_t w[U * W];
+    uint32_t pend = 0;
+    const bool on = b + tid < n;
+    const int e = on ? keys.list[b + tid] : 0;
+    int j0 = start + e / kTopThreads * (U * kTopThreads) + e % kTopThreads, j1 = on ? p.b : 0;
+    Group8<T> g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j0 + u * kTopThreads < j1) g[u].load(p.at(j0 + u * kTopThreads));
+      else g[u].fill();
+    }
+    if (e >= 0xfffe) {
+      j0 = p.edge(e - 0xfffe);
+      j1 = j0 + 1;
+      load_group(g[0], p.rv, j0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)  // a NaN counts
+        pend |= (j0 + u * kTopThreads < j1 && !(g[u].get(k) < bar.value) ? 1u : 0u) << (8 * u + k);
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[u * W + i] = g[u].w[i];
+    }
+    while (true) {
+      for (; pend; pend &= pend - 1) {
+        const int i = __ffs(pend) - 1;
+        const int v = p.rv.first(j0 + (i >> 3) * kTopThreads) + (i & 7);
+        float x;
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t two = pick(w, i >> 1);
+          x = (i & 1) ? bf16hi(two) : bf16lo(two);
+        } else {
+          x = __uint_as_float(pick(w, i));
+        }
+        const uint64_t key = ((uint64_t)value_key(x) << 32) | (0xffffffffu - (uint32_t)v);
+        if (v < 0 || v >= p.rv.V || key <= bar.key) continue;
+        const int at = atomicAdd(&keys.cnt, 1);
+        if (at >= kTopBuf) break;
+        keys.key[at] = key;
+      }
+      if (!Tm::any(pend != 0)) break;
+      // The buffer is full: keep its K largest, raise the bar, and try again with what is left.
+      sort_keys<Tm>(keys.key, kTopBuf, kTopBuf);
+      const uint64_t kth = keys.key[K - 1];
+      bar.raise(kth, key_value((uint32_t)(kth >> 32)));
+      if (tid == 0) keys.cnt = K;
+      Tm::sync();
+    }
+  }
+}
+
+// The columns that come into question of n swept rounds from group `start` on; `edges` with the edges of the
+// part.  The caller's barrier lies before it.
+template <typename Tm, typename T, int U>
+__device__ __forceinline__ void choose(const RowPart<T>& p, int start, int n, bool edges, int K, Bar& bar,
+                                       const TopSweep& sw, TopKeys<Tm>& keys) {
+  const int tid = Tm::tid();
+  if (tid < 32) {
+    const uint4* mine = reinterpret_cast<const uint4*>(sw.mine) + 2 * tid;
+    const uint4 a = mine[0], b = mine[1];
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    static_assert(kTopThreads == 32 * 16, "a warp reads all threads' maxima");
+    uint32_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+    const uint32_t t = kth_of_warp(v, K);
+    if (tid == 0) keys.kth = t;
+  }
+  Tm::sync();
+  if (const uint32_t t = keys.kth << 16; t > 0)
+    bar.raise(((uint64_t)t << 32) - 1, key_value(t));  // values equal to it stay in
+  if (edges && tid < 2 && p.edge(tid) >= 0) keys.list[atomicAdd(&keys.listed, 1)] = (uint16_t)(0xfffe + tid);
+  // Eight rounds' maxima a thread at a time; a warp numbers those that reach the bar.
+  const uint4* eight = reinterpret_cast<const uint4*>(sw.top);
+  const int lane = tid & 31, steps = n * (kTopThreads / 8);
+  static_assert(kTopThreads / 8 % 32 == 0, "whole warps");
+  int at = tid - lane;
+  bool more;
+  do {
+    const uint32_t least = (uint32_t)((bar.key + 1) >> 48);
+    for (; at < steps; at += Tm::N) {
+      const uint4 q = eight[at + lane];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      uint32_t hit = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        hit |= ((w[i] & 0xffffu) >= least ? 1u : 0u) << (2 * i);
+        hit |= ((w[i] >> 16) >= least ? 2u : 0u) << (2 * i);
+      }
+      const int cnt = __popc(hit);
+      int sum = cnt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const int total = __shfl_sync(0xffffffffu, sum, 31);
+      if (total == 0) continue;
+      int slot = 0;
+      if (lane == 0) slot = *(volatile int*)&keys.listed >= kTopList ? -1 : atomicAdd(&keys.listed, total);
+      slot = __shfl_sync(0xffffffffu, slot, 0);
+      if (slot < 0) break;  // the list is full: a step a warp may come on top of it
+      for (slot += sum - cnt; hit; hit &= hit - 1)
+        keys.list[slot++] = (uint16_t)(8 * (at + lane) + __ffs(hit) - 1);
+    }
+    more = Tm::any(at < steps);
+    absorb<Tm, T, U>(p, start, keys.listed, K, bar, keys);
+    Tm::sync();
+    if (tid == 0) keys.listed = 0;
+    Tm::sync();
+  } while (more);
+}
+
+// The K largest of n keys (n >= K) as a row's output.  A few keys are placed by counting the keys above each.
+template <typename Tm>
+__device__ __forceinline__ void write_topk(uint64_t* key, int n, int K, float m, float s, float inv_t,
+                                           float* __restrict__ logp, int64_t* __restrict__ ids) {
+  const float ls = log2f(s) * kLn2;
+  auto put = [&](int place, uint64_t k) {
+    logp[place] = (key_value((uint32_t)(k >> 32)) - m) * inv_t - ls;
+    ids[place] = (int64_t)(0xffffffffu - (uint32_t)k);
+  };
+  if (n * ((n + Tm::N - 1) / Tm::N) <= 320) {
+    for (int i = Tm::tid(); i < n; i += Tm::N) {
+      const uint64_t k = key[i];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) place += key[j] > k;
+      if (place < K) put(place, k);
+    }
+    return;
+  }
+  sort_keys<Tm>(key, n, pow2_at_least(n));
+  for (int i = Tm::tid(); i < K; i += Tm::N) put(i, key[i]);
+}
+
+// A block a row, or a cluster of blocks where there are few rows; the block that swept chooses.
 template <typename T, int U>
-__global__ void __launch_bounds__(kTopThreads, 2) topk_again_kernel(const T* __restrict__ logits, int64_t ld, int64_t N,
-                                                                    int V, int K, int segs, float c, float inv_t,
-                                                                    TopNotes notes, float* __restrict__ logp,
-                                                                    int64_t* __restrict__ ids) {
-  __shared__ TopShared sh;
-  bool any = false;
-  for (int64_t r = blockIdx.x + (int64_t)threadIdx.x * gridDim.x; r < N; r += (int64_t)gridDim.x * kTopThreads)
-    any |= notes.count[r * segs] > kNoteCap;
-  if (!__syncthreads_or(any)) return;
-  for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-    if (notes.count[r * segs] <= kNoteCap) continue;
-    float m, s;
-    const RowPart<T> p(logits, ld, r, V, 0, 1);
-    const int have = part_topk<T, U>(p, K, c, kTopBuf, m, s, sh);
-    write_topk<kTopThreads>(sh.buf, have, K, m, s, inv_t, logp + r * K, ids + r * K);
+__global__ void __launch_bounds__(kTopThreads, 3) topk_block_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                                                  int K, float c, float inv_t,
+                                                                  float* __restrict__ logp,
+                                                                  int64_t* __restrict__ ids) {
+  using Block = Team<0, kTopThreads, 0>;
+  constexpr int kRound = U * kTopThreads;
+  __shared__ __align__(16) TopSweep sw;
+  __shared__ TopKeys<Block> keys;
+  __shared__ float s_red[64], s_part[2][8];
+  __shared__ int s_have[8];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = (int)threadIdx.x;
+  const int64_t r = blockIdx.x / C;
+  const RowPart<T> p(logits, ld, r, V, rank, C);
+  if (tid == 0) keys.cnt = keys.listed = 0;
+  Bar bar;
+  float m = -INFINITY, s = 0.f, mine = -INFINITY;
+  sweep_edge(p, c, m, s, mine);
+  int jb = p.a;
+  do {
+    const int start = jb;
+    int n = 0;
+    for (; n < kTopRounds && jb < p.b; ++n, jb += kRound) {
+      Group8<T> g[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * kTopThreads + tid;
+        if (j < p.b) g[u].load(p.at(j));
+        else g[u].fill();
+      }
+      sw.top[n * kTopThreads + tid] = sweep_round<T, U>(g, c, m, s, mine, [](int) {});
+    }
+    sw.mine[tid] = key16(mine);
+    Block::sync();
+    choose<Block, T, U>(p, start, n, start == p.a, K, bar, sw, keys);
+  } while (jb < p.b);
+  block_online_merge(c, m, s, s_red);
+  if (tid == 0) {  // one thread's rounding for all: which thread writes an output depends on timing
+    s_part[0][0] = m;
+    s_part[1][0] = s;
+  }
+  __syncthreads();
+  int have = keys.cnt;
+  if (C == 1) {
+    write_topk<Block>(keys.key, have, K, s_part[0][0], s_part[1][0], inv_t, logp + r * K, ids + r * K);
+    return;
+  }
+  if (have > kTopBuf / C) {
+    sort_keys<Block>(keys.key, have, pow2_at_least(have));
+    have = K;
+  }
+  m = s_part[0][0];
+  s = s_part[1][0];
+  // Every block's keys go to the first one, behind those of the blocks before it.
+  cluster.sync();
+  if (tid < C) cluster.map_shared_rank(s_have, tid)[rank] = have;
+  if (tid == 0) {
+    float* part = cluster.map_shared_rank(&s_part[0][0], 0);
+    part[rank] = m;
+    part[8 + rank] = s;
+  }
+  cluster.sync();
+  int before = 0, total = 0;
+  for (int q = 0; q < C; ++q) {
+    before += q < rank ? s_have[q] : 0;
+    total += s_have[q];
+  }
+  if (rank > 0) {
+    uint64_t* dst = cluster.map_shared_rank(keys.key, 0);
+    for (int i = tid; i < have; i += kTopThreads) dst[before + i] = keys.key[i];
+  }
+  cluster.sync();
+  if (rank != 0) return;
+  m = -INFINITY;
+  s = 0.f;
+  for (int q = 0; q < C; ++q) online_merge(c, m, s, s_part[0][q], s_part[1][q]);
+  if (total > kMaxEntries) {  // what lies below the K-th largest of all (16 bits of it) goes first
+    uint64_t own[kTopBuf / kTopThreads];
+#pragma unroll
+    for (int i = 0; i < kTopBuf / kTopThreads; ++i) {
+      const bool ok = i * kTopThreads + tid < total;
+      own[i] = ok ? keys.key[i * kTopThreads + tid] : 0;
+    }
+    uint32_t t = 0;
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint64_t cand = (uint64_t)(t | (1u << bit)) << 48;
+      int reach = 0;
+#pragma unroll
+      for (int i = 0; i < kTopBuf / kTopThreads; ++i)
+        if (i * kTopThreads < total) reach += __syncthreads_count(own[i] >= cand);
+      if (reach >= K) t |= 1u << bit;
+    }
+    if (tid == 0) keys.cnt = 0;
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTopBuf / kTopThreads; ++i)
+      if (own[i] != 0 && own[i] >= ((uint64_t)t << 48)) keys.key[atomicAdd(&keys.cnt, 1)] = own[i];
+    __syncthreads();
+    total = keys.cnt;
+  }
+  write_topk<Block>(keys.key, total, K, m, s, inv_t, logp + r * K, ids + r * K);
+}
+
+// Many rows: resident blocks take row after row.  512 threads sweep and never stop for a choice: they hand
+// what they swept to 128 more, which choose and write the row's output while the next row is read.  Two
+// buffers between them; barriers 2, 3 say that one is full, 4, 5 that it is free.  Top 64 of 4096 rows of
+// 151936 bf16 columns: 256 us (4.9 TB/s), 244 us of it the sweep, where exponentials (63% of the special
+// function units' rate) and loads take turns; of 2048 fp32 rows 199 us (6.3 TB/s).
+constexpr int kChoosers = 128;
+constexpr int kStreamThreads = kTopThreads + kChoosers;
+template <typename T, int U>
+__global__ void __launch_bounds__(kStreamThreads, 2) topk_stream_kernel(const T* __restrict__ logits, int64_t ld, int64_t N,
+                                                                    int V, int K, float c, float inv_t,
+                                                                    float* __restrict__ logp,
+                                                                    int64_t* __restrict__ ids) {
+  using Choosers = Team<kTopThreads, kChoosers, 1>;
+  constexpr int kRound = U * kTopThreads;
+  __shared__ __align__(16) TopSweep sw[2];
+  __shared__ TopKeys<Choosers> keys;
+  const int tid = (int)threadIdx.x;
+  if (tid < kTopThreads) {
+    // g holds the next round: `left` groups from `src` (this thread's) to the end of its row
+    Group8<T> g[U];
+    const T* src = logits;
+    int left = 0;
+    auto load = [&](int u) {
+      if (left >= kRound) g[u].load(src + u * kTopThreads * 8);
+      else if (u * kTopThreads + tid < left) g[u].load(src + u * kTopThreads * 8);
+      else g[u].fill();
+    };
+    auto turn_to = [&](int64_t r) {
+      left = 0;
+      if (r >= N) return;
+      const RowPart<T> p(logits, ld, r, V, 0, 1);
+      left = p.b - p.a;
+      src = p.at(p.a + tid);
+    };
+    turn_to(blockIdx.x);
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u);
+    int unit = 0;
+    for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
+      float m = -INFINITY, s = 0.f, mine = -INFINITY;
+      sweep_edge(RowPart<T>(logits, ld, r, V, 0, 1), c, m, s, mine);
+      bool more = left > 0;
+      const bool none = !more;
+      do {
+        TopSweep& out = sw[unit & 1];
+        if (unit > 1) bar_sync(4 + (unit & 1), kStreamThreads);
+        for (int n = 0; n < kTopRounds && more; ++n) {
+          src += kRound * 8;
+          left -= kRound;
+          more = left > 0;
+          if (!more) turn_to(r + gridDim.x);
+          out.top[n * kTopThreads + tid] = sweep_round<T, U>(g, c, m, s, mine, load);
+        }
+        out.mine[tid] = key16(mine);
+        if (!more) {
+          float wm = m, ws = s;
+          warp_online_merge<32>(c, wm, ws);
+          if ((tid & 31) == 0) {
+            out.m[tid >> 5] = wm;
+            out.s[tid >> 5] = ws;
+          }
+        }
+        bar_arrive(2 + (unit & 1), kStreamThreads);
+        ++unit;
+      } while (more);
+      if (none) {  // no round of this row carried the next one's loads
+        turn_to(r + gridDim.x);
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(u);
+      }
+    }
+    return;
+  }
+  int unit = 0;
+  for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
+    const RowPart<T> p(logits, ld, r, V, 0, 1);
+    if (tid == kTopThreads) keys.cnt = keys.listed = 0;
+    Choosers::sync();
+    Bar bar;
+    int jb = p.a;
+    while (true) {
+      const TopSweep& in = sw[unit & 1];
+      bar_sync(2 + (unit & 1), kStreamThreads);
+      const int n = min(kTopRounds, (p.b - jb + kRound - 1) / kRound);
+      choose<Choosers, T, U>(p, jb, n, jb == p.a, K, bar, in, keys);
+      jb += n * kRound;
+      if (jb >= p.b) break;
+      bar_arrive(4 + (unit & 1), kStreamThreads);
+      ++unit;
+    }
+    float m = sw[unit & 1].m[tid & 15], s = sw[unit & 1].s[tid & 15];
+    warp_online_merge<16>(c, m, s);
+    m = __shfl_sync(0xffffffffu, m, 0);  // one rounding for all: which thread writes an output depends on timing
+    s = __shfl_sync(0xffffffffu, s, 0);
+    bar_arrive(4 + (unit & 1), kStreamThreads);
+    ++unit;
+    write_topk<Choosers>(keys.key, keys.cnt, K, m, s, inv_t, logp + r * K, ids + r * K);
+    Choosers::sync();  // the keys are read
   }
 }
 
 template <typename T> constexpr int top_unroll() { return sizeof(T) == 2 ? 4 : 2; }
-constexpr int64_t kTopFew = 2 * kNumSMs;  // rows up to which one launch with clusters takes them
-
-int top_parts(int64_t N, int V, int dtype) {
-  return dtype == IKRL_DTYPE_BF16 ? row_parts(N, V, 2, kTopThreads * top_unroll<uint16_t>())
-                                  : row_parts(N, V, 4, kTopThreads * top_unroll<float>());
-}
 
 template <typename T>
 int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c, float inv_t, float* logp,
-                int64_t* ids, void* ws, int segs, cudaStream_t s) {
+                int64_t* ids, cudaStream_t s) {
   constexpr int U = top_unroll<T>();
   const T* x = reinterpret_cast<const T*>(logits);
-  if (N > kTopFew) {
-    const int64_t parts = N * segs;
-    const TopNotes notes = top_notes(ws, parts);
-    topk_note_kernel<T, U, 3><<<(unsigned)parts, kTopThreads, 0, s>>>(x, ld, V, K, segs, c, parts, notes);
-    int rc = check_launch("topk_note_kernel");
-    if (rc) return rc;
-    topk_select_kernel<T><<<(unsigned)N, kSelectThreads, 0, s>>>(x, ld, V, K, segs, c, inv_t, parts, notes, logp, ids);
-    if ((rc = check_launch("topk_select_kernel"))) return rc;
-    topk_again_kernel<T, U><<<2 * kNumSMs, kTopThreads, 0, s>>>(x, ld, N, V, K, segs, c, inv_t, notes, logp, ids);
-    return check_launch("topk_again_kernel");
+  // Rows that all have a resident block need no streaming (444 rows of 151936 bf16 columns, K = 64: 41 us
+  // against 47; 600 rows: 59 against 53).  With many keys a row the choosers fall behind the sweep, and blocks
+  // that choose themselves are as fast or faster (4096 rows of 50257 fp32 columns, K = 200: 242 us against 289;
+  // 1776 rows of 151936 bf16 columns: K = 128 139 against 131, K = 256 174 against 176).
+  if (N > 3 * kNumSMs && K <= 128) {
+    topk_stream_kernel<T, U><<<2 * kNumSMs, kStreamThreads, 0, s>>>(x, ld, N, V, K, c, inv_t, logp, ids);
+    return check_launch("topk_stream_kernel");
   }
   const int C = row_cluster(N, V, kTopThreads);
   cudaLaunchConfig_t cfg = {};
@@ -501,9 +562,9 @@ int launch_topk(const void* logits, int64_t ld, int64_t N, int V, int K, float c
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kern = logits_topk_kernel<T, U>;
+  auto kern = topk_block_kernel<T, U>;
   IKRL_CUDA(cudaLaunchKernelEx(&cfg, kern, x, ld, V, K, c, inv_t, logp, ids));
-  return check_launch("logits_topk_kernel");
+  return check_launch("topk_block_kernel");
 }
 
 }  // namespace
@@ -513,13 +574,8 @@ using namespace ikrl;
 
 extern "C" {
 
-size_t ikrl_logits_topk_workspace_bytes(int32_t dtype, int64_t N, int32_t V) {
-  if (N <= kTopFew || V <= 0) return 0;
-  return top_notes_bytes(N * top_parts(N, V, dtype));
-}
-
 int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V, int32_t K,
-                     float temperature, float* logp, int64_t* ids, void* ws, size_t ws_bytes, void* stream) {
+                     float temperature, float* logp, int64_t* ids, void* stream) {
   clear_error();
   const char* what = "ikrl_logits_topk";
   int rc = check_logits_arg(what, logits, dtype, ld, N, V);
@@ -532,21 +588,11 @@ int ikrl_logits_topk(const void* logits, int32_t dtype, int64_t ld, int64_t N, i
                "%s: temperature %g must be positive and finite", what, (double)temperature);
   if (N == 0) return IKRL_OK;
   IKRL_REQUIRE(logits && logp && ids, IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  int segs = 1;
-  if (N > kTopFew) {
-    segs = top_parts(N, V, dtype);
-    while (segs * K > kSelectBuf / 2) segs /= 2;  // each part may leave a little more than K keys
-    IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need too many blocks", what,
-                 (long long)N, V);
-    const size_t need = top_notes_bytes(N * segs);
-    IKRL_REQUIRE(ws != nullptr && ws_bytes >= need, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes,
-                 need);
-    IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
-                 "%s: workspace must be 256-byte aligned", what);
-  }
+  IKRL_REQUIRE(N <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: N=%lld rows need too many blocks", what,
+               (long long)N);
   return dtype == IKRL_DTYPE_BF16
-             ? launch_topk<uint16_t>(logits, ld, N, V, K, c, inv_t, logp, ids, ws, segs, as_stream(stream))
-             : launch_topk<float>(logits, ld, N, V, K, c, inv_t, logp, ids, ws, segs, as_stream(stream));
+             ? launch_topk<uint16_t>(logits, ld, N, V, K, c, inv_t, logp, ids, as_stream(stream))
+             : launch_topk<float>(logits, ld, N, V, K, c, inv_t, logp, ids, as_stream(stream));
 }
 
 }  // extern "C"

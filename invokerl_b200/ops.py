@@ -737,11 +737,9 @@ def logits_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> tuple
     log_probs = x.new_empty(shape, dtype=torch.float32)
     ids = x.new_empty(shape, dtype=torch.int64)
     code = N.dtype_code(x)
-    nbytes = N.lib().ikrl_logits_topk_workspace_bytes(code, Nr, V)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with N.on_device(dev):
         call("ikrl_logits_topk", x.data_ptr(), code, _ld(x), Nr, V, k, t, log_probs.data_ptr(), ids.data_ptr(),
-             ws.data_ptr() if nbytes else None, nbytes, N.stream_handle(dev))
+             N.stream_handle(dev))
     return log_probs, ids
 
 

@@ -36,7 +36,8 @@ def check_topk(x, k, temperature=1.0):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,V,k", [(1, 1, 1), (1, 5, 5), (3, 17, 1), (7, 1001, 256), (2, 256, 256), (5, 50257, 33),
-                                   (2, 151936, 20), (320, 4097, 64), (1, 151936, 256), (700, 151, 16)])
+                                   (2, 151936, 20), (320, 4097, 64), (1, 151936, 256), (700, 151, 16), (1000, 5, 3),
+                                   (445, 9001, 128), (900, 40000, 30), (445, 200003, 64), (40, 200003, 128)])
 def test_topk_sizes(n, V, k, dtype):
     g = torch.Generator().manual_seed(n + V + k)
     check_topk((2 * torch.randn(n, V, generator=g)).to(dtype).to(DEV), k)
@@ -44,7 +45,7 @@ def test_topk_sizes(n, V, k, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["equal", "two", "rising", "falling", "masked", "lowest", "zeros"])
-@pytest.mark.parametrize("n,V,k", [(3, 40001, 100), (400, 20000, 256)])
+@pytest.mark.parametrize("n,V,k", [(3, 40001, 100), (400, 20000, 256), (450, 20000, 128), (446, 210000, 40)])
 def test_topk_orders_and_ties(kind, n, V, k, dtype):
     g = torch.Generator().manual_seed(V)
     x = torch.randn(n, V, generator=g)
@@ -74,12 +75,18 @@ def test_topk_layouts_temperature_and_empty():
     check_topk(base.to(torch.bfloat16)[:, 1, 1:], 17)
     check_topk(base.transpose(0, 2), 2)      # strided columns
     check_topk(base[:1, :1].expand(4, 2, 1100), 9)
+    many = torch.randn(500, 1015, generator=g).to(DEV)
+    for dtype in DTYPES:
+        check_topk(many.to(dtype)[:, 5:1011], 100)
+        check_topk(many.to(dtype)[1:451, 3:12], 9)
+    check_topk(many[:1].expand(450, 1015), 9)
     lp, ids = ops.logits_topk(torch.empty(0, 50, device=DEV), 4)
     assert lp.shape == ids.shape == (0, 4)
 
 
-def test_topk_nan_and_infinity():
-    x = torch.randn(4, 30000, generator=torch.Generator().manual_seed(1)).to(DEV)
+@pytest.mark.parametrize("n", [4, 450])
+def test_topk_nan_and_infinity(n):
+    x = torch.randn(n, 30000, generator=torch.Generator().manual_seed(1)).to(DEV)
     want = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :8]
     x[0, 12345] = math.nan
     x[1, 777] = math.inf
@@ -791,7 +798,7 @@ def test_teacher_and_student_policies():
         assert float((losses[fsdp][1][:, 1:].cpu() - want_ce).abs().max()) <= t
 
 
-@pytest.mark.parametrize("n,V,k", [(2, 40000, 50), (40, 1500, 12), (400, 20000, 200)])
+@pytest.mark.parametrize("n,V,k", [(2, 40000, 50), (40, 1500, 12), (400, 20000, 200), (700, 20000, 100)])
 def test_topk_repeats_bit_for_bit(n, V, k):
     """Ids and log-probs do not depend on the order in which columns reach the buffer."""
     x = torch.randn(n, V, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).to(DEV)
