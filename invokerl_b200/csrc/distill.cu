@@ -361,6 +361,7 @@ template <int WARPS>
 __global__ void __launch_bounds__(128) row_losses_kernel(const float* __restrict__ part_m,
                                                          const float* __restrict__ part_s,
                                                          const float* __restrict__ part_x, int sets,
+                                                         const int* __restrict__ sets_dev,
                                                          const int* __restrict__ pos, int64_t N, int K,
                                                          RowLossParams P, RowState st, float* __restrict__ loss,
                                                          const int* __restrict__ err) {
@@ -374,6 +375,7 @@ __global__ void __launch_bounds__(128) row_losses_kernel(const float* __restrict
   float m = -INFINITY, s = 0.f, sum = 0.f;
   if (id == kRowLive) {
     const int64_t at = pos ? pos[r] : r;
+    if (sets_dev != nullptr) sets = *sets_dev;
     for (int q = WARPS == 1 ? lane : (int)threadIdx.x; q < sets; q += 32 * WARPS) {
       online_merge(P.c, m, s, part_m[(int64_t)q * N + at], part_s[(int64_t)q * N + at]);
       if (part_x) sum += part_x[(int64_t)q * N + at];
@@ -448,7 +450,7 @@ int launch_fwd(const void* logits, int64_t ld, const int64_t* tids, const float*
   if ((rc = check_launch("row_sums_kernel"))) return rc;
   const float* part = st.part;
   return launch_row_losses(part, part + (int64_t)kMaxParts * N, sum ? part + (int64_t)2 * kMaxParts * N : nullptr,
-                           segs, nullptr, N, K, P, st, loss, nullptr, s);
+                           segs, nullptr, nullptr, N, K, P, st, loss, nullptr, s);
 }
 
 template <typename T>
@@ -537,15 +539,16 @@ int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, 
   return check_launch("row_entries_kernel");
 }
 
-int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const int* pos,
-                      int64_t N, int K, const RowLossParams& p, const RowState& st, float* loss, const int* err,
-                      cudaStream_t s) {
+int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets,
+                      const int* sets_dev, const int* pos, int64_t N, int K, const RowLossParams& p, const RowState& st,
+                      float* loss, const int* err, cudaStream_t s) {
   // Few rows come with many sets (a GEMM of one row tile cuts the columns as fine as it can).
   if (sets > 64 && N <= 4 * kNumSMs)
-    row_losses_kernel<4><<<(unsigned)N, 128, 0, s>>>(part_m, part_s, part_x, sets, pos, N, K, p, st, loss, err);
+    row_losses_kernel<4><<<(unsigned)N, 128, 0, s>>>(part_m, part_s, part_x, sets, sets_dev, pos, N, K, p, st, loss,
+                                                        err);
   else
-    row_losses_kernel<1><<<(unsigned)((N + 3) / 4), 128, 0, s>>>(part_m, part_s, part_x, sets, pos, N, K, p, st, loss,
-                                                                 err);
+    row_losses_kernel<1><<<(unsigned)((N + 3) / 4), 128, 0, s>>>(part_m, part_s, part_x, sets, sets_dev, pos, N, K,
+                                                                 p, st, loss, err);
   return check_launch("row_losses_kernel");
 }
 

@@ -90,11 +90,11 @@ int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossP
 int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, const RowLossParams& p,
                        const RowState& st, cudaStream_t s, int* clear = nullptr);
 // part_m / part_s / part_x: [sets][N] tail maxima, sums of 2^(c (x - max)), plain sums of all logits
-// (part_x null without label smoothing); pos: the place of each row in them, or null: itself; err: an
-// error word that makes every loss NaN, or null.
-int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const int* pos,
-                      int64_t N, int K, const RowLossParams& p, const RowState& st, float* loss, const int* err,
-                      cudaStream_t s);
+// (part_x null without label smoothing), the number of sets on the device where sets_dev is given; pos: the
+// place of each row in them, or null: itself; err: an error word that makes every loss NaN, or null.
+int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets, const int* sets_dev,
+                      const int* pos, int64_t N, int K, const RowLossParams& p, const RowState& st, float* loss,
+                      const int* err, cudaStream_t s);
 
 // ---- device side ---------------------------------------------------------------------------------
 
