@@ -152,7 +152,7 @@ def check_distill(x, ids, lp, up, kind="forward", tail=True, temperature=1.0, be
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind,tail", KINDS)
 @pytest.mark.parametrize("n,V,K", [(1, 1, 1), (2, 7, 3), (3, 1001, 16), (5, 1000, 256), (2, 50257, 64),
-                                   (300, 333, 5), (1, 151936, 100)])
+                                   (300, 333, 5), (1, 151936, 100), (100, 20011, 40), (330, 20011, 40)])
 def test_distill_sizes(n, V, K, kind, tail, dtype):
     x, ids, lp, up = make_rows(n, V, K, dtype, n + V + K)
     check_distill(x, ids, lp, up, kind, tail)
@@ -205,7 +205,7 @@ def test_distill_masked_columns(kind, hole, dtype):
     check_distill(x, ids, lp, up, kind)
 
 
-@pytest.mark.parametrize("n", [3, 80])  # one launch, and three
+@pytest.mark.parametrize("n", [3, 80, 310])  # one launch, and three
 @pytest.mark.parametrize("low", [-1e9, -1e30, torch.finfo(torch.float32).min])
 def test_losses_where_everything_is_masked(low, n):
     """Rows of one value, however low: a uniform softmax; and masks behind which whole vectors lie before
@@ -285,7 +285,8 @@ def test_losses_on_strided_and_unaligned_logits(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,V,ld,off", [(5, 1001, 1040, 0), (70, 1000, 1001, 1), (3, 2049, 2056, 7), (66, 9, 9, 5)])
+@pytest.mark.parametrize("n,V,ld,off", [(5, 1001, 1040, 0), (70, 1000, 1001, 1), (3, 2049, 2056, 7), (66, 9, 9, 5),
+                                        (310, 1000, 1001, 1), (300, 9, 9, 5)])
 def test_losses_on_a_matrix_with_a_row_stride(n, V, ld, off, dtype):
     """2-D views are taken as they are: rows of any alignment, gradients (dense) aligned otherwise."""
     x, ids, lp, up = make_rows(n, V, 7, dtype, n + ld)
@@ -307,7 +308,7 @@ def test_losses_on_a_matrix_with_a_row_stride(n, V, ld, off, dtype):
                    tol * (1 + span))
 
 
-@pytest.mark.parametrize("n", [3, 80])  # one launch, and three
+@pytest.mark.parametrize("n", [3, 80, 310])  # one launch, and three
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_bad_logits_stay_in_their_row(n, bad):
     x, ids, lp, up = make_rows(n, 3000, 5, torch.float32, 17)
@@ -369,7 +370,8 @@ def check_xent(x, t, up, smoothing, z):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("smoothing,z", [(0.0, 0.0), (0.1, 1e-3)])
-@pytest.mark.parametrize("n,V", [(1, 1), (2, 7), (9, 1001), (3, 50257), (400, 257), (2, 151936)])
+@pytest.mark.parametrize("n,V", [(1, 1), (2, 7), (9, 1001), (3, 50257), (400, 257), (2, 151936), (130, 20011),
+                                 (330, 20011)])
 def test_cross_entropy_sizes(n, V, smoothing, z, dtype):
     x, ids, _, up = make_rows(n, V, 1, dtype, n + V)
     t = ids[:, 0].clone()
