@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __re
                                                                    float* __restrict__ loss) {
   extern __shared__ uint32_t s_map[];
   __shared__ int s_col[kMaxEntries];
-  __shared__ __align__(16) int s_raw[kMaxEntries];
+  __shared__ int s_raw[kMaxEntries];
   __shared__ float s_lp[kMaxEntries], s_x[kMaxEntries], s_red[64], s_part[3][kMaxParts];
   constexpr int U = unroll_of<T>();
   cg::cluster_group cluster = cg::this_cluster();
@@ -327,11 +327,11 @@ __global__ void __launch_bounds__(kBwdThreads, MINB) row_loss_bwd_kernel(const T
   }
 }
 
-// Entries of each row: one block of at least K threads a row, or one thread for a single target.
+// Entries of each row: one block a row, or one thread for a single target.
 __global__ void row_entries_kernel(const int64_t* __restrict__ tids, const float* __restrict__ tlp, int K, int V,
                                    RowState st, int* __restrict__ clear) {
   __shared__ int s_col[kMaxEntries];
-  __shared__ __align__(16) int s_raw[kMaxEntries];
+  __shared__ int s_raw[kMaxEntries];
   __shared__ float s_lp[kMaxEntries];
   const int64_t r = blockIdx.x;
   int cnt = 0;
@@ -501,6 +501,7 @@ int distill_params(const char* what, const ikrl_distill_params* d, int V, int K,
                "%s: beta %g outside (0, 1)", what, (double)d->beta);
   IKRL_REQUIRE(K >= 1 && K <= kMaxEntries, IKRL_ERR_UNSUPPORTED, "%s: K=%d entries outside 1..%d", what, K,
                kMaxEntries);
+  IKRL_REQUIRE(V < 1 << 24, IKRL_ERR_UNSUPPORTED, "%s: V=%d needs more than 24 bits", what, V);  // row_entries
   RowLossParams p{};
   p.loss = d->kind == IKRL_DISTILL_FORWARD ? (d->tail ? ROW_FORWARD : ROW_FORWARD_TOPK)
                                            : (d->kind == IKRL_DISTILL_REVERSE ? ROW_REVERSE : ROW_JSD);
@@ -535,7 +536,7 @@ int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, 
     row_targets_kernel<<<(unsigned)((N + 255) / 256), 256, 0, s>>>(tids, N, p.V, st, clear);
     return check_launch("row_targets_kernel");
   }
-  row_entries_kernel<<<(unsigned)N, (unsigned)((K + 31) / 32 * 32), 0, s>>>(tids, tlp, K, p.V, st, clear);
+  row_entries_kernel<<<(unsigned)N, (unsigned)entry_threads(K), 0, s>>>(tids, tlp, K, p.V, st, clear);
   return check_launch("row_entries_kernel");
 }
 

@@ -181,7 +181,7 @@ def test_c_entries_refuse_before_any_cuda_call(lib):
                N.sz(state_bytes), N.i64(cache), p, p, q, ws, N.sz(nbytes), None)
 
     for kw, msg in [(dict(H=12), "multiple of 8"), (dict(n=-1), "bad sizes"), (dict(nbytes=256), "workspace"),
-                    (dict(state_bytes=64), "state"), (dict(ws=N.c_void_p(264)), "aligned"), (dict(K=300), "K=300"),
+                    (dict(state_bytes=64), "state"), (dict(ws=N.c_void_p(264)), "aligned"), (dict(K=300), "K=300"), (dict(V=1 << 24), "24 bits"),
                     (dict(cache=-1), "cache_rows"), (dict(cache=4, V=101), "multiple of 8"),
                     (dict(cache=4, V=104, q=None), "null cache"), (dict(cache=4, V=104, q=N.c_void_p(258)), "aligned")]:
         with pytest.raises(N.IkrlError, match=msg):
