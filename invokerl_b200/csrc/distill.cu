@@ -190,13 +190,19 @@ __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __re
 // Rows without entries are not read.
 template <typename T, bool SUM, int U, int MINB>
 __global__ void __launch_bounds__(kFwdThreads, MINB) row_sums_kernel(const T* __restrict__ logits, int64_t ld,
-                                                                     int segs, int K, float c, int V, RowState st,
+                                                                     RowCut cut, int K, float c, int V, RowState st,
                                                                      int64_t N) {
   extern __shared__ uint32_t s_map[];
   __shared__ int s_cols[kMaxEntries];
   __shared__ float s_red[64], s_sum[32];
-  const int64_t r = blockIdx.x / segs;
-  const int seg = (int)(blockIdx.x - r * segs);
+  int64_t r = blockIdx.x;
+  int seg = 0, segs = 1;
+  if (r >= cut.whole) {
+    const int64_t b = r - cut.whole;
+    segs = cut.parts;
+    r = cut.whole + b / segs;
+    seg = (int)(b % segs);
+  }
   const RowPart<T> p(logits, ld, r, V, seg, segs);
   Group8<T> g[U];
   if (whole_round<T, U>(p, p.a)) load_round<T, U>(g, p, p.a);  // a row that is not live costs this read
@@ -221,6 +227,11 @@ __global__ void __launch_bounds__(kFwdThreads, MINB) row_sums_kernel(const T* __
       st.part[(int64_t)seg * N + r] = m;
       st.part[((int64_t)kMaxParts + seg) * N + r] = s;
       if constexpr (SUM) st.part[((int64_t)2 * kMaxParts + seg) * N + r] = sum;
+    }
+    if (segs < cut.parts && threadIdx.x > 0 && threadIdx.x < cut.parts) {  // the parts that a whole row lacks
+      st.part[(int64_t)threadIdx.x * N + r] = -INFINITY;
+      st.part[((int64_t)kMaxParts + threadIdx.x) * N + r] = 0.f;
+      if constexpr (SUM) st.part[((int64_t)2 * kMaxParts + threadIdx.x) * N + r] = 0.f;
     }
   }
 }
@@ -441,16 +452,17 @@ int launch_fwd(const void* logits, int64_t ld, const int64_t* tids, const float*
   if (rc) return rc;
   constexpr int U = unroll_of<T>();
   static_assert(kMaxRowParts <= kMaxParts, "the state holds a sum for every part");
-  const int segs = row_parts(N, P.V, sizeof(T), kFwdThreads * U);
-  IKRL_REQUIRE(N * segs <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "N=%lld rows of V=%d need too many blocks",
+  const RowCut cut = row_cut(N, P.V, sizeof(T), kFwdThreads * U);
+  const int64_t blocks = cut.whole + (N - cut.whole) * cut.parts;
+  IKRL_REQUIRE(blocks <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "N=%lld rows of V=%d need too many blocks",
                (long long)N, P.V);
-  const size_t smem = (size_t)map_words((groups + segs - 1) / segs) * 4;
+  const size_t smem = (size_t)map_words(cut.whole > 0 ? groups : (groups + cut.parts - 1) / cut.parts) * 4;
   auto kern = sum ? row_sums_kernel<T, true, U, 3> : row_sums_kernel<T, false, U, 3>;
-  kern<<<(unsigned)(N * segs), kFwdThreads, smem, s>>>(x, ld, segs, K, P.c, P.V, st, N);
+  kern<<<(unsigned)blocks, kFwdThreads, smem, s>>>(x, ld, cut, K, P.c, P.V, st, N);
   if ((rc = check_launch("row_sums_kernel"))) return rc;
   const float* part = st.part;
   return launch_row_losses(part, part + (int64_t)kMaxParts * N, sum ? part + (int64_t)2 * kMaxParts * N : nullptr,
-                           segs, nullptr, nullptr, N, K, P, st, loss, nullptr, s);
+                           cut.parts, nullptr, nullptr, N, K, P, st, loss, nullptr, s);
 }
 
 template <typename T>

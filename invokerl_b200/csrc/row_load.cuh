@@ -259,24 +259,34 @@ inline int row_cluster(int64_t N, int V, int min_groups) {
   return c;
 }
 
-// Parts a row is cut into when many rows are read by one block a part.  Three blocks share an SM's 44
-// bytes a ns (of 6.5 TB/s), and a part costs its block about 2.8 us beside its bytes (sums of 4096 rows
-// of 151936 bf16 columns: 218, 258, 316, 420 us in 1, 2, 4, 8 parts), so rows are cut only where the
-// blocks would not come out even otherwise; a part keeps at least `round` groups.
+// How many rows are read by one block each, and into how many parts the others are cut.  Three blocks share an
+// SM's 44 bytes a ns (of 6.5 TB/s), and a part costs its block about 2.8 us beside its bytes (sums of 4096 rows
+// of 151936 bf16 columns: 218, 258, 316, 420 us in 1, 2, 4, 8 parts), so rows are cut only where the blocks would
+// not come out even otherwise and 5% is to be had: all of them, or those behind the last full round of whole
+// rows (distillation forward of 512 / 1024 / 4096 such rows: 52 / 79 / 239 us, 56 / 89 / 241 us with all rows cut
+// alike; 16384 rows of 32000: 355 us with a cut worth 2%, 345 without).  A part keeps at least `round` groups.
 constexpr int kMaxRowParts = 8;
-inline int row_parts(int64_t N, int V, int elem_bytes, int round) {
+struct RowCut {
+  int64_t whole;  // rows [0, whole) are whole
+  int parts;      // parts of each of the others
+};
+inline RowCut row_cut(int64_t N, int V, int elem_bytes, int round) {
   const int64_t resident = 3 * kNumSMs;
   const double row_us = (double)V * elem_bytes * 3.0 / 44e3;
-  int parts = 1;
-  double best = 0.0;
+  const int64_t full = N / resident * resident;
+  RowCut best{0, 1};
+  double least = 0.0;
   for (int q = 1; q <= kMaxRowParts && (q == 1 || V / 8 / q >= round); q *= 2) {
-    const double us = (double)((N * q + resident - 1) / resident) * (row_us / q + 2.8);
-    if (q == 1 || us < best) {
-      best = us;
-      parts = q;
+    for (const int64_t whole : {(int64_t)0, full}) {
+      const double us = (double)(whole / resident) * (row_us + 2.8) +
+                        (double)(((N - whole) * q + resident - 1) / resident) * (row_us / q + 2.8);
+      if (least == 0.0 || us < 0.95 * least) {
+        least = us;
+        best = {whole, q};
+      }
     }
   }
-  return parts;
+  return best;
 }
 
 }  // namespace ikrl
