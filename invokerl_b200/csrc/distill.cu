@@ -198,10 +198,10 @@ __global__ void __launch_bounds__(kFwdThreads, MINB) row_sums_kernel(const T* __
   int64_t r = blockIdx.x;
   int seg = 0, segs = 1;
   if (r >= cut.whole) {
-    const int64_t b = r - cut.whole;
-    segs = cut.parts;
-    r = cut.whole + b / segs;
-    seg = (int)(b % segs);
+    const unsigned b = (unsigned)(r - cut.whole);
+    segs = cut.parts;  // a power of two
+    r = cut.whole + (b >> (31 - __clz(segs)));
+    seg = (int)(b & (unsigned)(segs - 1));
   }
   const RowPart<T> p(logits, ld, r, V, seg, segs);
   Group8<T> g[U];

@@ -263,8 +263,8 @@ inline int row_cluster(int64_t N, int V, int min_groups) {
 // SM's 44 bytes a ns (of 6.5 TB/s), and a part costs its block about 2.8 us beside its bytes (sums of 4096 rows
 // of 151936 bf16 columns: 218, 258, 316, 420 us in 1, 2, 4, 8 parts), so rows are cut only where the blocks would
 // not come out even otherwise and 5% is to be had: all of them, or those behind the last full round of whole
-// rows (distillation forward of 512 / 1024 / 4096 such rows: 52 / 79 / 239 us, 56 / 89 / 241 us with all rows cut
-// alike; 16384 rows of 32000: 355 us with a cut worth 2%, 345 without).  A part keeps at least `round` groups.
+// rows (distillation forward of 512 / 1024 / 4096 such rows: 49 / 77 / 238 us, 56 / 89 / 241 us with all rows cut
+// alike).  A part keeps at least `round` groups.
 constexpr int kMaxRowParts = 8;
 struct RowCut {
   int64_t whole;  // rows [0, whole) are whole
