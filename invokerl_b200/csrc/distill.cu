@@ -41,22 +41,34 @@ __device__ __forceinline__ void mark_entry(const RowPart<T>& p, int col, uint32_
   if (j >= p.a && j < p.b) atomicOr(&map[(j - p.a) >> 5], 1u << ((j - p.a) & 31));
 }
 
-// First U groups a thread of a part: issued ahead of the work on the entries.
+// U groups a thread of a part from group jb on; behind the part's last, groups of -inf.
 template <typename T, int U>
 __device__ __forceinline__ void load_round(Group8<T> (&g)[U], const RowPart<T>& p, int jb) {
+  if (jb + U * kFwdThreads <= p.b) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kFwdThreads + (int)threadIdx.x));
+    for (int u = 0; u < U; ++u) g[u].load(p.at(jb + u * kFwdThreads + (int)threadIdx.x));
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int j = jb + u * kFwdThreads + (int)threadIdx.x;
+    if (j < p.b) g[u].load(p.at(j));
+    else g[u].fill();
+  }
 }
-template <typename T, int U>
-__device__ __forceinline__ bool whole_round(const RowPart<T>& p, int jb) {
-  return jb + U * kFwdThreads <= p.b;
+
+template <typename T>
+__device__ __forceinline__ float group_sum(const Group8<T>& g) {
+  float lo, hi;
+  unpack2(add2(add2(g.get2(0), g.get2(1)), add2(g.get2(2), g.get2(3))), lo, hi);
+  return lo + hi;
 }
 
 // Running sums of a part by a block: m, s over the tail and, with SUM, the sum of all logits.
 //
 // The loop over the part leaves out the groups that hold entries: their bits are one shared word a
 // warp and group, zero most of the time.  Those groups are taken one a thread, by the thread of their
-// first entry, and so are the groups that reach past the row.  g holds the first round, if whole.
+// first entry, and so are the groups that reach past the row.  g holds the first round.
 template <typename T, int U, bool SUM>
 __device__ __forceinline__ void sum_part(Group8<T> (&g)[U], const RowPart<T>& p, const RowEntries& e, float c, float& m,
                                          float& s, float& sum) {
@@ -95,35 +107,31 @@ __device__ __forceinline__ void sum_part(Group8<T> (&g)[U], const RowPart<T>& p,
   int jb = p.a;
   const uint32_t* word = e.map + (tid >> 5);
   const uint32_t bit = 1u << (tid & 31);
-  for (; whole_round<T, U>(p, jb); jb += U * kFwdThreads) {
+  for (; jb + U * kFwdThreads <= p.b; jb += U * kFwdThreads) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t wd = word[u * (kFwdThreads / 32)];
       if constexpr (SUM) {
-        uint64_t t = add2(add2(g[u].get2(0), g[u].get2(1)), add2(g[u].get2(2), g[u].get2(3)));
-        float lo, hi;
-        unpack2(t, lo, hi);
-        sum += (wd & bit) ? 0.f : lo + hi;
+        const float x = group_sum(g[u]);
+        sum += (wd & bit) ? 0.f : x;
       }
       if (wd != 0 && (wd & bit)) g[u].fill();
     }
     word += U * (kFwdThreads / 32);
     online_groups<T, U>(g, c, m, s);
-    if (whole_round<T, U>(p, jb + U * kFwdThreads)) load_round<T, U>(g, p, jb + U * kFwdThreads);
+    if (jb + U * kFwdThreads < p.b) load_round<T, U>(g, p, jb + U * kFwdThreads);
   }
-  for (; jb < p.b; jb += kFwdThreads) {  // what is left, a group a thread at a time
-    const int j = jb + tid;
-    Group8<T> h[1];
-    h[0].fill();
-    if (j < p.b && !(*word & bit)) {
-      h[0].load(p.at(j));
-      if constexpr (SUM) {
+  if (jb < p.b) {  // the last round, in part
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum += h[0].get(k);
+    for (int u = 0; u < U; ++u) {
+      const bool in = jb + u * kFwdThreads + tid < p.b;
+      const bool entry = jb + u * kFwdThreads < p.b && (word[u * (kFwdThreads / 32)] & bit);  // the map ends with p.b
+      if constexpr (SUM) {
+        if (in && !entry) sum += group_sum(g[u]);
       }
+      if (entry) g[u].fill();
     }
-    word += kFwdThreads / 32;
-    online_groups<T, 1>(h, c, m, s);
+    online_groups<T, U>(g, c, m, s);
   }
 }
 
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(kFwdThreads) row_loss_fwd_kernel(const T* __re
   const int64_t r = blockIdx.x / C;
   const RowPart<T> p(logits, ld, r, P.V, rank, C);
   Group8<T> g[U];
-  if (whole_round<T, U>(p, p.a)) load_round<T, U>(g, p, p.a);
+  load_round<T, U>(g, p, p.a);
 
   for (int i = threadIdx.x; i < map_words(p.b - p.a); i += kFwdThreads) s_map[i] = 0u;
   int cnt = 0;
@@ -205,7 +213,7 @@ __global__ void __launch_bounds__(kFwdThreads, MINB) row_sums_kernel(const T* __
   }
   const RowPart<T> p(logits, ld, r, V, seg, segs);
   Group8<T> g[U];
-  if (whole_round<T, U>(p, p.a)) load_round<T, U>(g, p, p.a);  // a row that is not live costs this read
+  load_round<T, U>(g, p, p.a);  // a row that is not live costs this read
   const int64_t id = st.row_ids[r];
   const int col = threadIdx.x < K ? st.cols[r * K + threadIdx.x] : kNoEntry;
   for (int i = threadIdx.x; i < map_words(p.b - p.a); i += kFwdThreads) s_map[i] = 0u;
@@ -457,7 +465,7 @@ int launch_fwd(const void* logits, int64_t ld, const int64_t* tids, const float*
   IKRL_REQUIRE(blocks <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "N=%lld rows of V=%d need too many blocks",
                (long long)N, P.V);
   const size_t smem = (size_t)map_words(cut.whole > 0 ? groups : (groups + cut.parts - 1) / cut.parts) * 4;
-  auto kern = sum ? row_sums_kernel<T, true, U, 3> : row_sums_kernel<T, false, U, 3>;
+  auto kern = sum ? row_sums_kernel<T, true, U, 4> : row_sums_kernel<T, false, U, 4>;
   kern<<<(unsigned)blocks, kFwdThreads, smem, s>>>(x, ld, cut, K, P.c, P.V, st, N);
   if ((rc = check_launch("row_sums_kernel"))) return rc;
   const float* part = st.part;

@@ -259,27 +259,26 @@ inline int row_cluster(int64_t N, int V, int min_groups) {
   return c;
 }
 
-// How many rows are read by one block each, and into how many parts the others are cut.  Three blocks share an
-// SM's 44 bytes a ns (of 6.5 TB/s), and a part costs its block about 2.8 us beside its bytes (sums of 4096 rows
-// of 151936 bf16 columns: 218, 258, 316, 420 us in 1, 2, 4, 8 parts), so rows are cut only where the blocks would
-// not come out even otherwise and 5% is to be had: all of them, or those behind the last full round of whole
-// rows (distillation forward of 512 / 1024 / 4096 such rows: 49 / 77 / 238 us, 56 / 89 / 241 us with all rows cut
-// alike).  A part keeps at least `round` groups.
+// How many rows are read by one block each, and into how many parts the others are cut.  An SM holds four blocks
+// and reads 44 bytes a ns (of 6.5 TB/s), and each of its rounds of four costs about 2.8 us beside the bytes
+// (forward of 4096 rows of 151936 bf16 columns in 1, 2, 4, 8 parts: 237, 257, 329, 479 us), so rows are cut only
+// where the SMs would not come out even otherwise and 5% is to be had: all of them, or those that are left when
+// every SM has as many whole rows.  A part keeps at least `round` groups.  (Forward of 300 / 512 such
+// rows: 45 / 53 us, 48 / 56 with all rows cut alike; 512 rows of 50257 columns: 35 us against 38.)
 constexpr int kMaxRowParts = 8;
 struct RowCut {
   int64_t whole;  // rows [0, whole) are whole
   int parts;      // parts of each of the others
 };
 inline RowCut row_cut(int64_t N, int V, int elem_bytes, int round) {
-  const int64_t resident = 3 * kNumSMs;
-  const double row_us = (double)V * elem_bytes * 3.0 / 44e3;
-  const int64_t full = N / resident * resident;
+  const double row_us = (double)V * elem_bytes / 44e3;
   RowCut best{0, 1};
   double least = 0.0;
   for (int q = 1; q <= kMaxRowParts && (q == 1 || V / 8 / q >= round); q *= 2) {
-    for (const int64_t whole : {(int64_t)0, full}) {
-      const double us = (double)(whole / resident) * (row_us + 2.8) +
-                        (double)(((N - whole) * q + resident - 1) / resident) * (row_us / q + 2.8);
+    for (const int64_t whole : {(int64_t)0, N / kNumSMs * kNumSMs}) {
+      const int64_t parts = (N - whole) * q;
+      const double rows = (double)(whole / kNumSMs) + (double)((parts + kNumSMs - 1) / kNumSMs) / q;
+      const double us = rows * row_us + (double)((whole + parts + 4 * kNumSMs - 1) / (4 * kNumSMs)) * 2.8;
       if (least == 0.0 || us < 0.95 * least) {
         least = us;
         best = {whole, q};

@@ -405,7 +405,8 @@ LOGIT_CACHE_STATS = {"rows": 0, "candidates": 0}
 
 
 def set_logit_cache(mode: str = "auto", reserve_bytes: int | None = None, fraction: float | None = None) -> dict:
-    """Set the logit-cache policy of `lmhead_logprob`; returns the previous one."""
+    """Set the logit-cache policy of `lmhead_logprob` and of the row losses through the head; returns the
+    previous one."""
     if mode not in ("auto", "off"):
         raise ValueError(f"logit cache mode {mode!r} is not 'auto' or 'off'")
     prev = dict(_LOGIT_CACHE)
