@@ -2231,10 +2231,27 @@ __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __
   if (two) ds[(rows + k) * ld_ds + col] = f32_to_bf16_rn(d - bf16_to_f32(hi));
 }
 
-// The hidden rows twice, one under the other: the dW operand beside a dS of two terms.
-__global__ void stack_rows_kernel(const uint4* __restrict__ h, int64_t n, uint4* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    out[i] = out[n + i] = h[i];
+// First launch of the backward of few rows, a block a row: clears the error word; with h2 the hidden rows
+// twice, one under the other (the dW operand beside a dS of two terms); with gs what row_scale_kernel leaves.
+__global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__ h, int vec_per_row, uint4* __restrict__ h2,
+                                                       const float* __restrict__ dloss,
+                                                       const int64_t* __restrict__ row_ids,
+                                                       const float* __restrict__ coef, float level,
+                                                       float* __restrict__ gs, float* __restrict__ level_out,
+                                                       int* __restrict__ err) {
+  const int64_t r = blockIdx.x;
+  if (r == 0 && threadIdx.x == 0) *err = 0;
+  if (gs != nullptr && threadIdx.x == 0) {
+    const float g = dloss[r];
+    const bool on = g != 0.f && row_ids[r] != kRowNone;
+    gs[r] = on ? g * coef[r] : 0.f;
+    level_out[r] = on ? g * level : 0.f;
+  }
+  if (h2 == nullptr) return;
+  const uint4* from = h + r * vec_per_row;
+  uint4* to = h2 + r * vec_per_row;
+  uint4* below = to + (int64_t)gridDim.x * vec_per_row;
+  for (int i = threadIdx.x; i < vec_per_row; i += blockDim.x) to[i] = below[i] = from[i];
 }
 
 // dH of a dS of two terms: out = bf16(sum over K ranges of the partials of row r and of row rows + r).
@@ -2860,20 +2877,21 @@ static int lmhead_row_loss_bwd_few(const char* what, const void* hidden, const v
   char* w = reinterpret_cast<char*>(ws);
   int* err = reinterpret_cast<int*>(w);
   uint16_t* ds = reinterpret_cast<uint16_t*>(w + L.ds_off);
-  IKRL_CUDA(cudaMemsetAsync(err, 0, sizeof(int), s));
+  const bool cached = cache.rows >= N;
+  float* gs = cached ? nullptr : reinterpret_cast<float*>(w + L.gs_off);
+  float* level = reinterpret_cast<float*>(w + L.level_off);
+  uint4* h2 = dweight ? reinterpret_cast<uint4*>(w + L.h_off) : nullptr;
+  few_rows_kernel<<<(unsigned)N, 128, 0, s>>>(reinterpret_cast<const uint4*>(hidden), H / 8, h2, dloss, rl.st.row_ids,
+                                              rl.st.coef, rl.level, gs, level, err);
+  if ((rc = check_launch("few_rows_kernel"))) return rc;
   // 1) dS, from the forward's numerators or by the GEMM again
-  if (cache.rows >= N) {
+  if (cached) {
     const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)), (unsigned)N);
     dtail_from_cache_kernel<true><<<grid, 256, 0, s>>>(cache.q, cache.m, L.lds, (int)cdiv64(V, 32), nullptr, nullptr,
                                                        dloss, rl.st.row_ids, rl.st.ref, rl.st.coef, rl.st.cols,
                                                        rl.st.grad, rl.K, rl.level, rl.c, 0, N, V, ds, L.lds);
     if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
   } else {
-    float* gs = reinterpret_cast<float*>(w + L.gs_off);
-    float* level = reinterpret_cast<float*>(w + L.level_off);
-    row_scale_kernel<<<(unsigned)cdiv64(N, 256), 256, 0, s>>>(dloss, rl.st.row_ids, rl.st.coef, nullptr, N, rl.level,
-                                                              gs, level);
-    if ((rc = check_launch("row_scale_kernel"))) return rc;
     CUtensorMap ta, tb, tb2, tds;
     if ((rc = make_tmap(&ta, hidden, H, N, H, BM, "hidden"))) return rc;
     if ((rc = make_tmap(&tb, weight, H, V, H, BN, "weight"))) return rc;
@@ -2893,11 +2911,6 @@ static int lmhead_row_loss_bwd_few(const char* what, const void* hidden, const v
   }
   // 2) dW (+)= [hi; lo]^T [h; h]
   if (dweight) {
-    uint4* h2 = reinterpret_cast<uint4*>(w + L.h_off);
-    const int64_t n = N * H / 8;
-    stack_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(n, 256), 148ll * 8), 256, 0, s>>>(
-        reinterpret_cast<const uint4*>(hidden), n, h2);
-    if ((rc = check_launch("stack_rows_kernel"))) return rc;
     CUtensorMap ta, tb;
     if ((rc = make_tmap(&ta, ds, V, 2 * N, L.lds, 64, "dS^T"))) return rc;
     if ((rc = make_tmap(&tb, h2, H, 2 * N, H, 64, "hidden^T"))) return rc;
@@ -2954,6 +2967,8 @@ static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void*
                                                                  accumulate_dweight);
     IKRL_REQUIRE(ws != nullptr && ws_bytes >= need, IKRL_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what,
                  ws_bytes, need);
+    IKRL_REQUIRE(((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15) == 0,
+                 IKRL_ERR_ALIGNMENT, "%s: hidden and weight must be 16-byte aligned", what);
     rl.st = row_state(const_cast<void*>(state), N, K);
   }
   rl.K = K;

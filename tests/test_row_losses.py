@@ -181,11 +181,24 @@ def test_c_entries_refuse_before_any_cuda_call(lib):
                N.sz(state_bytes), N.i64(cache), p, p, q, ws, N.sz(nbytes), None)
 
     for kw, msg in [(dict(H=12), "multiple of 8"), (dict(n=-1), "bad sizes"), (dict(nbytes=256), "workspace"),
-                    (dict(state_bytes=64), "state"), (dict(ws=N.c_void_p(264)), "aligned"), (dict(K=300), "K=300"), (dict(V=1 << 24), "24 bits"),
+                    (dict(state_bytes=64), "state"), (dict(ws=N.c_void_p(264)), "aligned"), (dict(K=300), "K=300"),
+                    (dict(V=1 << 24), "24 bits"),
                     (dict(cache=-1), "cache_rows"), (dict(cache=4, V=101), "multiple of 8"),
                     (dict(cache=4, V=104, q=None), "null cache"), (dict(cache=4, V=104, q=N.c_void_p(258)), "aligned")]:
         with pytest.raises(N.IkrlError, match=msg):
             head(**kw)
+    def head_bwd(n, hidden=p, nbytes=1 << 26, state_bytes=1 << 20, ws=p, g=p, dh=p, dw=p):
+        N.call("ikrl_lmhead_distill_bwd", hidden, p, N.i64(n), N.i32(64), N.i32(100), N.i32(3), params(), p,
+               N.sz(state_bytes), g, N.i64(0), dh, dw, N.i32(N.IKRL_DTYPE_BF16), N.i32(0), N.i64(0), None, None, None,
+               ws, N.sz(nbytes), None)
+
+    odd = N.c_void_p(264)
+    for n in (4, 400):
+        for kw, msg in [(dict(hidden=odd), "aligned"), (dict(nbytes=512), "workspace"), (dict(state_bytes=64), "state"),
+                        (dict(ws=odd), "aligned"), (dict(dh=odd), "aligned"), (dict(dw=odd), "aligned"),
+                        (dict(g=None), "null pointer"), (dict(dh=None, dw=None), "null pointer")]:
+            with pytest.raises(N.IkrlError, match=msg):
+                head_bwd(n, **kw)
     with pytest.raises(N.IkrlError, match="bf16 dweight"):
         N.call("ikrl_lmhead_cross_entropy_bwd", p, p, N.i64(4), N.i32(64), N.i32(100), N.f32(0), N.f32(0), p,
                N.sz(1 << 20), p, N.i64(0), p, p, N.i32(N.IKRL_DTYPE_BF16), N.i32(1), N.i64(0), None, None, None, p,
