@@ -808,3 +808,58 @@ def test_topk_repeats_bit_for_bit(n, V, k):
     for _ in range(5):
         lp2, ids2 = ops.logits_topk(x, k, 1.3)
         assert torch.equal(lp, lp2) and torch.equal(ids, ids2)
+
+
+# ---- offsets past 32 bits -------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [5, 310, 460])
+def test_rows_far_apart(n):
+    """Rows whose offsets pass 2^31 elements give what the same rows side by side give."""
+    V, stride = 1003, (2 ** 31 + 2 ** 20) // (n - 1) // 8 * 8
+    store = torch.empty((n - 1) * stride + V, dtype=torch.bfloat16, device=DEV)
+    far = store.as_strided((n, V), (stride, 1))
+    x, ids, lp, up = make_rows(n, V, 9, torch.bfloat16, n)
+    near = torch.empty(n, 1008, dtype=torch.bfloat16, device=DEV)[:, :V]  # rows aligned alike
+    far.copy_(x)
+    near.copy_(x)
+    res = []
+    for logits in (far, near):
+        a = logits.detach().requires_grad_(True)
+        out = list(ops.logits_topk(a, 20))
+        for loss in (ops.logits_distill(a, ids.to(DEV), lp.to(DEV), "jsd"),
+                     ops.logits_cross_entropy(a, ids[:, 0].contiguous().to(DEV), 0.1)):
+            g, = torch.autograd.grad(loss, a, up.to(DEV))
+            out += [loss.detach(), g]
+        res.append(out)
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_gradients_past_2_31_elements():
+    """Equal rows of a matrix of more than 2^31 elements: the first and the last get the same."""
+    n, V, H = 14200, 151936, 1024
+    assert n * V > 2 ** 31
+    g = torch.Generator().manual_seed(2)
+    row = (2 * torch.randn(V, generator=g)).to(torch.bfloat16).to(DEV)
+    ids = torch.randperm(V, generator=g)[:7].expand(n, 7).contiguous().to(DEV)
+    lp = (torch.log_softmax(torch.randn(7, generator=g), 0) - 0.1).expand(n, 7).contiguous().to(DEV)
+    up = torch.ones(n, device=DEV)
+
+    def first_and_last(loss, grad):
+        assert bool((loss == loss[0]).all()) and bool(loss[0].isfinite())
+        assert torch.equal(grad[0], grad[-1]) and float(grad[-1].abs().max()) > 0
+
+    x = row.expand(n, V).contiguous().requires_grad_(True)
+    top, _ = ops.logits_topk(x, 5)
+    assert torch.equal(top[0], top[-1])
+    for loss in (ops.logits_distill(x, ids, lp, "reverse"), ops.logits_cross_entropy(x, ids[:, 0].contiguous())):
+        d, = torch.autograd.grad(loss, x, up)
+        first_and_last(loss.detach(), d)
+        del d
+    del x, loss
+    w = (0.03 * torch.randn(V, H, generator=g)).to(torch.bfloat16).to(DEV).requires_grad_(True)
+    h = torch.randn(H, generator=g).to(torch.bfloat16).to(DEV).expand(n, H).contiguous().requires_grad_(True)
+    for loss in (ops.lmhead_distill(h, w, ids, lp, "reverse"), ops.lmhead_cross_entropy(h, w, ids[:, 0].contiguous())):
+        dh, dw = torch.autograd.grad(loss, (h, w), up)
+        first_and_last(loss.detach(), dh)
+        assert bool(dw[-1].isfinite().all())
