@@ -414,8 +414,9 @@ IKRL_API int ikrl_lmhead_noalloc_status(int32_t* status_out, void* stream);
  * ikrl_lmhead_cache_row_elems; its 16-bit numerators are fp16 here), cache_rows = 0 for none; slots
  * go to the rows that have entries (or a target), in row order, and those rows alone take part in the
  * GEMMs.  The backward gets what the forward filled.
- * Up to 256 rows all rows take part, neither direction synchronises, chunk_rows is without effect, and a
- * cache is used when it has room for all rows (row r in slot r, cache_slot left alone). */
+ * Up to 256 rows, and up to 1024 where N H V <= 2^34, all rows take part, neither direction
+ * synchronises, chunk_rows is without effect, and a cache is used when it has room for all rows (row r in
+ * slot r, cache_slot left alone). */
 IKRL_API size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V);
 IKRL_API size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
                                                          int32_t dweight_dtype, int32_t accumulate_dweight);

@@ -2326,10 +2326,16 @@ size_t cache_fwd_workspace_bytes(int64_t N, int H, int V) {
   return base + ((((size_t)std::max<int64_t>(1, cdiv64(N, kCompactRows)) * 4) + 255) & ~size_t(255));
 }
 
-// A row loss of at most this many rows runs its GEMMs on all of them: one row pair of tiles costs
-// the same however many of its rows count, and the compaction's host synchronisation and launches
-// would cost more than they save.  Its backward is lmhead_row_loss_bwd_few.
-constexpr int64_t kRowLossDense = 256;
+// A row loss of few rows runs its GEMMs on all of them, whichever count: up to 256, where one row pair of
+// tiles costs the same however many of its rows count, and up to 1024 while the products are small enough
+// that the compaction's host synchronisation and launches cost more than they save.  Its backward is
+// lmhead_row_loss_bwd_few.  (Distillation forward and backward, a third without gradient: 300 rows of 512 against
+// 32003 columns 176 us, 206 with the compaction; 512 of 1024 against 32000 229 / 259 us, without a cache 268 / 260.)
+constexpr int64_t kRowLossDense = 256, kRowLossDenseMost = 1024;
+constexpr double kRowLossDenseWork = 17179869184.0;  // N H V
+static bool row_loss_dense(int64_t N, int H, int V) {
+  return N <= kRowLossDense || (N <= kRowLossDenseMost && (double)N * H * V <= kRowLossDenseWork);
+}
 
 // Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums
 // of all logits (up to 3 times the forward's splits, which the balance rule may take), and the
@@ -2343,7 +2349,7 @@ struct RowLossFwdLayout {
 static RowLossFwdLayout row_loss_fwd_layout(int64_t N, int H, int V) {
   RowLossFwdLayout L;
   L.splits = fwd_layout(N, H, V).splits;
-  L.gather = N > kRowLossDense;
+  L.gather = !row_loss_dense(N, H, V);
   const size_t part = align256((size_t)kWideGroups * 3 * L.splits * N * 4);
   size_t o = 256;  // the error word
   L.pm_off = o; o += part;
@@ -2836,7 +2842,7 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
                            K, P, st, loss, err, s);
 }
 
-// Backward of a row loss of few rows (N <= kRowLossDense), all of them in one chunk, without the
+// Backward of a row loss of few rows (row_loss_dense), all of them in one chunk, without the
 // compaction and its host synchronisation.  dS is held in two terms, hi = bf16(d) and lo = bf16(d - hi),
 // stacked as 2N rows: dW = [hi; lo]^T [h; h], dH = hi W + lo W.  With few rows a sum over the rows averages
 // little of dS's rounding away, and one term alone would leave dW with up to twice the error that its own
@@ -2975,7 +2981,7 @@ static int lmhead_row_loss_bwd(const char* what, const void* hidden, const void*
   rl.c = P.c;
   rl.level = P.loss == ROW_XENT ? -P.smoothing / (float)V : 0.f;
   rl.all_cached = cache.rows >= N;
-  if (N > 0 && N <= kRowLossDense)
+  if (N > 0 && row_loss_dense(N, H, V))
     return lmhead_row_loss_bwd_few(what, hidden, weight, dloss, N, H, V, rl, dhidden, dweight, dweight_dtype,
                                    accumulate_dweight, cache, ws, stream);
   const bool cached = cache.rows > 0;
@@ -2995,7 +3001,7 @@ size_t ikrl_lmhead_row_loss_fwd_workspace_bytes(int64_t N, int32_t H, int32_t V)
 size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V, int64_t chunk_rows,
                                                 int32_t dweight_dtype, int32_t accumulate_dweight) {
   if (N <= 0 || H <= 0 || V <= 0) return 256;
-  if (N <= kRowLossDense) return few_layout(N, H, V).total;
+  if (row_loss_dense(N, H, V)) return few_layout(N, H, V).total;
   return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + align256((size_t)N * 4);
 }
 

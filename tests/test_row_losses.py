@@ -209,8 +209,9 @@ def test_workspace_sizes_grow_with_their_parts(lib):
     s = lib.ikrl_row_loss_state_bytes
     assert s(0, 5) == 256 and s(100, 64) >= 100 * (8 + 4 + 4 + 64 * 12 + 12)
     f = lib.ikrl_lmhead_row_loss_fwd_workspace_bytes
-    # three sets of partial sums, the rows that count gathered (above 256 rows)
-    assert f(1000, 1024, 5000) >= lib.ikrl_lmhead_fwd_workspace_bytes(1000, 1024, 5000) + 1000 * 1024 * 2
-    assert f(256, 1024, 5000) < f(257, 1024, 5000) - 256 * 1024 * 2
+    # three sets of partial sums, the rows that count gathered (above 1024 rows, or 256 of a large product)
+    assert f(2000, 1024, 5000) >= lib.ikrl_lmhead_fwd_workspace_bytes(2000, 1024, 5000) + 2000 * 1024 * 2
+    assert f(1024, 1024, 5000) < f(1025, 1024, 5000) - 1024 * 1024 * 2
+    assert f(256, 4096, 50000) < f(257, 4096, 50000) - 256 * 4096 * 2
     b = lib.ikrl_lmhead_row_loss_bwd_workspace_bytes
-    assert b(1000, 1024, 5000, 0, 1, 0) >= lib.ikrl_lmhead_bwd_workspace_bytes(1000, 1024, 5000, 0, 1, 0) + 4000
+    assert b(2000, 1024, 5000, 0, 1, 0) >= lib.ikrl_lmhead_bwd_workspace_bytes(2000, 1024, 5000, 0, 1, 0) + 8000

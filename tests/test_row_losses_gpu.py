@@ -510,7 +510,8 @@ def run_head(f, h, w, up, *args, **kw):
     return (loss.detach(), *torch.autograd.grad(loss, (hd, wd), up.to(DEV)))
 
 
-HEADS = [(1, 8, 5, 2), (130, 64, 1001, 16), (257, 512, 3000, 33), (64, 1024, 5003, 8), (300, 2048, 1536, 256)]
+HEADS = [(1, 8, 5, 2), (130, 64, 1001, 16), (257, 512, 3000, 33), (64, 1024, 5003, 8), (300, 2048, 1536, 256),
+         (1100, 256, 1003, 20)]
 
 
 @pytest.mark.parametrize("kind,tail", KINDS)
@@ -552,9 +553,12 @@ def test_head_cross_entropy(n, H, V, K, smoothing, z):
         assert float(got[0][1].abs()) == 0.0 and float(got[1][1].float().abs().max()) == 0.0
 
 
-@pytest.mark.parametrize("knobs", [dict(cta_pairs=0), dict(wide=0), dict(wide=1), dict(skip_zero_rows=0)])
-def test_head_under_each_kernel_choice(knobs):
-    h, w, ids, lp, up = make_head(200, 1024, 2050, 12, 21)
+@pytest.mark.parametrize("n", [200, 1100])
+@pytest.mark.parametrize("knobs", [dict(cta_pairs=0), dict(wide=0), dict(wide=1), dict(skip_zero_rows=0),
+                                   dict(balance_splits=0)])
+def test_head_under_each_kernel_choice(knobs, n):
+    h, w, ids, lp, up = make_head(n, 1024, 2050, 12, 21)
+    ids[5] = -1
     with N.tuning(**knobs):
         got = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="jsd")
     span = span_of(h.double() @ w.double().t(), ids, lp, 1.0)
@@ -564,7 +568,8 @@ def test_head_under_each_kernel_choice(knobs):
 
 @pytest.mark.parametrize("loss", ["jsd", "xent"])
 @pytest.mark.parametrize("n,H,V,slots", [(200, 1024, 2056, 200), (3, 64, 40, 3), (600, 1024, 1000, 600),
-                                         (600, 1024, 1000, 250), (600, 256, 1000, 1)])
+                                         (600, 1024, 1000, 250), (600, 256, 1000, 1),
+                                         (1100, 1024, 1000, 1100), (1100, 1024, 1000, 450), (1100, 256, 1000, 1)])
 def test_head_with_the_logit_cache(n, H, V, slots, loss, monkeypatch):
     """dS from stored numerators: all rows in the cache, some, one; rows without entries hold no slot; a
     second backward, without the cache, agrees within the roundings; the kernel choices share it."""
@@ -594,7 +599,7 @@ def test_head_with_the_logit_cache(n, H, V, slots, loss, monkeypatch):
     for knobs in ({}, dict(wide=0), dict(wide=1), dict(cta_pairs=0), dict(skip_zero_rows=0)):
         with N.tuning(**knobs):
             check_head(h, w, up, run_head(f, h, w, up, *args, **kw), rows, scale, 9, span, cached=True)
-    assert bool(asked) == (n > 256)
+    assert bool(asked) == (n > 1024)
     hd, wd = h.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
     out = f(hd, wd, *[a.to(DEV) for a in args], **kw)
     first = torch.autograd.grad(out, (hd, wd), up.to(DEV), retain_graph=True)
@@ -603,8 +608,9 @@ def test_head_with_the_logit_cache(n, H, V, slots, loss, monkeypatch):
         assert float((g1.float() - g2.float()).norm()) <= 4 * 2 ** -8 * float(g2.float().norm())
 
 
-def test_head_in_chunks_one_sided_and_bad_rows():
-    h, w, ids, lp, up = make_head(400, 256, 1000, 6, 22)
+@pytest.mark.parametrize("n", [400, 1100])
+def test_head_in_chunks_one_sided_and_bad_rows(n):
+    h, w, ids, lp, up = make_head(n, 256, 1000, 6, 22)
     up = up + 0.01
     whole = run_head(ops.lmhead_distill, h, w, up, ids, lp)
     parts = run_head(ops.lmhead_distill, h, w, up, ids, lp, chunk_rows=128)
@@ -626,10 +632,11 @@ def test_head_in_chunks_one_sided_and_bad_rows():
     assert bool(got[1].isfinite().all()) and bool(got[2].isfinite().all())
 
 
-def test_head_cache_in_chunks(monkeypatch):
-    h, w, ids, lp, up = make_head(600, 256, 1000, 6, 24)
+@pytest.mark.parametrize("n", [600, 1100])
+def test_head_cache_in_chunks(n, monkeypatch):
+    h, w, ids, lp, up = make_head(n, 256, 1000, 6, 24)
     monkeypatch.setattr(ops, "_ROW_CACHE_MIN_HIDDEN", 1)
-    for slots in (600, 300):
+    for slots in (n, n // 2):
         monkeypatch.setattr(ops, "logit_cache_rows", lambda *a: slots)
         span = span_of(h.double() @ w.double().t(), ids, lp, 1.0)
         got = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="reverse", chunk_rows=256)
@@ -637,7 +644,7 @@ def test_head_cache_in_chunks(monkeypatch):
                    lambda x: grad_scale(x, ids, lp, up), 6, span, cached=True)
 
 
-@pytest.mark.parametrize("n", [60, 400])
+@pytest.mark.parametrize("n", [60, 400, 1100])
 def test_head_c_entry_accumulates_an_fp32_dweight(n):
     """dW added to what is there, in fp32; dH left out; nothing written behind the outputs."""
     H, V = 128, 600
