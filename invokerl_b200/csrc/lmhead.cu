@@ -128,7 +128,7 @@ struct GemmParams {
   const int* cols;        // [original rows][n_cols] entry columns ascending, then kNoEntry (TAIL)
   int n_cols;
   float* xk;              // [original rows][n_cols] logits at the entries, or null (TAIL)
-  int64_t cache_cap;      // TAIL_CACHED: slots; a row's slot is slot[row] (row itself with row_idx)
+  int64_t cache_cap;      // TAIL_CACHED: slots; a row's slot is its place in the launch
   float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
   const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
   uint16_t* out_lo;       // what rounding to out_bf16 leaves, itself rounded, or null (DTAIL)
@@ -220,8 +220,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   int cslot0 = 0;
   if constexpr (is_cached(EPI)) {
     if constexpr (EPI == EPI_TAIL_CACHED) {
-      if (row_ok) cslot = (p.row_idx != nullptr || p.slot == nullptr) ? grow : p.slot[grow];
-      if (cslot >= p.cache_cap) cslot = -1;
+      if (row_ok && grow < p.cache_cap) cslot = grow;  // slots go by place in the launch
     } else if (row_ok && p.slot != nullptr) {
       cslot = p.slot[grow];
     }
@@ -2818,7 +2817,6 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
     pos = posw;
     p.m_dev = count;
     p.row_idx = idx;
-    p.slot = posw;
   }
   if (cached) {
     p.cache_cap = cache.rows;
