@@ -269,8 +269,9 @@ IKRL_API int ikrl_logits_logprob_bwd(const void* logits, int64_t ld, const int64
  *
  * Rows have logits x [V], z = x / temperature, p = softmax(z).  Distillation: each row has K teacher
  * entries (id, log-prob), q = exp(log-prob), in any order, K <= 256.  An entry counts when its id is
- * >= 0 and its log-prob is above -inf, and a repeated id at its first place only; a row without
- * entries has loss 0 and no gradient; an id >= V makes the row's loss and gradient NaN.  Outcomes
+ * >= 0 and its log-prob is not -inf, and a repeated id at its first place only; a row without
+ * entries has loss 0 and no gradient; an id >= V, or an entry that counts with a log-prob of NaN, makes
+ * the row's loss and gradient NaN.  Outcomes
  * are the entries' columns and, with `tail`, one more: any other column, of student mass p_t (the
  * sum over those columns) and teacher mass q_t = 1 - sum q (0 when that is below 2^-20).
  *   IKRL_DISTILL_FORWARD  KL(q | p); without `tail`, q is renormalised over the entries

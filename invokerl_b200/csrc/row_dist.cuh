@@ -132,7 +132,7 @@ __device__ __forceinline__ int64_t row_entries(const int64_t* __restrict__ tids,
   bool bad = false;
   if (t < K) {
     const int64_t id = tids[t];
-    const bool use = id >= 0 && !(tlp[t] == -INFINITY);  // a NaN log-prob counts and makes the row NaN
+    const bool use = id >= 0 && !(tlp[t] == -INFINITY);  // a NaN log-prob counts (row_loss makes the row NaN)
     bad = use && id >= V;
     if (use && !bad) key = (uint32_t)id << 8 | (uint32_t)t;
   }
@@ -242,6 +242,15 @@ __device__ inline void row_loss(const RowLossParams& P, int64_t row_id, int cnt,
   double q64 = 0.0;
   for (int k = lane; k < cnt; k += 32) q64 += exp((double)lp[k]);
   q64 = warp_sum(q64);
+  if (q64 != q64) {  // an entry's log-prob is NaN: so are the row's loss and gradient
+    for (int k = lane; k < cnt; k += 32) grad[k] = nan_f32();
+    if (lane == 0) {
+      *loss = nan_f32();
+      *ref = r;
+      *coef = nan_f32();
+    }
+    return;
+  }
   // ROW_FORWARD_TOPK renormalises the teacher over its entries.
   const double lq64 = P.loss == ROW_FORWARD_TOPK ? log(q64) : 0.0;
   const double left = 1.0 - q64;

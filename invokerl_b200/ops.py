@@ -793,8 +793,9 @@ def logits_distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log_
 
     p = softmax(logits / temperature); the teacher's log-probs are taken as they are.  An entry with
     an id below 0 or a log-prob of -inf is no entry, a repeated id counts at its first place, a row
-    without entries has loss 0, an id past the vocabulary makes its row NaN.  With `tail` the tokens
-    that are not entries form one more outcome, of teacher mass 1 - sum q (0 below 2^-20).
+    without entries has loss 0, an id past the vocabulary or an entry's log-prob of NaN makes its row's
+    loss and gradient NaN.  With `tail` the tokens that are not entries form one more outcome, of
+    teacher mass 1 - sum q (0 below 2^-20).
     kind "forward": KL(q | p), without `tail` over the renormalised entries; "reverse": KL(p | q);
     "jsd": beta KL(q | m) + (1 - beta) KL(p | m), m = beta q + (1 - beta) p.  The gradient goes to
     the logits only (it reads them again: do not overwrite them in between)."""

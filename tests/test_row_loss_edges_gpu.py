@@ -1,0 +1,57 @@
+"""Row losses on the GPU where their inputs are not what a healthy step gives them."""
+
+import math
+
+import pytest
+import torch
+
+from invokerl_b200 import ops
+from test_row_losses_gpu import DEV, KINDS, check_distill, make_head, make_rows, run_distill, run_head
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- teachers -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind,tail", KINDS)
+@pytest.mark.parametrize("n", [4, 310])  # one launch, and three
+def test_nan_log_prob_of_an_entry_makes_its_row_nan(n, kind, tail):
+    """Where the entry counts: not behind an id below 0, and not as a repeat of a column that is there already."""
+    x, ids, lp, up = make_rows(n, 700, 6, torch.float32, 41)
+    up = up.abs() + 0.1
+    lp[1, 2] = math.nan
+    ids[2, 3], lp[2, 3] = -1, math.nan
+    ids[0, 4], lp[0, 4] = ids[0, 1], math.nan
+    lp[3] = math.nan
+    loss, d = check_distill(x, ids, lp, up, kind, tail)
+    nan = torch.arange(n) % 2 == 1
+    nan[4:] = False
+    assert torch.equal(loss.isnan().cpu(), nan) and torch.equal(d.isnan().all(1).cpu(), nan)
+
+
+@pytest.mark.parametrize("kind,tail", KINDS)
+@pytest.mark.parametrize("n", [30, 1100])
+def test_nan_log_prob_through_the_head(n, kind, tail):
+    h, w, ids, lp, up = make_head(n, 64, 1000, 6, 42)
+    up = up.abs() + 0.1
+    want = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind=kind, tail=tail)
+    lp[3, 2] = math.nan
+    loss, dh, dw = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind=kind, tail=tail)
+    ok = torch.arange(n) != 3
+    assert bool(loss[3].isnan()) and bool(dh[3].isnan().all()) and bool(dw.isnan().all())
+    assert torch.equal(loss[ok], want[0][ok]) and torch.equal(dh[ok], want[1][ok])
+    up[3] = 0.0
+    _, dh, dw = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind=kind, tail=tail)
+    assert bool(dh.isfinite().all()) and bool(dw.isfinite().all())
+
+
+@pytest.mark.parametrize("kind,tail", KINDS)
+def test_nan_in_the_teachers_logits_reaches_the_students_loss(kind, tail):
+    x, _, _, _ = make_rows(5, 3000, 4, torch.bfloat16, 43)
+    t = x.clone()
+    t[2, 1717] = math.nan
+    lp, ids = ops.logits_topk(t.to(DEV), 8)
+    loss, d = run_distill(x, ids, lp, torch.ones(5), kind=kind, tail=tail)
+    assert loss.isnan().tolist() == [False, False, True, False, False]
+    assert d.isnan().all(1).tolist() == [False, False, True, False, False]
