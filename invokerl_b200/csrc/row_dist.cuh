@@ -251,8 +251,21 @@ __device__ inline void row_loss(const RowLossParams& P, int64_t row_id, int cnt,
     }
     return;
   }
-  // ROW_FORWARD_TOPK renormalises the teacher over its entries.
-  const double lq64 = P.loss == ROW_FORWARD_TOPK ? log(q64) : 0.0;
+  // ROW_FORWARD_TOPK renormalises the teacher over its entries: log q = lp - top - lq64.  Where their mass leaves
+  // the range of 64 bits (entries near e^-745 and below) it is summed from its largest.
+  double top = 0.0, lq64 = 0.0;
+  if (P.loss == ROW_FORWARD_TOPK) {
+    double mass = q64;
+    if (q64 < 1e-290) {
+      float hi = -INFINITY;
+      for (int k = lane; k < cnt; k += 32) hi = fmaxf(hi, lp[k]);
+      top = (double)warp_max(hi);
+      mass = 0.0;
+      for (int k = lane; k < cnt; k += 32) mass += exp((double)lp[k] - top);
+      mass = warp_sum(mass);
+    }
+    lq64 = log(mass);
+  }
   const double left = 1.0 - q64;
   const bool columns_left = cnt < P.V;
   float qt = 0.f, log_qt = 0.f;
@@ -281,7 +294,7 @@ __device__ inline void row_loss(const RowLossParams& P, int64_t row_id, int cnt,
   };
   for (int k = lane; k < cnt; k += 32) {
     const float log_p = (x[k] - m) * P.inv_t - ls * kLn2, p = exp2f((x[k] - m) * P.c - ls);
-    const float lq = (float)((double)lp[k] - lq64);
+    const float lq = (float)((double)lp[k] - top - lq64);
     float ck;
     sum += outcome(log_p, p, lq, expf(lq), ck);
     mean += p > 0.f ? p * ck : 0.f;
@@ -296,7 +309,7 @@ __device__ inline void row_loss(const RowLossParams& P, int64_t row_id, int cnt,
   const float S = P.loss == ROW_FORWARD_TOPK ? 1.f : (float)(q64 + (double)qt);
   for (int k = lane; k < cnt; k += 32) {
     const float log_p = (x[k] - m) * P.inv_t - ls * kLn2, p = exp2f((x[k] - m) * P.c - ls);
-    const float lq = (float)((double)lp[k] - lq64);
+    const float lq = (float)((double)lp[k] - top - lq64);
     const float q = expf(lq);
     float d;
     if (P.loss == ROW_FORWARD || P.loss == ROW_FORWARD_TOPK) {

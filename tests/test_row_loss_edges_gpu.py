@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from invokerl_b200 import ops
-from test_row_losses_gpu import DEV, KINDS, check_distill, make_head, make_rows, run_distill, run_head
+from row_loss_math import check_grad, check_loss, distill_rows, fp32_tol, grad_scale, loss_and_grad, loss_size
+from test_row_losses_gpu import DEV, KINDS, check_distill, make_head, make_rows, run_distill, run_head, span_of
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,20 @@ def test_nan_in_the_teachers_logits_reaches_the_students_loss(kind, tail):
     loss, d = run_distill(x, ids, lp, torch.ones(5), kind=kind, tail=tail)
     assert loss.isnan().tolist() == [False, False, True, False, False]
     assert d.isnan().all(1).tolist() == [False, False, True, False, False]
+
+
+@pytest.mark.parametrize("n", [4, 310])
+def test_renormalised_teacher_of_any_mass(n):
+    """Without the tail only the entries' ratios count, also where their mass is 0 in 64 bits; entries masked
+    with a very low value beside others weigh nothing."""
+    x, ids, lp, up = make_rows(n, 700, 6, torch.float32, 44)
+    lp[0, 3] = -1e30
+    lp[1] -= 2000
+    lp[2] = -1e30
+    lp[3] = torch.finfo(torch.float32).min
+    loss, d = run_distill(x, ids, lp, up, kind="forward", tail=False)
+    ratios = torch.log_softmax(lp.double(), 1)
+    want, dw = loss_and_grad(lambda y: distill_rows(y, ids, ratios, tail=False), x, up)
+    tol = fp32_tol(700, 6, span_of(x, ids, ratios, 1.0))
+    check_loss(loss, want, tol * loss_size(x, ids, ratios, tail=False))
+    check_grad(d, dw, x.dtype, grad_scale(x, ids, ratios, up), tol)
