@@ -57,14 +57,16 @@ __device__ __forceinline__ void load_round(Group8<T> (&g)[U], const RowPart<T>& 
   }
 }
 
+// Sum of a group in units of kSumUnit.
 template <typename T>
 __device__ __forceinline__ float group_sum(const Group8<T>& g) {
+  const uint64_t u = pack2(1.f / kSumUnit, 1.f / kSumUnit);
   float lo, hi;
-  unpack2(add2(add2(g.get2(0), g.get2(1)), add2(g.get2(2), g.get2(3))), lo, hi);
+  unpack2(add2(fma2(g.get2(1), u, mul2(g.get2(0), u)), fma2(g.get2(3), u, mul2(g.get2(2), u))), lo, hi);
   return lo + hi;
 }
 
-// Running sums of a part by a block: m, s over the tail and, with SUM, the sum of all logits.
+// Running sums of a part by a block: m, s over the tail and, with SUM, the sum of all logits (in kSumUnit).
 //
 // The loop over the part leaves out the groups that hold entries: their bits are one shared word a
 // warp and group, zero most of the time.  Those groups are taken one a thread, by the thread of their
@@ -98,7 +100,7 @@ __device__ __forceinline__ void sum_part(Group8<T> (&g)[U], const RowPart<T>& p,
     if constexpr (SUM) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (v0 + k >= 0 && v0 + k < p.rv.V) sum += h[0].get(k);
+        if (v0 + k >= 0 && v0 + k < p.rv.V) sum = fmaf(h[0].get(k), 1.f / kSumUnit, sum);
     }
     for (; first < e.cnt && e.col[first] < v0 + 8; ++first) e.x[first] = h[0].take(e.col[first] - v0);
     online_groups<T, 1>(h, c, m, s);
@@ -546,6 +548,7 @@ int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossP
   p.inv_t = 1.f;
   p.smoothing = smoothing;
   p.zeta = z_loss;
+  p.sum_unit = 1.f;
   *out = p;
   return IKRL_OK;
 }
@@ -578,8 +581,9 @@ int launch_row_losses(const float* part_m, const float* part_s, const float* par
 using namespace ikrl;
 
 static int logits_loss_fwd(const char* what, const void* logits, int32_t dtype, int64_t ld, int64_t N, int32_t V,
-                           const int64_t* tids, const float* tlp, int32_t K, const RowLossParams& P, float* loss,
+                           const int64_t* tids, const float* tlp, int32_t K, RowLossParams P, float* loss,
                            void* state, size_t state_bytes, void* stream) {
+  P.sum_unit = kSumUnit;
   int rc = check_logits_arg(what, logits, dtype, ld, N, V);
   if (rc || N == 0) return rc;
   IKRL_REQUIRE(logits && tids && loss, IKRL_ERR_INVALID_ARGUMENT, "%s: null pointer", what);

@@ -22,6 +22,10 @@ constexpr int kMaxVocab = 1 << 21;         // columns of the kernels on logits
 constexpr int kMaxParts = 8;               // parts a row of logits may be cut into
 constexpr int kNoEntry = 0x7fffffff;       // pads a row's sorted entry columns
 constexpr double kTailEps = 1.0 / (1 << 20);
+// Sums of logits in memory are kept in this unit, a power of two above their number: a row masked with the
+// type's lowest value has a mean in range although its plain sum is not.
+constexpr float kSumUnit = 4194304.f;
+static_assert(kMaxVocab < 4194304, "the unit keeps every row's sum in range");
 
 // What a row's id says (the compaction of the LM-head backward skips kRowNone rows).
 constexpr int64_t kRowNone = -100;  // no entries (or an ignored target): loss 0, no gradient
@@ -43,6 +47,7 @@ struct RowLossParams {
   float inv_t;  // 1 / T
   float beta;   // ROW_JSD
   float smoothing, zeta;  // ROW_XENT
+  float sum_unit;         // ROW_XENT: unit of the sums of all logits
 };
 
 // What a forward keeps for its backward, in one caller-owned buffer.
@@ -180,8 +185,8 @@ __device__ __forceinline__ int64_t row_entries(const int64_t* __restrict__ tids,
 }
 
 // One row's loss and gradient by one warp.  x[k], lp[k], k < cnt: the logits and teacher log-probs
-// of its entries; the tail has maximum tm and sum ts of 2^(c (x - tm)); sum_x: the sum of all logits
-// (ROW_XENT).  Writes *loss, *ref, *coef and grad[k] (grad may be lp's array: each lane reads its
+// of its entries; the tail has maximum tm and sum ts of 2^(c (x - tm)); sum_x: the sum of all logits in
+// units of P.sum_unit (ROW_XENT).  Writes *loss, *ref, *coef and grad[k] (grad may be lp's array: each lane reads its
 // entries before it writes them).
 //
 // log p is formed as (x - m) / T - log(s) with the row's maximum m: both terms are small, so nothing
@@ -226,7 +231,7 @@ __device__ inline void row_loss(const RowLossParams& P, int64_t row_id, int cnt,
       // -log p of the target: log1p of the others' sum over its own where that is the smaller
       const float nll = (rest && tm > xy) ? ls * kLn2 - (xy - m)
                                           : log1pf(rest ? ts * exp2f((tm - xy) * P.c) : 0.f);
-      const float mean = P.smoothing != 0.f ? sum_x / (float)P.V : 0.f;
+      const float mean = P.smoothing != 0.f ? sum_x / (float)P.V * P.sum_unit : 0.f;
       const float smooth = P.smoothing != 0.f ? P.smoothing * (xy - mean) : 0.f;
       *loss = nll + smooth + P.zeta * lse * lse;
       const float a1 = 2.f * P.zeta * lse;

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from invokerl_b200 import ops
-from row_loss_math import check_grad, check_loss, distill_rows, fp32_tol, grad_scale, loss_and_grad, loss_size
+from row_loss_math import (check_grad, check_loss, distill_rows, fp32_tol, grad_scale, loss_and_grad, loss_size,
+                           xent_rows)
 from test_row_losses_gpu import DEV, KINDS, check_distill, make_head, make_rows, run_distill, run_head, span_of
 
 pytestmark = pytest.mark.gpu
@@ -73,3 +74,32 @@ def test_renormalised_teacher_of_any_mass(n):
     tol = fp32_tol(700, 6, span_of(x, ids, ratios, 1.0))
     check_loss(loss, want, tol * loss_size(x, ids, ratios, tail=False))
     check_grad(d, dw, x.dtype, grad_scale(x, ids, ratios, up), tol)
+
+
+# ---- masks ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,V", [(4, 9001), (310, 9001), (3, 17), (330, 9)])
+def test_label_smoothing_beside_the_lowest_value(n, V, dtype):
+    """The mean of a row half masked with the type's lowest value is in range, its sum is not."""
+    x, ids, _, up = make_rows(n, V, 1, dtype, 45)
+    t = ids[:, 0]
+    g = torch.Generator().manual_seed(n)
+    keep = (torch.rand(n, V, generator=g) < 0.5).scatter_(1, ids, True)
+    keep[:, V - 3:] = False
+    keep.scatter_(1, ids, True)
+    x = torch.where(keep, x, torch.finfo(dtype).min)
+    xd = x.to(DEV).requires_grad_(True)
+    loss = ops.logits_cross_entropy(xd, t.to(DEV), 0.1)
+    d, = torch.autograd.grad(loss, xd, up.to(DEV))
+    want, dw = loss_and_grad(lambda y: xent_rows(y, t, 0.1), x, up)
+    # nearly all of it is 0.1 of the mean, a sum of values of one sign
+    check_loss(loss.detach(), want, fp32_tol(V, 1, 1.0) * want.abs())
+    logp = torch.log_softmax(x.double(), 1)
+    span = float(logp[keep].abs().max())
+    p = logp.exp()
+    scale = p.scatter(1, ids, 1 - p.gather(1, ids) + 0.1) + 0.1 / V
+    # the 64-bit p_y - 1 is rounded at the size of 1 and of the logits it comes from
+    ref_err = up.double().abs()[:, None] * 2.0 ** -52 * (1 + float(x[keep].double().abs().max()))
+    check_grad(d, dw, dtype, up.double().abs()[:, None] * scale, fp32_tol(V, 1, span), ref_err)
