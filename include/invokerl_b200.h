@@ -411,6 +411,8 @@ IKRL_API int ikrl_lmhead_noalloc_status(int32_t* status_out, void* stream);
  * dweight_dtype and accumulation, ikrl_lmhead_status on the workspace).  The [N, V] logits are never
  * in memory.  state: ikrl_row_loss_state_bytes(N, K), K = 1 for the cross entropy, as the forward
  * left it; dloss[N] fp32 is the upstream gradient of the row losses.
+ * Rows that have no entries (or no target), and rows whose dloss is 0, reach neither gradient, whatever
+ * their hidden state holds (NaN in padding); their dhidden is 0.
  * cache_*: a logit cache as ikrl_lmhead_logprob_fwd_cached has it (sizes from
  * ikrl_lmhead_cache_row_elems; its 16-bit numerators are fp16 here), cache_rows = 0 for none; slots
  * go to the rows that have entries (or a target), in row order, and those rows alone take part in the

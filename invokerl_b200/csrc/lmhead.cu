@@ -249,11 +249,13 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
     }
   }
   float level = 0.f;
+  bool still = true;  // DTAIL: a row without a gradient, whose logits (padding may hold NaN) do not matter
   if constexpr (EPI == EPI_DTAIL) {
     if (row_ok) {
       lse2 = p.lse[grow] * p.c;
       gval = p.g[grow];
       level = p.level[grow];
+      still = gval == 0.f && level == 0.f;
     }
   }
   if constexpr (EPI == EPI_DLOGITS) {
@@ -390,8 +392,8 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         if constexpr (EPI == EPI_DTAIL) {
-          v[i] = fmaf(gval, fast_exp2(fmaf(v[i], p.c, -lse2)), level);
-          v[i + 1] = fmaf(gval, fast_exp2(fmaf(v[i + 1], p.c, -lse2)), level);
+          v[i] = still ? 0.f : fmaf(gval, fast_exp2(fmaf(v[i], p.c, -lse2)), level);
+          v[i + 1] = still ? 0.f : fmaf(gval, fast_exp2(fmaf(v[i + 1], p.c, -lse2)), level);
           w[i >> 1] = pack_bf16x2(v[i], v[i + 1]);
           continue;
         }
@@ -2232,6 +2234,7 @@ __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __
 
 // First launch of the backward of few rows, a block a row: clears the error word; with h2 the hidden rows
 // twice, one under the other (the dW operand beside a dS of two terms); with gs what row_scale_kernel leaves.
+// Rows without a gradient go in as zeros: padding may hold NaN, and 0 NaN would reach all of dW.
 __global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__ h, int vec_per_row, uint4* __restrict__ h2,
                                                        const float* __restrict__ dloss,
                                                        const int64_t* __restrict__ row_ids,
@@ -2240,9 +2243,9 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__
                                                        int* __restrict__ err) {
   const int64_t r = blockIdx.x;
   if (r == 0 && threadIdx.x == 0) *err = 0;
+  const float g = dloss[r];
+  const bool on = g != 0.f && row_ids[r] != kRowNone;
   if (gs != nullptr && threadIdx.x == 0) {
-    const float g = dloss[r];
-    const bool on = g != 0.f && row_ids[r] != kRowNone;
     gs[r] = on ? g * coef[r] : 0.f;
     level_out[r] = on ? g * level : 0.f;
   }
@@ -2250,7 +2253,20 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__
   const uint4* from = h + r * vec_per_row;
   uint4* to = h2 + r * vec_per_row;
   uint4* below = to + (int64_t)gridDim.x * vec_per_row;
-  for (int i = threadIdx.x; i < vec_per_row; i += blockDim.x) to[i] = below[i] = from[i];
+  for (int i = threadIdx.x; i < vec_per_row; i += blockDim.x)
+    to[i] = below[i] = on ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// The dW operand where the rows are not gathered (a capture): rows without a gradient as zeros, as above.
+__global__ void live_rows_kernel(const uint4* __restrict__ h, int64_t n, int vec_per_row,
+                                 const float* __restrict__ dloss, const int64_t* __restrict__ row_ids,
+                                 uint4* __restrict__ out) {
+  const int64_t total = n * vec_per_row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / vec_per_row;
+    const bool on = dloss[r] != 0.f && row_ids[r] != kRowNone;
+    out[i] = on ? h[i] : make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 // dH of a dS of two terms: out = bf16(sum over K ranges of the partials of row r and of row rows + r).
@@ -2524,7 +2540,8 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   int64_t n_cached = 0;                                      // leading compacted rows whose dS is cached
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   IKRL_CUDA(cudaStreamIsCapturing(s, &cap));
-  if (skip_zero_rows_enabled() && cap == cudaStreamCaptureStatusNone && N <= INT32_MAX) {
+  const bool skip_rows = skip_zero_rows_enabled() && cap == cudaStreamCaptureStatusNone && N <= INT32_MAX;
+  if (skip_rows) {
     int* counts = reinterpret_cast<int*>(w + L.cnt_off);
     int64_t* n_act_d = reinterpret_cast<int64_t*>(w + L.nact_off);
     int* idx = reinterpret_cast<int*>(w + L.idx_off);
@@ -2563,6 +2580,16 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       // dH of a chunk overwrites that chunk's gathered rows once dW has read them.
       if (dhidden) { dh_out = h_c; pos = posw; }
     }
+  }
+
+  const uint16_t* hw = hsrc;  // the dW operand
+  if (rl && !skip_rows && dweight) {
+    uint4* h_c = reinterpret_cast<uint4*>(w + L.hc_off);
+    const int vpr = H / 8;
+    live_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(N * vpr, 256), 148ll * 16), 256, 0, s>>>(
+        reinterpret_cast<const uint4*>(hidden), N, vpr, dlogp, ids, h_c);
+    if ((rc = check_launch("live_rows_kernel"))) return rc;
+    hw = reinterpret_cast<const uint16_t*>(h_c);
   }
 
   float* level = nullptr;
@@ -2609,7 +2636,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     const int64_t c0 = chunks[ci].c0;
     const int64_t rows = chunks[ci].rows;
     const int m_tiles = (int)cdiv64(rows, BM);
-    const uint16_t* hc = hsrc + c0 * H;
+    const uint16_t* hc = hw + c0 * H;
     // 1) dS = g * (onehot - softmax(h W^T)) for this chunk: from the logit cache, or recomputed
     const int64_t from_cache = chunks[ci].cached;  // leading rows of the chunk
     if (from_cache > 0 && rl) {
