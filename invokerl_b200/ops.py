@@ -410,6 +410,7 @@ def set_logit_cache(mode: str = "auto", reserve_bytes: int | None = None, fracti
     if mode not in ("auto", "off"):
         raise ValueError(f"logit cache mode {mode!r} is not 'auto' or 'off'")
     prev = dict(_LOGIT_CACHE)
+    _SMALL_ROOM.clear()  # found under the previous policy
     _LOGIT_CACHE["mode"] = mode
     if reserve_bytes is not None:
         _LOGIT_CACHE["reserve_bytes"] = int(reserve_bytes)
@@ -818,7 +819,7 @@ def logits_cross_entropy(logits: torch.Tensor, targets: torch.Tensor, label_smoo
 
 
 # A head call of up to this many rows keeps all of them in the logit cache, where that takes at most
-# 256 MB, without asking how much memory is free.
+# 256 MB and the policy's memory allows it.
 _ROW_CACHE_SMALL = 1024
 # The row losses' cache pays from this H on: at 1024 the forward and backward of 16,384 rows, two thirds
 # with targets, took 10.3 ms with it and 11.2 ms without.
@@ -843,15 +844,38 @@ def _free_bytes(device: torch.device) -> int:
     return total - outside - stats["allocated_bytes"]["all"]["current"]
 
 
+# What the policy leaves small caches of each device, and when that was last found out: asking even torch's
+# allocator takes 10 us, a tenth of a small step.
+_SMALL_ROOM: dict[int, tuple[float, float]] = {}
+
+
+def _small_cache_fits(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> bool:
+    """Whether the policy of `set_logit_cache` has room for a cache of all rows beside the backward's workspace and
+    outputs.  The room is asked for once a second, and again when the caches since then have used it up."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    cache = n_rows * (2 * ((V + 63) // 64 * 64) + 4 * ((V + 31) // 32))
+    ws = N.lib().ikrl_lmhead_row_loss_bwd_workspace_bytes(n_rows, H, V, chunk_rows or 0, N.IKRL_DTYPE_BF16, 0)
+    rest = (ws + 2 * (n_rows + V) * H) * _LOGIT_CACHE["fraction"]
+    now = time.monotonic()
+    asked, room = _SMALL_ROOM.get(index, (-1e9, 0.0))
+    if now - asked > 1.0 or cache + rest > room:
+        room = (_free_bytes(device) - _LOGIT_CACHE["reserve_bytes"]) * _LOGIT_CACHE["fraction"]
+        asked = now
+    fits = cache + rest <= room
+    _SMALL_ROOM[index] = (asked, room - cache if fits else room)
+    return fits
+
+
 def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> LogitCache | None:
     """Logit cache of a row loss's forward under the policy of `set_logit_cache`, or None."""
     if _LOGIT_CACHE["mode"] == "off" or V % 8 or n_rows == 0 or torch.cuda.is_current_stream_capturing():
         return None
     if n_rows <= _ROW_CACHE_SMALL and n_rows * V <= 1 << 27:
-        return LogitCache(n_rows, V, n_rows, device)
-    if H < _ROW_CACHE_MIN_HIDDEN:
+        rows = n_rows if _small_cache_fits(n_rows, H, V, device, chunk_rows) else 0
+    elif H < _ROW_CACHE_MIN_HIDDEN:
         return None
-    rows = logit_cache_rows(n_rows, H, V, device, n_rows, chunk_rows, _ROW_CACHE_MIN_HIDDEN, _free_bytes(device))
+    else:
+        rows = logit_cache_rows(n_rows, H, V, device, n_rows, chunk_rows, _ROW_CACHE_MIN_HIDDEN, _free_bytes(device))
     if rows <= 0:
         return None
     try:

@@ -153,3 +153,30 @@ def test_padding_rows_may_hold_nan(n, cache, captured, loss):
         assert bool(g.isfinite().all())
         assert float((g.float() - ref.float()).norm()) <= 2 ** -6 * float(ref.float().norm())
         assert float(got[1][3].float().abs().max()) == float(got[1][5].float().abs().max()) == 0.0
+
+
+# ---- memory ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [60, 300])
+def test_a_small_cache_is_only_taken_where_memory_is_left(n, monkeypatch):
+    """Neither a reserve that leaves nothing nor an allocation that fails stops a call: it recomputes the logits."""
+    h, w, ids, lp, up = make_head(n, 64, 1000, 6, 47)
+    prev = ops.set_logit_cache("off")
+    try:
+        want = run_head(ops.lmhead_distill, h, w, up, ids, lp)
+        made = []
+
+        class Failing(ops.LogitCache):
+            def __init__(self, *a):
+                made.append(a)
+                raise torch.OutOfMemoryError("no memory left")
+
+        monkeypatch.setattr(ops, "LogitCache", Failing)
+        for reserve, tried in ((1 << 50, 0), (0, 1)):
+            ops.set_logit_cache("auto", reserve)
+            got = run_head(ops.lmhead_distill, h, w, up, ids, lp)
+            assert len(made) == tried
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    finally:
+        ops.set_logit_cache(prev["mode"], prev["reserve_bytes"], prev["fraction"])
