@@ -108,6 +108,11 @@ class PolicyModel:
             return None, self.model.model(input_ids=token_ids, attention_mask=attention_mask).last_hidden_state
 
     @staticmethod
+    def _row_logits(logits: Tensor) -> Tensor:
+        """Logits as the row losses and the top-k read them: bf16 and fp32 as they are, others in fp32."""
+        return logits if logits.dtype in (torch.bfloat16, torch.float32) else logits.float()
+
+    @staticmethod
     def _at_next_token(rows: Tensor) -> Tensor:
         """[B, T] row values (row t is about token t + 1) moved to the token they are about; 0 at position 0."""
         return torch.cat([torch.zeros_like(rows[:, :1]), rows[:, :-1]], dim=1)
@@ -125,9 +130,7 @@ class PolicyModel:
         log_probs = torch.full((B, T, k), -torch.inf, dtype=torch.float32, device=token_ids.device)
         ids = torch.full((B, T, k), -1, dtype=torch.int64, device=token_ids.device)
         if hidden is None:
-            if logits.dtype != torch.bfloat16:
-                logits = logits.to(torch.bfloat16)
-            lp, top = ops.logits_topk(logits, k, temperature)
+            lp, top = ops.logits_topk(self._row_logits(logits), k, temperature)
             log_probs[:, 1:], ids[:, 1:] = lp[:, :-1], top[:, :-1]
         else:
             # logits of at most 1 GiB of rows at a time
@@ -156,7 +159,7 @@ class PolicyModel:
         lp = torch.roll(teacher_log_probs, -1, dims=1)
         args = (ids, lp, kind, beta, temperature, tail)
         if hidden is None:
-            rows = ops.logits_distill(logits.to(torch.bfloat16), *args)
+            rows = ops.logits_distill(self._row_logits(logits), *args)
         else:
             rows = ops.lmhead_distill(hidden, self.model.lm_head.weight, *args)
         return self._at_next_token(rows)
@@ -173,7 +176,7 @@ class PolicyModel:
         targets = torch.full_like(token_ids, -100)
         targets[:, :-1] = torch.where(keep[:, 1:], token_ids[:, 1:], -100)
         if hidden is None:
-            rows = ops.logits_cross_entropy(logits.to(torch.bfloat16), targets, label_smoothing, z_loss)
+            rows = ops.logits_cross_entropy(self._row_logits(logits), targets, label_smoothing, z_loss)
         else:
             rows = ops.lmhead_cross_entropy(hidden, self.model.lm_head.weight, targets, label_smoothing, z_loss)
         return self._at_next_token(rows)

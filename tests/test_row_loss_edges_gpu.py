@@ -8,7 +8,8 @@ import torch
 from invokerl_b200 import ops
 from row_loss_math import (check_grad, check_loss, distill_rows, fp32_tol, grad_scale, loss_and_grad, loss_size,
                            xent_rows)
-from test_row_losses_gpu import DEV, KINDS, check_distill, make_head, make_rows, run_distill, run_head, span_of
+from test_row_losses_gpu import (DEV, KINDS, _tiny_policy, check_distill, make_head, make_rows, run_distill, run_head,
+                                 span_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -180,3 +181,29 @@ def test_a_small_cache_is_only_taken_where_memory_is_left(n, monkeypatch):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
     finally:
         ops.set_logit_cache(prev["mode"], prev["reserve_bytes"], prev["fraction"])
+
+
+# ---- policies -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_policies_with_logits_in_memory_keep_their_bits(dtype):
+    """Models that yield fp32 (or fp16) logits: their losses and top log-probs are those of the logits themselves."""
+    from invokerl_b200.policy import PolicyModel
+
+    policy = PolicyModel.from_model(_tiny_policy(2).to(dtype), fsdp_wrapped=True)
+    g = torch.Generator().manual_seed(4)
+    tok = torch.randint(0, 1000, (2, 20), generator=g).to(DEV)
+    am = torch.ones_like(tok)
+    lp, ids = policy.topk_log_probs(tok, am, 9, temperature=1.3)
+    x = policy.model(input_ids=tok, attention_mask=am).logits.detach()[:, :-1].reshape(-1, 1000)
+    assert x.dtype == dtype
+    wl, wi = ops.logits_topk(x.float(), 9, 1.3)
+    assert torch.equal(ids[:, 1:].reshape(-1, 9), wi) and torch.equal(lp[:, 1:].reshape(-1, 9), wl)
+    other = torch.log_softmax(torch.randn(2, 20, 9, generator=g), -1).to(DEV) - 0.1
+    kl = policy.distill_loss(tok, am, ids, other, kind="jsd")
+    assert torch.equal(kl[:, 1:].reshape(-1), ops.logits_distill(x.float(), wi, other[:, 1:].reshape(-1, 9), "jsd"))
+    ce = policy.cross_entropy_loss(tok, am, 0.1, 1e-4)
+    assert torch.equal(ce[:, 1:].reshape(-1), ops.logits_cross_entropy(x.float(), tok[:, 1:].reshape(-1), 0.1, 1e-4))
+    (kl.sum() + ce.sum()).backward()
+    assert all(bool(p.grad.isfinite().all()) for p in policy.model.parameters())
