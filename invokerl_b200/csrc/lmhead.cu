@@ -1418,7 +1418,10 @@ template <int EPI, bool A_MN, bool B_MN, bool WIDE>
 int launch_gemm_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap* c, const GemmParams& p_in,
                      int m_tiles, cudaStream_t s) {
   GemmParams p = p_in;
-  auto kern = WIDE ? lmhead_gemm_wide_kernel<EPI, A_MN, B_MN> : lmhead_gemm_pair_kernel<EPI, A_MN, B_MN>;
+  const auto kern = [] {
+    if constexpr (WIDE) return lmhead_gemm_wide_kernel<EPI, A_MN, B_MN>;
+    else return lmhead_gemm_pair_kernel<EPI, A_MN, B_MN>;
+  }();
   p.ds_tma = (WIDE && c != nullptr && is_staged(EPI)) ? 1 : 0;
   const uint32_t smem_bytes = WIDE ? (p.ds_tma ? kWideDsSmemBytes : kWideSmemBytes) : kPairSmemBytes;
   IKRL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes));
