@@ -129,6 +129,7 @@ struct GemmParams {
   int n_cols;
   float* xk;              // [original rows][n_cols] logits at the entries, or null (TAIL)
   int64_t cache_cap;      // TAIL_CACHED: slots; a row's slot is its place in the launch
+  int part_cap;           // sets that part_m, part_s and part_x hold (TAIL)
   float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
   const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
   uint16_t* out_lo;       // what rounding to out_bf16 leaves, itself rounded, or null (DTAIL)
@@ -1513,17 +1514,19 @@ int64_t pair_makespan(int64_t m_pairs, int n_tiles, int tps, int64_t npairs) {
 
 // Balance of the persistent pairs: the L2 rule's split count can leave a last round of units on
 // a few pairs only (14 m-pairs x 11 splits = 154 units over 74 pairs runs 3 rounds where the mean
-// is 2.1).  Up to 3x the hinted count, take a larger count when it shortens the busiest pair's
-// work by at least 5%; more splits mean more W re-reads, so near-balanced hints stay.  Used for
-// the backward's dS launches, which have no per-split workspace.  IKRL_TUNE_BALANCE_SPLITS = 0
-// keeps the hint.
+// is 2.1).  Up to kBalanceMost times the hinted count, take a larger count when it shortens the busiest
+// pair's work by at least 5%; more splits mean more W re-reads, so near-balanced hints stay.  Used for the
+// backward's dS launches, which have no per-split workspace, and for the row losses' forward, whose workspace
+// holds that many sets (row_loss_fwd_layout; launch_k1 checks it).  IKRL_TUNE_BALANCE_SPLITS = 0 keeps the
+// hint.
+constexpr int kBalanceMost = 3;
 bool balance_splits_enabled() { return tuning(IKRL_TUNE_BALANCE_SPLITS) != 0; }
 
 int balanced_tiles_per_split(int64_t m_tiles, int n_tiles, int splits_hint, int64_t npairs) {
   const int64_t m_pairs = (m_tiles + 1) / 2;
   int best_tps = (int)cdiv64(n_tiles, splits_hint);
   int64_t best = pair_makespan(m_pairs, n_tiles, best_tps, npairs);
-  for (int sp = splits_hint + 1; sp <= std::min(3 * splits_hint, n_tiles); ++sp) {
+  for (int sp = splits_hint + 1; sp <= std::min(kBalanceMost * splits_hint, n_tiles); ++sp) {
     const int tps = (int)cdiv64(n_tiles, sp);
     if (tps == best_tps) continue;
     const int64_t ms = pair_makespan(m_pairs, n_tiles, tps, npairs);
@@ -1653,6 +1656,8 @@ int launch_k1(const CUtensorMap& a_single, const CUtensorMap& b_single, const CU
   p.splits = pl.splits;
   p.split_major = 1;
   p.part_sets = p.splits * (kind == 2 ? kWideGroups : 1);
+  if constexpr (is_tail(EPI))
+    IKRL_REQUIRE(p.part_sets <= p.part_cap, IKRL_ERR_WORKSPACE, "%d partial sets, room for %d", p.part_sets, p.part_cap);
   {
     // L2 policy of the A and B loads of the wide kernel (0 normal, 1 evict-last, 2 evict-first),
     // IKRL_TUNE_L2_POLICY = 10 * a + b.  Default: A (re-read by every tile of a unit) evict-last,
@@ -2355,20 +2360,21 @@ static bool row_loss_dense(int64_t N, int H, int V) {
   return N <= kRowLossDense || (N <= kRowLossDenseMost && (double)N * H * V <= kRowLossDenseWork);
 }
 
-// Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums
-// of all logits (up to 3 times the forward's splits, which the balance rule may take), and the
-// numbering of the rows that count with their hidden rows gathered.
+// Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums of all logits (`sets` of
+// each: the wide kernel's column groups of up to kBalanceMost times the forward's splits, which the balance
+// rule may take), and the numbering of the rows that count with their hidden rows gathered.
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 struct RowLossFwdLayout {
   size_t pm_off, ps_off, px_off, counts_off, count_off, pos_off, idx_off, hc_off, total;
-  int splits;
+  int splits, sets;
   bool gather;  // the rows that count are gathered before the GEMM
 };
 static RowLossFwdLayout row_loss_fwd_layout(int64_t N, int H, int V) {
   RowLossFwdLayout L;
   L.splits = fwd_layout(N, H, V).splits;
   L.gather = !row_loss_dense(N, H, V);
-  const size_t part = align256((size_t)kWideGroups * 3 * L.splits * N * 4);
+  L.sets = kWideGroups * kBalanceMost * L.splits;
+  const size_t part = align256((size_t)L.sets * N * 4);
   size_t o = 256;  // the error word
   L.pm_off = o; o += part;
   L.ps_off = o; o += part;
@@ -2808,6 +2814,7 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   p.M = (int)N; p.N = V; p.K = H;
   p.part_m = reinterpret_cast<float*>(w + L.pm_off);
   p.part_s = reinterpret_cast<float*>(w + L.ps_off);
+  p.part_cap = L.sets;
   p.part_x = P.loss == ROW_XENT && P.smoothing != 0.f ? reinterpret_cast<float*>(w + L.px_off) : nullptr;
   p.err = err;
   p.c = P.c;
@@ -2834,8 +2841,11 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
     LiveSplit ls{pl.n_tiles, pl.tiles_per_split, pl.splits, 0, 0, std::max(1, nsm / 2), pl.kind == 2 ? kWideGroups : 1};
     if (pl.kind != 0 && persistent_pairs() && balance_splits_enabled()) {
       ls.least = std::min(L.splits, pl.n_tiles);
-      ls.most = std::min(3 * L.splits, pl.n_tiles);  // as many sets as the workspace has
+      ls.most = std::min(kBalanceMost * L.splits, pl.n_tiles);
     }
+    IKRL_REQUIRE(std::max(ls.most, ls.splits) * ls.groups <= L.sets, IKRL_ERR_WORKSPACE,
+                 "%s: %d column ranges of %d groups, room for %d sets", what, std::max(ls.most, ls.splits), ls.groups,
+                 L.sets);
     row_index_kernel<<<(unsigned)cdiv64(N, 256), 256, 0, s>>>(posw, N, cache.rows, idx, cached ? cache.slot : nullptr,
                                                               counts, nb, ls, count);
     if ((rc = check_launch("row_index_kernel"))) return rc;
