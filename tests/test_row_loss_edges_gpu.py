@@ -6,10 +6,10 @@ import pytest
 import torch
 
 from invokerl_b200 import ops
-from row_loss_math import (check_grad, check_loss, distill_rows, fp32_tol, grad_scale, loss_and_grad, loss_size,
-                           xent_rows)
-from test_row_losses_gpu import (DEV, KINDS, _tiny_policy, check_distill, make_head, make_rows, run_distill, run_head,
-                                 span_of)
+from row_loss_math import (EPS32, check_grad, check_loss, distill_rows, fp32_tol, grad_scale, loss_and_grad,
+                           loss_size, xent_rows)
+from test_row_losses_gpu import (DEV, KINDS, _tiny_policy, check_distill, check_head, make_head, make_rows, run_distill,
+                                 run_head, span_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -207,3 +207,72 @@ def test_policies_with_logits_in_memory_keep_their_bits(dtype):
     assert torch.equal(ce[:, 1:].reshape(-1), ops.logits_cross_entropy(x.float(), tok[:, 1:].reshape(-1), 0.1, 1e-4))
     (kl.sum() + ce.sum()).backward()
     assert all(bool(p.grad.isfinite().all()) for p in policy.model.parameters())
+
+
+# ---- many column tiles ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("loss", ["reverse", "xent"])
+@pytest.mark.parametrize("n,H,V", [(1100, 64, 40000), (1100, 1024, 40001), (2300, 1024, 32000), (4500, 128, 9001)])
+def test_gathered_rows_over_many_column_tiles(n, H, V, loss):
+    """Some tens of column tiles, dealt out on the device for the rows that count: every column is in every row's
+    sums once.  A logit errs by at most 2 H half-steps of fp32 (the accumulators cut) of its terms' magnitudes, E;
+    a loss by the sum of its derivatives times E beside its own arithmetic; the gradients' whole as check_head."""
+    h, w, ids, lp, up = make_head(n, H, V, 20 if loss == "reverse" else 1, n + H)
+    off = torch.arange(n) % 3 == 1
+    t = torch.where(off, -100, ids[:, 0])
+    ids[off] = -1
+    if loss == "reverse":
+        got = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="reverse")
+        rows = lambda y: distill_rows(y, ids, lp, "reverse")  # noqa: E731
+    else:
+        got = run_head(ops.lmhead_cross_entropy, h, w, up, t, label_smoothing=0.1)
+        rows = lambda y: xent_rows(y, t, 0.1)  # noqa: E731
+    h, w, ids, lp, up, t = (a.to(DEV) for a in (h, w, ids, lp, up, t))
+    x = h.double() @ w.double().t()
+    err = 2 * H * EPS32 * (h.double().abs() @ w.double().abs().t())
+    want, ds = loss_and_grad(rows, x, torch.ones(n, device=DEV))
+    span = float((x.amax(1) - x.amin(1)).max())
+    tol = fp32_tol(V, ids.shape[1], span) * (1 + span) + 1.01 * (ds.abs() * err).sum(1)
+    check_loss(got[0], want, tol.cpu())
+    ds *= up.double()[:, None]
+    for g, ref in ((got[1], ds @ w.double()), (got[2], ds.t() @ h.double())):
+        assert float((g.double() - ref).norm() / ref.norm()) <= 2 ** -7 + 8 * float(err.max())
+
+
+@pytest.mark.parametrize("loss", ["jsd", "xent"])
+@pytest.mark.parametrize("slots", [0, 1, 250, 599, 600])
+def test_a_cache_of_some_rows_of_a_small_batch(slots, loss, monkeypatch):
+    """Up to 1024 rows a cache is used when it holds all of them, and otherwise left alone: both directions of the C
+    entries agree on which."""
+    n, H, V = 600, 64, 1000
+    h, w, ids, lp, up = make_head(n, H, V, 9, 48)
+    ids[1::3] = -1
+    made = []
+
+    def some(*a):
+        made.append(ops.LogitCache(n, V, slots, torch.device(DEV, 0)) if slots else None)
+        if slots:
+            made[-1].slot.fill_(7)
+            made[-1].q.fill_(3.0)
+        return made[-1]
+
+    monkeypatch.setattr(ops, "_row_cache", some)
+    if loss == "jsd":
+        got = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="jsd", temperature=1.3)
+        rows, scale = lambda y: distill_rows(y, ids, lp, "jsd", 0.5, 1.3), lambda x: grad_scale(x, ids, lp, up, 1.3)
+        span = span_of(h.double() @ w.double().t(), ids, lp, 1.3)
+    else:
+        t = torch.where(ids[:, 0] < 0, -100, ids[:, 0])
+        got = run_head(ops.lmhead_cross_entropy, h, w, up, t, label_smoothing=0.1)
+        rows = lambda y: xent_rows(y, t, 0.1)  # noqa: E731
+        x = h.double() @ w.double().t()
+        span = float((x.amax(1) - x.amin(1)).max())
+
+        def scale(x):
+            p = torch.softmax(x, 1)
+            return up.double().abs()[:, None] * (p + 0.1 / V).scatter(1, t.clamp(min=0)[:, None], 1.0)
+
+    check_head(h, w, up, got, rows, scale, 9, span, cached=True)
+    if slots:
+        assert bool((made[0].slot == 7).all()) and bool((made[0].q == 3.0).all()) == (slots < n)
