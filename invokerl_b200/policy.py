@@ -136,7 +136,7 @@ class PolicyModel:
             # logits of at most 1 GiB of rows at a time
             w = self.model.lm_head.weight.to(torch.bfloat16)
             h = hidden.to(torch.bfloat16)
-            step = max(1, (1 << 30) // (2 * w.shape[0] * B))
+            step = max(1, (1 << 30) // (2 * w.shape[0] * max(1, B)))
             for s in range(0, T - 1, step):
                 e = min(s + step, T - 1)
                 lp, top = ops.logits_topk(torch.nn.functional.linear(h[:, s:e], w), k, temperature)

@@ -1,6 +1,7 @@
 """Row losses on the GPU where their inputs are not what a healthy step gives them."""
 
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -207,6 +208,36 @@ def test_policies_with_logits_in_memory_keep_their_bits(dtype):
     assert torch.equal(ce[:, 1:].reshape(-1), ops.logits_cross_entropy(x.float(), tok[:, 1:].reshape(-1), 0.1, 1e-4))
     (kl.sum() + ce.sum()).backward()
     assert all(bool(p.grad.isfinite().all()) for p in policy.model.parameters())
+
+
+@pytest.mark.parametrize("fsdp", [False, True])
+@pytest.mark.parametrize("B,T", [(0, 7), (2, 1), (1, 2)])
+def test_policies_on_the_smallest_batches(B, T, fsdp):
+    """No sequences, and sequences without a second token: nothing to learn from, and no error."""
+    from invokerl_b200.policy import PolicyModel
+
+    w = torch.randn(50, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+
+    class Body:
+        lm_head = SimpleNamespace(weight=w)
+
+        def model(self, input_ids, attention_mask):
+            return SimpleNamespace(last_hidden_state=torch.ones(*input_ids.shape, 64, device=DEV, dtype=w.dtype))
+
+        def __call__(self, input_ids, attention_mask):
+            return SimpleNamespace(logits=self.model(input_ids, attention_mask).last_hidden_state @ w.t())
+
+    policy = PolicyModel.from_model(Body(), fsdp_wrapped=fsdp)
+    tok = torch.zeros(B, T, dtype=torch.int64, device=DEV)
+    am = torch.ones_like(tok)
+    lp, ids = policy.topk_log_probs(tok, am, 3)
+    assert lp.shape == ids.shape == (B, T, 3) and bool((ids[:, :1] == -1).all())
+    ce = policy.cross_entropy_loss(tok, am)
+    assert bool((ce[:, 1:] > 0).all())
+    for loss in (policy.distill_loss(tok, am, ids, lp), ce):
+        assert loss.shape == (B, T) and not bool(loss[:, :1].any()) and bool(loss.isfinite().all())
+        dw, = torch.autograd.grad(loss.sum(), w)
+        assert bool(dw.isfinite().all())
 
 
 # ---- many column tiles ----------------------------------------------------------------------------
