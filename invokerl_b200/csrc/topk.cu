@@ -437,8 +437,9 @@ __global__ void __launch_bounds__(kTopThreads, 3) topk_block_kernel(const T* __r
 // Many rows: resident blocks take row after row.  512 threads sweep and never stop for a choice: they hand
 // what they swept to 128 more, which choose and write the row's output while the next row is read.  Two
 // buffers between them; barriers 2, 3 say that one is full, 4, 5 that it is free.  Top 64 of 4096 rows of
-// 151936 bf16 columns: 256 us (4.9 TB/s), 244 us of it the sweep, where exponentials (63% of the special
-// function units' rate) and loads take turns; of 2048 fp32 rows 199 us (6.3 TB/s).
+// 151936 bf16 columns: 247 us in a row of calls, 256 from a cold L2, 270 after other work (4.6 to 5.0 TB/s), nearly
+// all of it the sweep, where exponentials (67% of the special function units' rate) and loads take turns; of
+// 2048 fp32 rows 194 us (6.4 TB/s).
 constexpr int kChoosers = 128;
 constexpr int kStreamThreads = kTopThreads + kChoosers;
 template <typename T, int U>

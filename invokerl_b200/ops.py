@@ -374,8 +374,9 @@ def default_chunk_rows(N: int, V: int, budget_bytes: int | None = None) -> int:
 
 
 class LogitCache:
-    """Softmax numerators the forward stored for up to `rows` rows (bf16, relative to each
-    32-column chunk's maximum) and those maxima (fp32), with each row's slot (-1: not cached).
+    """Softmax numerators the forward stored for up to `rows` rows (16 bits each, relative to each
+    32-column chunk's maximum: bf16 for `lmhead_logprob`; the row losses put fp16 bits into `q`,
+    whatever its dtype says) and those maxima (fp32), with each row's slot (-1: not cached).
     The backward forms the cached rows' dlogits from it instead of recomputing their logits."""
 
     def __init__(self, n_rows: int, V: int, rows: int, device):
@@ -400,7 +401,7 @@ class LogitCache:
 # numerators: on B200 the Qwen3-8B head (H = 4096) step ran 17% faster with it, the Qwen3-0.6B
 # head (H = 1024) 9% slower, so "auto" caches from H = 2048 (min_hidden).
 _LOGIT_CACHE = {"mode": "auto", "reserve_bytes": 4 << 30, "fraction": 0.9, "min_rows": 1024, "min_hidden": 2048}
-# Cache rows and candidate rows of the last forward that needed a gradient (for reports).
+# Cache rows and candidate rows of the last `lmhead_logprob` that needed a gradient (for reports).
 LOGIT_CACHE_STATS = {"rows": 0, "candidates": 0}
 
 
@@ -867,7 +868,8 @@ def _small_cache_fits(n_rows: int, H: int, V: int, device, chunk_rows: int | Non
 
 
 def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> LogitCache | None:
-    """Logit cache of a row loss's forward under the policy of `set_logit_cache`, or None."""
+    """Logit cache of a row loss's forward under the policy of `set_logit_cache`, or None.  A capture has none: its
+    pool would hold the memory for as long as the graph lives."""
     if _LOGIT_CACHE["mode"] == "off" or V % 8 or n_rows == 0 or torch.cuda.is_current_stream_capturing():
         return None
     if n_rows <= _ROW_CACHE_SMALL and n_rows * V <= 1 << 27:
@@ -969,7 +971,13 @@ def lmhead_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
                    teacher_log_probs: torch.Tensor, kind: str = "forward", beta: float = 0.5,
                    temperature: float = 1.0, tail: bool = True, chunk_rows: int | None = None) -> torch.Tensor:
     """`logits_distill` of the logits hidden [..., H] @ weight [V, H].T, which are never in memory:
-    fp32 loss [...], gradients to hidden and weight.  `chunk_rows` as in `lmhead_logprob`."""
+    fp32 loss [...], gradients to hidden and weight.
+
+    `chunk_rows` as in `lmhead_logprob`, except that up to 256 rows, and up to 1024 where
+    rows * H * V <= 2^34, it is without effect: all rows' dlogits are formed at once, in two bf16
+    terms (4 bytes an element of [rows, V]), which leaves the gradients the error of their own rounding.
+    Above that they are formed in one term, as in `lmhead_logprob`, and the gradients err by about
+    1.4 times as much."""
     params = _distill_params(kind, beta, temperature, tail)
     N.require_cuda(hidden, weight, teacher_ids, teacher_log_probs)
     h, w = _head_rows(hidden, weight)
@@ -982,7 +990,7 @@ def lmhead_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
                          label_smoothing: float = 0.0, z_loss: float = 0.0,
                          chunk_rows: int | None = None) -> torch.Tensor:
     """`logits_cross_entropy` of the logits hidden [..., H] @ weight [V, H].T, which are never in
-    memory: fp32 loss [...], gradients to hidden and weight.  `chunk_rows` as in `lmhead_logprob`."""
+    memory: fp32 loss [...], gradients to hidden and weight.  `chunk_rows` as in `lmhead_distill`."""
     label_smoothing, z_loss = _check_xent(label_smoothing, z_loss)
     N.require_cuda(hidden, weight, targets)
     h, w = _head_rows(hidden, weight)

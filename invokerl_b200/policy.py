@@ -122,7 +122,9 @@ class PolicyModel:
                        temperature: float = 1.0) -> tuple[Tensor, Tensor]:
         """As a teacher: (log_probs fp32, ids int64), both [B, T, k], where position t holds the k
         likeliest tokens given the tokens before t.  Position 0 and unattended positions hold no
-        entries (-inf, -1), which `distill_loss` skips."""
+        entries (-inf, -1), which `distill_loss` skips.  Without FSDP the logits are formed in bf16, as
+        the model's own head gives them: log-probs carry that rounding (2^-8 of a logit), which the
+        student's, summed in fp32 by the fused head, do not."""
         token_ids = token_ids.to(self.device)
         attention_mask = attention_mask.to(self.device)
         logits, hidden = self._body(token_ids, attention_mask)
