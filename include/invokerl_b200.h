@@ -411,6 +411,8 @@ IKRL_API int ikrl_lmhead_noalloc_status(int32_t* status_out, void* stream);
  * dweight_dtype and accumulation, ikrl_lmhead_status on the workspace).  The [N, V] logits are never
  * in memory.  state: ikrl_row_loss_state_bytes(N, K), K = 1 for the cross entropy, as the forward
  * left it; dloss[N] fp32 is the upstream gradient of the row losses.
+ * dW and dH have the error of their final rounding (dS is held in two bf16 terms up to the limit below, in
+ * fp16 with a scale per row above it; the workspace then holds a scaled fp16 copy of the weight, V H 2 bytes).
  * Rows that have no entries (or no target), and rows whose dloss is 0, reach neither gradient, whatever
  * their hidden state holds (NaN in padding); their dhidden is 0.
  * cache_*: a logit cache as ikrl_lmhead_logprob_fwd_cached has it (sizes from

@@ -84,6 +84,8 @@ constexpr int epi_kind(int epi) {
          : epi == EPI_STORE_TMA           ? (int)EPI_STORE_BF16
                                           : epi;
 }
+// Epilogues whose GEMM may have fp16 operands.
+constexpr bool takes_f16(int epi) { return epi == EPI_F32 || epi == EPI_STORE_BF16 || epi == EPI_STORE_TMA; }
 enum F32Mode : int { F32_STORE = 0, F32_ADD = 1, F32_ADD_TO_BF16 = 2 };
 
 struct GemmParams {
@@ -133,6 +135,10 @@ struct GemmParams {
   float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
   const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
   uint16_t* out_lo;       // what rounding to out_bf16 leaves, itself rounded, or null (DTAIL)
+  // Products of fp16 operands scaled by powers of two (the row losses' dW and dH; see RowRange)
+  int f16;                // A and B are fp16 (F32, STORE_BF16, STORE_TMA); the output is (DTAIL)
+  const float* out_scale; // what the output is multiplied by, one for all or (scale_rows) each row's, or null
+  int scale_rows;
 };
 
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err) {
@@ -148,6 +154,11 @@ __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, i
 
 __device__ __forceinline__ void st_global_v4(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // What a row loss's forward over gathered rows runs with: the rows there are (known on the device only), the
@@ -269,6 +280,10 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   // Column index of the target in this W (a vocab shard starts at id_offset); ignore_index rows
   // keep -100, which matches no column.
   if (tgt != -100) tgt -= p.id_offset;
+  float out_scale = 1.f;
+  if constexpr (takes_f16(EPI)) {
+    if (p.out_scale != nullptr) out_scale = p.scale_rows ? (row_ok ? p.out_scale[grow] : 0.f) : p.out_scale[0];
+  }
   float run_m = -INFINITY, run_s = 0.f, tval = 0.f;
   bool found = false;
 
@@ -290,16 +305,12 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
     }
   };
   // The numerators v of a chunk whose maximum is cm into the logit cache.  They are at most 1: a row
-  // loss keeps them in fp16, whose 11 bits leave the one rounding of dS to bf16 (in bf16 the two
-  // together took dH and dW from 1.4 to 1.55 times the error of a single final rounding); what lies
-  // below 2^-14 of its chunk's maximum loses bits that the sums over the vocabulary do not see.
+  // loss keeps them in fp16, whose 11 bits its dS has as well (bf16's 8 would be most of its gradients'
+  // error); what lies below 2^-14 of its chunk's maximum loses bits that the sums over the vocabulary
+  // do not see.
   auto pack16 = [](float lo, float hi) -> uint32_t {
-    if constexpr (EPI == EPI_TAIL_CACHED) {
-      const __half2 h = __floats2half2_rn(lo, hi);
-      return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      return pack_bf16x2(lo, hi);
-    }
+    if constexpr (EPI == EPI_TAIL_CACHED) return pack_f16x2(lo, hi);
+    else return pack_bf16x2(lo, hi);
   };
   auto store_numerators = [&](const float* v, int col0, float cm) {
     uint32_t w[16];
@@ -319,6 +330,12 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   // The epilogue of one 32-column chunk of this thread's row, columns [col0, col0 + 32) of the
   // output (col0 < N; the chunk may end past N).  Warp-uniform control flow.
   auto chunk = [&](float* v, int col0) {
+    if constexpr (takes_f16(EPI)) {
+      if (p.out_scale != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= out_scale;
+      }
+    }
     const int nvalid = min(32, p.N - col0);
     if constexpr (is_lse(EPI)) {
       float cm = -INFINITY;
@@ -395,7 +412,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
         if constexpr (EPI == EPI_DTAIL) {
           v[i] = still ? 0.f : fmaf(gval, fast_exp2(fmaf(v[i], p.c, -lse2)), level);
           v[i + 1] = still ? 0.f : fmaf(gval, fast_exp2(fmaf(v[i + 1], p.c, -lse2)), level);
-          w[i >> 1] = pack_bf16x2(v[i], v[i + 1]);
+          w[i >> 1] = p.f16 ? pack_f16x2(v[i], v[i + 1]) : pack_bf16x2(v[i], v[i + 1]);
           continue;
         }
         const float p0 = fast_exp2(fmaf(v[i], kLog2e, -lse2));
@@ -666,7 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (lane == 0 && ntiles > 0) {
-      constexpr uint32_t idesc = idesc_bf16_f32(BM, BN, A_MN, B_MN);
+      uint32_t idesc = idesc_bf16_f32(BM, BN, A_MN, B_MN);
+      if constexpr (takes_f16(EPI)) idesc = p.f16 ? idesc_f16_f32(BM, BN, A_MN, B_MN) : idesc;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -889,7 +907,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA only) ----------------
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16_f32(2 * BM, BN, A_MN, B_MN);
+      uint32_t idesc = idesc_bf16_f32(2 * BM, BN, A_MN, B_MN);
+      if constexpr (takes_f16(EPI)) idesc = p.f16 ? idesc_f16_f32(2 * BM, BN, A_MN, B_MN) : idesc;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -1100,7 +1119,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA only) ----------------
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16_f32(2 * BM, BN, A_MN, B_MN);
+      uint32_t idesc = idesc_bf16_f32(2 * BM, BN, A_MN, B_MN);
+      if constexpr (takes_f16(EPI)) idesc = p.f16 ? idesc_f16_f32(2 * BM, BN, A_MN, B_MN) : idesc;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -2024,22 +2044,24 @@ __global__ void __launch_bounds__(256) ds_from_cache_kernel(
 
 // The same for a row loss: dS = g (coef q 2^(c (m - ref)) + level), then g grad at the row's entries,
 // written behind a barrier by the block that holds their columns.  slot null: row r has slot r; idx null:
-// chunk row k is row c0 + k.  Rows without a gradient (or a slot) are zeros.  TWO: dS in two terms, what the
-// rounding to bf16 leaves (rounded itself) `rows` rows below.
+// chunk row k is row c0 + k.  Rows without a gradient (or a slot) are zeros.  TWO: dS in two bf16 terms, what the
+// rounding of the first leaves (rounded itself) `rows` rows below; otherwise dS times mul[c0 + k] in fp16.
 template <bool TWO>
 __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
     const uint16_t* __restrict__ cache_q, const float* __restrict__ cache_m, int64_t ld_cache, int n_mchunks,
     const int* __restrict__ slot, const int* __restrict__ idx, const float* __restrict__ dloss,
     const int64_t* __restrict__ row_ids, const float* __restrict__ refs, const float* __restrict__ coefs,
-    const int* __restrict__ cols, const float* __restrict__ grads, int K, float level, float c, int64_t c0,
-    int64_t rows, int V, uint16_t* __restrict__ ds, int64_t ld_ds) {
+    const int* __restrict__ cols, const float* __restrict__ grads, const float* __restrict__ mul, int K, float level,
+    float c, int64_t c0, int64_t rows, int V, uint16_t* __restrict__ ds, int64_t ld_ds) {
   const int vec = V >> 3;
   const int jb = blockIdx.x * blockDim.x * kDsUnroll + threadIdx.x;  // gridDim.x covers the columns
   for (int64_t k = blockIdx.y; k < rows; k += gridDim.y) {
     const int64_t r = idx ? idx[c0 + k] : c0 + k;
     const int64_t sl = slot ? slot[r] : r;
-    const float g = dloss[r], ref = refs[r], coef = coefs[r];
+    float g = dloss[r];
+    const float ref = refs[r], coef = coefs[r];
     const bool on = sl >= 0 && g != 0.f && row_ids[r] != kRowNone;
+    if constexpr (!TWO) g *= mul[c0 + k];
     const float gs = g * coef, lv = on ? g * level : 0.f;
     const uint16_t* qrow = cache_q + (on ? sl : 0) * ld_cache;
     const float* mrow = cache_m + (on ? sl : 0) * n_mchunks;
@@ -2068,8 +2090,12 @@ __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
       for (int e = 0; e < 4; ++e) {
         const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
         const float d0 = fmaf(q.x, sc, lv), d1 = fmaf(q.y, sc, lv);
-        o[e] = pack_bf16x2(d0, d1);
-        if constexpr (TWO) lo[e] = pack_bf16x2(d0 - bf16lo(o[e]), d1 - bf16hi(o[e]));
+        if constexpr (TWO) {
+          o[e] = pack_bf16x2(d0, d1);
+          lo[e] = pack_bf16x2(d0 - bf16lo(o[e]), d1 - bf16hi(o[e]));
+        } else {
+          o[e] = pack_f16x2(d0, d1);
+        }
       }
       *reinterpret_cast<uint4*>(drow + (jv << 3)) = make_uint4(o[0], o[1], o[2], o[3]);
       if constexpr (TWO) *reinterpret_cast<uint4*>(lrow + (jv << 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -2081,8 +2107,12 @@ __global__ void __launch_bounds__(256) dtail_from_cache_kernel(
         const int col = cols[r * K + e];
         if (col == kNoEntry || col < lo || col >= hi) continue;
         const float d = g * grads[r * K + e];
-        drow[col] = f32_to_bf16_rn(d);
-        if constexpr (TWO) lrow[col] = f32_to_bf16_rn(d - bf16_to_f32(drow[col]));
+        if constexpr (TWO) {
+          drow[col] = f32_to_bf16_rn(d);
+          lrow[col] = f32_to_bf16_rn(d - bf16_to_f32(drow[col]));
+        } else {
+          drow[col] = __half_as_ushort(__float2half_rn(d));
+        }
       }
     }
   }
@@ -2206,26 +2236,130 @@ __global__ void scatter_rows_kernel(const uint4* __restrict__ src, const int* __
   }
 }
 
-// Row losses, backward: what the dS epilogue multiplies and adds for compacted row k (row idx[k]; k
-// itself when idx is null), gs = g coef and level_out = g level; 0 for rows without a gradient.
-__global__ void row_scale_kernel(const float* __restrict__ dloss, const int64_t* __restrict__ row_ids,
-                                 const float* __restrict__ coef, const int* __restrict__ idx, int64_t n, float level,
-                                 float* __restrict__ gs, float* __restrict__ level_out) {
-  const int64_t k = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+// The backward of a row loss multiplies fp16 operands.  Rounded to bf16, dS took dH and dW to 1.4 times the error of
+// their own final rounding (1.7 times where the upstream gradients are all alike and round the same way); in fp16 it
+// leaves them at 1.0 times.  bf16 hidden rows and weights fit fp16 as they are, 8 bits in 11, and what fp16 lacks in
+// range powers of two supply, which the epilogues take out again:
+//   dS'_k = dS_k 2^(14 - e_k)        2^e_k above the largest |dS_k|
+//   h'_k  = h_k 2^(e_k - 14 - X)     X one for all, so that the largest is below 2^15
+//   W'    = W 2^(15 - e_W)           2^e_W above the largest |W|
+//   dW    = 2^X dS'^T h',            dH_k = 2^(e_k + e_W - 29) dS'_k W'
+// What lies more than 2^29 below its largest loses bits, one for each further 2, which is 2^-40 of that largest at most.
+// Rows without a gradient are zeros in both operands (padding may hold NaN).  Infinities and NaN do not count for the
+// ranges and stay what they are.  One more pass over W and a copy: 0.5 ms of 20 (8192 x 4096 x 151936).
+struct RowRange {
+  int* e;           // [rows] e_k, or kNoRange: no gradient
+  float* mul;       // [rows] 2^(14 - e_k)
+  float* gs;        // [rows] g coef mul and
+  float* level;     // [rows] g level mul: what the dS epilogue multiplies and adds
+  float* dh_scale;  // [rows] 2^(e_k + e_W - 29)
+  unsigned* top;    // [0] largest e_k plus exponent of |h_k|, biased, 0: no row; [1] largest |W|, its bits;
+  float* dw_scale;  // [1] 2^X
+  uint16_t* h;      // [rows][H] h'
+  uint16_t* w;      // [V][H] W'
+};
+constexpr int kNoRange = INT_MIN;
+constexpr int kRangeBias = 1024;
+
+// Exponent e with |x| < 2^e of a bf16 magnitude's bits (2^(e - 1) <= |x| too where x is a normal number).
+__device__ __forceinline__ int bf16_exponent(uint32_t bits) { return (int)(bits >> 7) - 126; }
+// e_W from the bits of the largest |W| (0: W is not wanted, or all of it is 0).
+__device__ __forceinline__ int weight_exponent(unsigned bits) { return bits == 0 ? 0 : max(bf16_exponent(bits), -111); }
+__device__ __forceinline__ uint32_t largest_finite(uint32_t m, uint32_t w) {
+  const uint32_t lo = w & 0x7fffu, hi = (w >> 16) & 0x7fffu;
+  m = max(m, lo < 0x7f80u ? lo : 0u);
+  return max(m, hi < 0x7f80u ? hi : 0u);
+}
+__device__ __forceinline__ uint32_t largest_finite(uint32_t m, uint4 v) {
+  return largest_finite(largest_finite(largest_finite(largest_finite(m, v.x), v.y), v.z), v.w);
+}
+
+// Ranges of rows [0, n): one warp a row (row idx[k], k itself when idx is null).
+__global__ void __launch_bounds__(256) row_range_kernel(const float* __restrict__ dloss,
+                                                        const int64_t* __restrict__ row_ids,
+                                                        const float* __restrict__ coefs, const int* __restrict__ cols,
+                                                        const float* __restrict__ grads, int K,
+                                                        const int* __restrict__ idx, int64_t n, float level,
+                                                        const uint4* __restrict__ h, int vec_per_row, RowRange R) {
+  const int64_t k = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
   if (k >= n) return;
   const int64_t r = idx ? idx[k] : k;
-  const float g = dloss[r];
+  const float g = dloss[r], coef = coefs[r];
   const bool on = g != 0.f && row_ids[r] != kRowNone;
-  gs[k] = on ? g * coef[r] : 0.f;
-  level_out[k] = on ? g * level : 0.f;
+  float most = fabsf(coef);
+  for (int e = lane; e < K; e += 32)
+    if (cols[r * K + e] != kNoEntry) most = fmaxf(most, fabsf(grads[r * K + e]));
+  most = (warp_max(most) + fabsf(level)) * fabsf(g);
+  uint32_t hm = 0;
+  for (int i = lane; i < vec_per_row; i += 32) hm = largest_finite(hm, h[k * vec_per_row + i]);
+  hm = __reduce_max_sync(0xffffffffu, hm);
+  if (lane != 0) return;
+  int e = kNoRange;
+  float mul = 0.f;
+  if (on) {
+    e = 0;  // of an infinite or NaN gradient
+    if (most < INFINITY) frexpf(most, &e);
+    e = max(e, max(-100, -120 - weight_exponent(R.top[1])));  // 2^(e + e_W - 29) is a number
+    mul = ldexpf(1.f, 14 - e);
+    if (hm > 0) atomicMax(&R.top[0], (unsigned)(kRangeBias + e + bf16_exponent(hm)));
+  }
+  R.e[k] = e;
+  R.mul[k] = mul;
+  R.gs[k] = on ? g * mul * coef : 0.f;
+  R.level[k] = on ? g * mul * level : 0.f;
+}
+
+__global__ void __launch_bounds__(256) weight_range_kernel(const uint4* __restrict__ w, int64_t n,
+                                                           unsigned* __restrict__ top) {
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+    m = largest_finite(m, w[i]);
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m > 0) atomicMax(top, m);
+}
+
+__device__ __forceinline__ uint32_t scale_to_f16(uint32_t w, float f) { return pack_f16x2(bf16lo(w) * f, bf16hi(w) * f); }
+__device__ __forceinline__ uint4 scale_to_f16(uint4 v, float f) {
+  return make_uint4(scale_to_f16(v.x, f), scale_to_f16(v.y, f), scale_to_f16(v.z, f), scale_to_f16(v.w, f));
+}
+
+// h' and the products' scales (h null: the scales only).
+__global__ void __launch_bounds__(256) scale_rows_kernel(const uint4* __restrict__ h, int64_t n, int vec_per_row,
+                                                         RowRange R) {
+  // 2^X is a normal number: rows so small that it is not keep fewer bits of theirs
+  const int X = min(max((int)R.top[0] - kRangeBias - 29, -126), 127);
+  const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (first == 0) R.dw_scale[0] = ldexpf(1.f, X);
+  const int ew = weight_exponent(R.top[1]);
+  const int64_t total = h != nullptr ? n * vec_per_row : n;
+  const int per = h != nullptr ? vec_per_row : 1;
+  for (int64_t i = first; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t k = i / per;
+    const int e = R.e[k];
+    if (i == k * per) R.dh_scale[k] = e == kNoRange ? 1.f : ldexpf(1.f, e + ew - 29);
+    if (h != nullptr)
+      reinterpret_cast<uint4*>(R.h)[i] =
+          e == kNoRange ? make_uint4(0u, 0u, 0u, 0u) : scale_to_f16(h[i], ldexpf(1.f, min(e - 14 - X, 126)));
+  }
+}
+
+__global__ void __launch_bounds__(256) scale_weight_kernel(const uint4* __restrict__ w, int64_t n, RowRange R) {
+  const float f = ldexpf(1.f, 15 - weight_exponent(R.top[1]));
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+    reinterpret_cast<uint4*>(R.w)[i] = scale_to_f16(w[i], f);
 }
 
 // Row losses, backward: the gradient at the entries of chunk rows [c0, c0 + rows) goes over what the
-// dS epilogue wrote there.  One block of threads per 256 entries.  two: the second term too, `rows` rows
-// below the first.
+// dS epilogue wrote there.  One block of threads per 256 entries.  TWO: two bf16 terms, the second `rows` rows
+// below the first; otherwise times mul[c0 + k] in fp16.
+template <bool TWO>
 __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __restrict__ cols,
-                                  const float* __restrict__ grad, int K, const int* __restrict__ idx, int64_t c0,
-                                  int64_t rows, uint16_t* __restrict__ ds, int64_t ld_ds, bool two) {
+                                  const float* __restrict__ grad, const float* __restrict__ mul, int K,
+                                  const int* __restrict__ idx, int64_t c0, int64_t rows, uint16_t* __restrict__ ds,
+                                  int64_t ld_ds) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= rows * K) return;
   const int64_t k = i / K;
@@ -2234,14 +2368,19 @@ __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __
   const int col = cols[r * K + e];
   if (col == kNoEntry) return;
   const float g = dloss[r];
-  const float d = g != 0.f ? g * grad[r * K + e] : 0.f;
-  const uint16_t hi = f32_to_bf16_rn(d);
-  ds[k * ld_ds + col] = hi;
-  if (two) ds[(rows + k) * ld_ds + col] = f32_to_bf16_rn(d - bf16_to_f32(hi));
+  if constexpr (TWO) {
+    const float d = g != 0.f ? g * grad[r * K + e] : 0.f;
+    const uint16_t hi = f32_to_bf16_rn(d);
+    ds[k * ld_ds + col] = hi;
+    ds[(rows + k) * ld_ds + col] = f32_to_bf16_rn(d - bf16_to_f32(hi));
+  } else {
+    ds[k * ld_ds + col] = __half_as_ushort(__float2half_rn(g != 0.f ? g * mul[c0 + k] * grad[r * K + e] : 0.f));
+  }
 }
 
 // First launch of the backward of few rows, a block a row: clears the error word; with h2 the hidden rows
-// twice, one under the other (the dW operand beside a dS of two terms); with gs what row_scale_kernel leaves.
+// twice, one under the other (the dW operand beside a dS of two terms); with gs what the dS epilogue multiplies and
+// adds.
 // Rows without a gradient go in as zeros: padding may hold NaN, and 0 NaN would reach all of dW.
 __global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__ h, int vec_per_row, uint4* __restrict__ h2,
                                                        const float* __restrict__ dloss,
@@ -2263,18 +2402,6 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__
   uint4* below = to + (int64_t)gridDim.x * vec_per_row;
   for (int i = threadIdx.x; i < vec_per_row; i += blockDim.x)
     to[i] = below[i] = on ? from[i] : make_uint4(0u, 0u, 0u, 0u);
-}
-
-// The dW operand where the rows are not gathered (a capture): rows without a gradient as zeros, as above.
-__global__ void live_rows_kernel(const uint4* __restrict__ h, int64_t n, int vec_per_row,
-                                 const float* __restrict__ dloss, const int64_t* __restrict__ row_ids,
-                                 uint4* __restrict__ out) {
-  const int64_t total = n * vec_per_row;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / vec_per_row;
-    const bool on = dloss[r] != 0.f && row_ids[r] != kRowNone;
-    out[i] = on ? h[i] : make_uint4(0u, 0u, 0u, 0u);
-  }
 }
 
 // dH of a dS of two terms: out = bf16(sum over K ranges of the partials of row r and of row rows + r).
@@ -2486,6 +2613,26 @@ static int launch_short_dw(const CUtensorMap& ta, const CUtensorMap& tb, GemmPar
   return launch_k1<EPI_STORE_BF16, true, true>(ta, tb, ta, tb, p, v_tiles, 0, s);
 }
 
+// The workspace of a RowRange.
+static size_t row_range_bytes(int64_t N, int H, int V) {
+  return 256 + 5 * align256((size_t)N * 4) + align256((size_t)N * H * 2) + align256((size_t)V * H * 2);
+}
+static RowRange row_range(char* w, int64_t N, int H) {
+  RowRange R;
+  const size_t n4 = align256((size_t)N * 4);
+  R.top = reinterpret_cast<unsigned*>(w);
+  R.dw_scale = reinterpret_cast<float*>(w) + 2;
+  w += 256;
+  R.e = reinterpret_cast<int*>(w);
+  R.mul = reinterpret_cast<float*>(w + n4);
+  R.gs = reinterpret_cast<float*>(w + 2 * n4);
+  R.level = reinterpret_cast<float*>(w + 3 * n4);
+  R.dh_scale = reinterpret_cast<float*>(w + 4 * n4);
+  R.h = reinterpret_cast<uint16_t*>(w + 5 * n4);
+  R.w = reinterpret_cast<uint16_t*>(w + 5 * n4 + align256((size_t)N * H * 2));
+  return R;
+}
+
 // A row loss (row_dist.cuh) behind the LM head's backward: the state its forward left, and its level
 // (the constant part of the gradient).
 struct RowLossBwd {
@@ -2498,10 +2645,7 @@ struct RowLossBwd {
 // cache_slot / cache_q / cache_m: the logit cache a forward filled (all null: no cache).  Active
 // rows with a slot take their dS from the cache; the others are recomputed by the dS GEMM.
 // rl: null for log p(ids); otherwise the row loss whose gradient dlogp is, with ids and lse its
-// state's row_ids and ref.  dS is rounded to bf16, the type of the products' operands, for both: a relative error
-// of up to 2^-8 an element, of which a sum over many rows or columns keeps little (8192 x 4096 x 151936: dH and dW err
-// by 2.3e-3 of their size, 1.7e-3 is their own rounding).  A second term, as few rows have it, would double the
-// two products that are two thirds of the step.
+// state's row_ids and ref, and the workspace has a RowRange behind the layout's.
 static int lmhead_bwd_impl(const char* what, const void* hidden, const void* weight, const int64_t* ids,
                            const float* lse, const float* dlogp, int64_t N, int32_t H, int32_t V, int64_t vocab_start,
                            int64_t chunk_rows, void* dhidden, void* dweight, int32_t dweight_dtype,
@@ -2520,7 +2664,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   IKRL_REQUIRE(lse && dlogp && (dhidden || dweight), IKRL_ERR_INVALID_ARGUMENT,
                "%s: null pointer", what);
   const BwdLayout L = bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
-  const size_t ws_need = L.total + (rl ? align256((size_t)N * 4) : 0);
+  const size_t ws_need = L.total + (rl ? row_range_bytes(N, H, V) : 0);
   IKRL_REQUIRE(ws != nullptr && ws_bytes >= ws_need, IKRL_ERR_WORKSPACE,
                "%s: workspace %zu < %zu bytes", what, ws_bytes, ws_need);
   IKRL_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 255) == 0, IKRL_ERR_ALIGNMENT,
@@ -2595,23 +2739,30 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   }
 
   const uint16_t* hw = hsrc;  // the dW operand
-  if (rl && !skip_rows && dweight) {
-    uint4* h_c = reinterpret_cast<uint4*>(w + L.hc_off);
+  RowRange R{};
+  if (rl) {
+    R = row_range(w + L.total, N, H);
     const int vpr = H / 8;
-    live_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(N * vpr, 256), 148ll * 16), 256, 0, s>>>(
-        reinterpret_cast<const uint4*>(hidden), N, vpr, dlogp, ids, h_c);
-    if ((rc = check_launch("live_rows_kernel"))) return rc;
-    hw = reinterpret_cast<const uint16_t*>(h_c);
-  }
-
-  float* level = nullptr;
-  if (rl && !(rl->all_cached && cache_slot != nullptr)) {  // what the dS epilogue multiplies and adds
-    float* gs = reinterpret_cast<float*>(w + L.gc_off);
-    level = reinterpret_cast<float*>(w + L.total);
-    row_scale_kernel<<<(unsigned)cdiv64(Nw, 256), 256, 0, s>>>(dlogp, rl->st.row_ids, rl->st.coef, idx_c, Nw,
-                                                               rl->level, gs, level);
-    if ((rc = check_launch("row_scale_kernel"))) return rc;
-    gsrc = gs;
+    IKRL_CUDA(cudaMemsetAsync(R.top, 0, 2 * sizeof(unsigned), s));
+    const uint4* hv = reinterpret_cast<const uint4*>(hsrc);
+    const int64_t nw = (int64_t)V * vpr;
+    const unsigned wb = (unsigned)std::min<int64_t>(cdiv64(nw, 256), 148ll * 8);
+    if (dhidden) {
+      weight_range_kernel<<<wb, 256, 0, s>>>(reinterpret_cast<const uint4*>(weight), nw, R.top + 1);
+      if ((rc = check_launch("weight_range_kernel"))) return rc;
+    }
+    row_range_kernel<<<(unsigned)cdiv64(Nw, 8), 256, 0, s>>>(dlogp, rl->st.row_ids, rl->st.coef, rl->st.cols, rl->st.grad,
+                                                             rl->K, idx_c, Nw, rl->level, hv, vpr, R);
+    if ((rc = check_launch("row_range_kernel"))) return rc;
+    scale_rows_kernel<<<(unsigned)std::min<int64_t>(cdiv64(dweight ? Nw * vpr : Nw, 256), 148ll * 8), 256, 0, s>>>(
+        dweight ? hv : nullptr, Nw, vpr, R);
+    if ((rc = check_launch("scale_rows_kernel"))) return rc;
+    if (dhidden) {
+      scale_weight_kernel<<<wb, 256, 0, s>>>(reinterpret_cast<const uint4*>(weight), nw, R);
+      if ((rc = check_launch("scale_weight_kernel"))) return rc;
+    }
+    gsrc = R.gs;
+    hw = R.h;
   }
 
   const BwdLayout Lw = bwd_layout(Nw, H, V, chunk_rows, dweight_dtype, accumulate_dweight);
@@ -2642,7 +2793,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
   CUtensorMap t_w_k, t_w_k2, t_w_mn;
   if ((rc = make_tmap(&t_w_k, weight, H, V, H, BN, "weight"))) return rc;
   if ((rc = make_tmap(&t_w_k2, weight, H, V, H, BN / 2, "weight"))) return rc;
-  if ((rc = make_tmap(&t_w_mn, weight, H, V, H, 64, "weight^T"))) return rc;
+  if ((rc = make_tmap(&t_w_mn, rl && dhidden ? (const void*)R.w : weight, H, V, H, 64, "weight^T"))) return rc;
 
   for (int64_t ci = 0; ci < nchunks; ++ci) {
     const int64_t c0 = chunks[ci].c0;
@@ -2656,8 +2807,8 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
                       (unsigned)std::min<int64_t>(from_cache, 65535));
       dtail_from_cache_kernel<false><<<grid, 256, 0, s>>>(
           cache_q, cache_m, L.lds, (int)cdiv64(V, 32), cache_slot, idx_c, dlogp,
-          rl->st.row_ids, rl->st.ref, rl->st.coef, rl->st.cols, rl->st.grad, rl->K, rl->level, rl->c, c0, from_cache, V,
-          dS, L.lds);
+          rl->st.row_ids, rl->st.ref, rl->st.coef, rl->st.cols, rl->st.grad, R.mul, rl->K, rl->level, rl->c, c0,
+          from_cache, V, dS, L.lds);
       if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
     } else if (from_cache > 0) {
       const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)),
@@ -2681,8 +2832,9 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       p.out_bf16 = dS_r; p.ld_bf16 = L.lds;
       p.err = err;
       if (rl) {
-        p.level = level + r0;
+        p.level = R.level + r0;
         p.c = rl->c;
+        p.f16 = 1;
         if ((rc = launch_k1<EPI_DTAIL, false, false>(ta, t_w_k, ta, t_w_k2, p, nr_tiles, sp, s, &tds))) return rc;
       } else {
         if ((rc = launch_k1<EPI_DLOGITS, false, false>(ta, t_w_k, ta, t_w_k2, p, nr_tiles, sp, s, &tds))) return rc;
@@ -2690,9 +2842,8 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
     }
     if (rl && from_cache < rows) {
       const int64_t n = rows - from_cache;
-      ds_entries_kernel<<<(unsigned)cdiv64(n * rl->K, 256), 256, 0, s>>>(dlogp, rl->st.cols, rl->st.grad, rl->K, idx_c,
-                                                                         c0 + from_cache, n, dS + from_cache * L.lds,
-                                                                         L.lds, false);
+      ds_entries_kernel<false><<<(unsigned)cdiv64(n * rl->K, 256), 256, 0, s>>>(
+          dlogp, rl->st.cols, rl->st.grad, R.mul, rl->K, idx_c, c0 + from_cache, n, dS + from_cache * L.lds, L.lds);
       if ((rc = check_launch("ds_entries_kernel"))) return rc;
     }
     // 2) dW (+)= dS^T h[chunk]
@@ -2703,6 +2854,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       GemmParams p{};
       p.M = V; p.N = H; p.K = (int)rows;
       p.err = err;
+      if (rl) { p.f16 = 1; p.out_scale = R.dw_scale; }
       const int v_tiles = (int)cdiv64(V, BM);
       const bool last = ci == nchunks - 1;
       if (dweight_dtype == IKRL_DTYPE_BF16 && !use_dw32 && rl && rows < kShortDw) {
@@ -2730,6 +2882,7 @@ static int lmhead_bwd_impl(const char* what, const void* hidden, const void* wei
       GemmParams p{};
       p.M = (int)rows; p.N = H; p.K = V;
       p.err = err;
+      if (rl) { p.f16 = 1; p.out_scale = R.dh_scale + c0; p.scale_rows = 1; }
       const int ks = dh_split_k(m_tiles, H, V, rows, L.part_elems, nsm, rl != nullptr);
       if (ks > 1) {
         float* part = reinterpret_cast<float*>(w + L.part_off);
@@ -2936,7 +3089,7 @@ static int lmhead_row_loss_bwd_few(const char* what, const void* hidden, const v
     const dim3 grid((unsigned)std::max<int64_t>(1, cdiv64(V / 8, 256 * kDsUnroll)), (unsigned)N);
     dtail_from_cache_kernel<true><<<grid, 256, 0, s>>>(cache.q, cache.m, L.lds, (int)cdiv64(V, 32), nullptr, nullptr,
                                                        dloss, rl.st.row_ids, rl.st.ref, rl.st.coef, rl.st.cols,
-                                                       rl.st.grad, rl.K, rl.level, rl.c, 0, N, V, ds, L.lds);
+                                                       rl.st.grad, nullptr, rl.K, rl.level, rl.c, 0, N, V, ds, L.lds);
     if ((rc = check_launch("dtail_from_cache_kernel"))) return rc;
   } else {
     CUtensorMap ta, tb, tb2, tds;
@@ -2952,8 +3105,8 @@ static int lmhead_row_loss_bwd_few(const char* what, const void* hidden, const v
     const int m_tiles = (int)cdiv64(N, BM);
     const int sp = choose_splits(m_tiles, (int)cdiv64(V, BN), H);
     if ((rc = launch_k1<EPI_DTAIL, false, false>(ta, tb, ta, tb2, p, m_tiles, sp, s, &tds))) return rc;
-    ds_entries_kernel<<<(unsigned)cdiv64(N * rl.K, 256), 256, 0, s>>>(dloss, rl.st.cols, rl.st.grad, rl.K, nullptr, 0,
-                                                                      N, ds, L.lds, true);
+    ds_entries_kernel<true><<<(unsigned)cdiv64(N * rl.K, 256), 256, 0, s>>>(dloss, rl.st.cols, rl.st.grad, nullptr, rl.K,
+                                                                            nullptr, 0, N, ds, L.lds);
     if ((rc = check_launch("ds_entries_kernel"))) return rc;
   }
   // 2) dW (+)= [hi; lo]^T [h; h]
@@ -3043,7 +3196,7 @@ size_t ikrl_lmhead_row_loss_bwd_workspace_bytes(int64_t N, int32_t H, int32_t V,
                                                 int32_t dweight_dtype, int32_t accumulate_dweight) {
   if (N <= 0 || H <= 0 || V <= 0) return 256;
   if (row_loss_dense(N, H, V)) return few_layout(N, H, V).total;
-  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + align256((size_t)N * 4);
+  return bwd_layout(N, H, V, chunk_rows, dweight_dtype, accumulate_dweight).total + row_range_bytes(N, H, V);
 }
 
 int ikrl_lmhead_distill_fwd(const void* hidden, const void* weight, const int64_t* teacher_ids,

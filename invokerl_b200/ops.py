@@ -421,9 +421,10 @@ def set_logit_cache(mode: str = "auto", reserve_bytes: int | None = None, fracti
 
 
 def logit_cache_rows(n_rows: int, H: int, V: int, device, candidates: int, chunk_rows: int | None = None,
-                     min_hidden: int | None = None, free: int | None = None) -> int:
+                     min_hidden: int | None = None, free: int | None = None, workspace: int | None = None) -> int:
     """Cache rows the policy allows for a forward of n_rows rows with `candidates` cacheable rows
-    (min_hidden: another smallest H; free: the bytes free for it, asked of the driver when None)."""
+    (min_hidden: another smallest H; free: the bytes free for it, asked of the driver when None;
+    workspace: the backward's bytes, `lmhead_logprob`'s when None)."""
     if min_hidden is None:
         min_hidden = _LOGIT_CACHE["min_hidden"]
     if _LOGIT_CACHE["mode"] == "off" or V % 8 or candidates <= 0 or H < min_hidden:
@@ -433,9 +434,10 @@ def logit_cache_rows(n_rows: int, H: int, V: int, device, candidates: int, chunk
         free += torch.cuda.memory_reserved(device) - torch.cuda.memory_allocated(device)
     if chunk_rows is None:
         chunk_rows = default_chunk_rows(n_rows, V)
-    bwd = int(N.lib().ikrl_lmhead_bwd_workspace_bytes(n_rows, H, V, chunk_rows, N.IKRL_DTYPE_BF16, 0))
+    if workspace is None:
+        workspace = int(N.lib().ikrl_lmhead_bwd_workspace_bytes(n_rows, H, V, chunk_rows, N.IKRL_DTYPE_BF16, 0))
     outputs = n_rows * H * 2 + V * H * 2  # dhidden and dweight of the backward
-    avail = (free - bwd - outputs - _LOGIT_CACHE["reserve_bytes"]) * _LOGIT_CACHE["fraction"]
+    avail = (free - workspace - outputs - _LOGIT_CACHE["reserve_bytes"]) * _LOGIT_CACHE["fraction"]
     rows = min(candidates, max(0, int(avail) // LogitCache.bytes_per_row(V)))
     return rows if rows >= _LOGIT_CACHE["min_rows"] else 0
 
@@ -877,7 +879,9 @@ def _row_cache(n_rows: int, H: int, V: int, device, chunk_rows: int | None) -> L
     elif H < _ROW_CACHE_MIN_HIDDEN:
         return None
     else:
-        rows = logit_cache_rows(n_rows, H, V, device, n_rows, chunk_rows, _ROW_CACHE_MIN_HIDDEN, _free_bytes(device))
+        ws = N.lib().ikrl_lmhead_row_loss_bwd_workspace_bytes(
+            n_rows, H, V, default_chunk_rows(n_rows, V) if chunk_rows is None else chunk_rows, N.IKRL_DTYPE_BF16, 0)
+        rows = logit_cache_rows(n_rows, H, V, device, n_rows, chunk_rows, _ROW_CACHE_MIN_HIDDEN, _free_bytes(device), ws)
     if rows <= 0:
         return None
     try:
@@ -975,9 +979,9 @@ def lmhead_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
 
     `chunk_rows` as in `lmhead_logprob`, except that up to 256 rows, and up to 1024 where
     rows * H * V <= 2^34, it is without effect: all rows' dlogits are formed at once, in two bf16
-    terms (4 bytes an element of [rows, V]), which leaves the gradients the error of their own rounding.
-    Above that they are formed in one term, as in `lmhead_logprob`, and the gradients err by about
-    1.4 times as much."""
+    terms (4 bytes an element of [rows, V]).  Above that they are formed in fp16 with a scale per row,
+    and the backward's workspace holds a scaled copy of the weight.  Either way the gradients have
+    the error of their own rounding to bf16."""
     params = _distill_params(kind, beta, temperature, tail)
     N.require_cuda(hidden, weight, teacher_ids, teacher_log_probs)
     h, w = _head_rows(hidden, weight)

@@ -307,3 +307,77 @@ def test_a_cache_of_some_rows_of_a_small_batch(slots, loss, monkeypatch):
     check_head(h, w, up, got, rows, scale, 9, span, cached=True)
     if slots:
         assert bool((made[0].slot == 7).all()) and bool((made[0].q == 3.0).all()) == (slots < n)
+
+
+# ---- the gradients' precision and range -------------------------------------------------------------
+
+
+def own_rounding(ref):
+    """Size of what rounding the 64-bit value to bf16 alone leaves."""
+    return float((ref.bfloat16().double() - ref).norm())
+
+
+@pytest.mark.parametrize("cache", ["auto", "off"])
+@pytest.mark.parametrize("loss", ["reverse", "jsd", "xent"])
+@pytest.mark.parametrize("n,H,V", [(1500, 72, 5000), (1100, 1024, 2056), (3000, 128, 1003)])
+def test_gradients_of_gathered_rows_err_by_their_own_rounding(n, H, V, loss, cache, monkeypatch):
+    """dS is rounded to fp16 (twice, with numerators from a cache), whose half step is an eighth of bf16's: beside
+    the final rounding, sqrt(1 + 2 / 64) = 1.016 times its error; the logits' own errors are far below.  With equal
+    upstream gradients, which round alike, a bf16 dS would leave 1.4 to 1.7 times."""
+    monkeypatch.setattr(ops, "_ROW_CACHE_MIN_HIDDEN", 1)
+    h, w, ids, lp, _ = make_head(n, H, V, 12, n + V)
+    up = torch.where(torch.arange(n) % 3 == 1, 0.0, 1.0 / n)
+    prev = ops.set_logit_cache(cache)
+    try:
+        if loss == "xent":
+            got = run_head(ops.lmhead_cross_entropy, h, w, up, ids[:, 0].contiguous(), label_smoothing=0.05)
+        else:
+            got = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind=loss)
+    finally:
+        ops.set_logit_cache(prev["mode"])
+    h, w, ids, lp, up = (a.to(DEV) for a in (h, w, ids, lp, up))
+    rows = (lambda y: xent_rows(y, ids[:, 0], 0.05)) if loss == "xent" else (lambda y: distill_rows(y, ids, lp, loss))
+    _, ds = loss_and_grad(rows, h.double() @ w.double().t(), up)
+    for g, ref in ((got[1], ds @ w.double()), (got[2], ds.t() @ h.double())):
+        assert float((g.double() - ref).norm()) <= 1.05 * own_rounding(ref)
+
+
+@pytest.mark.parametrize("cache", ["auto", "off"])
+@pytest.mark.parametrize("ws,us", [(-40, 0), (30, 0), (0, -60), (0, 40), (-20, -50), (25, 30)])
+def test_powers_of_two_pass_through_the_gradients(ws, us, cache, monkeypatch):
+    """2^ws W and 2^-ws h have the same logits: dW and dH are 2^-ws and 2^ws times as large, bit for bit, and 2^us
+    times with an upstream gradient that is."""
+    monkeypatch.setattr(ops, "_ROW_CACHE_MIN_HIDDEN", 1)
+    n = 1100
+    h, w, ids, lp, up = make_head(n, 64, 1000, 9, 51)
+    prev = ops.set_logit_cache(cache)
+    try:
+        want = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="jsd")
+        got = run_head(ops.lmhead_distill, h * 2.0 ** -ws, w * 2.0 ** ws, up * 2.0 ** us, ids, lp, kind="jsd")
+    finally:
+        ops.set_logit_cache(prev["mode"])
+    assert torch.equal(got[0], want[0])
+    assert torch.equal(got[1].double(), want[1].double() * 2.0 ** (us + ws))
+    assert torch.equal(got[2].double(), want[2].double() * 2.0 ** (us - ws))
+
+
+def test_rows_of_very_different_gradients():
+    """Each row's dH keeps its bits beside rows with a gradient 2^40 times as large, and infinite ones; dW is the
+    large rows'."""
+    n = 1100
+    h, w, ids, lp, up = make_head(n, 64, 1000, 9, 52)
+    up = up.abs() + 0.5
+    want = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="reverse")
+    small = torch.arange(n) % 2 == 1
+    few = torch.where(small, 2.0 ** -40, 1.0)
+    got = run_head(ops.lmhead_distill, h, w, up * few, ids, lp, kind="reverse")
+    assert torch.equal(got[1].double(), want[1].double() * few.to(DEV)[:, None].double())
+    large = run_head(ops.lmhead_distill, h, w, torch.where(small, 0.0, up), ids, lp, kind="reverse")
+    # both within half a bf16 step (2^-8) of fp32 sums of the same large terms in another order
+    assert float((got[2].double() - large[2].double()).norm()) <= 2.0 ** -7 * 1.01 * float(large[2].double().norm())
+    up[6] = math.inf
+    _, dh, dw = run_head(ops.lmhead_distill, h, w, up, ids, lp, kind="reverse")
+    ok = torch.arange(n) != 6
+    assert torch.equal(dh[ok], want[1][ok]) and not bool(dh[6].isfinite().any()) and not bool(dw.isfinite().all())
+    zero = run_head(ops.lmhead_distill, h, torch.zeros_like(w), up.clamp(max=1.0), ids, lp, kind="reverse")
+    assert not bool(zero[1].any()) and bool(zero[2].isfinite().all())
