@@ -566,8 +566,7 @@ int launch_row_entries(const int64_t* tids, const float* tlp, int64_t N, int K, 
 int launch_row_losses(const float* part_m, const float* part_s, const float* part_x, int sets,
                       const int* sets_dev, const int* pos, int64_t N, int K, const RowLossParams& p, const RowState& st,
                       float* loss, const int* err, cudaStream_t s) {
-  // Few rows come with many sets (a GEMM of one row tile cuts the columns as fine as it can).
-  if (sets > 64 && N <= 4 * kNumSMs)
+  if (row_takes_a_block(sets, N))
     row_losses_kernel<4><<<(unsigned)N, 128, 0, s>>>(part_m, part_s, part_x, sets, sets_dev, pos, N, K, p, st, loss,
                                                         err);
   else

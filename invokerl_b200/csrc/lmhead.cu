@@ -131,6 +131,7 @@ struct GemmParams {
   int n_cols;
   float* xk;              // [original rows][n_cols] logits at the entries, or null (TAIL)
   int64_t cache_cap;      // TAIL_CACHED: slots; a row's slot is its place in the launch
+  int* part_c;            // [splits][M] columns of the maxima in part_m, or null (TAIL)
   int part_cap;           // sets that part_m, part_s and part_x hold (TAIL)
   float* part_x;          // [splits][M] sum of all logits, or null (TAIL)
   const float* level;     // [M] constant part of the gradient (DTAIL); lse: the row's ref, g: its coef
@@ -244,6 +245,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
   float* entry_x = nullptr;
   int next = kNoEntry, at = 0;
   float sum_x = 0.f;
+  int run_c = 0;
   auto advance = [&]() { next = ++at < p.n_cols ? next_col[at] : kNoEntry; };
   if constexpr (is_tail(EPI)) {
     if (row_ok) {
@@ -391,6 +393,12 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (i < nvalid) cm = fmaxf(cm, v[i]);
+      if (p.part_c != nullptr && cm > run_m) {
+        int at_max = 0;  // columns past N come last, so the lowest of equal ones is a column
+#pragma unroll
+        for (int i = 31; i >= 0; --i) at_max = v[i] == cm ? i : at_max;
+        run_c = col0 + at_max;
+      }
       const float from = cm == -INFINITY ? 0.f : cm;  // a chunk of entries only sums to 0
       float cs = 0.f;
 #pragma unroll
@@ -578,6 +586,7 @@ __device__ __forceinline__ bool epilogue_role(const GemmParams& p, uint32_t tmem
       p.part_m[o] = run_m;
       p.part_s[o] = run_s;
       if (p.part_x != nullptr) p.part_x[o] = sum_x;
+      if (p.part_c != nullptr) p.part_c[o] = run_c;
     }
   }
   return ok;
@@ -2179,26 +2188,11 @@ __global__ void gather_live_rows_kernel(const uint4* __restrict__ h, const int* 
   }
 }
 
-// A distillation's logits at the entries, xk[r][e] = h_r . w_col, one warp an entry: 32-bit sums of
-// exact products, rounded.  The GEMM's accumulators cut every partial sum to 24 bits towards zero,
-// which at K = 4096 takes 4e-6 of a logit of 12 away; the student's likely tokens are mostly among the
-// entries, so this leaves little of it (loss of an 8B-sized head against 64 bits: 1.3e-5 -> 2.5e-6).
-// A cross entropy takes its target's logit from the accumulators instead: there the likely tokens stay
-// in the tail, and target and tail are short by about the same (2e-6 against 1e-5 with only the target
-// exact).
-__global__ void __launch_bounds__(256) entry_logits_kernel(const uint4* __restrict__ h, const uint4* __restrict__ w,
-                                                           const int* __restrict__ cols, int64_t n, int K,
-                                                           int vec_per_row, float* __restrict__ xk) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= n) return;
-  const int col = cols[i];
-  if (col == kNoEntry) return;
-  const uint4* a = h + i / K * vec_per_row;
-  const uint4* b = w + (int64_t)col * vec_per_row;
+// h . w by one warp, in every lane: 32-bit sums of exact products.
+__device__ __forceinline__ float warp_dot(const uint4* __restrict__ a, const uint4* __restrict__ b, int vec_per_row) {
   float s0 = 0.f, s1 = 0.f;
 #pragma unroll 4
-  for (int v = lane; v < vec_per_row; v += 32) {
+  for (int v = threadIdx.x & 31; v < vec_per_row; v += 32) {
     const uint4 x = a[v], y = b[v];
     s0 = fmaf(bf16lo(x.x), bf16lo(y.x), s0);
     s1 = fmaf(bf16hi(x.x), bf16hi(y.x), s1);
@@ -2209,8 +2203,105 @@ __global__ void __launch_bounds__(256) entry_logits_kernel(const uint4* __restri
     s0 = fmaf(bf16lo(x.w), bf16lo(y.w), s0);
     s1 = fmaf(bf16hi(x.w), bf16hi(y.w), s1);
   }
-  const float s = warp_sum(s0 + s1);
-  if (lane == 0) xk[i] = s;
+  return warp_sum(s0 + s1);
+}
+
+// The logits at the entries, xk[r][e] = h_r . w_col, one warp an entry.  The GEMM's accumulators cut every
+// partial sum to 24 bits towards zero, which takes about 1e-9 H of a logit away; a distilled student's likely
+// tokens are mostly among the entries, so this leaves little of it (loss of an 8B-sized head against 64 bits:
+// 1.3e-5 -> 2.5e-6).  A cross entropy takes its target's logit from here where exact_tops_kernel deals with its
+// tail as well, and from the accumulators below kExactTopsHidden: target and tail are then short by about the
+// same.
+__global__ void __launch_bounds__(256) entry_logits_kernel(const uint4* __restrict__ h, const uint4* __restrict__ w,
+                                                           const int* __restrict__ cols, int64_t n, int K,
+                                                           int vec_per_row, float* __restrict__ xk) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const int col = cols[i];
+  if (col == kNoEntry) return;
+  const float s = warp_dot(h + i / K * vec_per_row, w + (int64_t)col * vec_per_row, vec_per_row);
+  if ((threadIdx.x & 31) == 0) xk[i] = s;
+}
+
+// The tail's likely tokens, with logits as exact as the entries': of each partial set whose largest column holds
+// 2^-10 of its row's sum or more, that column's share is taken from warp_dot instead of the accumulators.  WARPS warps
+// a row, as row_losses_kernel; they share the columns found.  The other columns are many and unlikely, and their
+// logits small, so what the accumulators cut of them does not show (a set's second likely token keeps its cut logit:
+// 14 rows of 1992 against 1174 columns, five sets, stay at 2e-6).  Cross entropy against 64 bits: 4 rows of 3904
+// against 17394 columns 3e-6 -> 5e-7, 16384 of 1024 against 151936 1.2e-6 -> 2e-7 (34 us for 8192 of those).
+constexpr int kExactTopsHidden = 1024;
+constexpr float kTopShare = 1.f / 1024.f;
+template <int WARPS>
+__global__ void __launch_bounds__(128) exact_tops_kernel(const uint4* __restrict__ h, const uint4* __restrict__ w,
+                                                         int vec_per_row, const float* __restrict__ part_m,
+                                                         const int* __restrict__ part_c, float* __restrict__ part_s,
+                                                         int sets, const int* __restrict__ sets_dev,
+                                                         const int* __restrict__ pos,
+                                                         const int64_t* __restrict__ row_ids,
+                                                         const float* __restrict__ xk, const int* __restrict__ cols,
+                                                         int K, int64_t N, int V, float c,
+                                                         const int* __restrict__ err) {
+  static_assert(WARPS == 1 || WARPS == 4, "a block's four warps take four rows or one");
+  constexpr int kList = 256;  // sets taken at a time
+  __shared__ float s_m[4], s_s[4];
+  __shared__ int s_list[4 / WARPS][kList], s_count[4 / WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * (4 / WARPS) + (WARPS == 1 ? warp : 0);
+  if (r >= N || row_ids[r] != kRowLive || *err != 0) return;  // after an error the sets may hold anything
+  const int64_t at = pos ? pos[r] : r;
+  if (sets_dev != nullptr) sets = *sets_dev;
+  const int first = WARPS == 1 ? lane : (int)threadIdx.x;
+  int* list = s_list[WARPS == 1 ? warp : 0];
+  int& count = s_count[WARPS == 1 ? warp : 0];
+  auto sync = [&]() {
+    if constexpr (WARPS == 1) __syncwarp();
+    else __syncthreads();
+  };
+  // the row's maximum m and its sum s of 2^(c (x - m)), over sets and entries
+  float m = -INFINITY, s = 0.f;
+  auto merge = [&](float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    if (mm > -INFINITY) {
+      s = s * exp2f((m - mm) * c) + s2 * exp2f((m2 - mm) * c);
+      m = mm;
+    }
+  };
+#pragma unroll 4
+  for (int q = first; q < sets; q += 32 * WARPS)
+    merge(part_m[(int64_t)q * N + at], part_s[(int64_t)q * N + at]);
+  for (int k = first; k < K; k += 32 * WARPS)
+    if (cols[r * K + k] != kNoEntry) merge(xk[r * K + k], 1.f);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    merge(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  if constexpr (WARPS == 4) {
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_s[warp] = s;
+    }
+    __syncthreads();
+    m = -INFINITY;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) merge(s_m[i], s_s[i]);
+  }
+  const float least = s * kTopShare;
+  const uint4* row = h + r * vec_per_row;
+  for (int q0 = 0; q0 < sets; q0 += kList) {
+    if (first == 0) count = 0;
+    sync();
+    for (int q = q0 + first; q < min(sets, q0 + kList); q += 32 * WARPS)
+      if (exp2f((part_m[(int64_t)q * N + at] - m) * c) >= least) list[atomicAdd(&count, 1)] = q;  // not for NaN
+    sync();
+    for (int i = WARPS == 1 ? 0 : warp; i < count; i += WARPS) {
+      const int64_t o = (int64_t)list[i] * N + at;
+      const int col = part_c[o];
+      if (col < 0 || col >= V) continue;
+      const float x = warp_dot(row, w + (int64_t)col * vec_per_row, vec_per_row);
+      if (lane == 0) part_s[o] += exp2f((x - part_m[o]) * c) - 1.f;
+    }
+    sync();
+  }
 }
 
 // h_c[k] = h[idx[k]] for k < n, 16 bytes per thread.
@@ -2487,12 +2578,12 @@ static bool row_loss_dense(int64_t N, int H, int V) {
   return N <= kRowLossDense || (N <= kRowLossDenseMost && (double)N * H * V <= kRowLossDenseWork);
 }
 
-// Workspace of a row loss.  Its forward's: the GEMM's partial maxima, sums and sums of all logits (`sets` of
-// each: the wide kernel's column groups of up to kBalanceMost times the forward's splits, which the balance
+// Workspace of a row loss.  Its forward's: the GEMM's partial maxima, their columns, sums and sums of all logits
+// (`sets` of each: the wide kernel's column groups of up to kBalanceMost times the forward's splits, which the balance
 // rule may take), and the numbering of the rows that count with their hidden rows gathered.
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 struct RowLossFwdLayout {
-  size_t pm_off, ps_off, px_off, counts_off, count_off, pos_off, idx_off, hc_off, total;
+  size_t pm_off, ps_off, px_off, pc_off, counts_off, count_off, pos_off, idx_off, hc_off, total;
   int splits, sets;
   bool gather;  // the rows that count are gathered before the GEMM
 };
@@ -2506,6 +2597,7 @@ static RowLossFwdLayout row_loss_fwd_layout(int64_t N, int H, int V) {
   L.pm_off = o; o += part;
   L.ps_off = o; o += part;
   L.px_off = o; o += part;
+  L.pc_off = o; o += part;
   L.counts_off = o; o += align256((size_t)std::max<int64_t>(1, cdiv64(N, kCompactRows)) * 4);
   L.count_off = o; o += 256;
   L.pos_off = o; o += align256((size_t)N * 4);
@@ -2956,7 +3048,8 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   if ((rc = launch_row_entries(tids, tlp, N, K, P, st, s, err))) return rc;
   const int vpr = H / 8;
   GemmParams p{};
-  if (P.loss == ROW_XENT) {
+  const bool exact_tops = H >= kExactTopsHidden;
+  if (P.loss == ROW_XENT && !exact_tops) {
     p.xk = st.xk;
   } else {
     IKRL_REQUIRE(cdiv64(N * K, 8) <= 0x7fffffffLL, IKRL_ERR_UNSUPPORTED, "%s: %lld rows of %d entries", what,
@@ -2970,6 +3063,7 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   p.M = (int)N; p.N = V; p.K = H;
   p.part_m = reinterpret_cast<float*>(w + L.pm_off);
   p.part_s = reinterpret_cast<float*>(w + L.ps_off);
+  p.part_c = exact_tops ? reinterpret_cast<int*>(w + L.pc_off) : nullptr;
   p.part_cap = L.sets;
   p.part_x = P.loss == ROW_XENT && P.smoothing != 0.f ? reinterpret_cast<float*>(w + L.px_off) : nullptr;
   p.err = err;
@@ -3032,8 +3126,16 @@ static int lmhead_row_loss_fwd(const char* what, const void* hidden, const void*
   } else {
     if ((rc = launch_k1<EPI_TAIL, false, false>(ta, tb, ta, tb2, p, m_tiles, L.splits, s))) return rc;
   }
-  return launch_row_losses(p.part_m, p.part_s, p.part_x, p.part_sets, p.m_dev ? p.m_dev + LIVE_SETS : nullptr, pos, N,
-                           K, P, st, loss, err, s);
+  const int* sets_dev = p.m_dev ? p.m_dev + LIVE_SETS : nullptr;
+  if (exact_tops) {
+    const bool wide_rows = row_takes_a_block(p.part_sets, N);
+    auto kern = wide_rows ? exact_tops_kernel<4> : exact_tops_kernel<1>;
+    kern<<<(unsigned)(wide_rows ? N : cdiv64(N, 4)), 128, 0, s>>>(
+        reinterpret_cast<const uint4*>(hidden), reinterpret_cast<const uint4*>(weight), vpr, p.part_m, p.part_c, p.part_s,
+        p.part_sets, sets_dev, pos, st.row_ids, st.xk, st.cols, K, N, V, P.c, err);
+    if ((rc = check_launch("exact_tops_kernel"))) return rc;
+  }
+  return launch_row_losses(p.part_m, p.part_s, p.part_x, p.part_sets, sets_dev, pos, N, K, P, st, loss, err, s);
 }
 
 // Backward of a row loss of few rows (row_loss_dense), all of them in one chunk, without the

@@ -89,6 +89,10 @@ int check_logits_arg(const char* what, const void* logits, int32_t dtype, int64_
 int distill_params(const char* what, const ikrl_distill_params* d, int V, int K, RowLossParams* out);
 int xent_params(const char* what, float smoothing, float z_loss, int V, RowLossParams* out);
 
+// Few rows come with many partial sets (a GEMM of one row tile cuts the columns as fine as it can): a block a row
+// joins them, otherwise a warp.
+inline bool row_takes_a_block(int sets, int64_t N) { return sets > 64 && N <= 4 * kNumSMs; }
+
 // The LM head's use of the two kernels in distill.cu: entries before its GEMM, losses after it.
 // tids / tlp: the teacher's [N][K], or targets with K = 1 and tlp null (ROW_XENT); clear: a word to
 // zero, or null.

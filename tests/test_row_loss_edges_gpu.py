@@ -381,3 +381,33 @@ def test_rows_of_very_different_gradients():
     assert torch.equal(dh[ok], want[1][ok]) and not bool(dh[6].isfinite().any()) and not bool(dw.isfinite().all())
     zero = run_head(ops.lmhead_distill, h, torch.zeros_like(w), up.clamp(max=1.0), ids, lp, kind="reverse")
     assert not bool(zero[1].any()) and bool(zero[2].isfinite().all())
+
+
+def likely_head(n, H, V, seed):
+    """Rows with eight likely tokens, as a trained model's: logits from 12 down over others of deviation 1.3.  Each
+    lies in another eighth of the vocabulary."""
+    g = torch.Generator().manual_seed(seed)
+    w = (0.02 * torch.randn(V, H, generator=g)).to(torch.bfloat16)
+    ids = torch.randint(0, V // 8, (n, 8), generator=g) + V // 8 * torch.arange(8)
+    boost = 12.0 - 0.8 * torch.arange(8) + torch.randn(n, 8, generator=g)
+    h = torch.randn(n, H, generator=g) + ((boost / (H * 4e-4))[:, :, None] * w[ids].float()).sum(1)
+    return h.to(torch.bfloat16), w, ids
+
+
+@pytest.mark.parametrize("loss", ["xent", "reverse"])
+@pytest.mark.parametrize("n,H,V", [(4, 4096, 6000), (14, 1992, 9001), (40, 1024, 20000), (1100, 4096, 20000)])
+def test_losses_through_a_wide_head(n, H, V, loss):
+    """The accumulators cut 1e-9 H of a logit; the likely tokens' logits are summed again in fp32.  Those err by 2^-24
+    of a logit of 12, about 2e-7 of a loss of 4; the unlikely tokens, a fifth of the mass with logits of about 2, by
+    4e-6 of that, 4e-7 of the loss.  With the likely ones from the accumulators it was 2e-6 to 5e-6."""
+    h, w, ids = likely_head(n, H, V, n + H)
+    if loss == "xent":
+        got = ops.lmhead_cross_entropy(h.to(DEV), w.to(DEV), ids[:, 0].contiguous().to(DEV))
+        rows = lambda y: xent_rows(y, ids[:, 0])  # noqa: E731
+    else:
+        few = ids[:, :2].contiguous()
+        lp = torch.log_softmax(torch.randn(n, 2, generator=torch.Generator().manual_seed(n)), 1) - 0.5
+        got = ops.lmhead_distill(h.to(DEV), w.to(DEV), few.to(DEV), lp.to(DEV), kind="reverse")
+        rows = lambda y: distill_rows(y, few, lp, "reverse")  # noqa: E731
+    want = rows(h.double() @ w.double().t())
+    assert float((got.double().cpu() - want).norm()) <= 1e-6 * float(want.norm())
