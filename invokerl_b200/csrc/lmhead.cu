@@ -2228,7 +2228,7 @@ __global__ void __launch_bounds__(256) entry_logits_kernel(const uint4* __restri
 // a row, as row_losses_kernel; they share the columns found.  The other columns are many and unlikely, and their
 // logits small, so what the accumulators cut of them does not show (a set's second likely token keeps its cut logit:
 // 14 rows of 1992 against 1174 columns, five sets, stay at 2e-6).  Cross entropy against 64 bits: 4 rows of 3904
-// against 17394 columns 3e-6 -> 5e-7, 16384 of 1024 against 151936 1.2e-6 -> 2e-7 (34 us for 8192 of those).
+// against 17394 columns 3e-6 -> 5e-7, 16384 of 1024 against 151936 1.2e-6 -> 2e-7 (38 us for 8192 of those).
 constexpr int kExactTopsHidden = 1024;
 constexpr float kTopShare = 1.f / 1024.f;
 template <int WARPS>
@@ -2337,7 +2337,7 @@ __global__ void scatter_rows_kernel(const uint4* __restrict__ src, const int* __
 //   dW    = 2^X dS'^T h',            dH_k = 2^(e_k + e_W - 29) dS'_k W'
 // What lies more than 2^29 below its largest loses bits, one for each further 2, which is 2^-40 of that largest at most.
 // Rows without a gradient are zeros in both operands (padding may hold NaN).  Infinities and NaN do not count for the
-// ranges and stay what they are.  One more pass over W and a copy: 0.5 ms of 20 (8192 x 4096 x 151936).
+// ranges and stay what they are.  One more pass over W and a copy: 0.6 ms of 21 (8192 x 4096 x 151936).
 struct RowRange {
   int* e;           // [rows] e_k, or kNoRange: no gradient
   float* mul;       // [rows] 2^(14 - e_k)
@@ -2471,8 +2471,7 @@ __global__ void ds_entries_kernel(const float* __restrict__ dloss, const int* __
 
 // First launch of the backward of few rows, a block a row: clears the error word; with h2 the hidden rows
 // twice, one under the other (the dW operand beside a dS of two terms); with gs what the dS epilogue multiplies and
-// adds.
-// Rows without a gradient go in as zeros: padding may hold NaN, and 0 NaN would reach all of dW.
+// adds.  Rows without a gradient go in as zeros: padding may hold NaN, and 0 NaN would reach all of dW.
 __global__ void __launch_bounds__(128) few_rows_kernel(const uint4* __restrict__ h, int vec_per_row, uint4* __restrict__ h2,
                                                        const float* __restrict__ dloss,
                                                        const int64_t* __restrict__ row_ids,
